@@ -206,6 +206,69 @@ int jgq_w4_matmul_noalloc(const void* x, int x_dtype, const uint8_t* packed,
                           const void* zero, const void* scale, int zs_dtype,
                           void* out, int64_t M, int64_t N, int64_t K, void* stream);
 
+/* ---- weights with a scale and a zero point per GROUP of the contraction axis (no counterpart in the reference, whose
+ * scales are per output channel, gptq.py:105-118) ---------------------------------------------------------------
+ * group_size: a positive multiple of 32; there are ceil(K / group_size) groups, the last one may be shorter.  scale and
+ * zero are (groups, N) row-major.
+ *     w[k, n] = scale[k / group_size, n] * (code[k, n] - zero[k / group_size, n])
+ * jgq_group_params: jgq_col_params of every group.  jgq_gptq_quantize_groups: jgq_gptq_quantize with those params; a block
+ * of the loop must lie in one group (group_size % block_size == 0).  jgq_w4_group_matmul: jgq_w4_matmul with them; the
+ * first 16384 bytes of its workspace must be zero before its first use (the kernels leave them zero). */
+int jgq_group_params(const float* W, int64_t K, int64_t N, int group_size, int maxq, float* scale, float* zero, void* stream);
+int jgq_gptq_quantize_groups(float* W, const float* L, const float* scale, const float* zero,
+                             int64_t K, int64_t N, int group_size, int block_size, int maxq,
+                             void* Q, int q_dtype, uint8_t* codes,
+                             void* ws, size_t ws_bytes, void* stream);
+size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int group_size, int transpose_b);
+int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed,
+                        const void* zero, const void* scale, int zs_dtype,
+                        void* out, int64_t M, int64_t N, int64_t K, int group_size, int flags,
+                        void* ws, size_t ws_bytes, void* stream);
+
+/* ---- paged cache of 8-bit keys and values (no counterpart in the reference) -----------------------------------------
+ * A page holds page_size (64, 128 or 256) tokens of every kv head.  Codes are bytes in excess 128 of rows padded to DW =
+ * 64, 128 or 256 channels (the smallest that holds head_dim <= 256), with one fp32 scale per page and head:
+ *     k (pages, kv_heads, page_size, DW)      v (pages, kv_heads, page_size / 64, DW, 64)      value = (byte - 128) * scale
+ * jgq_kv_write: row t of k_new, v_new (tokens, kv_heads, head_dim; strides in elements, the last axis contiguous) goes to
+ *     slot slots[t] = page * page_size + offset; a slot outside the cache is passed over.  The rows of one page must be
+ *     consecutive rows with ascending slots (as jgq_kv_reserve makes them).  A page's scale is set when its first token is
+ *     written and grows by powers of two when later tokens need it; the codes that are there are then rounded again.
+ * jgq_kv_read: out (count, kv_heads, page_size, head_dim) of the pages index[i]; NaN where there is no such page.
+ * jgq_kv_attend: q (tokens, q_heads, head_dim; strides in elements), out and lse (tokens, q_heads[, head_dim]) contiguous, lse
+ *     (natural logarithm of the sum of exponentials) may be null.  Sequence r has lengths[r] tokens (at most
+ *     table_width * page_size are looked at) in the pages block_table[r][...]; its rows are cu_seqlens[r] .. cu_seqlens[r + 1] - 1, or
+ *     row r where cu_seqlens is null; row i of n sees the first lengths[r] - n + i + 1 tokens, and is zero where that is none.
+ *     max_new is the expected largest n (a larger one is computed all the same).  Rows behind cu_seqlens[requests] are left as
+ *     they were, or zeroed with JGQ_KV_ZERO_REST.  A page number outside [0, pages) makes its rows NaN.
+ *     The first 16384 bytes of the workspace must be zero before its first use (the kernels leave them zero).
+ * jgq_kv_reserve: pages of finished requests (finished[r] != 0; may be null) back to the stack free_pages[0 .. free_count), pages
+ *     for lengths[r] + added[r] tokens of every request from it into block_table, held[r] (pages of a request) with them;
+ *     then slots and positions of the added tokens (-1 and 0 behind the last one, up to max_tokens), cu_seqlens (requests + 1) and
+ *     lengths_out = lengths + added.  All or nothing: otherwise a bit is or-ed into *status, no page is taken, every slot
+ *     is -1, cu_seqlens is zero and lengths_out = lengths.  Any page_size >= 1.
+ * jgq_capture_id: 0 if the stream is not being captured, else a number of the capture (host; launches nothing). */
+enum { JGQ_KV_ZERO_REST = 1 };
+enum { JGQ_KV_NO_PAGES = 1, JGQ_KV_ROW_FULL = 2, JGQ_KV_TOO_MANY_TOKENS = 4, JGQ_KV_BAD_LENGTH = 8, JGQ_KV_BAD_TABLE = 16 };
+int jgq_kv_write(const void* k_new, const void* v_new, int dtype, int64_t k_token_stride, int64_t k_head_stride,
+                 int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                 uint8_t* k, uint8_t* v, float* k_scale, float* v_scale,
+                 int64_t pages, int page_size, int64_t kv_heads, int64_t head_dim, void* stream);
+int jgq_kv_read(const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
+                int64_t pages, int page_size, int64_t kv_heads, int64_t head_dim,
+                const int64_t* index, int64_t count, void* k_out, void* v_out, int dtype, void* stream);
+size_t jgq_kv_attend_workspace_bytes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, int q_dtype);
+int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride, void* out, float* lse,
+                  const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale, int64_t pages, int page_size,
+                  const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths,
+                  const int32_t* cu_seqlens, int64_t tokens, int64_t requests, int64_t max_new,
+                  int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale, int flags,
+                  void* ws, size_t ws_bytes, void* stream);
+int jgq_kv_reserve(int32_t* block_table, int64_t table_stride, int64_t table_width, int32_t* held, int32_t* free_pages,
+                   int32_t* free_count, int64_t pages, int page_size, const int32_t* lengths, const int32_t* added,
+                   const uint8_t* finished, int64_t requests, int64_t* slots, int32_t* positions, int64_t max_tokens,
+                   int32_t* cu_seqlens, int32_t* lengths_out, int32_t* status, void* stream);
+uint64_t jgq_capture_id(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,6 @@
 """B200 (sm_100a) implementation of the jax-gptq hot path: GPTQ layer quantization,
 int4 pack/unpack and the packed-int4 matmul, behind the reference's own function
-names.  All arithmetic runs in libjgq.so (hand-written CUDA behind a C ABI).
+names, and a paged cache of 8-bit keys and values for serving what it made.  All arithmetic runs in libjgq.so (hand-written CUDA behind a C ABI).
 
 The public names are resolved on first use so that ``jax_gptq_b200.build`` can be
 imported (and run) before the shared library exists; touching any operator
@@ -12,7 +12,8 @@ _GPTQ_NAMES = ('QuantizedMatrix', 'accumulate_H', 'get_col_quantize_params', 'pa
                'unpack_matrix', 'pack_along_axis', 'unpack_along_axis', 'pack_rowwise', 'pack_colwise',
                'unpack_rowwise', 'unpack_colwise', 'quant_matrix_shape')
 _OP_NAMES = ('quantized_matmul',)
-__all__ = list(_GPTQ_NAMES + _OP_NAMES)
+_CACHE_NAMES = ('KVCache', 'PageTable')
+__all__ = list(_GPTQ_NAMES + _OP_NAMES + _CACHE_NAMES)
 
 
 def _load_public():
@@ -23,10 +24,13 @@ def _load_public():
         ns[n] = getattr(g, n)
     for n in _OP_NAMES:
         ns[n] = getattr(o, n)
+    c = importlib.import_module(__name__ + '.cache')
+    for n in _CACHE_NAMES:
+        ns[n] = getattr(c, n)
 
 
 def __getattr__(name):
-    if name in ('gptq', 'op'):      # submodules, as in the reference: jax_gptq.gptq.gptq(W, xs)
+    if name in ('gptq', 'op', 'cache'):      # submodules, as in the reference: jax_gptq.gptq.gptq(W, xs)
         return importlib.import_module(__name__ + '.' + name)
     if name in __all__:
         _load_public()

@@ -15,6 +15,9 @@ F32, F16, BF16, U8, I32 = 0, 1, 2, 3, 4
 STATUS_NOT_PD, STATUS_NAN, STATUS_TIMEOUT = 1, 2, 4
 W4_TRANSPOSE_B, W4_WEIGHTS_SETTLED = 1, 2
 
+KV_ZERO_REST = 1
+KV_NO_PAGES, KV_ROW_FULL, KV_TOO_MANY_TOKENS, KV_BAD_LENGTH, KV_BAD_TABLE = 1, 2, 4, 8, 16
+
 _i64, _int, _vp, _sz = C.c_int64, C.c_int, C.c_void_p, C.c_size_t
 
 # name -> (restype, argtypes); mirrors include/jgq.h one to one
@@ -53,6 +56,17 @@ SIGNATURES = {
     'jgq_w4_matmul': (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
     'jgq_w4_matmul_noalloc_max_bytes': (_sz, []),
     'jgq_w4_matmul_noalloc': (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp]),
+    'jgq_group_params': (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _vp]),
+    'jgq_gptq_quantize_groups': (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _vp, _int, _vp, _vp, _sz, _vp]),
+    'jgq_w4_group_matmul_workspace_bytes': (_sz, [_i64, _i64, _i64, _int, _int]),
+    'jgq_w4_group_matmul': (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _int, _int, _vp, _sz, _vp]),
+    'jgq_kv_write': (_int, [_vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _int, _i64, _i64, _vp]),
+    'jgq_kv_read': (_int, [_vp, _vp, _vp, _vp, _i64, _int, _i64, _i64, _vp, _i64, _vp, _vp, _int, _vp]),
+    'jgq_kv_attend_workspace_bytes': (_sz, [_i64, _i64, _i64, _i64, _int]),
+    'jgq_kv_attend': (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                             _i64, _i64, _i64, _i64, C.c_float, _int, _vp, _sz, _vp]),
+    'jgq_kv_reserve': (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _int, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    'jgq_capture_id': (C.c_uint64, [_vp]),
 }
 
 

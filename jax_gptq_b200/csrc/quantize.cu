@@ -525,7 +525,7 @@ gptq_block_kernel(const QuantParams p) {
 
 template <typename QT>
 static int run_quantize(float* W, const float* L, const float* scale, const float* zero,
-                        int K, int64_t N, int bs, int maxq, QT* Q, uint8_t* codes, float* P, cudaStream_t s) {
+                        int K, int64_t N, int group, int bs, int maxq, QT* Q, uint8_t* codes, float* P, cudaStream_t s) {
   auto kern = gptq_block_kernel<QT>;
   struct AttrTag {};
   once_per_device<AttrTag>([&]() {
@@ -544,6 +544,8 @@ static int run_quantize(float* W, const float* L, const float* scale, const floa
   p.P = P;
   for (int start = 0; start < K; start += bs) {
     p.start = start;
+    p.scale = scale + (start / group) * N;       // a block lies in one group
+    p.zero = zero + (start / group) * N;
     p.apply_prev = fused && start > 0;
     const int rest = K - (start + bs);
     p.make_next = fused && rest > 0;
@@ -581,10 +583,11 @@ extern "C" size_t jgq_gptq_quantize_workspace_bytes(int64_t K, int64_t N, int bl
   return align_up((size_t)block_size * (size_t)N * sizeof(float), 256);
 }
 
-extern "C" int jgq_gptq_quantize(float* W, const float* L, const float* scale, const float* zero,
-                                 int64_t K, int64_t N, int block_size, int maxq,
-                                 void* Q, int q_dtype, uint8_t* codes,
-                                 void* ws, size_t ws_bytes, void* stream) {
+// `group`: rows that share a scale and a zero point (K: all)
+static int quantize(float* W, const float* L, const float* scale, const float* zero,
+                    int64_t K, int64_t N, int64_t group, int block_size, int maxq,
+                    void* Q, int q_dtype, uint8_t* codes,
+                    void* ws, size_t ws_bytes, void* stream) {
   JGQ_REQUIRE(K > 0 && N > 0, JGQ_ERR_ARG, "gptq_quantize: bad shape K=%lld N=%lld", (long long)K, (long long)N);
   JGQ_REQUIRE(K <= 46340 && N <= 2147483647LL, JGQ_ERR_LIMIT, "gptq_quantize: shape too large");
   JGQ_REQUIRE(block_size >= 1 && block_size <= 128, JGQ_ERR_ARG, "gptq_quantize: block_size %d not in [1,128]", block_size);
@@ -598,15 +601,31 @@ extern "C" int jgq_gptq_quantize(float* W, const float* L, const float* scale, c
               "gptq_quantize: workspace %zu < %zu bytes", ws_bytes, jgq_gptq_quantize_workspace_bytes(K, N, block_size));
   JGQ_REQUIRE(aligned(ws, 16), JGQ_ERR_ALIGN, "gptq_quantize: workspace must be 16-byte aligned");
   // K / block_size launches whose arguments depend on these values alone: replayed as a graph when they recur
-  struct { int tag; int block_size, maxq, q_dtype; int64_t K, N; const void *W, *L, *scale, *zero, *Q, *codes, *ws; } key;
+  struct { int tag; int block_size, maxq, q_dtype; int64_t K, N, group; const void *W, *L, *scale, *zero, *Q, *codes, *ws; } key;
   memset(&key, 0, sizeof(key));
-  key.tag = 2; key.block_size = block_size; key.maxq = maxq; key.q_dtype = q_dtype; key.K = K; key.N = N;
+  key.tag = 2; key.block_size = block_size; key.maxq = maxq; key.q_dtype = q_dtype; key.K = K; key.N = N; key.group = group;
   key.W = W; key.L = L; key.scale = scale; key.zero = zero; key.Q = Q; key.codes = codes; key.ws = ws;
   return run_replayed(key, (cudaStream_t)stream, [&](cudaStream_t s) {
     switch (q_dtype) {
-      case JGQ_F32:  return run_quantize<float>(W, L, scale, zero, (int)K, N, block_size, maxq, (float*)Q, codes, (float*)ws, s);
-      case JGQ_F16:  return run_quantize<__half>(W, L, scale, zero, (int)K, N, block_size, maxq, (__half*)Q, codes, (float*)ws, s);
-      default:       return run_quantize<__nv_bfloat16>(W, L, scale, zero, (int)K, N, block_size, maxq, (__nv_bfloat16*)Q, codes, (float*)ws, s);
+      case JGQ_F32:  return run_quantize<float>(W, L, scale, zero, (int)K, N, (int)group, block_size, maxq, (float*)Q, codes, (float*)ws, s);
+      case JGQ_F16:  return run_quantize<__half>(W, L, scale, zero, (int)K, N, (int)group, block_size, maxq, (__half*)Q, codes, (float*)ws, s);
+      default:       return run_quantize<__nv_bfloat16>(W, L, scale, zero, (int)K, N, (int)group, block_size, maxq, (__nv_bfloat16*)Q, codes, (float*)ws, s);
     }
   });
+}
+
+extern "C" int jgq_gptq_quantize(float* W, const float* L, const float* scale, const float* zero,
+                                 int64_t K, int64_t N, int block_size, int maxq,
+                                 void* Q, int q_dtype, uint8_t* codes,
+                                 void* ws, size_t ws_bytes, void* stream) {
+  return quantize(W, L, scale, zero, K, N, K, block_size, maxq, Q, q_dtype, codes, ws, ws_bytes, stream);
+}
+
+extern "C" int jgq_gptq_quantize_groups(float* W, const float* L, const float* scale, const float* zero,
+                                        int64_t K, int64_t N, int group_size, int block_size, int maxq,
+                                        void* Q, int q_dtype, uint8_t* codes,
+                                        void* ws, size_t ws_bytes, void* stream) {
+  JGQ_REQUIRE(group_size > 0 && block_size > 0 && group_size % block_size == 0, JGQ_ERR_ARG,
+              "gptq_quantize: group_size %d is not a multiple of block_size %d", group_size, block_size);
+  return quantize(W, L, scale, zero, K, N, group_size, block_size, maxq, Q, q_dtype, codes, ws, ws_bytes, stream);
 }

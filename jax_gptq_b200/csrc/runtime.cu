@@ -142,3 +142,9 @@ namespace jgq { unsigned long long launches(); }
 extern "C" int jgq_version(void) { return 100; }
 extern "C" uint64_t jgq_launch_count(void) { return (uint64_t)jgq::launches(); }
 extern "C" const char* jgq_last_error(void) { return jgq::error_buffer(); }
+extern "C" uint64_t jgq_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) { cudaGetLastError(); return 0; }
+  return status == cudaStreamCaptureStatusActive ? (uint64_t)id + 1 : 0;
+}

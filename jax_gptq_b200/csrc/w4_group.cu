@@ -1,0 +1,372 @@
+// Packed-int4 matmul with a scale and a zero point per GROUP of the contraction axis and output channel:
+//
+//   w[k, n] = scale[k / g, n] * (code[k, n] - zero[k / g, n])
+//   forward      out[m, n] = sum_k x[m, k] w[k, n]
+//   transposed   out[m, k] = sum_n x[m, n] w[k, n]
+//
+// This file holds the dispatcher and the general kernel (any M, N, even K, pointers aligned to their element).
+//
+// General kernel: mma.sync with the weights as the 16-row operand, always as exact codes; what depends on the
+// group is applied to fp32 numbers, so nothing but the sums is rounded:
+//   forward      the sums of one group are finished with  total += scale * (sum - zero * xsum[m, group])  before the next
+//                group's begin; xsum comes from a small kernel in front;
+//   transposed   scale varies along the contraction, the group along the rows: a tile's rows lie in one group, the
+//                activations are multiplied with that group's scales while they are staged (products in fp32, split into
+//                bf16 planes), and sum_n x scale zero is summed up beside it.
+// 16-bit activations enter the forward product as they are; x * scale as two bf16 planes (16 bits of the product, below
+// the result's own rounding); fp32 activations as three (all 24 bits).
+// A long contraction with few tiles is split; the slices are added in order by the kernel behind.
+#include "w4_common.cuh"
+#include "w4_plans.cuh"
+#include <algorithm>
+#include <cstring>
+
+namespace jgq {
+
+constexpr int WG_TOK = 64;                  // tokens per tile
+constexpr int WG_KC = 32;                   // contraction indices per stage: a group is a multiple of it
+constexpr int WG_THREADS = 128;
+constexpr int WG_XSTRIDE = WG_KC + 8;       // elements per staged row: 80 bytes, eight rows start on eight different 16-byte banks
+
+template <typename XT, bool TB> struct GroupType {                 // operand type and planes of the activations
+  using CT = typename std::conditional<std::is_same<XT, __half>::value && !TB, __half, __nv_bfloat16>::type;
+  static constexpr int PL = std::is_same<XT, float>::value ? 3 : (TB ? 2 : 1);
+};
+
+struct GroupParams {
+  const void* x; const uint8_t* packed; const void* zero; const void* scale; void* out;
+  const float* xsum;           // forward: [M][groups]
+  float* part;                 // [splits][M][rows] when the contraction is split
+  int64_t M, N, K;
+  int64_t rows, depth;         // weight rows of the product (N or K) and its contraction length (K or N)
+  int group, groups;
+  int chunks_per_split, splits;
+  int vec_w;                   // 4-byte loads of codes are legal
+  int vec_x;                   // 16-byte loads of activations are legal
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <typename CT> __device__ __forceinline__ uint32_t pair_bits(float a, float b);
+template <> __device__ __forceinline__ uint32_t pair_bits<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pair_bits<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// sums of the activations per group: xsum[m][i] = sum of x[m, i g .. i g + g - 1]; one warp per (row, group)
+template <typename XT>
+__global__ void __launch_bounds__(256) w4_group_xsum_kernel(const XT* __restrict__ x, float* __restrict__ xsum, int64_t M, int64_t K, int group, int groups) {
+  const int64_t item = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (item >= M * groups) return;
+  const int64_t m = item / groups, i = item % groups;
+  const int64_t k0 = i * group, k1 = min(K, k0 + group);
+  float s = 0.f;
+  for (int64_t k = k0 + lane; k < k1; k += 32) s += to_f32<XT>(x[m * K + k]);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) xsum[item] = s;
+}
+
+// BM: weight rows per tile (32 or 64; in the transposed product a tile lies in one group)
+template <typename XT, typename ZST, bool TB, int BM>
+__global__ void __launch_bounds__(WG_THREADS)
+w4_group_kernel(const GroupParams p) {
+  using CT = typename GroupType<XT, TB>::CT;
+  constexpr int PL = GroupType<XT, TB>::PL;
+  constexpr int WM = BM / 32, WN = 4 / WM;             // warps along rows and tokens
+  constexpr int NTW = WG_TOK / WN / 8;                 // token octets per warp
+  constexpr int ASTRIDE = TB ? WG_KC + 8 : BM + 8;     // elements; forward: [contraction][row], transposed: [row][contraction]
+  constexpr int AROWS = TB ? BM : WG_KC;
+  constexpr int WORDS = BM * WG_KC / 8 / WG_THREADS;   // 4-byte words of codes per thread and stage
+  __shared__ __align__(16) CT sa[2][AROWS * ASTRIDE];
+  __shared__ __align__(16) CT sx[2][PL][WG_TOK * WG_XSTRIDE];
+  __shared__ float scz[WG_TOK];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int wm = (warp % WM) * 32, wn = (warp / WM) * (WG_TOK / WN);
+  const int64_t row0 = (int64_t)blockIdx.x * BM, tok0 = (int64_t)blockIdx.y * WG_TOK;
+  const int64_t chunks = (p.depth + WG_KC - 1) / WG_KC;
+  const int64_t c_begin = (int64_t)blockIdx.z * p.chunks_per_split, c_end = min(chunks, c_begin + p.chunks_per_split);
+  const int64_t tb_group = TB ? row0 / p.group : 0;
+
+  uint32_t wreg[WORDS];
+  float xreg[16], cz = 0.f;
+  const int xt = tid >> 1, xh = (tid & 1) * 16;        // this thread's token of the tile and half of the stage's indices
+  const XT* xrow = reinterpret_cast<const XT*>(p.x) + (tok0 + xt) * p.depth;
+  const bool xlive = tok0 + xt < p.M;
+
+  auto fetch = [&](int64_t c) {
+    const int64_t d0 = c * WG_KC;
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) {
+      const int i = tid + WG_THREADS * u;
+      // forward: BM / 4 words of each of 16 byte rows; transposed: 8 words of each of BM / 2 byte rows
+      const int64_t br = TB ? row0 / 2 + i / 8 : d0 / 2 + i / (BM / 4);
+      const int64_t n = TB ? d0 + 4 * (i % 8) : row0 + 4 * (i % (BM / 4));
+      uint32_t w = 0;
+      if (2 * br < p.K && n < p.N) {
+        const uint8_t* src = p.packed + br * p.N + n;
+        if (p.vec_w) w = *reinterpret_cast<const uint32_t*>(src);       // N % 4 == 0: the word is inside the row
+        else
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (n + b < p.N) w |= (uint32_t)src[b] << (8 * b);
+      }
+      wreg[u] = w;
+    }
+    const int64_t d = d0 + xh;
+    if (xlive && p.vec_x && d + 16 <= p.depth) {
+      __align__(16) XT e[16];
+#pragma unroll
+      for (int v = 0; v < (int)sizeof(XT); ++v) reinterpret_cast<uint4*>(e)[v] = reinterpret_cast<const uint4*>(xrow + d)[v];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) xreg[i] = to_f32<XT>(e[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) xreg[i] = (xlive && d + i < p.depth) ? to_f32<XT>(xrow[d + i]) : 0.f;
+    }
+    if (TB) {                                          // times this tile's scales; sum_n x scale zero beside it
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = d + i < p.depth;
+        const int64_t o = tb_group * p.N + (in ? d + i : 0);
+        xreg[i] = in ? __fmul_rn(xreg[i], zs_to_f32<ZST>(p.scale, o)) : 0.f;
+        cz = fmaf(xreg[i], zs_to_f32<ZST>(p.zero, o), cz);
+      }
+    }
+  };
+  auto stage = [&](int buf) {
+    CT* a = sa[buf];
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) {
+      const int i = tid + WG_THREADS * u;
+      const uint32_t w = wreg[u];
+      uint32_t e[2], o[2];                             // four channels of the even and of the odd contraction-axis index
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t b = __byte_perm(w, 0, h ? 0x4342 : 0x4140);       // two channels' bytes in the halves of a word
+        e[h] = MmaType<CT>::expand(b);
+        o[h] = MmaType<CT>::expand(b >> 4);
+      }
+      const int r = TB ? 2 * (i / 8) : 2 * (i / (BM / 4)), c = TB ? 4 * (i % 8) : 4 * (i % (BM / 4));
+      *reinterpret_cast<uint2*>(a + r * ASTRIDE + c) = make_uint2(e[0], e[1]);
+      *reinterpret_cast<uint2*>(a + (r + 1) * ASTRIDE + c) = make_uint2(o[0], o[1]);
+    }
+#pragma unroll
+    for (int pl = 0; pl < PL; ++pl) {
+      uint32_t b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        b[i] = pair_bits<CT>(xreg[2 * i], xreg[2 * i + 1]);
+        if (pl + 1 < PL) {                             // what this plane leaves; bf16 is the upper half of an fp32
+          xreg[2 * i] -= __uint_as_float(b[i] << 16);
+          xreg[2 * i + 1] -= __uint_as_float(b[i] & 0xffff0000u);
+        }
+      }
+      uint4* dst = reinterpret_cast<uint4*>(&sx[buf][pl][xt * WG_XSTRIDE + xh]);
+      dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
+      dst[1] = make_uint4(b[4], b[5], b[6], b[7]);
+    }
+  };
+
+  float acc[2][NTW][4], total[TB ? 1 : 2][TB ? 1 : NTW][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NTW; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { acc[i][j][e] = 0.f; if (!TB) total[i][j][e] = 0.f; }
+
+  // the sums of one group into the totals; a group that two slices share gives its zero point to the one it begins in
+  auto finish_group = [&](int64_t grp) {
+    const bool begins = grp * p.group >= c_begin * WG_KC;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t n = row0 + wm + 16 * i + g + 8 * h;
+        float s = 0.f, z = 0.f;
+        if (n < p.rows) { s = zs_to_f32<ZST>(p.scale, grp * p.N + n); z = zs_to_f32<ZST>(p.zero, grp * p.N + n); }
+#pragma unroll
+        for (int j = 0; j < NTW; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int64_t m = tok0 + wn + 8 * j + 2 * q + e;
+            const float xs = begins && m < p.M ? p.xsum[m * p.groups + grp] : 0.f;
+            if (!TB) total[i][j][2 * h + e] = fmaf(s, acc[i][j][2 * h + e] - z * xs, total[i][j][2 * h + e]);
+            acc[i][j][2 * h + e] = 0.f;
+          }
+      }
+  };
+
+  if (c_begin < c_end) {
+    fetch(c_begin);
+    stage(0);
+  }
+  __syncthreads();
+  for (int64_t c = c_begin; c < c_end; ++c) {
+    const int buf = (int)((c - c_begin) & 1);
+    if (c + 1 < c_end) fetch(c + 1);
+    const uint32_t ab = (uint32_t)__cvta_generic_to_shared(sa[buf]);
+#pragma unroll
+    for (int k16 = 0; k16 < WG_KC; k16 += 16) {
+      uint32_t a[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (TB) ldsm_x4(a[i], ab + 2 * ((wm + 16 * i + (lane & 15)) * ASTRIDE + k16 + 8 * (lane >> 4)));
+        else    ldsm_x4_t(a[i], ab + 2 * ((k16 + (lane & 7) + 8 * (lane >> 4)) * ASTRIDE + wm + 16 * i + 8 * ((lane >> 3) & 1)));
+      }
+#pragma unroll
+      for (int pl = 0; pl < PL; ++pl) {
+        const uint32_t xb = (uint32_t)__cvta_generic_to_shared(sx[buf][pl]);
+#pragma unroll
+        for (int j = 0; j < NTW; j += 2) {
+          uint32_t b[4];
+          ldsm_x4(b, xb + 2 * ((wn + 8 * j + (lane & 7) + 8 * (lane >> 4)) * WG_XSTRIDE + k16 + 8 * ((lane >> 3) & 1)));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            MmaType<CT>::mma(acc[i][j], a[i], b[0], b[1]);
+            MmaType<CT>::mma(acc[i][j + 1], a[i], b[2], b[3]);
+          }
+        }
+      }
+    }
+    if (!TB && ((c + 1) * WG_KC % p.group == 0 || c + 1 == c_end)) finish_group(c * WG_KC / p.group);
+    if (c + 1 < c_end) stage(buf ^ 1);
+    __syncthreads();
+  }
+  if (TB) {
+    cz += __shfl_xor_sync(0xffffffffu, cz, 1);
+    if ((tid & 1) == 0) scz[xt] = cz;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < NTW; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = wn + 8 * j + 2 * q + e;
+      const int64_t m = tok0 + t;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t r = row0 + wm + 16 * i + g + 8 * h;
+          if (r >= p.rows) continue;
+          const float v = TB ? acc[i][j][2 * h + e] - scz[t] : total[TB ? 0 : i][TB ? 0 : j][2 * h + e];
+          if (p.splits > 1) p.part[((int64_t)blockIdx.z * p.M + m) * p.rows + r] = v;
+          else reinterpret_cast<XT*>(p.out)[m * p.rows + r] = from_f32<XT>(v);
+        }
+    }
+}
+
+// the slices of a split contraction, added in order
+template <typename XT>
+__global__ void __launch_bounds__(256) w4_group_join_kernel(const float* __restrict__ part, XT* __restrict__ out, int64_t count, int splits) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
+    float s = 0.f;
+    for (int z = 0; z < splits; ++z) s += part[z * count + i];
+    out[i] = from_f32<XT>(s);
+  }
+}
+
+// ------------------------------------------------------------------ host ----
+struct GroupPlan { int bm, tiles, mtiles, splits, chunks_per_split; size_t xsum_bytes, part_bytes; };
+
+static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int transpose_b) {
+  GroupPlan pl;
+  memset(&pl, 0, sizeof(pl));
+  const int64_t rows = transpose_b ? K : N, depth = transpose_b ? N : K, chunks = cdiv(depth, WG_KC);
+  pl.mtiles = (int)cdiv(M, WG_TOK);
+  pl.bm = 64;
+  // a transposed tile lies in one group; narrower tiles where the wide ones leave most SMs without one
+  while (pl.bm > 32 && ((transpose_b && group % pl.bm != 0) || cdiv(rows, pl.bm) * pl.mtiles < sm_count() / 2)) pl.bm /= 2;
+  pl.tiles = (int)cdiv(rows, pl.bm);
+  const int64_t want = std::max<int64_t>(1, 3 * (int64_t)sm_count() / ((int64_t)pl.tiles * pl.mtiles));
+  const int64_t splits = std::min<int64_t>({want, cdiv(chunks, 8), 64});       // at least eight stages each
+  pl.chunks_per_split = (int)cdiv(chunks, splits);
+  pl.splits = (int)cdiv(chunks, pl.chunks_per_split);
+  pl.xsum_bytes = transpose_b ? 0 : align_up((size_t)M * cdiv(K, group) * sizeof(float), 256);
+  pl.part_bytes = pl.splits > 1 ? align_up((size_t)pl.splits * M * rows * sizeof(float), 256) : 0;
+  return pl;
+}
+
+template <typename XT, typename ZST, bool TB>
+static int launch_group(const GroupPlan& pl, GroupParams& p, uint8_t* ws, cudaStream_t s) {
+  if (!TB) {
+    float* xsum = reinterpret_cast<float*>(ws);
+    w4_group_xsum_kernel<XT><<<(unsigned)cdiv(p.M * p.groups, 8), 256, 0, s>>>((const XT*)p.x, xsum, p.M, p.K, p.group, p.groups);
+    JGQ_LAUNCHED();
+    p.xsum = xsum;
+  }
+  p.part = reinterpret_cast<float*>(ws + pl.xsum_bytes);
+  const dim3 grid((unsigned)pl.tiles, (unsigned)pl.mtiles, (unsigned)pl.splits);
+  if (pl.bm == 64) w4_group_kernel<XT, ZST, TB, 64><<<grid, WG_THREADS, 0, s>>>(p);
+  else             w4_group_kernel<XT, ZST, TB, 32><<<grid, WG_THREADS, 0, s>>>(p);
+  if (pl.splits > 1) {
+    JGQ_LAUNCHED();
+    const int64_t count = p.M * p.rows;
+    w4_group_join_kernel<XT><<<(unsigned)std::min<int64_t>(cdiv(count, 256), 8 * (int64_t)sm_count()), 256, 0, s>>>(p.part, (XT*)p.out, count, pl.splits);
+  }
+  return check_launch("w4_group_matmul");
+}
+
+}  // namespace jgq
+
+using namespace jgq;
+
+extern "C" size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int group_size, int transpose_b) {
+  if (M <= 0 || N <= 0 || K <= 0 || group_size <= 0) return 0;
+  const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
+  return W4_TICKET_REGION + pl.xsum_bytes + pl.part_bytes;
+}
+
+extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale, int zs_dtype,
+                                   void* out, int64_t M, int64_t N, int64_t K, int group_size, int flags,
+                                   void* ws, size_t ws_bytes, void* stream) {
+  JGQ_REQUIRE((flags & ~(JGQ_W4_TRANSPOSE_B | JGQ_W4_WEIGHTS_SETTLED)) == 0, JGQ_ERR_ARG, "w4_group_matmul: unknown flag bits %d", flags);
+  const int transpose_b = flags & JGQ_W4_TRANSPOSE_B;
+  JGQ_REQUIRE(x_dtype == JGQ_F32 || x_dtype == JGQ_F16 || x_dtype == JGQ_BF16, JGQ_ERR_ARG, "w4_group_matmul: activation dtype must be f32/f16/bf16");
+  JGQ_REQUIRE(zs_dtype == JGQ_F32 || zs_dtype == JGQ_F16, JGQ_ERR_ARG, "w4_group_matmul: zero/scale dtype must be f32/f16");
+  JGQ_REQUIRE(M >= 0 && N > 0 && K > 0, JGQ_ERR_ARG, "w4_group_matmul: bad shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  JGQ_REQUIRE(K % 2 == 0, JGQ_ERR_ARG, "w4_group_matmul: K=%lld must be even (two codes per byte)", (long long)K);
+  JGQ_REQUIRE(group_size > 0 && group_size % WG_KC == 0, JGQ_ERR_ARG, "w4_group_matmul: group_size %d is not a positive multiple of %d", group_size, WG_KC);
+  // tokens: the grid's second dimension in tiles of 64
+  JGQ_REQUIRE(M <= 65535ll * WG_TOK && N <= 2147483647LL / 4 && K <= 2147483647LL / 4, JGQ_ERR_LIMIT, "w4_group_matmul: shape too large");
+  if (M == 0) return JGQ_OK;
+  JGQ_REQUIRE(x && packed && zero && scale && out, JGQ_ERR_ARG, "w4_group_matmul: null pointer");
+  const size_t zb = dtype_size(zs_dtype), xb = dtype_size(x_dtype);
+  JGQ_REQUIRE(aligned(x, xb) && aligned(out, xb) && aligned(zero, zb) && aligned(scale, zb), JGQ_ERR_ALIGN, "w4_group_matmul: a pointer is not aligned to its element");
+  const size_t need = jgq_w4_group_matmul_workspace_bytes(M, N, K, group_size, transpose_b);
+  JGQ_REQUIRE(ws && ws_bytes >= need, JGQ_ERR_WORKSPACE, "w4_group_matmul: workspace %zu < %zu bytes", ws_bytes, need);
+  JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_group_matmul: workspace must be 256-byte aligned");
+  cudaStream_t s = (cudaStream_t)stream;
+  const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
+  GroupParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.packed = packed; p.zero = zero; p.scale = scale; p.out = out;
+  p.M = M; p.N = N; p.K = K;
+  p.rows = transpose_b ? K : N; p.depth = transpose_b ? N : K;
+  p.group = group_size; p.groups = (int)cdiv(K, group_size);
+  p.chunks_per_split = pl.chunks_per_split; p.splits = pl.splits;
+  p.vec_w = N % 4 == 0 && aligned(packed, 4);
+  p.vec_x = p.depth * xb % 16 == 0 && aligned(x, 16);
+  uint8_t* w = (uint8_t*)ws + W4_TICKET_REGION;
+  const bool zf = zs_dtype == JGQ_F32;
+#define JGQ_GROUP(XT)                                                                                                      \
+  return transpose_b ? (zf ? launch_group<XT, float, true>(pl, p, w, s) : launch_group<XT, __half, true>(pl, p, w, s))       \
+                     : (zf ? launch_group<XT, float, false>(pl, p, w, s) : launch_group<XT, __half, false>(pl, p, w, s))
+  if (x_dtype == JGQ_F32) { JGQ_GROUP(float); }
+  if (x_dtype == JGQ_F16) { JGQ_GROUP(__half); }
+  JGQ_GROUP(__nv_bfloat16);
+#undef JGQ_GROUP
+}

@@ -10,6 +10,7 @@ libjgq.so; there is no PyTorch or CPU implementation behind these functions.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -76,6 +77,26 @@ def _workspace(nbytes, zeroed=False, tag='ws'):
         size = max(int(nbytes), 1 << 20)
         buf = (torch.zeros if zeroed else torch.empty)(size, dtype=torch.uint8, device=_dev())
         _ws_cache[key] = buf
+    return buf
+
+
+_capture_ws = {}
+
+
+def _scratch(nbytes, tag):
+    """A zeroed workspace of the current device and stream for kernels that leave their tickets zero.  While the stream is
+    being captured the buffer belongs to that capture (allocated and cleared inside it, once), so that no two graphs, and no
+    graph and an eager call, ever share one."""
+    dev = torch.cuda.current_device()
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    capture = lib.jgq_capture_id(stream) if torch.cuda.is_current_stream_capturing() else 0
+    if not capture:
+        return _workspace(nbytes, zeroed=True, tag=tag)
+    key = (dev, stream, tag)
+    owner, buf = _capture_ws.get(key, (0, None))
+    if owner != capture or buf.numel() < nbytes:
+        buf = torch.zeros(int(nbytes), dtype=torch.uint8, device=torch.device('cuda', dev))
+        _capture_ws[key] = (capture, buf)
     return buf
 
 
@@ -154,14 +175,19 @@ class QuantizedMatrix:
 
     ``bits`` is 4 for the reference's format (two codes per byte, gptq.py:237-249).  ``bits=3`` marks the
     3-bit storage format of this library (eight codes in three bytes along the contraction axis), which the
-    reference does not have; `pack_matrix(..., bits=3)` produces it."""
+    reference does not have; `pack_matrix(..., bits=3)` produces it.
 
-    def __init__(self, int_weight, zero, scale, contraction_axis=0, bits=4):
+    ``group_size`` (not in the reference either) marks a 2-D matrix, packed along axis 0, whose scale and zero are
+    (groups, N): rows [i * group_size, (i + 1) * group_size) share row i of them, the last group may be shorter.  It
+    is a positive multiple of 32."""
+
+    def __init__(self, int_weight, zero, scale, contraction_axis=0, bits=4, group_size=None):
         self.int_weight = int_weight
         self.zero = zero
         self.scale = scale
         self.contraction_axis = contraction_axis
         self.bits = bits
+        self.group_size = None if group_size is None else _check_group_size(group_size)
 
     @property
     def shape(self):
@@ -173,11 +199,26 @@ class QuantizedMatrix:
 
     def tree_flatten(self):
         """Children / aux data in the reference's pytree order (gptq.py:24-32)."""
-        return (self.int_weight, self.zero, self.scale), self.contraction_axis
+        aux = self.contraction_axis if self.group_size is None else (self.contraction_axis, self.group_size)
+        return (self.int_weight, self.zero, self.scale), aux
 
     @classmethod
     def tree_unflatten(cls, contraction_axis, children):
-        return cls(*children, contraction_axis=contraction_axis)
+        contraction_axis, group_size = contraction_axis if isinstance(contraction_axis, tuple) else (contraction_axis, None)
+        return cls(*children, contraction_axis=contraction_axis, group_size=group_size)
+
+
+def _check_group_size(group_size):
+    g = int(group_size)
+    if g <= 0 or g % 32 != 0:
+        raise ValueError(f'group_size must be a positive multiple of 32, not {group_size}')
+    return g
+
+
+def _group_parts(K, group_size):
+    """The groups of K rows as (first row, first group, groups, rows per group): the full ones, then a shorter last one."""
+    full, rest = divmod(K, group_size)
+    return ([(0, 0, full, group_size)] if full else []) + ([(full * group_size, full, 1, rest)] if rest else [])
 
 
 def quant_matrix_shape(quantized_matrix, bits=4):
@@ -351,8 +392,15 @@ def accumulate_H(xs, use_fp64=False):
 # --------------------------------------------------------------------------
 # quantization parameters                             reference gptq.py:105-118
 # --------------------------------------------------------------------------
-def _col_params(Wf, bits=4):
+def _col_params(Wf, bits=4, group_size=None):
     K, N = Wf.shape
+    if group_size is not None:
+        group_size = _check_group_size(group_size)
+        groups, maxq = -(-K // group_size), 2 ** bits - 1
+        scale = torch.empty((groups, N), dtype=torch.float32, device=Wf.device)
+        zero = torch.empty((groups, N), dtype=torch.float32, device=Wf.device)
+        check(lib.jgq_group_params(Wf.data_ptr(), K, N, group_size, maxq, scale.data_ptr(), zero.data_ptr(), _stream()))
+        return {'scale': scale, 'zero': zero, 'maxq': maxq, 'group_size': group_size}
     scale = torch.empty(N, dtype=torch.float32, device=Wf.device)
     zero = torch.empty(N, dtype=torch.float32, device=Wf.device)
     maxq = 2 ** bits - 1
@@ -360,14 +408,15 @@ def _col_params(Wf, bits=4):
     return {'scale': scale, 'zero': zero, 'maxq': maxq}
 
 
-def get_col_quantize_params(W, bits=4):
-    """Per-output-channel scale / zero of a (K, N) matrix (gptq.py:118)."""
+def get_col_quantize_params(W, bits=4, group_size=None):
+    """Per-output-channel scale / zero of a (K, N) matrix (gptq.py:118).  ``group_size`` (not in the reference): per group
+    of that many rows and channel, (groups, N), and the result says so under 'group_size'."""
     as_np = _is_np(W)
     Wf = _to_dev(W, torch.float32).contiguous()
     if Wf.dim() != 2:
         raise ValueError('get_col_quantize_params expects a 2-D matrix')
-    p = _col_params(Wf, bits)
-    return {'scale': _out(p['scale'], as_np), 'zero': _out(p['zero'], as_np), 'maxq': p['maxq']}
+    p = _col_params(Wf, bits, group_size)
+    return {**p, 'scale': _out(p['scale'], as_np), 'zero': _out(p['zero'], as_np)}
 
 
 # --------------------------------------------------------------------------
@@ -401,8 +450,16 @@ def _quantize(Wf, L, params, block_size, out_dtype, want_codes=False):
     K, N = Wf.shape
     Q = _tmp('Q', (K, N), out_dtype)
     codes = _tmp('codes', (K, N), torch.uint8) if want_codes else None
+    group_size = params.get('group_size')
+    if group_size is not None:
+        block_size = math.gcd(block_size, group_size)        # a block of the loop lies in one group
     need = lib.jgq_gptq_quantize_workspace_bytes(K, N, block_size)
     ws = _workspace_for(need)
+    if group_size is not None:
+        check(lib.jgq_gptq_quantize_groups(Wf.data_ptr(), L.data_ptr(), params['scale'].data_ptr(), params['zero'].data_ptr(), K, N,
+                                           group_size, block_size, params['maxq'], Q.data_ptr(), _DT[out_dtype], _ptr(codes),
+                                           ws.data_ptr(), need, _stream()))
+        return Q, codes
     check(lib.jgq_gptq_quantize(Wf.data_ptr(), L.data_ptr(), params['scale'].data_ptr(),
                                 params['zero'].data_ptr(), K, N, block_size, params['maxq'],
                                 Q.data_ptr(), _DT[out_dtype], _ptr(codes), ws.data_ptr(), need, _stream()))
@@ -419,7 +476,7 @@ def _raise_status(st):
 
 
 def gptq(W, xs, block_size=128, actorder=False, damping=0.01, use_fp64=False, *,
-         bits=4, H=None, return_codes=False, return_packed=False, _defer=None, _hess=None):
+         bits=4, group_size=None, H=None, return_codes=False, return_packed=False, _defer=None, _hess=None):
     """Quantize W (K x N) with calibration batches xs.  Returns (Q, params) like the
     reference (gptq.py:182-212): Q holds the dequantised values in W's dtype and
     params = {'scale', 'zero', 'maxq'}.
@@ -428,7 +485,9 @@ def gptq(W, xs, block_size=128, actorder=False, damping=0.01, use_fp64=False, *,
     reference does under ``enable_x64`` (gptq.py:186-197); the loop itself stays fp32.
 
     Keyword-only extras (not in the reference): ``bits`` (3-bit uses maxq=7 with
-    the same nibble container), ``H`` (a finalized Hessian to reuse, e.g. for
+    the same nibble container), ``group_size`` (a scale and a zero point per that many rows and channel instead of per
+    channel, taken from W before the loop as the reference's are; params then hold (groups, N) arrays and 'group_size'; not
+    together with ``actorder``, which would spread a group's rows), ``H`` (a finalized Hessian to reuse, e.g. for
     linears fed by the same activation), ``return_packed`` (also return the QuantizedMatrix, packed
     straight from the integer codes the loop produced instead of recovering them from Q by
     round(Q / scale + zero) as quantize_interpreter.py:285 / gptq.py:221 do - the same bytes, one pass
@@ -439,13 +498,17 @@ def gptq(W, xs, block_size=128, actorder=False, damping=0.01, use_fp64=False, *,
     Wd = _to_dev(W)
     if Wd.dim() != 2:
         raise ValueError('gptq expects a 2-D weight (K, N)')
+    if group_size is not None:
+        group_size = _check_group_size(group_size)
+        if actorder:
+            raise ValueError('group_size does not go with actorder: the groups are consecutive rows')
     orig_dtype = Wd.dtype if Wd.dtype in _DT else torch.float32
     Wf = _tmp('Wf', tuple(Wd.shape), torch.float32)           # gptq.py:184 (private copy, updated in place)
     Wf.copy_(Wd)
     K, N = Wf.shape
     if K % block_size != 0:
         raise ValueError(f'K={K} must be a multiple of block_size={block_size}')
-    params = _col_params(Wf, bits)                           # gptq.py:185 (before any fix-up)
+    params = _col_params(Wf, bits, group_size)               # gptq.py:185 (before any fix-up)
     h_status = _tmp('h_status', (1,), torch.int32, zero=True) if _hess is None else None
     hdtype = torch.float64 if use_fp64 else torch.float32
     if _hess is not None:
@@ -483,8 +546,8 @@ def gptq(W, xs, block_size=128, actorder=False, damping=0.01, use_fp64=False, *,
         # Inside a job pipeline every buffer the two sequential stages touch sits at a fixed address per
         # compute stream, so that the library can replay their launch sequences (recorded once per shape
         # and stream) instead of enqueueing them kernel by kernel.
-        loop_params = {'scale': _tmp('scale', (N,), torch.float32), 'zero': _tmp('zero', (N,), torch.float32),
-                       'maxq': params['maxq']}
+        shape = tuple(params['scale'].shape)
+        loop_params = {**params, 'scale': _tmp('scale', shape, torch.float32), 'zero': _tmp('zero', shape, torch.float32)}
         loop_params['scale'].copy_(params['scale'])
         loop_params['zero'].copy_(params['zero'])
     Q, codes = _quantize(Wf, L, loop_params, block_size, orig_dtype, return_codes or return_packed)
@@ -506,12 +569,11 @@ def gptq(W, xs, block_size=128, actorder=False, damping=0.01, use_fp64=False, *,
     else:
         st_host = torch.stack((status.reshape(()), h_status.reshape(()))).tolist()     # gptq.py:194-196 (one host sync per call)
         _raise_status(int(st_host[0]) | (int(st_host[1]) << 8))
-    out_params = {'scale': _out(params['scale'], as_np), 'zero': _out(params['zero'], as_np),
-                  'maxq': params['maxq']}
+    out_params = {**params, 'scale': _out(params['scale'], as_np), 'zero': _out(params['zero'], as_np)}
     extras = ()
     if return_packed:
         packed = pack_along_axis(0, codes)       # the nibble container, whatever `bits` (like pack_matrix's default)
-        extras += (QuantizedMatrix(_out(packed, as_np), out_params['zero'], out_params['scale'], 0),)
+        extras += (QuantizedMatrix(_out(packed, as_np), out_params['zero'], out_params['scale'], 0, group_size=group_size),)
     if return_codes:
         extras += (_out(codes, as_np),)
     return (_out(Q, as_np), out_params) + extras
@@ -588,7 +650,8 @@ def unpack_colwise(w):
 
 def pack_matrix(Q, params, contraction_axis=0, bits=4):
     """codes = round(Q / scale + zero) packed along `contraction_axis` (gptq.py:214-228).  ``bits=3`` stores a
-    3-bit result (maxq = 7) in the 3-bit format instead of one nibble per code."""
+    3-bit result (maxq = 7) in the 3-bit format instead of one nibble per code.  Params with a 'group_size' (from
+    `get_col_quantize_params` or `gptq`) give a matrix with that group size (2-D, axis 0)."""
     as_np = _is_np(Q)
     Qd = _to_dev(Q)
     if Qd.dtype not in _DT:
@@ -599,13 +662,22 @@ def pack_matrix(Q, params, contraction_axis=0, bits=4):
     scale = _to_dev(params['scale'], torch.float32).contiguous()
     zero = _to_dev(params['zero'], torch.float32).contiguous()
     outer, alen, inner = _view3(Qd.shape, contraction_axis)
-    if scale.numel() != outer * inner or zero.numel() != outer * inner:
+    group_size = params.get('group_size')
+    if group_size is not None:
+        group_size = _check_group_size(group_size)
+        _check_groups(Qd.dim(), contraction_axis, alen, inner, group_size, scale, zero)
+    elif scale.numel() != outer * inner or zero.numel() != outer * inner:
         raise ValueError('scale/zero must have the shape of Q without the contraction axis')
     shape = list(Qd.shape)
     shape[contraction_axis] = alen // 2
     packed = torch.empty(shape, dtype=torch.uint8, device=Qd.device)
-    check(lib.jgq_pack_matrix(Qd.data_ptr(), _DT[Qd.dtype], scale.data_ptr(), zero.data_ptr(),
-                              packed.data_ptr(), outer, alen, inner, _stream()))
+    if group_size is not None:
+        for r0, i, outer, rows in _group_parts(alen, group_size):
+            check(lib.jgq_pack_matrix(Qd[r0:].data_ptr(), _DT[Qd.dtype], scale[i:].data_ptr(), zero[i:].data_ptr(),
+                                      packed[r0 // 2:].data_ptr(), outer, rows, inner, _stream()))
+    else:
+        check(lib.jgq_pack_matrix(Qd.data_ptr(), _DT[Qd.dtype], scale.data_ptr(), zero.data_ptr(),
+                                  packed.data_ptr(), outer, alen, inner, _stream()))
     if bits == 3:
         # the fused kernel rounds to codes and packs nibbles; the 3-bit format is made from those codes
         codes = unpack_along_axis(contraction_axis, packed)
@@ -613,7 +685,15 @@ def pack_matrix(Q, params, contraction_axis=0, bits=4):
             raise ValueError('pack_matrix(bits=3): codes above 7; the matrix was not quantized to 3 bits')
         packed = pack_along_axis(contraction_axis, codes, bits=3)
     return QuantizedMatrix(int_weight=_out(packed, as_np), zero=_out(zero, as_np), scale=_out(scale, as_np),
-                           contraction_axis=contraction_axis, bits=bits)
+                           contraction_axis=contraction_axis, bits=bits, group_size=group_size)
+
+
+def _check_groups(dims, contraction_axis, K, N, group_size, scale, zero):
+    if dims != 2 or contraction_axis != 0:
+        raise ValueError('group_size is for 2-D matrices packed along axis 0')
+    want = (-(-K // group_size), N)
+    if tuple(scale.shape) != want or tuple(zero.shape) != want:
+        raise ValueError(f'scale/zero of groups of {group_size} must have shape {want}, not {tuple(scale.shape)} and {tuple(zero.shape)}')
 
 
 def unpack_matrix(weight, dtype=None):
@@ -627,6 +707,18 @@ def unpack_matrix(weight, dtype=None):
     outer, plen, inner = _view3(packed.shape, axis)
     shape = list(packed.shape)
     out_dtype = dtype or torch.float32
+    group_size = getattr(weight, 'group_size', None)
+    if group_size is not None:
+        three = getattr(weight, 'bits', 4) == 3
+        K = plen * 8 // 3 if three else plen * 2
+        _check_groups(packed.dim(), axis, K, inner, group_size, scale, zero)
+        fn = lib.jgq_unpack_matrix3 if three else lib.jgq_unpack_matrix
+        out = torch.empty((K, inner), dtype=out_dtype, device=packed.device)
+        for r0, i, outer, rows in _group_parts(K, group_size):
+            b0, blen = (r0 * 3 // 8, rows * 3 // 8) if three else (r0 // 2, rows // 2)
+            check(fn(packed[b0:].data_ptr(), zero[i:].data_ptr(), scale[i:].data_ptr(), out[r0:].data_ptr(), _DT[out_dtype],
+                     outer, blen, inner, _stream()))
+        return _out(out, as_np)
     if getattr(weight, 'bits', 4) == 3:
         shape[axis] = plen * 8 // 3
         out = torch.empty(shape, dtype=out_dtype, device=packed.device)
@@ -652,7 +744,7 @@ def to_int4_layout(weight):
     shape[axis] = plen * 4 // 3
     out = torch.empty(shape, dtype=torch.uint8, device=packed.device)
     check(lib.jgq_repack_int3_to_int4(packed.data_ptr(), out.data_ptr(), outer, plen, inner, _stream()))
-    return QuantizedMatrix(out, weight.zero, weight.scale, axis, bits=4)
+    return QuantizedMatrix(out, weight.zero, weight.scale, axis, bits=4, group_size=getattr(weight, 'group_size', None))
 
 
 # --------------------------------------------------------------------------
@@ -663,7 +755,7 @@ _trace = None            # measurement: a list that receives (job, 'hessian' | '
 
 
 def gptq_many(jobs, block_size=128, actorder=False, damping=0.01, bits=4, pack=True, out_host=None, streams=8,
-              hessian_stream=True):
+              hessian_stream=True, group_size=None):
     """Run ``gptq`` (and ``pack_matrix`` when `pack`) over a sequence of independent ``(W, xs)`` jobs.
 
     This is the loop the reference's interpreter runs layer by layer
@@ -685,7 +777,7 @@ def gptq_many(jobs, block_size=128, actorder=False, damping=0.01, bits=4, pack=T
     * the NaN / not-positive-definite status words are read once, after all jobs were issued.
 
     `out_host`, if given, is a list of ``(packed, scale, zero)`` pinned host tensors that receive
-    each packed result (device->host, asynchronously).  Returns the list of results
+    each packed result (device->host, asynchronously).  ``group_size`` as in `gptq`.  Returns the list of results
     (QuantizedMatrix when `pack`, else ``(Q, params)``), valid after the function returns.
     """
     global _ARENA
@@ -876,7 +968,7 @@ def gptq_many(jobs, block_size=128, actorder=False, damping=0.01, bits=4, pack=T
                 _ARENA = arenas[wi]
                 try:
                     got = gptq(Wd, xd, block_size=block_size, actorder=actorder, damping=damping, bits=bits,
-                               return_packed=pack, _defer=deferred, _hess=hess)
+                               group_size=group_size, return_packed=pack, _defer=deferred, _hess=hess)
                     Q, params = got[0], got[1]
                 finally:
                     _ARENA = None

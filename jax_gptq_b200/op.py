@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _to_dev, _out, _is_np, _workspace, _DT
+from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _check_groups, _DT
 
 _functorch_active = torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._get_tracing_state
@@ -69,6 +69,46 @@ def _launch(x, w, zero, scale, transpose_b):
     return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
 
 
+def _launch_groups(x, w, zero, scale, group_size, transpose_b):
+    """The product with a scale and a zero point per group of `group_size` rows of the weights."""
+    shape = x.shape
+    if len(shape) > 2:
+        x = x.reshape(-1, shape[-1])
+    if not x.is_contiguous():
+        x = x.contiguous()
+    M, K = x.shape
+    Kw, Nw = w.shape
+    Kw *= 2
+    K2, out_n = (Nw, Kw) if transpose_b else (Kw, Nw)
+    assert K == K2, f'Inner dim mismatch: {K} != {K2}'
+    with torch.cuda.device(x.device):
+        out = x.new_empty((M, out_n))
+        if M == 0:
+            return out.reshape(shape[:-1] + (out_n,))
+        need = lib.jgq_w4_group_matmul_workspace_bytes(M, Nw, Kw, group_size, int(transpose_b))
+        ws = _scratch(need, 'w4g')
+        flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
+        check(lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
+                                      out.data_ptr(), M, Nw, Kw, group_size, flags, ws.data_ptr(), need, _raw_stream(x.device.index)))
+    return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
+
+
+class _GroupMatmul(torch.autograd.Function):
+    """forward: x @ W ; backward w.r.t. x: y_bar @ W^T, for weights with groups."""
+
+    @staticmethod
+    def forward(ctx, x, w, zero, scale, group_size, transpose_b):
+        ctx.save_for_backward(w, zero, scale)
+        ctx.group_size, ctx.transpose_b = group_size, transpose_b
+        return _launch_groups(x, w, zero, scale, group_size, transpose_b)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, y_bar):
+        w, zero, scale = ctx.saved_tensors
+        return _launch_groups(y_bar, w, zero, scale, ctx.group_size, not ctx.transpose_b), None, None, None, None, None
+
+
 class _QuantizedMatmul(torch.autograd.Function):
     """forward: x @ W ; backward w.r.t. x: y_bar @ W^T via the transposed kernel (op.py:71-81)."""
 
@@ -101,7 +141,8 @@ def _needs_function(x, zero, scale):
 
 
 def quantized_matmul(x, quantized_matrix, transpose_b=False):
-    """x @ dequant(quantized_matrix) (or its transpose); result in x's dtype."""
+    """x @ dequant(quantized_matrix) (or its transpose); result in x's dtype.  A matrix with a ``group_size`` has a scale and
+    a zero point per group of rows and channel, one without per channel."""
     as_np = _is_np(x)
     xd = x if type(x) is torch.Tensor and x.is_cuda else _to_dev(x)
     if xd.dtype not in _DT:
@@ -123,6 +164,16 @@ def quantized_matmul(x, quantized_matrix, transpose_b=False):
         if zero.dtype not in _ZS or zero.dtype != scale.dtype:
             zero, scale = zero.to(torch.float32), scale.to(torch.float32)
     zero, scale = _on_device(zero), _on_device(scale)
+    group_size = getattr(quantized_matrix, 'group_size', None)
+    if group_size is not None:
+        _check_groups(w.dim(), 0, 2 * w.shape[0], w.shape[1], group_size, scale, zero)
+        if not (xd.device == w.device == zero.device == scale.device):
+            raise ValueError(f'x is on {xd.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
+        if _needs_function(xd, zero, scale):
+            out = _GroupMatmul.apply(xd, w, zero, scale, group_size, bool(transpose_b))
+        else:
+            out = _launch_groups(xd, w, zero, scale, group_size, bool(transpose_b))
+        return _out(out, as_np)
     if _needs_function(xd, zero, scale):
         out = _QuantizedMatmul.apply(xd, w, zero, scale, bool(transpose_b))
     else:
