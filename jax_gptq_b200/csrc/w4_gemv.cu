@@ -36,6 +36,12 @@
 // Measured (GPU time per call, back to back): bf16 8 x 4096 x 11008 20.1 -> 18.0 us against the streaming kernel; f16 32 x 768 x
 // 2304 28.5 -> 12.3 us against two passes of it.
 //
+// Scales per group of the contraction (FU > 0): a warp keeps the sums of the current group apart and, where the group ends,
+// adds scale * (sum - zero * sum_k x) to totals, in fp32.  The scales and zero points of the next group are requested
+// when the current one begins.  FU is the number of 32-index units between two looks for a group's end: 4 where groups
+// are multiples of 128, else 1.  A slice then holds the totals alone.  fp32 activations take three planes here (all 24
+// bits), and codes other than f16's enter as code - 8, which halves what the zero point takes off again.
+//
 // Launch overlap: the kernel is launched with programmatic stream serialization.  It sets up its
 // barriers and, when the caller declared the weights settled (JGQ_W4_WEIGHTS_SETTLED), issues its
 // first boxes before `griddepcontrol.wait`, i.e. while the previous kernel on the stream is still
@@ -68,6 +74,8 @@ struct GemvParams {
   int G;                       // CTAs
   int maxc;                    // slice slots per group
   int early;                   // 1: weights may be fetched before the stream's previous kernel has finished
+  int group;                   // contraction indices per group
+  int zs_f16;                  // scale and zero point are f16 (with groups; without, a template parameter says so)
 };
 
 __device__ __forceinline__ int gemv_cta_of(int64_t idx, int64_t S, int G) {
@@ -112,6 +120,7 @@ template <> struct GemvType<__half> {
   static constexpr float UP = 16777216.f;                              // 2^24: the codes enter as code * 2^-24
   static constexpr uint32_t ONES = 0x3C003C00u;
   // four operand registers (low / high nibbles of two channels) of the two byte rows' permuted bytes
+  template <bool CENTRED>
   __device__ static __forceinline__ void expand(uint32_t p0, uint32_t p1, uint32_t (&a)[4]) {
     a[0] = p0 & 0x000F000Fu; a[1] = p1 & 0x000F000Fu; a[2] = p0 & 0x00F000F0u; a[3] = p1 & 0x00F000F0u;
   }
@@ -124,13 +133,15 @@ template <> struct GemvType<__nv_bfloat16> {
   static constexpr int ACCS = 1;
   static constexpr float UP = 1.f;
   static constexpr uint32_t ONES = 0x3F803F80u;
+  template <bool CENTRED>
   __device__ static __forceinline__ uint32_t code(uint32_t v) {
     uint32_t r = (v & 0x000F000Fu) | 0x43004300u;
-    const __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), __float2bfloat162_rn(128.f));
+    const __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), __float2bfloat162_rn(CENTRED ? 136.f : 128.f));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  template <bool CENTRED>
   __device__ static __forceinline__ void expand(uint32_t p0, uint32_t p1, uint32_t (&a)[4]) {
-    a[0] = code(p0); a[1] = code(p1); a[2] = code(p0 >> 4); a[3] = code(p1 >> 4);
+    a[0] = code<CENTRED>(p0); a[1] = code<CENTRED>(p1); a[2] = code<CENTRED>(p0 >> 4); a[3] = code<CENTRED>(p1 >> 4);
   }
   __device__ static __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     mma_bf16(d, a0, a1, a2, a3, b0, b1);
@@ -143,12 +154,16 @@ __host__ __device__ constexpr int gemv_ctas(int nt, int planes) { return nt * pl
 
 // NT: token rows staged per warp (1, 2, 4, 8, 16 or 32 >= M); the MMA's n dimension holds eight of them, more
 // rows are further such groups fed from the same expanded weights.  ROWS: byte rows per stage (64 or 128).
-template <typename XT, int NT, typename ZST>
-__global__ void __launch_bounds__(GV_THREADS, gemv_ctas(NT, GemvType<XT>::PLANES))
+// FU: see above; 0: one scale per channel.
+template <typename XT, int FU> __host__ __device__ constexpr int gemv_planes() { return std::is_same<XT, float>::value ? (FU ? 3 : 2) : 1; }
+template <typename XT, int NT, typename ZST, int FU>
+__global__ void __launch_bounds__(GV_THREADS, gemv_ctas(NT, gemv_planes<XT, FU>()))
 w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
   using namespace umma;
   using T = GemvType<XT>;
-  constexpr int PL = T::PLANES;
+  constexpr int PL = gemv_planes<XT, FU>();
+  constexpr bool GROUPED = FU > 0;
+  constexpr bool CENTRED = GROUPED && !std::is_same<XT, __half>::value;
   constexpr int ROWS = gemv_rows(NT, PL);
   constexpr int STAGE_BYTES = ROWS * WCOLS;
   constexpr int STEPS = ROWS / 8;                  // 8 byte rows (16 contraction indices) per MMA step
@@ -218,6 +233,56 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
       }
   };
   clear_acc();
+  // with groups: totals of this lane's channels and tokens, scale and zero point of the current group and of the next
+  float tot[GROUPED ? NG : 1][2][4];
+  uint4 zs_now[2], zs_next[2];
+  auto clear_tot = [&]() {
+#pragma unroll
+    for (int q = 0; q < (GROUPED ? NG : 1); ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { tot[q][0][i] = 0.f; tot[q][1][i] = 0.f; }
+  };
+  clear_tot();
+  // (ordinary loads, as for the activations below) the four channels of a lane: 16 bytes of fp32 or 8 of f16, behind the matrix nothing
+  auto fetch_zs = [&](uint4 (&zs)[2], int cgr, int64_t k) {
+    const int n0 = cgr * WCOLS + 32 * warp + 4 * g;
+    zs[0] = zs[1] = make_uint4(0, 0, 0, 0);
+    if (n0 < p.N && k < p.K) {
+      const int64_t at = (k / p.group) * p.N + n0;
+      if (p.zs_f16) {
+        const uint2 a = *reinterpret_cast<const uint2*>((const __half*)p.scale + at), b = *reinterpret_cast<const uint2*>((const __half*)p.zero + at);
+        zs[0].x = a.x; zs[0].y = a.y; zs[1].x = b.x; zs[1].y = b.y;
+      } else {
+        zs[0] = *reinterpret_cast<const uint4*>((const float*)p.scale + at);
+        zs[1] = *reinterpret_cast<const uint4*>((const float*)p.zero + at);
+      }
+    }
+  };
+  auto zs_values = [&](const uint4& v, float (&f)[4]) {
+    if (p.zs_f16) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    } else {
+      f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+    }
+  };
+  // the sums since the last call, which belong to one group, into the totals
+  auto finish_group = [&]() {
+    float sc[4], z[4];
+    zs_values(zs_now[0], sc);
+    zs_values(zs_now[1], z);
+#pragma unroll
+    for (int q = 0; q < (GROUPED ? NG : 1); ++q)
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                  // channel 2 tile + i / 2 of the four, token 2 t + i % 2
+          const int c = 2 * tile + (i >> 1);
+          const float v = ACCS == 2 ? fmaf(acc[q][tile][ACCS - 1][i], 0.0625f, acc[q][tile][0][i]) : acc[q][tile][0][i];
+          tot[q][tile][i] = fmaf(sc[c], fmaf(-(CENTRED ? z[c] - 8.f : z[c]), accx[q][i & 1], v * T::UP), tot[q][tile][i]);
+        }
+    clear_acc();
+  };
 
   const uint32_t ring_u32 = smem_u32(ring);
   const uint32_t xs_warp = smem_u32(xs_all) + warp * XWARP;
@@ -236,6 +301,13 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
   constexpr uint32_t ones = T::ONES;
 
   int gid = g_begin, st = st_begin;
+  int64_t group_end = 0;               // contraction index behind the current group
+  if (GROUPED) {
+    const int64_t k = (int64_t)st * (2 * ROWS);
+    group_end = (k / p.group + 1) * p.group;
+    fetch_zs(zs_now, gid, k);
+    fetch_zs(zs_next, gid, group_end);
+  }
   bool alive = true;
   for (int s = 0; s < nstage; ++s) {
     const int cg = gid;
@@ -268,16 +340,22 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
         const uint32_t dst = xs_warp + r * XROW + (lane + 32 * h) * 8;
         if constexpr (kF32) {
           const float f[4] = {xv[r][h].x, xv[r][h].z, xv[r][h].y, xv[r][h].w};
-          uint32_t hi[2], lo[2];
+          uint32_t hi[2], lo[2], least[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const __nv_bfloat16 h0 = __float2bfloat16_rn(f[2 * i]), h1 = __float2bfloat16_rn(f[2 * i + 1]);
-            const __nv_bfloat16 l0 = __float2bfloat16_rn(f[2 * i] - __bfloat162float(h0)), l1 = __float2bfloat16_rn(f[2 * i + 1] - __bfloat162float(h1));
+            const float r0 = f[2 * i] - __bfloat162float(h0), r1 = f[2 * i + 1] - __bfloat162float(h1);
+            const __nv_bfloat16 l0 = __float2bfloat16_rn(r0), l1 = __float2bfloat16_rn(r1);
             hi[i] = (uint32_t)__bfloat16_as_ushort(h0) | ((uint32_t)__bfloat16_as_ushort(h1) << 16);
             lo[i] = (uint32_t)__bfloat16_as_ushort(l0) | ((uint32_t)__bfloat16_as_ushort(l1) << 16);
+            if (PL == 3) {
+              const __nv_bfloat16 m0 = __float2bfloat16_rn(r0 - __bfloat162float(l0)), m1 = __float2bfloat16_rn(r1 - __bfloat162float(l1));
+              least[i] = (uint32_t)__bfloat16_as_ushort(m0) | ((uint32_t)__bfloat16_as_ushort(m1) << 16);
+            }
           }
           sts64(dst, hi[0], hi[1]);
           sts64(dst + NT * XROW, lo[0], lo[1]);
+          if (PL == 3) sts64(dst + 2 * NT * XROW, least[0], least[1]);
         } else {
           const uint32_t ev = __byte_perm(xv[r][h].x, xv[r][h].y, 0x5410);
           const uint32_t od = __byte_perm(xv[r][h].x, xv[r][h].y, 0x7632);
@@ -294,15 +372,14 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     __syncwarp();
     if (alive) {
       const uint32_t tile = ring_u32 + slot * STAGE_BYTES;
-#pragma unroll
-      for (int sl = 0; sl < STEPS; sl += ACCS) {
+      auto steps = [&](int sl) {                     // ACCS steps of 16 contraction indices
         uint32_t a0[ACCS][4], a1[ACCS][4];         // per step: low nibbles, then high nibbles, of the two channel tiles
 #pragma unroll
         for (int h = 0; h < ACCS; ++h) {
           const uint32_t w1 = lds32(tile + (sl + h) * (8 * WCOLS) + off0);
           const uint32_t w2 = lds32(tile + (sl + h) * (8 * WCOLS) + off1);
-          T::expand(__byte_perm(w1, w2, 0x4400), __byte_perm(w1, w2, 0x5511), a0[h]);
-          T::expand(__byte_perm(w1, w2, 0x6622), __byte_perm(w1, w2, 0x7733), a1[h]);
+          T::template expand<CENTRED>(__byte_perm(w1, w2, 0x4400), __byte_perm(w1, w2, 0x5511), a0[h]);
+          T::template expand<CENTRED>(__byte_perm(w1, w2, 0x6622), __byte_perm(w1, w2, 0x7733), a1[h]);
         }
 #pragma unroll
         for (int q = 0; q < NG; ++q)
@@ -324,6 +401,24 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
               T::mma(accx[q], ones, ones, ones, ones, xb.x, xb.y);
             }
           }
+      };
+      if constexpr (!GROUPED) {
+#pragma unroll
+        for (int sl = 0; sl < STEPS; sl += ACCS) steps(sl);
+      } else {
+        int64_t k = (int64_t)st * (2 * ROWS);
+#pragma unroll 1
+        for (int s0 = 0; s0 < STEPS; s0 += 2 * FU) {
+#pragma unroll
+          for (int sl = 0; sl < 2 * FU; sl += ACCS) steps(s0 + sl);
+          k += 32 * FU;
+          if (k == group_end && s0 + 2 * FU <= STEPS) {
+            finish_group();
+            zs_now[0] = zs_next[0]; zs_now[1] = zs_next[1];
+            group_end += p.group;
+            fetch_zs(zs_next, gid, group_end);
+          }
+        }
       }
       __syncwarp();
       if (lane == 0) {
@@ -344,10 +439,11 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     const bool last_of_group = (st_now == p.spc - 1) || (s == nstage - 1);
     if (!last_of_group) continue;
     if (s == nstage - 1) GTRACE(3);
+    if (GROUPED) finish_group();                     // what the last group has here (none: sums of zero)
 
     // ---- flush this warp's 32 channels of group cg ----
     // lane (g, t): tokens 2t and 2t+1; channels n0 .. n0+3 = (tile 0 row g, tile 0 row g+8, tile 1 row g, tile 1 row g+8)
-    const float kUp = T::UP;
+    const float kUp = GROUPED ? 1.f : T::UP;
     const int n0 = cg * WCOLS + 32 * warp + 4 * g;
     const int first_c = gemv_cta_of((int64_t)cg * p.spc, p.S, p.G);
     const int last_c = gemv_cta_of((int64_t)(cg + 1) * p.spc - 1, p.S, p.G);
@@ -360,7 +456,8 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         auto sum = [&](int tile, int i) {
-          if constexpr (ACCS == 2) return fmaf(acc[q][tile][1][i], 0.0625f, acc[q][tile][0][i]) + poison;
+          if constexpr (GROUPED) return tot[q][tile][i] + poison;
+          else if constexpr (ACCS == 2) return fmaf(acc[q][tile][1][i], 0.0625f, acc[q][tile][0][i]) + poison;
           else return acc[q][tile][0][i] + poison;
         };
         v[q][e] = make_float4(sum(0, e), sum(0, 2 + e), sum(1, e), sum(1, 2 + e));
@@ -378,7 +475,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
           const int tok = 8 * q + 2 * t + e;
           if (tok < p.M && tok < NT) {
             *reinterpret_cast<float4*>(mine + tok * 32 + 4 * g) = v[q][e];
-            if (g == 0) mine[NT * 32 + tok] = xsum[q][e];
+            if (!GROUPED && g == 0) mine[NT * 32 + tok] = xsum[q][e];
           }
         }
       __threadfence();
@@ -405,7 +502,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
                 const float* src = base + (int64_t)zc * WWARPS * SL;
                 const float4 a = __ldcg(reinterpret_cast<const float4*>(src + tok * 32 + 4 * g));
                 v[q][e].x += a.x; v[q][e].y += a.y; v[q][e].z += a.z; v[q][e].w += a.w;
-                xsum[q][e] += __ldcg(src + NT * 32 + tok);
+                if (!GROUPED) xsum[q][e] += __ldcg(src + NT * 32 + tok);
               }
             }
           }
@@ -414,15 +511,15 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     if (write_out && n0 < p.N) {               // N % 16 == 0: the four channels are inside together
       float sc[4], z[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { sc[i] = zs_to_f32<ZST>(p.scale, n0 + i); z[i] = zs_to_f32<ZST>(p.zero, n0 + i); }
+      for (int i = 0; i < 4; ++i) { sc[i] = 1.f; z[i] = 0.f; if (!GROUPED) { sc[i] = zs_to_f32<ZST>(p.scale, n0 + i); z[i] = zs_to_f32<ZST>(p.zero, n0 + i); } }
 #pragma unroll
       for (int q = 0; q < NG; ++q)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int tok = 8 * q + 2 * t + e;
           if (tok < p.M && tok < NT) {
-            const float o0 = sc[0] * (kUp * v[q][e].x - z[0] * xsum[q][e]), o1 = sc[1] * (kUp * v[q][e].y - z[1] * xsum[q][e]);
-            const float o2 = sc[2] * (kUp * v[q][e].z - z[2] * xsum[q][e]), o3 = sc[3] * (kUp * v[q][e].w - z[3] * xsum[q][e]);
+            const float o0 = GROUPED ? v[q][e].x : sc[0] * (kUp * v[q][e].x - z[0] * xsum[q][e]), o1 = GROUPED ? v[q][e].y : sc[1] * (kUp * v[q][e].y - z[1] * xsum[q][e]);
+            const float o2 = GROUPED ? v[q][e].z : sc[2] * (kUp * v[q][e].z - z[2] * xsum[q][e]), o3 = GROUPED ? v[q][e].w : sc[3] * (kUp * v[q][e].w - z[3] * xsum[q][e]);
             XT* dst = (XT*)p.out + (int64_t)tok * p.N + n0;
             if constexpr (kF32) {
               *reinterpret_cast<float4*>(dst) = make_float4(o0, o1, o2, o3);
@@ -434,6 +531,14 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
         }
     }
     clear_acc();
+    if (GROUPED) {                                   // the next channel group begins at contraction index 0
+      clear_tot();
+      group_end = p.group;
+      if (s + 1 < nstage) {
+        fetch_zs(zs_now, gid, 0);
+        fetch_zs(zs_next, gid, group_end);
+      }
+    }
   }
 
   GTRACE(4);
@@ -452,11 +557,11 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
 
 // ------------------------------------------------------------------ host ----
 
-GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype) {
+GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped) {
   GemvPlan pl;
   memset(&pl, 0, sizeof(pl));
-  const int planes = x_dtype == JGQ_F32 ? 2 : 1;
-  if (M < 1 || M > (planes == 2 ? 16 : 32) || N % 16 != 0 || K % 8 != 0) return pl;
+  const int planes = x_dtype == JGQ_F32 ? (grouped ? 3 : 2) : 1;
+  if (M < 1 || M > (planes > 1 ? 16 : 32) || N % 16 != 0 || K % 8 != 0) return pl;
   pl.ncg = (int)cdiv(N, WCOLS);
   if (pl.ncg * WWARPS > GV_TICKET_BYTES / (int)sizeof(int)) return pl;
   pl.use = 1;
@@ -476,9 +581,9 @@ GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype) {
   return pl;
 }
 
-template <typename XT, int NT, typename ZST>
+template <typename XT, int NT, typename ZST, int FU>
 static int launch_gemv_inst(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, cudaStream_t s) {
-  auto kern = w4_gemv_kernel<XT, NT, ZST>;
+  auto kern = w4_gemv_kernel<XT, NT, ZST, FU>;
   struct AttrTag {};
   const int arc = once_per_device<AttrTag>([&]() {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem_bytes);
@@ -504,22 +609,22 @@ static int launch_gemv_inst(const GemvPlan& pl, const GemvParams& p, const CUten
   return JGQ_OK;
 }
 
-template <typename XT, typename ZST>
+template <typename XT, typename ZST, int FU>
 static int launch_gemv_type(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, cudaStream_t s) {
   switch (pl.nt) {
-    case 1:  return launch_gemv_inst<XT, 1, ZST>(pl, p, wmap, s);
-    case 2:  return launch_gemv_inst<XT, 2, ZST>(pl, p, wmap, s);
-    case 4:  return launch_gemv_inst<XT, 4, ZST>(pl, p, wmap, s);
-    case 8:  return launch_gemv_inst<XT, 8, ZST>(pl, p, wmap, s);
-    case 16: return launch_gemv_inst<XT, 16, ZST>(pl, p, wmap, s);
+    case 1:  return launch_gemv_inst<XT, 1, ZST, FU>(pl, p, wmap, s);
+    case 2:  return launch_gemv_inst<XT, 2, ZST, FU>(pl, p, wmap, s);
+    case 4:  return launch_gemv_inst<XT, 4, ZST, FU>(pl, p, wmap, s);
+    case 8:  return launch_gemv_inst<XT, 8, ZST, FU>(pl, p, wmap, s);
+    case 16: return launch_gemv_inst<XT, 16, ZST, FU>(pl, p, wmap, s);
     default:
-      if constexpr (GemvType<XT>::PLANES == 1) return launch_gemv_inst<XT, 32, ZST>(pl, p, wmap, s);
+      if constexpr (GemvType<XT>::PLANES == 1) return launch_gemv_inst<XT, 32, ZST, FU>(pl, p, wmap, s);
       return fail(JGQ_ERR_ARG, "w4_gemv: bad plan");
   }
 }
 
 int launch_w4_gemv(const GemvPlan& pl, const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale,
-                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, void* ws, int settled, cudaStream_t s) {
+                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int group, void* ws, int settled, cudaStream_t s) {
   CUtensorMap wmap;
   const int rc = encode_tmap_2d_u8(&wmap, packed, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)N, WCOLS, (uint32_t)pl.rows, 1);
   if (rc) return rc;
@@ -531,11 +636,20 @@ int launch_w4_gemv(const GemvPlan& pl, const void* x, int x_dtype, const uint8_t
   p.M = (int)M; p.N = (int)N; p.K = (int)K;
   p.ncg = pl.ncg; p.spc = pl.spc; p.S = pl.S; p.G = pl.G; p.maxc = pl.maxc;
   p.early = settled ? 1 : 0;
+  if (group > 0) {
+    p.group = group;
+    p.zs_f16 = zs_dtype == JGQ_F16;
+#define JGQ_GEMV(XT) return group % 128 == 0 ? launch_gemv_type<XT, float, 4>(pl, p, wmap, s) : launch_gemv_type<XT, float, 1>(pl, p, wmap, s)
+    if (x_dtype == JGQ_F16) { JGQ_GEMV(__half); }
+    if (x_dtype == JGQ_BF16) { JGQ_GEMV(__nv_bfloat16); }
+    JGQ_GEMV(float);
+#undef JGQ_GEMV
+  }
   const bool zf = zs_dtype == JGQ_F32;
-  if (x_dtype == JGQ_F16) return zf ? launch_gemv_type<__half, float>(pl, p, wmap, s) : launch_gemv_type<__half, __half>(pl, p, wmap, s);
+  if (x_dtype == JGQ_F16) return zf ? launch_gemv_type<__half, float, 0>(pl, p, wmap, s) : launch_gemv_type<__half, __half, 0>(pl, p, wmap, s);
   if (x_dtype == JGQ_BF16)
-    return zf ? launch_gemv_type<__nv_bfloat16, float>(pl, p, wmap, s) : launch_gemv_type<__nv_bfloat16, __half>(pl, p, wmap, s);
-  return zf ? launch_gemv_type<float, float>(pl, p, wmap, s) : launch_gemv_type<float, __half>(pl, p, wmap, s);
+    return zf ? launch_gemv_type<__nv_bfloat16, float, 0>(pl, p, wmap, s) : launch_gemv_type<__nv_bfloat16, __half, 0>(pl, p, wmap, s);
+  return zf ? launch_gemv_type<float, float, 0>(pl, p, wmap, s) : launch_gemv_type<float, __half, 0>(pl, p, wmap, s);
 }
 
 }  // namespace jgq

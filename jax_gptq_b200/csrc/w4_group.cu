@@ -4,7 +4,8 @@
 //   forward      out[m, n] = sum_k x[m, k] w[k, n]
 //   transposed   out[m, k] = sum_n x[m, n] w[k, n]
 //
-// This file holds the dispatcher and the general kernel (any M, N, even K, pointers aligned to their element).
+// This file holds the dispatcher and the general kernel (any M, N, even K, pointers aligned to their element).  The decode
+// kernel (w4_gemv.cu) and the kernel on CTA pairs (w4_pair.cu) take what fits them.
 //
 // General kernel: mma.sync with the weights as the 16-row operand, always as exact codes; what depends on the
 // group is applied to fp32 numbers, so nothing but the sums is rounded:
@@ -13,6 +14,8 @@
 //   transposed   scale varies along the contraction, the group along the rows: a tile's rows lie in one group, the
 //                activations are multiplied with that group's scales while they are staged (products in fp32, split into
 //                bf16 planes), and sum_n x scale zero is summed up beside it.
+// Codes enter as code - 8 (exact): the sums and what the zero point takes off them are half as large.  The tensor core's
+// sums truncate, so they are handed to fp32 totals at the latest every 128 indices (28672 in one chain: relative error 3.7e-5).
 // 16-bit activations enter the forward product as they are; x * scale as two bf16 planes (16 bits of the product, below
 // the result's own rounding); fp32 activations as three (all 24 bits).
 // A long contraction with few tiles is split; the slices are added in order by the kernel behind.
@@ -52,6 +55,18 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// the low nibbles of the two halves, less 8
+template <typename CT> __device__ __forceinline__ uint32_t centred(uint32_t v);
+template <> __device__ __forceinline__ uint32_t centred<__half>(uint32_t v) {
+  uint32_t r = (v & 0x000F000Fu) | 0x64006400u;
+  const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__float2half_rn(1032.f)));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t centred<__nv_bfloat16>(uint32_t v) {
+  uint32_t r = (v & 0x000F000Fu) | 0x43004300u;
+  const __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), __float2bfloat162_rn(136.f));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <typename CT> __device__ __forceinline__ uint32_t pair_bits(float a, float b);
 template <> __device__ __forceinline__ uint32_t pair_bits<__half>(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -140,7 +155,7 @@ w4_group_kernel(const GroupParams p) {
         const bool in = d + i < p.depth;
         const int64_t o = tb_group * p.N + (in ? d + i : 0);
         xreg[i] = in ? __fmul_rn(xreg[i], zs_to_f32<ZST>(p.scale, o)) : 0.f;
-        cz = fmaf(xreg[i], zs_to_f32<ZST>(p.zero, o), cz);
+        cz = fmaf(xreg[i], zs_to_f32<ZST>(p.zero, o) - 8.f, cz);
       }
     }
   };
@@ -154,8 +169,8 @@ w4_group_kernel(const GroupParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t b = __byte_perm(w, 0, h ? 0x4342 : 0x4140);       // two channels' bytes in the halves of a word
-        e[h] = MmaType<CT>::expand(b);
-        o[h] = MmaType<CT>::expand(b >> 4);
+        e[h] = centred<CT>(b);
+        o[h] = centred<CT>(b >> 4);
       }
       const int r = TB ? 2 * (i / 8) : 2 * (i / (BM / 4)), c = TB ? 4 * (i % 8) : 4 * (i % (BM / 4));
       *reinterpret_cast<uint2*>(a + r * ASTRIDE + c) = make_uint2(e[0], e[1]);
@@ -178,31 +193,33 @@ w4_group_kernel(const GroupParams p) {
     }
   };
 
-  float acc[2][NTW][4], total[TB ? 1 : 2][TB ? 1 : NTW][4];
+  float acc[2][NTW][4], total[2][NTW][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < NTW; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { acc[i][j][e] = 0.f; if (!TB) total[i][j][e] = 0.f; }
+      for (int e = 0; e < 4; ++e) { acc[i][j][e] = 0.f; total[i][j][e] = 0.f; }
 
-  // the sums of one group into the totals; a group that two slices share gives its zero point to the one it begins in
-  auto finish_group = [&](int64_t grp) {
+  // The sums since the last call, all of one group (transposed: of any), into the totals.  Where the group ends, or the
+  // slice, the zero point's part: a group that two slices share gives it to the one it begins in.
+  auto hand_over = [&](int64_t grp, bool ends) {
     const bool begins = grp * p.group >= c_begin * WG_KC;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t n = row0 + wm + 16 * i + g + 8 * h;
-        float s = 0.f, z = 0.f;
-        if (n < p.rows) { s = zs_to_f32<ZST>(p.scale, grp * p.N + n); z = zs_to_f32<ZST>(p.zero, grp * p.N + n); }
+        float s = 1.f, z = 0.f;
+        if (!TB && n < p.rows) { s = zs_to_f32<ZST>(p.scale, grp * p.N + n); z = zs_to_f32<ZST>(p.zero, grp * p.N + n) - 8.f; }
 #pragma unroll
         for (int j = 0; j < NTW; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int64_t m = tok0 + wn + 8 * j + 2 * q + e;
-            const float xs = begins && m < p.M ? p.xsum[m * p.groups + grp] : 0.f;
-            if (!TB) total[i][j][2 * h + e] = fmaf(s, acc[i][j][2 * h + e] - z * xs, total[i][j][2 * h + e]);
+            float v = acc[i][j][2 * h + e];
+            if (!TB && ends && begins && m < p.M) v = fmaf(-z, p.xsum[m * p.groups + grp], v);
+            total[i][j][2 * h + e] = TB ? total[i][j][2 * h + e] + v : fmaf(s, v, total[i][j][2 * h + e]);
             acc[i][j][2 * h + e] = 0.f;
           }
       }
@@ -240,7 +257,11 @@ w4_group_kernel(const GroupParams p) {
         }
       }
     }
-    if (!TB && ((c + 1) * WG_KC % p.group == 0 || c + 1 == c_end)) finish_group(c * WG_KC / p.group);
+    {
+      const int64_t k = (c + 1) * WG_KC;
+      const bool ends = c + 1 == c_end || (!TB && k % p.group == 0);
+      if (ends || k % 128 == 0) hand_over(TB ? 0 : c * WG_KC / p.group, ends);
+    }
     if (c + 1 < c_end) stage(buf ^ 1);
     __syncthreads();
   }
@@ -262,7 +283,7 @@ w4_group_kernel(const GroupParams p) {
         for (int h = 0; h < 2; ++h) {
           const int64_t r = row0 + wm + 16 * i + g + 8 * h;
           if (r >= p.rows) continue;
-          const float v = TB ? acc[i][j][2 * h + e] - scz[t] : total[TB ? 0 : i][TB ? 0 : j][2 * h + e];
+          const float v = TB ? total[i][j][2 * h + e] - scz[t] : total[i][j][2 * h + e];
           if (p.splits > 1) p.part[((int64_t)blockIdx.z * p.M + m) * p.rows + r] = v;
           else reinterpret_cast<XT*>(p.out)[m * p.rows + r] = from_f32<XT>(v);
         }
@@ -280,6 +301,17 @@ __global__ void __launch_bounds__(256) w4_group_join_kernel(const float* __restr
 }
 
 // ------------------------------------------------------------------ host ----
+// ---- which kernel ----
+// Up to 32 rows, forward: the decode kernel (fp32 activations in passes of 16 rows).
+constexpr int64_t kGroupDecodeRows = 32, kGroupPassRows = 16;
+static bool group_decodes(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b) {
+  return !transpose_b && M <= kGroupDecodeRows && plan_w4_gemv(x_dtype == JGQ_F32 ? std::min(M, kGroupPassRows) : M, N, K, x_dtype, 1).use;
+}
+// 16-bit activations, more rows or transposed: CTA pairs.
+static PairPlan group_pairs(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b, int group) {
+  return plan_w4_pair(M, N, K, x_dtype, transpose_b, group);
+}
+
 struct GroupPlan { int bm, tiles, mtiles, splits, chunks_per_split; size_t xsum_bytes, part_bytes; };
 
 static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int transpose_b) {
@@ -326,8 +358,19 @@ using namespace jgq;
 
 extern "C" size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int group_size, int transpose_b) {
   if (M <= 0 || N <= 0 || K <= 0 || group_size <= 0) return 0;
+  // over all activation types, and over the kernels that the alignment of the pointers chooses between
   const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
-  return W4_TICKET_REGION + pl.xsum_bytes + pl.part_bytes;
+  size_t bytes = W4_TICKET_REGION + pl.xsum_bytes + pl.part_bytes;
+  for (int dt : {JGQ_F32, JGQ_F16, JGQ_BF16}) {
+    if (group_decodes(M, N, K, dt, transpose_b))
+      for (int64_t rows : {std::min(M, kGroupPassRows), M}) {
+        const GemvPlan gp = plan_w4_gemv(rows, N, K, dt, 1);
+        if (gp.use) bytes = std::max(bytes, gp.ws_bytes);
+      }
+    const PairPlan pp = group_pairs(M, N, K, dt, transpose_b, group_size);
+    if (pp.use) bytes = std::max(bytes, pp.ws_bytes);
+  }
+  return bytes;
 }
 
 extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale, int zs_dtype,
@@ -350,6 +393,20 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   JGQ_REQUIRE(ws && ws_bytes >= need, JGQ_ERR_WORKSPACE, "w4_group_matmul: workspace %zu < %zu bytes", ws_bytes, need);
   JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_group_matmul: workspace must be 256-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
+  if (group_decodes(M, N, K, x_dtype, transpose_b) && aligned(packed, 16) && aligned(x, 16) && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) &&
+      aligned(scale, 4 * zb) && aligned(zero, 4 * zb)) {
+    const int64_t step = x_dtype == JGQ_F32 ? kGroupPassRows : M;
+    for (int64_t r0 = 0; r0 < M; r0 += step) {
+      const int64_t rows = std::min(step, M - r0);
+      const int rc = launch_w4_gemv(plan_w4_gemv(rows, N, K, x_dtype, 1), (const char*)x + (size_t)r0 * K * xb, x_dtype, packed, zero, scale,
+                                    zs_dtype, (char*)out + (size_t)r0 * N * xb, rows, N, K, group_size, ws, (flags & JGQ_W4_WEIGHTS_SETTLED) != 0, s);
+      if (rc) return rc;
+    }
+    return JGQ_OK;
+  }
+  const PairPlan pp = group_pairs(M, N, K, x_dtype, transpose_b, group_size);
+  if (pp.use && aligned(packed, 16) && aligned(x, 16))
+    return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, transpose_b, group_size, ws, s);
   const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
   GroupParams p;
   memset(&p, 0, sizeof(p));

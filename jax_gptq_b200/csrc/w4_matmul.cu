@@ -428,7 +428,7 @@ extern "C" int jgq_w4_matmul(const void* x, int x_dtype, const uint8_t* packed,
     JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_matmul: workspace must be 256-byte aligned");
     const PairPlan pp = w4_pair_choice(M, N, K, x_dtype, 1);
     if (pp.use && pp.ws_bytes <= ws_bytes && aligned(packed, 16))
-      return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, 1, ws, s);
+      return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, 1, 0, ws, s);
     return launch_w4_tb(x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, ws, ws_bytes, s);
   }
   JGQ_REQUIRE(aligned(x, 8), JGQ_ERR_ALIGN, "w4_matmul: x must be 8-byte aligned");
@@ -449,7 +449,7 @@ extern "C" int jgq_w4_matmul(const void* x, int x_dtype, const uint8_t* packed,
       for (int64_t r0 = 0; r0 < M; r0 += step) {
         const int64_t rows = std::min<int64_t>(step, M - r0);
         const int rc = launch_w4_gemv(plan_w4_gemv(rows, N, K, x_dtype), (const char*)x + (size_t)r0 * K * elt, x_dtype, packed, zero,
-                                      scale, zs_dtype, (char*)out + (size_t)r0 * N * elt, rows, N, K, ws, settled, s);
+                                      scale, zs_dtype, (char*)out + (size_t)r0 * N * elt, rows, N, K, 0, ws, settled, s);
         if (rc) return rc;
       }
       return JGQ_OK;
@@ -481,7 +481,7 @@ extern "C" int jgq_w4_matmul(const void* x, int x_dtype, const uint8_t* packed,
   if (!w4_force_mma_sync()) {
     const PairPlan pp = w4_pair_choice(M, N, K, x_dtype, 0);
     if (pp.use && pp.ws_bytes <= ws_bytes && aligned(x, 16) && aligned(packed, 16))
-      return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, 0, ws, s);
+      return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, 0, 0, ws, s);
     const UmmaPlan up = plan_w4_umma(M, N, K, x_dtype);
     if (M > 16 && up.use && aligned(x, 16) && aligned(packed, 16) && aligned(out, 4))
       return launch_w4_umma(up, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, ws, s);

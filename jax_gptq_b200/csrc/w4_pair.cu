@@ -36,6 +36,13 @@
 // (bytes of both CTAs' loads) and acc_empty (arrivals of both CTAs' epilogue warps) live in the even CTA; a_empty, x_empty
 // and acc_full exist in both and are signalled by two commits each.  No load uses multicast.  Waits are bounded: a timed-out product writes NaN.
 //
+// Scales per group of the contraction axis (GR): they cannot leave the contraction, so the weights become 16-bit operands
+// themselves: w = scale (code - zero) in fp32, one multiply-add per code from tables  a = 128 scale f,  b = -(128 + zero) scale f
+// (1 + code / 128 is an fp32 with the code in its mantissa), rounded once to the activations' type, which costs a result
+// what its own rounding does.  The tables come from a small kernel in front and reach the expanding warps by TMA beside the
+// raw bytes.  For f16, f is the power of two that brings the largest weight of an output channel (transposed: of a
+// group) to [2^13, 2^14); the epilogue takes it off again.  One plane of activations in both directions, in their own order.
+//
 // Measured (replayed over rotating weights): forward, 2048 x 4096 x 11008, bf16: 291 us on the single-CTA kernel, 177 with a
 // tile per pair and launch, 152 now, 1.22 PFLOP/s (of 1.67 measured with cuBLAS in a burst; 175 us in a loop of calls that
 // changes its inputs); transposed, 2048 rows on 11008 x 4096: 894 with mma.sync, 275, 244, 1.52 PFLOP/s executed for two
@@ -67,6 +74,8 @@ constexpr int P_OUT_STRIDE = 32 * 4 + 16;            // bytes per token in a war
 constexpr int P_OUT_BYTES = P_EPI_WARPS * 32 * P_OUT_STRIDE;
 constexpr int P_SMEM_BYTES = P_RING_BYTES + P_OUT_BYTES + 512;
 constexpr int P_TMEM_COLS = 512;
+constexpr int P_TAB_BYTES = 2048;                    // with groups, per raw stage: two tables of up to 1 KB
+constexpr int P_SMEM_BYTES_GR = P_SMEM_BYTES + P_RAW_ST * P_TAB_BYTES;
 
 struct PairParams {
   const void* zero; const void* scale; void* out;
@@ -79,6 +88,8 @@ struct PairParams {
   int nt;                      // tokens per block: 256; fewer only if all tokens fit one block
   int x_blk, x_slot, x_st;     // activation ring: bytes per block (a CTA's half) and per slot, slots
   uint32_t emask_lo, emask_hi, emagic;
+  const float* inv;            // with groups: what the epilogue multiplies by, per channel (transposed: per group); null: nothing
+  int group, tab_rows;         // contraction-axis indices per group, groups per stage's table (transposed: per 128 rows)
 };
 
 struct PairItem { int rp, m0, nh; };            // row pair, first token, tiles taken together (1 or 2)
@@ -97,10 +108,37 @@ __device__ __forceinline__ PairItem pair_item(const PairParams& p, int t) {
   return s;
 }
 
-template <typename XT, typename ZST, int FMT, bool TB>
+// nibble i of a word as the fp32 1 + nibble / 128
+template <int I>
+__device__ __forceinline__ float nibble_float(uint32_t w) {
+  constexpr int sh = 16 - 4 * I;
+  const uint32_t v = sh > 0 ? w << (sh > 0 ? sh : 0) : w >> (sh > 0 ? 0 : -sh);
+  return __uint_as_float((v & 0x000F0000u) | 0x3F800000u);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if (FMT == 0) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// a word (four channels, two contraction-axis indices) as weights: e the even index' channels in order, o the odd one's
+template <int FMT>
+__device__ __forceinline__ void expand_word_scaled(uint32_t w, const float (&a)[4], const float (&b)[4], uint32_t& e0, uint32_t& e1, uint32_t& o0,
+                                                   uint32_t& o1) {
+  e0 = pack_pair<FMT>(fmaf(nibble_float<0>(w), a[0], b[0]), fmaf(nibble_float<2>(w), a[1], b[1]));
+  e1 = pack_pair<FMT>(fmaf(nibble_float<4>(w), a[2], b[2]), fmaf(nibble_float<6>(w), a[3], b[3]));
+  o0 = pack_pair<FMT>(fmaf(nibble_float<1>(w), a[0], b[0]), fmaf(nibble_float<3>(w), a[1], b[1]));
+  o1 = pack_pair<FMT>(fmaf(nibble_float<5>(w), a[2], b[2]), fmaf(nibble_float<7>(w), a[3], b[3]));
+}
+
+// GR: scales per group; xmap1 and zmap are then the maps of the tables a and b
+template <typename XT, typename ZST, int FMT, bool TB, bool GR>
 __global__ void __launch_bounds__(P_THREADS, 1)
 w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap0,
-               const __grid_constant__ CUtensorMap xmap1, const PairParams p) {
+               const __grid_constant__ CUtensorMap xmap1, const __grid_constant__ CUtensorMap zmap, const PairParams p) {
   using namespace umma;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
@@ -108,7 +146,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
   uint8_t* a_ring = raw_ring + P_RAW_ST * P_RAW_BYTES;
   uint8_t* x_ring = a_ring + P_A_ST * P_A_BYTES;
   uint8_t* out_buf = smem + P_RING_BYTES;
-  uint64_t* raw_full = reinterpret_cast<uint64_t*>(out_buf + P_OUT_BYTES);
+  uint8_t* tab_ring = out_buf + P_OUT_BYTES;
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(tab_ring + (GR ? P_RAW_ST * P_TAB_BYTES : 0));
   uint64_t* raw_empty = raw_full + P_RAW_ST;
   uint64_t* a_full = raw_empty + P_RAW_ST;
   uint64_t* a_empty = a_full + P_A_ST;
@@ -136,7 +175,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     fence_barrier_init();
     prefetch_tensormap(&wmap);
     prefetch_tensormap(&xmap0);
-    if (p.planes > 1) prefetch_tensormap(&xmap1);
+    if (GR || p.planes > 1) prefetch_tensormap(&xmap1);
+    if (GR) prefetch_tensormap(&zmap);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)P_TMEM_COLS) : "memory");
@@ -155,6 +195,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     int issued = 0, rs = 0;
     uint32_t rph = 0;
     bool ok = true;
+    const uint32_t tab = GR ? (uint32_t)(p.tab_rows * (TB ? P_STAGE_K : 128) * 4) : 0u;      // bytes of one table
+    if (GR) asm volatile("griddepcontrol.wait;" ::: "memory");                                 // the tables come from the previous kernel
     for (int t = pair; t < w_end && ok; t += p.G) {
       const PairItem sg = pair_item(p, t);
       const int row0 = sg.rp * 256 + 128 * (int)rank;
@@ -162,9 +204,14 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         if (issued >= P_RAW_ST) ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], rph ^ 1, abort_flag));
         if (!ok) break;
         if (lane == 0) {
-          mbar_expect_tx(&raw_full[rs], P_RAW_BYTES);
+          mbar_expect_tx(&raw_full[rs], P_RAW_BYTES + 2 * tab);
           if (TB) tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, st * P_STAGE_K, row0 / 2, &raw_full[rs]);
           else    tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, row0, st * (P_STAGE_K / 2), &raw_full[rs]);
+          if (GR) {
+            const int cx = TB ? st * P_STAGE_K : row0, cy = (TB ? row0 : st * P_STAGE_K) / p.group;
+            tma_load_2d(tab_ring + rs * P_TAB_BYTES, &xmap1, cx, cy, &raw_full[rs]);
+            tma_load_2d(tab_ring + rs * P_TAB_BYTES + P_TAB_BYTES / 2, &zmap, cx, cy, &raw_full[rs]);
+          }
         }
         __syncwarp();
         ++issued;
@@ -264,6 +311,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     bool ok = true;
     int rs = as;
     uint32_t rph = 0, aph = 0;
+    int row0 = 0, st = as, t_now = pair - p.G;         // with groups: the tile's first row, and where in its item the stage is
+    if (GR) st += nst;                                 // (the first step takes the first item)
     const int total = pair < w_end ? (w_end - 1 - pair) / p.G * nst + nst : 0;      // stages of all items
     for (int i = as; i < total; i += P_A_ST) {
       ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[rs], rph, abort_flag));
@@ -282,13 +331,44 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         tc_fence_after();
       }
       uint8_t* at = a_ring + as * P_A_BYTES;
+      if (GR) {
+        while (st >= nst) {
+          st -= nst;
+          t_now += p.G;
+          row0 = pair_item(p, t_now).rp * 256 + 128 * (int)rank;
+        }
+      }
+      float ta[GR ? 16 : 1], tb[GR ? 16 : 1];          // the tables' entries of this lane's 16 channels
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        uint32_t e[8], o[8];     // low nibbles / high nibbles: 16 channels each, in expanded order
+        uint32_t e[8], o[8];     // low nibbles / high nibbles: 16 channels each, in expanded order (with groups: as they are)
+        if constexpr (GR) {
+          // the 32 contraction-axis indices from here on lie in one group: all of a forward warp's, half of a transposed one's
+          if (u == 0 || (TB && u == 2)) {
+            const int k = TB ? row0 + 16 * (u0 + u) : st * P_STAGE_K + 8 * u0;
+            const int first = (TB ? row0 : st * P_STAGE_K) / p.group;
+            const uint32_t at_tab = smem_u32(tab_ring + rs * P_TAB_BYTES) + (uint32_t)((k / p.group - first) * (TB ? P_STAGE_K : 128) * 4 +
+                                                                                      (TB ? lane & 3 : lane & 7) * 64);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(ta[4 * c]), "=f"(ta[4 * c + 1]), "=f"(ta[4 * c + 2]), "=f"(ta[4 * c + 3])
+                           : "r"(at_tab + 16 * c) : "memory");
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(tb[4 * c]), "=f"(tb[4 * c + 1]), "=f"(tb[4 * c + 2]), "=f"(tb[4 * c + 3])
+                           : "r"(at_tab + P_TAB_BYTES / 2 + 16 * c) : "memory");
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float a4[4] = {ta[4 * c], ta[4 * c + 1], ta[4 * c + 2], ta[4 * c + 3]};
+            const float b4[4] = {tb[4 * c], tb[4 * c + 1], tb[4 * c + 2], tb[4 * c + 3]};
+            expand_word_scaled<FMT>(c == 0 ? v[u].x : c == 1 ? v[u].y : c == 2 ? v[u].z : v[u].w, a4, b4, e[2 * c], e[2 * c + 1], o[2 * c], o[2 * c + 1]);
+          }
+        } else {
         expand_word<FMT>(v[u].x, p.emask_lo, p.emask_hi, p.emagic, e[0], e[1], o[0], o[1]);
         expand_word<FMT>(v[u].y, p.emask_lo, p.emask_hi, p.emagic, e[2], e[3], o[2], o[3]);
         expand_word<FMT>(v[u].z, p.emask_lo, p.emask_hi, p.emagic, e[4], e[5], o[4], o[5]);
         expand_word<FMT>(v[u].w, p.emask_lo, p.emask_hi, p.emagic, e[6], e[7], o[6], o[7]);
+        }
         const uint4 e0 = make_uint4(e[0], e[1], e[2], e[3]), e1 = make_uint4(e[4], e[5], e[6], e[7]);
         const uint4 o0 = make_uint4(o[0], o[1], o[2], o[3]), o1 = make_uint4(o[4], o[5], o[6], o[7]);
         if (TB) {
@@ -316,6 +396,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
       // the raw slot goes back only after the fence: its next writer is the async proxy
       if (lane == 0) { mbar_arrive_cluster(a_full0 + (uint32_t)(as * 8)); mbar_arrive(&raw_empty[rs]); }
       aph ^= 1;
+      if (GR) st += P_A_ST;
       rs += P_A_ST;
       if (rs >= P_RAW_ST) { rs -= P_RAW_ST; rph ^= 1; }
     }
@@ -328,7 +409,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     const bool helper = warp < P_XWARP;
     const int q = warp & 3;                                                  // TMEM lanes 32 q .. + 31
     const int share = helper ? 1 + ((warp - 2) >> 2) : 0;                    // of the three warps with this q
-    const int lrow = TB ? lane : ((lane & ~3) | ((lane & 1) << 1) | ((lane >> 1) & 1));      // forward: channels 0, 2, 1, 3
+    const int lrow = TB || GR ? lane : ((lane & ~3) | ((lane & 1) << 1) | ((lane >> 1) & 1));      // forward: channels 0, 2, 1, 3
     const int64_t ld = TB ? p.K : p.N;
     // helpers use the A ring: by then every MMA has read its operands
     uint8_t* buf = helper ? a_ring + (warp - 2) * 32 * P_OUT_STRIDE : out_buf + (warp - P_XWARP - 1) * 32 * P_OUT_STRIDE;
@@ -343,7 +424,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
       const int row32 = it.rp * 256 + 128 * (int)rank + 32 * q;
       const int row = row32 + lrow;
       float sc = 1.f, zr = 1.f;
-      if (!TB && row < p.rows) { sc = zs_to_f32<ZST>(p.scale, row); zr = zs_to_f32<ZST>(p.zero, row); }
+      if (GR && p.inv && row < p.rows) sc = p.inv[TB ? row / p.group : row];
+      if (!GR && !TB && row < p.rows) { sc = zs_to_f32<ZST>(p.scale, row); zr = zs_to_f32<ZST>(p.zero, row); }
       const int piece = lane % LT, n_left = p.rows - row32 - piece * V;
       const bool wide = n_left >= V && (ld * (int64_t)sizeof(XT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
       for (int h = 0; h < it.nh; ++h, ++use) {
@@ -356,7 +438,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         for (int c = final_item ? 32 * share : 0; c < ntok; c += final_item ? 96 : 32) {
           // one value per token comes by shuffle, a pair through the 16 bytes that every token's row of the buffer has left
           float tok = 0.f;
-          if (TB) {
+          if (GR) {
+          } else if (TB) {
             if (c + lane < ntok)
               *reinterpret_cast<float2*>(buf + lane * P_OUT_STRIDE + 128) = *reinterpret_cast<const float2*>(p.tok + 2 * (int64_t)(m0 + c + lane));
             __syncwarp();
@@ -374,7 +457,9 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             float o;
-            if (TB) {
+            if (GR) {
+              o = __uint_as_float(v[i]) * sc;
+            } else if (TB) {
               const float2 t = *reinterpret_cast<const float2*>(buf + i * P_OUT_STRIDE + 128);
               o = fmaf(__uint_as_float(v[i]), t.y, -t.x);
             } else {
@@ -418,11 +503,12 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 }
 
 // ------------------------------------------------------------------ host ----
-PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b) {
+PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b, int group) {
   PairPlan pl;
   memset(&pl, 0, sizeof(pl));
   if (M < 1 || N % 16 != 0 || (!transpose_b && K % 8 != 0)) return pl;
-  pl.planes = (transpose_b || x_dtype == JGQ_F32) ? 2 : 1;
+  if (group > 0 && x_dtype == JGQ_F32) return pl;
+  pl.planes = group == 0 && (transpose_b || x_dtype == JGQ_F32) ? 2 : 1;
   pl.rows = (int)(transpose_b ? K : N);
   pl.depth = (int)(transpose_b ? N : K);
   pl.nrp = (int)cdiv(pl.rows, 256);
@@ -447,27 +533,32 @@ PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpos
   pl.Np = cdiv(N, P_STAGE_K) * P_STAGE_K;
   pl.plane_bytes = pl.planes == 1 ? 0 : align_up((size_t)M * (transpose_b ? pl.Np : K) * 2, 256);
   pl.tok_bytes = align_up((size_t)M * (transpose_b ? sizeof(float2) : sizeof(float)), 256);
+  if (group > 0) {                              // two tables, and the factors in place of the tokens' sums
+    pl.plane_bytes = align_up((size_t)cdiv(K, group) * N * sizeof(float), 256);
+    pl.tok_bytes = align_up((size_t)std::max<int64_t>(N, cdiv(K, group)) * sizeof(float), 256);
+  }
   pl.ws_bytes = W4_TICKET_REGION + pl.tok_bytes + 2 * pl.plane_bytes;
   pl.use = 1;
   return pl;
 }
 
-template <typename XT, typename ZST, int FMT, bool TB>
+template <typename XT, typename ZST, int FMT, bool TB, bool GR>
 static int launch_pair_inst(const PairPlan& pl, const PairParams& p, const CUtensorMap& wmap, const CUtensorMap& x0,
-                            const CUtensorMap& x1, cudaStream_t s) {
-  auto kern = w4_pair_kernel<XT, ZST, FMT, TB>;
+                            const CUtensorMap& x1, const CUtensorMap& z, cudaStream_t s) {
+  auto kern = w4_pair_kernel<XT, ZST, FMT, TB, GR>;
+  constexpr int smem = GR ? P_SMEM_BYTES_GR : P_SMEM_BYTES;
   struct AttrTag {};
   const int arc = once_per_device<AttrTag>([&]() {
     cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 0);
     cudaGetLastError();
-    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM_BYTES);
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (arc != 0) return fail(JGQ_ERR_CUDA, "w4_matmul: cannot raise the dynamic shared memory limit");
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)(2 * pl.G));
   cfg.blockDim = dim3(P_THREADS);
-  cfg.dynamicSmemBytes = P_SMEM_BYTES;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -476,7 +567,7 @@ static int launch_pair_inst(const PairPlan& pl, const PairParams& p, const CUten
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, wmap, x0, x1, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, wmap, x0, x1, z, p);
   note_launches(1);
   if (e != cudaSuccess) { cudaGetLastError(); return fail(JGQ_ERR_CUDA, "w4_pair: %s", cudaGetErrorString(e)); }
   return JGQ_OK;
@@ -519,12 +610,78 @@ static int launch_pair_type(const PairPlan& pl, PairParams& p, const void* x, co
     rc = encode_tmap_2d_b16(&xm[b], plane[b], cols, (uint64_t)M, cols * 2, P_STAGE_K, (uint32_t)pl.nt / 2);
     if (rc) return rc;
   }
-  if (transpose_b) return launch_pair_inst<XT, ZST, 0, true>(pl, p, wmap, xm[0], xm[1], s);
-  return launch_pair_inst<XT, ZST, std::is_same<XT, __half>::value ? 0 : 1, false>(pl, p, wmap, xm[0], xm[1], s);
+  if (transpose_b) return launch_pair_inst<XT, ZST, 0, true, false>(pl, p, wmap, xm[0], xm[1], xm[1], s);
+  return launch_pair_inst<XT, ZST, std::is_same<XT, __half>::value ? 0 : 1, false, false>(pl, p, wmap, xm[0], xm[1], xm[1], s);
+}
+
+// The tables of the weights with groups (see above).  FACTOR: with the power of two per channel, or per group (TB).
+// A CTA has 32 channels of every group, or, per group, one group's channels.
+template <typename ZST, bool FACTOR, bool TB>
+__global__ void __launch_bounds__(512) w4_group_tables_kernel(const ZST* __restrict__ scale, const ZST* __restrict__ zero, int64_t N, int64_t groups,
+                                                              float* __restrict__ a, float* __restrict__ b, float* __restrict__ inv) {
+  constexpr bool ROW = FACTOR && TB;
+  __shared__ float top[16][33];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t n = ROW ? (int64_t)threadIdx.x : blockIdx.x * 32ll + lane, n_step = ROW ? 512 : N;      // this thread's channels
+  const int64_t g0 = ROW ? blockIdx.x : w, g1 = ROW ? g0 + 1 : groups;                                   // and groups
+  float f = 1.f;
+  if (FACTOR) {
+    float big = 0.f;
+    for (int64_t g = g0; g < g1; g += 16)
+      for (int64_t c = n; c < N; c += n_step) {
+        const float z = to_f32<ZST>(zero[g * N + c]);
+        big = fmaxf(big, fabsf(to_f32<ZST>(scale[g * N + c])) * fmaxf(fabsf(z), fabsf(15.f - z)));
+      }
+    if (ROW) for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    top[w][lane] = big;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) big = fmaxf(big, top[i][ROW ? 0 : lane]);
+    const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
+    f = __uint_as_float((267u - e) << 23);
+    if (ROW ? threadIdx.x == 0 : (w == 0 && n < N)) inv[ROW ? g0 : n] = __uint_as_float((e - 13u) << 23);
+  }
+  for (int64_t g = g0; g < g1; g += 16)
+    for (int64_t c = n; c < N; c += n_step) {
+      const float s = to_f32<ZST>(scale[g * N + c]) * f, z = to_f32<ZST>(zero[g * N + c]);
+      a[g * N + c] = 128.f * s;
+      b[g * N + c] = -(128.f + z) * s;
+    }
+}
+
+template <typename XT, typename ZST>
+static int launch_pair_groups(const PairPlan& pl, PairParams& p, const void* x, const uint8_t* packed, int transpose_b, int group, uint8_t* ws, cudaStream_t s) {
+  constexpr bool FACTOR = std::is_same<XT, __half>::value;
+  constexpr int FMT = FACTOR ? 0 : 1;
+  const int64_t M = p.M, N = p.N, K = p.K, groups = cdiv(K, group);
+  float* inv = (float*)(ws + W4_TICKET_REGION);
+  float* a = (float*)(ws + W4_TICKET_REGION + pl.tok_bytes);
+  float* b = (float*)(ws + W4_TICKET_REGION + pl.tok_bytes + pl.plane_bytes);
+  const ZST *sc = (const ZST*)p.scale, *z = (const ZST*)p.zero;
+  if (FACTOR && transpose_b) w4_group_tables_kernel<ZST, FACTOR, true><<<(unsigned)groups, 512, 0, s>>>(sc, z, N, groups, a, b, inv);
+  else                       w4_group_tables_kernel<ZST, FACTOR, false><<<(unsigned)cdiv(N, 32), 512, 0, s>>>(sc, z, N, groups, a, b, inv);
+  int rc = check_launch("w4_group_tables");
+  if (rc) return rc;
+  p.inv = FACTOR ? inv : nullptr;
+  p.group = group;
+  p.tab_rows = transpose_b ? (group % 128 == 0 ? 1 : 4) : (group % P_STAGE_K == 0 ? 1 : 2);
+  CUtensorMap wmap, xm, am, bm;
+  rc = transpose_b ? encode_tmap_2d_u8(&wmap, packed, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)N, 64, 64, 0)
+                   : encode_tmap_2d_u8(&wmap, packed, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)N, 128, 32, 0);
+  if (rc) return rc;
+  const uint64_t depth = (uint64_t)(transpose_b ? N : K);
+  rc = encode_tmap_2d_b16(&xm, x, depth, (uint64_t)M, depth * 2, P_STAGE_K, (uint32_t)pl.nt / 2);
+  if (rc) return rc;
+  rc = encode_tmap_2d_f32(&am, a, (uint64_t)N, (uint64_t)groups, (uint64_t)N * 4, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
+  if (rc) return rc;
+  rc = encode_tmap_2d_f32(&bm, b, (uint64_t)N, (uint64_t)groups, (uint64_t)N * 4, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
+  if (rc) return rc;
+  if (transpose_b) return launch_pair_inst<XT, float, FMT, true, true>(pl, p, wmap, xm, am, bm, s);
+  return launch_pair_inst<XT, float, FMT, false, true>(pl, p, wmap, xm, am, bm, s);
 }
 
 int launch_w4_pair(const PairPlan& pl, const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale,
-                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int transpose_b, void* ws, cudaStream_t s) {
+                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int transpose_b, int group, void* ws, cudaStream_t s) {
   PairParams p;
   memset(&p, 0, sizeof(p));
   p.nst = (int)cdiv(pl.depth, P_STAGE_K);
@@ -538,6 +695,10 @@ int launch_w4_pair(const PairPlan& pl, const void* x, int x_dtype, const uint8_t
   p.rows = pl.rows; p.depth = pl.depth; p.planes = pl.planes; p.nrp = pl.nrp;
   uint8_t* w = (uint8_t*)ws;
   const bool zf = zs_dtype == JGQ_F32;
+  if (group > 0) {
+    if (x_dtype == JGQ_F16) return zf ? launch_pair_groups<__half, float>(pl, p, x, packed, transpose_b, group, w, s) : launch_pair_groups<__half, __half>(pl, p, x, packed, transpose_b, group, w, s);
+    return zf ? launch_pair_groups<__nv_bfloat16, float>(pl, p, x, packed, transpose_b, group, w, s) : launch_pair_groups<__nv_bfloat16, __half>(pl, p, x, packed, transpose_b, group, w, s);
+  }
 #define JGQ_PAIR(XT) return zf ? launch_pair_type<XT, float>(pl, p, x, packed, transpose_b, w, s) : launch_pair_type<XT, __half>(pl, p, x, packed, transpose_b, w, s)
   if (x_dtype == JGQ_F32) { JGQ_PAIR(float); }
   if (x_dtype == JGQ_F16) { JGQ_PAIR(__half); }

@@ -41,9 +41,10 @@ struct PairPlan {
   int G;                            // pairs
   double us;                        // estimate
 };
-PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b);
+// group: contraction indices per scale (0: one per channel); not for fp32 activations
+PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b, int group = 0);
 int launch_w4_pair(const PairPlan& pl, const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale,
-                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int transpose_b, void* ws, cudaStream_t s);
+                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int transpose_b, int group, void* ws, cudaStream_t s);
 
 // decode kernel, M <= 32, fp32 activations M <= 16 (w4_gemv.cu)
 struct GemvPlan {
@@ -52,8 +53,9 @@ struct GemvPlan {
   size_t ws_bytes;       // tickets + slices
   int smem_bytes;        // dynamic shared memory per CTA
 };
-GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype);
+// group: contraction indices per scale (0: one per channel); grouped: whether there are such
+GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped = 0);
 int launch_w4_gemv(const GemvPlan& pl, const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale,
-                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, void* ws, int settled, cudaStream_t s);
+                   int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int group, void* ws, int settled, cudaStream_t s);
 
 }  // namespace jgq
