@@ -19,14 +19,28 @@
 //     half a step of 2^-11, as an f16 result is).
 //   * running maximum and sum per row (in log2 units), fp32 accumulators; scales meet fp32 numbers only.
 //
-// Work: the list of all (sequence, kv head, 8 NT rows, 64-token tile) is cut into equal contiguous ranges, one per CTA, at
-// least four tiles each; the ranges follow from the lengths on the device.  In a CTA four warps take tiles in turn and
-// are joined through shared memory; an item that several CTAs share is joined by the one that draws the last ticket, in
-// CTA order.  A CTA shares at most two items (its first and its last), so two slices per CTA are all the scratch there is.
+// Keys and values of 64 tokens are contiguous: they come by bulk copies in units of 8 KB (DW = 64: 4 KB), a ring of NSLOT
+// units ahead of their use.
+//
+// Work: the list of all (sequence, kv head, NC rows of q, 64-token tile) is cut into equal contiguous ranges, one per CTA; the
+// ranges follow from the lengths on the device.  Two ways to share a CTA's piece of an item among its four warps:
+//   few rows (NC = 8 NT): the warps take tiles in turn, each with a ring of its own, and are joined through shared memory;
+//   COLS (NC = 32 NT): every warp has 8 NT rows of its own and all walk the same tiles in one ring, refilled by the warp
+//   that is the last to have read a unit.  A warp passes over tiles that none of its rows sees.
+// An item that several CTAs share is joined by the one that draws the last ticket, in CTA order.  A CTA shares at most two
+// items (its first and its last), so two slices per CTA are all the scratch there is.
+// Where the rows of a sequence make several row tiles, the earlier ones see fewer tokens: tile counts are a linear function
+// rounded down, whose sums have a closed form (floor_sum).
 #include "kv_cache.cuh"
+#include "umma.cuh"
+#include "trace.cuh"
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
+
+// measurement builds, per CTA: 0 entry, 1 range known, 2 first piece's tiles done, 3 first piece done, 4 last piece's tiles done, 5 exit
+JGQ_TRACE_DEFINE(attend, 8 * 1024)
+#define ATRACE(i) JGQ_TRACE_CTA(attend, i, 1024)
 
 namespace jgq {
 
@@ -41,7 +55,7 @@ struct AttendParams {
   int64_t table_stride;
   int32_t* tickets; float* slices;
   int T, B, W, Hq, Hkv, group, D, P, pages;
-  int vec_q;                   // 16-byte loads of q are legal
+  int vec_q, vec_o;            // 16-byte loads of q, stores of four channels are legal
   int zero_rest;               // rows behind the last sequence are zeroed
   int G;                       // CTAs
   float scale;                 // of the scores, times log2(e)
@@ -57,6 +71,11 @@ __device__ __forceinline__ void mma_h(float (&d)[4], uint32_t a0, uint32_t a1, u
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_h0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // d = a b
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -67,10 +86,14 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(umma::smem_u32(bar)) : "memory");
 }
 
 // two codes of a word as f16: as subnormals with their excess, or exact
@@ -96,38 +119,98 @@ __device__ __forceinline__ int seq_len(const AttendParams& p, int r) {
   return (int)min((int64_t)max(0, p.lengths[r]), (int64_t)p.W * p.P);
 }
 
-template <typename XT, int DW, int NT>
-__global__ void __launch_bounds__(KA_THREADS)
+// sum over i < n of floor((a i + b) / m); a, b >= 0
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    if (a >= m) { sum += n * (n - 1) / 2 * (a / m); a %= m; }
+    if (b >= m) { sum += n * (b / m); b %= m; }
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;                                         // the lattice points below the line, counted along the other axis
+    b = y % m;
+    const int64_t t = a; a = m; m = t;
+  }
+  return sum;
+}
+
+// a sequence's part of the list: row tiles per head, and units of row tile c: floor((a c + b) / m), COST in front and a tile each
+struct SeqWork {
+  int n, L, ct;
+  int64_t m, a, b;
+};
+template <int NC, int COST>
+__device__ __forceinline__ SeqWork seq_work(const AttendParams& p, int r) {
+  SeqWork w;
+  w.n = seq_rows(p, r);
+  w.L = seq_len(p, r);
+  w.ct = (w.n * p.group + NC - 1) / NC;
+  w.m = 1; w.a = 0; w.b = COST + max(1, (w.L + KV_TILE - 1) / KV_TILE);
+  if (w.ct > 1 && w.L >= w.n) {                        // what the last row of row tile c sees, in tokens times group, rounded up
+    w.m = (int64_t)KV_TILE * p.group;
+    w.a = NC;
+    w.b = (int64_t)(w.L - w.n) * p.group + NC + p.group - 1 + w.m - 1 + COST * w.m;
+  }
+  return w;
+}
+
+__host__ __device__ constexpr int attend_unit(int dw) { return dw == 64 ? 4096 : 8192; }      // bytes
+__host__ __device__ constexpr int attend_slots(int dw, bool cols) { return cols ? (dw == 64 ? 8 : 6) : (dw == 64 ? 4 : dw == 128 ? 2 : 3); }   // units per ring
+__host__ __device__ constexpr int attend_ctas(int dw, int nt, bool f32, bool cols) { return cols ? (dw == 64 && nt == 1 ? 3 : 2) : (dw <= 128 && nt == 1 && !f32 ? 3 : 2); }
+__host__ __device__ constexpr int attend_ring_bytes(int dw, bool cols) { return attend_unit(dw) * attend_slots(dw, cols) * (cols ? 1 : KA_WARPS); }
+__host__ __device__ constexpr int attend_smem(int dw, bool cols) {
+  return 1024 + attend_ring_bytes(dw, cols);
+}
+
+template <typename XT, int DW, int NT, bool COLS>
+__global__ void __launch_bounds__(KA_THREADS, attend_ctas(DW, NT, std::is_same<XT, float>::value, COLS))
 kv_attend_kernel(const AttendParams p) {
+  using namespace umma;
   constexpr bool F32 = std::is_same<XT, float>::value;
   constexpr bool EXACT = F32;
   constexpr int QP = F32 ? 2 : 1;                      // planes of q and of p
-  constexpr int NC = 8 * NT;                           // rows of q per item
+  // What beginning and finishing an item takes, in tiles: units in front of its tiles that only weigh in the cut.  Without
+  // them a CTA with many short sequences took 215 us where the others took 119.
+  constexpr int kPieceCost = COLS ? 8 : 6;
+  constexpr int NC = 8 * NT * (COLS ? KA_WARPS : 1);   // rows of q per item
   constexpr int CH = DW / 64;                          // 64-channel chunks of a row
   constexpr int DT = DW / 16;                          // 16-channel tiles of the output
+  constexpr int UNIT = attend_unit(DW), NSLOT = attend_slots(DW, COLS);
+  constexpr int UPT = 2 * 64 * DW / UNIT, KU = UPT / 2;                // units per tile; of keys
+  constexpr int DTU = DT / KU;                         // channel tiles per unit of values
   constexpr int SLICE = NC * (DW + 2);                 // floats: sums, then (max, sum) per row
   constexpr float UP24 = EXACT ? 1.f : 16777216.f;
-  extern __shared__ __align__(16) float smem[];        // [warp][NC][DW] sums, [warp][NC][2]
-  float* so = smem;
-  float* sml = smem + KA_WARPS * NC * DW;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  uint64_t* full_all = reinterpret_cast<uint64_t*>(smem_raw);          // [rings][NSLOT]
+  int* done = reinterpret_cast<int*>(smem_raw + 512);                  // [NSLOT] warps that have read a unit (COLS)
+  uint8_t* ring_all = smem_raw + 1024;
+  // few rows: a warp's sums [NC][DW] lie in its own ring, which is empty by then
+  static_assert(COLS || NC * DW * 4 <= NSLOT * UNIT, "a warp's sums fit its ring");
+  auto sums_of = [&](int w) { return reinterpret_cast<float*>(ring_all + w * (NSLOT * UNIT)); };
+  __shared__ __align__(16) float sml[COLS ? 1 : KA_WARPS * NC * 2];                  // [warp][NC] maximum, sum
   __shared__ int64_t s_pre[KA_THREADS + 1];
   __shared__ int64_t s_found[2];
-  __shared__ int s_flag;
+  __shared__ int s_flag, s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  auto units = [&](int r, int& ct, int& tiles) {       // work of a sequence: kv heads x row tiles x token tiles (one at least)
-    const int n = seq_rows(p, r);
-    ct = (n * p.group + NC - 1) / NC;
-    tiles = n > 0 ? max(1, (seq_len(p, r) + KV_TILE - 1) / KV_TILE) : 0;
-    return (int64_t)p.Hkv * ct * tiles;
+  volatile int* abort_flag = &s_abort;
+  ATRACE(0);
+  if (tid == 0) {
+    for (int i = 0; i < NSLOT * (COLS ? 1 : KA_WARPS); ++i) mbar_init(&full_all[i], 1);
+    for (int i = 0; i < NSLOT; ++i) done[i] = 0;
+    s_abort = 0;
+    fence_barrier_init();
+  }
+  auto units = [&](int r) {                            // work of a sequence
+    const SeqWork w = seq_work<NC, kPieceCost>(p, r);
+    return w.n > 0 ? (int64_t)p.Hkv * (w.a ? floor_sum(w.ct, w.m, w.a, w.b) : w.ct * w.b) : 0;
   };
 
   // ---- this CTA's range ----
   const int per = (p.B + KA_THREADS - 1) / KA_THREADS;
   {
     int64_t sum = 0;
-    int ct, tiles;
-    for (int r = tid * per; r < min(p.B, (tid + 1) * per); ++r) sum += units(r, ct, tiles);
+    for (int r = tid * per; r < min(p.B, (tid + 1) * per); ++r) sum += units(r);
     int64_t inc = sum;
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -150,14 +233,13 @@ kv_attend_kernel(const AttendParams p) {
     if (p.lse)
       for (int64_t i = first * p.Hq + blockIdx.x * (int64_t)KA_THREADS + tid; i < (int64_t)p.T * p.Hq; i += (int64_t)gridDim.x * KA_THREADS) p.lse[i] = -INFINITY;
   }
-  const int G = (int)min((int64_t)p.G, (S + KA_WARPS - 1) / KA_WARPS);
+  const int G = (int)min((int64_t)p.G, (S + kPieceCost + KA_WARPS - 1) / (kPieceCost + KA_WARPS));
   if ((int)blockIdx.x >= G) return;
   const int64_t idx_begin = (int64_t)blockIdx.x * S / G, idx_end = ((int64_t)blockIdx.x + 1) * S / G;
   if (s_pre[tid] <= idx_begin && idx_begin < s_pre[tid + 1]) {
     int64_t at = s_pre[tid];
-    int ct, tiles;
     for (int r = tid * per;; ++r) {
-      const int64_t u = units(r, ct, tiles);
+      const int64_t u = units(r);
       if (idx_begin < at + u) { s_found[0] = r; s_found[1] = at; break; }
       at += u;
     }
@@ -166,18 +248,76 @@ kv_attend_kernel(const AttendParams p) {
   int r = (int)s_found[0];
   int64_t seq_at = s_found[1];                         // first unit of the sequence
 
+  uint64_t* full = full_all + (COLS ? 0 : warp * NSLOT);
+  const uint32_t ring = smem_u32(ring_all) + (COLS ? 0 : warp * NSLOT * UNIT);
+  int slot = 0;                                        // of the ring's next unit, and the parity its arrival has
+  uint32_t phase = 0;
+  bool alive = true;
+  ATRACE(1);
+  const int page_shift = p.P == 64 ? 0 : p.P == 128 ? 1 : 2;          // tiles per page
+
   // ---- pieces: the part of one item (sequence, head, row tile) in this range ----
   for (int64_t idx = idx_begin; idx < idx_end;) {
-    int ct, tiles;
-    int64_t u = units(r, ct, tiles);
-    while (idx >= seq_at + u) { seq_at += u; ++r; u = units(r, ct, tiles); }
-    const int64_t in_seq = idx - seq_at;
-    const int item = (int)(in_seq / tiles), h = item / ct, c0 = (item % ct) * NC;
-    const int64_t item_at = seq_at + (int64_t)item * tiles;
-    const int t_first = (int)(idx - item_at), t_last = (int)min((int64_t)tiles, idx_end - item_at);
-    const int n = seq_rows(p, r), L = seq_len(p, r), row_first = p.cu ? max(0, min(p.cu[r], p.T)) : r;
+    int64_t u = units(r);
+    while (idx >= seq_at + u) { seq_at += u; ++r; u = units(r); }
+    const SeqWork wk = seq_work<NC, kPieceCost>(p, r);
+    const int n = wk.n, L = wk.L;
+    const int64_t per_head = u / p.Hkv;
+    const int h = (int)((idx - seq_at) / per_head);
+    int64_t in_head = (idx - seq_at) - h * per_head;
+    int row_tile, tiles;
+    if (wk.a) {                                        // the row tile by bisection in the sums
+      int lo = 0, hi = wk.ct;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (floor_sum(mid, wk.m, wk.a, wk.b) <= in_head) lo = mid; else hi = mid;
+      }
+      row_tile = lo;
+      in_head -= floor_sum(lo, wk.m, wk.a, wk.b);
+      tiles = (int)((wk.a * lo + wk.b) / wk.m) - kPieceCost;
+    } else {
+      row_tile = (int)(in_head / wk.b);
+      in_head -= row_tile * wk.b;
+      tiles = (int)wk.b - kPieceCost;
+    }
+    const int c0 = row_tile * NC;
+    const int64_t item_at = idx - in_head;
+    const int64_t tile_at = item_at + kPieceCost;
+    const int t_first = (int)max((int64_t)0, idx - tile_at), t_last = (int)max((int64_t)0, min((int64_t)tiles, idx_end - tile_at));
+    if (t_last <= t_first) { idx = idx_end; break; }   // the item's tiles begin behind this range
+    const int row_first = p.cu ? max(0, min(p.cu[r], p.T)) : r;
     const int rows = min(NC, n * p.group - c0);        // rows of q of this item
-    const int seen_least = max(0, L - n + c0 / p.group + 1);          // what its first row sees
+    const int w0 = COLS ? 8 * NT * warp : 0;           // this warp's first one
+    const int mine = COLS ? max(0, min(8 * NT, rows - w0)) : rows;
+    // tokens that the first and the last of this warp's rows see, and the last of the item's
+    const int seen_least = max(0, L - n + (c0 + w0) / p.group + 1);
+    const int seen_most = mine > 0 ? max(0, L - n + (c0 + w0 + mine - 1) / p.group + 1) : 0;
+    const int seen_item = max(0, L - n + (c0 + rows - 1) / p.group + 1);
+    const int t_end = min(t_last, (seen_item + KV_TILE - 1) / KV_TILE);
+
+    // ---- the ring: unit i of this piece's tiles ----
+    const int t_begin = COLS ? t_first : t_first + warp, t_step = COLS ? 1 : KA_WARPS;
+    const int my_tiles = t_begin < t_end ? (t_end - t_begin + t_step - 1) / t_step : 0;
+    const int32_t* row_of_table = p.table + (int64_t)r * p.table_stride;
+    auto page_of = [&](int k) { return k < my_tiles ? row_of_table[(t_begin + k * t_step) >> page_shift] : -1; };
+    auto issue = [&](int to, int k, int part, int page) {         // part `part` of tile k, on that page, into a slot; one lane
+      const int tile = t_begin + k * t_step;
+      const int64_t block = (int64_t)(page < 0 || page >= p.pages ? 0 : page) * p.Hkv + h;
+      const int64_t at = ((block << page_shift) + (tile & ((1 << page_shift) - 1))) * (int64_t)(DW * KV_TILE) + (part % KU) * UNIT;
+      mbar_expect_tx(&full[to], UNIT);
+      bulk_load(ring + to * UNIT, (part < KU ? p.k : p.v) + at, UNIT, &full[to]);
+    };
+    int page_now = page_of(0), page_1 = page_of(1), page_2 = page_of(2);
+    // Tiles in front of the ring's end: units are requested NSLOT ahead, that is up to AHEAD tiles.
+    constexpr int AHEAD = (NSLOT + UPT - 1) / UPT;
+    static_assert(AHEAD <= 4, "page numbers are kept two tiles ahead, further ones are looked up");
+    if (alive && lane == 0 && (!COLS || warp == 0)) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < NSLOT; ++i)
+        if (i / UPT < my_tiles)
+          issue(slot + i < NSLOT ? slot + i : slot + i - NSLOT, i / UPT, i % UPT, i / UPT == 0 ? page_now : i / UPT == 1 ? page_1 : i / UPT == 2 ? page_2 : page_of(i / UPT));
+    }
 
     // ---- q: the lane's operands, and per column (2 t, 2 t + 1 of each octet) limit, factor and sum ----
     uint32_t qf[NT][QP][CH][4][2];
@@ -186,8 +326,8 @@ kv_attend_kernel(const AttendParams p) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[CH][16], big = 0.f, sum = 0.f;
-      const int c = 8 * nt + g, row = c0 + c;
-      const bool live = c < rows;
+      const int c = 8 * nt + g, row = c0 + w0 + c;
+      const bool live = c < mine;
       const XT* src = reinterpret_cast<const XT*>(p.q) + (int64_t)(row_first + (live ? row / p.group : 0)) * p.q_token +
                       (int64_t)(h * p.group + (live ? row % p.group : 0)) * p.q_head;
 #pragma unroll
@@ -233,7 +373,7 @@ kv_attend_kernel(const AttendParams p) {
         const float fc = __shfl_sync(0xffffffffu, f, from);
         qscale[nt][b] = fc * UP24;
         qbias[nt][b] = EXACT ? 0.f : -128.f * __shfl_sync(0xffffffffu, sum, from) * fc;
-        limit[nt][b] = col < rows ? L - n + (c0 + col) / p.group + 1 : 0;
+        limit[nt][b] = col < mine ? L - n + (c0 + w0 + col) / p.group + 1 : 0;
       }
     }
 
@@ -249,155 +389,320 @@ kv_attend_kernel(const AttendParams p) {
     }
 
     // ---- tiles ----
-    const int32_t* row_of_table = p.table + (int64_t)r * p.table_stride;
-    const int tiles_per_page = p.P / KV_TILE;
-    const int k_lane = (16 * (g >> 1) + (g & 1)) * DW + 16 * t, v_lane = 64 * g + 16 * t;
-    const int t_end = L > 0 ? t_last : t_first;        // a sequence without tokens has one unit and no tile
-    for (int tile = t_first + warp; tile < t_end; tile += KA_WARPS) {
-      int page = row_of_table[tile / tiles_per_page];
-      const bool bad = page < 0 || page >= p.pages;    // no such page: the result is NaN
-      if (bad) page = 0;
-      const int64_t block = (int64_t)page * p.Hkv + h;
-      const int sub = tile % tiles_per_page;
-      const uint8_t* kp = p.k + (block * p.P + (int64_t)sub * KV_TILE) * DW + k_lane;
-      const uint8_t* vp = p.v + (block * tiles_per_page + sub) * (int64_t)(DW * KV_TILE) + v_lane;
-      const float ks = bad ? __int_as_float(0x7fc00000) : p.k_scale[block], vs = p.v_scale[block];
-
-      // scores of 64 tokens: tile i has tokens 16 (g / 2) + 4 i + (g & 1), and those plus two
-      float s[4][NT][4];
+    // `ahead` units behind the ring's next one: its slot and parity
+    auto slot_of = [&](int ahead) { return slot + ahead < NSLOT ? slot + ahead : slot + ahead - NSLOT; };
+    auto wait_unit = [&](int ahead) {
+      const uint32_t ph = slot + ahead < NSLOT ? phase : phase ^ 1u;
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&full[slot_of(ahead)], ph, abort_flag));
+      return ring + (uint32_t)slot_of(ahead) * UNIT;
+    };
+    // gives back the ring's next unit, part `part` of tile k, and has the one NSLOT further on fetched into its place
+    auto pass_unit = [&](int k, int part) {
+      __syncwarp();
+      if (lane == 0 && alive) {
+        bool refill = true;
+        if (COLS) {
+          int old;
+          asm volatile("atom.acq_rel.cta.shared.add.u32 %0, [%1], 1;" : "=r"(old) : "r"(smem_u32(&done[slot])) : "memory");
+          refill = old == KA_WARPS - 1;                // every warp has read the unit
+          if (refill) done[slot] = 0;
+        }
+        const int ahead = part + NSLOT, k2 = k + ahead / UPT;
+        if (refill && k2 < my_tiles) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          issue(slot, k2, ahead % UPT, ahead / UPT == 0 ? page_now : ahead / UPT == 1 ? page_1 : ahead / UPT == 2 ? page_2 : page_of(k2));
+        }
+      }
+      if (++slot == NSLOT) { slot = 0; phase ^= 1u; }
+    };
+    const uint32_t k_lane = (uint32_t)((16 * (g >> 1) + (g & 1)) * DW + 16 * t), v_lane = (uint32_t)(64 * g + 16 * t);
+    float ks = 0.f, vs = 0.f;
+    if (my_tiles > 0) {
+      const bool bad = page_now < 0 || page_now >= p.pages;            // no such page: the result is NaN
+      const int64_t block = (int64_t)(bad ? 0 : page_now) * p.Hkv + h;
+      ks = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+      vs = p.v_scale[block];
+    }
+    for (int k = 0; k < my_tiles; ++k) {
+      const int tile = t_begin + k * t_step;
+      // scales of the next tile, page number of the one after the next
+      float ks_next = 0.f, vs_next = 0.f;
+      const int page_3 = page_of(k + 3);
+      if (k + 1 < my_tiles) {
+        const bool bad = page_1 < 0 || page_1 >= p.pages;
+        const int64_t block = (int64_t)(bad ? 0 : page_1) * p.Hkv + h;
+        ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+        vs_next = p.v_scale[block];
+      }
+      if (COLS && tile * KV_TILE >= seen_most) {       // nothing for this warp's rows
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+        for (int part = 0; part < UPT; ++part) { wait_unit(0); pass_unit(k, part); }
+      } else {
+        // scores of 64 tokens: tile i has tokens 16 (g / 2) + 4 i + (g & 1), and those plus two
+        float s[4][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int part = 0; part < KU; ++part) wait_unit(part);
+        if (alive) {
+          const uint32_t slot0 = ring + (uint32_t)slot * UNIT, slot1 = ring + (uint32_t)slot_of(KU - 1) * UNIT;
+          // rows 16 (g / 2) + ..: with two units of 32 tokens, lanes g < 4 read the first and g >= 4 the second
+          const uint32_t at = KU == 1 ? slot0 + k_lane : (g < 4 ? slot0 + k_lane : slot1 + k_lane - 32 * DW);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][nt][e] = 0.f;
+          for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          const uint4 wa = load16(kp + 4 * i * DW + 64 * ch), wb = load16(kp + (4 * i + 2) * DW + 64 * ch);
+            for (int ch = 0; ch < CH; ++ch) {
+              const uint4 wa = lds16(at + 4 * i * DW + 64 * ch), wb = lds16(at + (4 * i + 2) * DW + 64 * ch);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a0 = code_pair<EXACT>(word_of(wa, j), 0), a2 = code_pair<EXACT>(word_of(wa, j), 1);
-            const uint32_t a1 = code_pair<EXACT>(word_of(wb, j), 0), a3 = code_pair<EXACT>(word_of(wb, j), 1);
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t a0 = code_pair<EXACT>(word_of(wa, j), 0), a2 = code_pair<EXACT>(word_of(wa, j), 1);
+                const uint32_t a1 = code_pair<EXACT>(word_of(wb, j), 0), a3 = code_pair<EXACT>(word_of(wb, j), 1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int pl = 0; pl < QP; ++pl) {
+                    if (ch == 0 && j == 0 && pl == 0) mma_h0(s[i][nt], a0, a1, a2, a3, qf[nt][pl][ch][j][0], qf[nt][pl][ch][j][1]);
+                    else                              mma_h(s[i][nt], a0, a1, a2, a3, qf[nt][pl][ch][j][0], qf[nt][pl][ch][j][1]);
+                  }
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int pl = 0; pl < QP; ++pl) mma_h(s[i][nt], a0, a1, a2, a3, qf[nt][pl][ch][j][0], qf[nt][pl][ch][j][1]);
+              for (int e = 0; e < 4; ++e) s[i][nt][e] = __int_as_float(0x7fc00000);
+        }
+#pragma unroll
+        for (int part = 0; part < KU; ++part) pass_unit(k, part);
+        const bool masked = (tile + 1) * KV_TILE > seen_least;
+        uint32_t pb[4][NT][QP][2];                       // p as operands of the products with the values
+        float alpha[NT][2], psum[NT][2], vsc[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float top[2] = {-INFINITY, -INFINITY};
+          const float fs[2] = {qscale[nt][0] * ks, qscale[nt][1] * ks}, fb[2] = {qbias[nt][0] * ks, qbias[nt][1] * ks};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v = fmaf(s[i][nt][e], fs[e & 1], fb[e & 1]);
+              if (masked && tile * KV_TILE + 16 * (g >> 1) + 4 * i + (g & 1) + (e & 2) >= limit[nt][e & 1]) v = -INFINITY;
+              s[i][nt][e] = v;
+              top[e & 1] = fmaxf(top[e & 1], v);         // passes a NaN over: its p is one
+            }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top[b] = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], x));
+            const float now = fmaxf(m[nt][b], top[b]), ref = now == -INFINITY ? 0.f : now;
+            alpha[nt][b] = exp2_fast(m[nt][b] - ref);
+            m[nt][b] = now;
+            top[b] = ref;
+          }
+          float ones[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float pv[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pv[e] = exp2_fast(s[i][nt][e] - top[e & 1]);
+            uint32_t ra = half2_bits(pv[0], pv[1]), rb = half2_bits(pv[2], pv[3]);
+            pb[i][nt][0][0] = transpose8x8(ra);
+            pb[i][nt][0][1] = transpose8x8(rb);
+            mma_h(ones, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[i][nt][0][0], pb[i][nt][0][1]);
+            if (QP == 2) {
+              const float2 fa = half2_floats(ra), fb = half2_floats(rb);
+              pb[i][nt][QP - 1][0] = transpose8x8(half2_bits(pv[0] - fa.x, pv[1] - fa.y));
+              pb[i][nt][QP - 1][1] = transpose8x8(half2_bits(pv[2] - fb.x, pv[3] - fb.y));
+              mma_h(ones, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[i][nt][QP - 1][0], pb[i][nt][QP - 1][1]);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            l[nt][b] = fmaf(l[nt][b], alpha[nt][b], ones[b]);
+            psum[nt][b] = EXACT ? 0.f : -128.f * ones[b];
+            vsc[nt][b] = ones[b] == 0.f ? 0.f : vs;      // a row that sees none of the tile takes nothing of it, not even a NaN
           }
         }
-      }
-      const bool masked = (tile + 1) * KV_TILE > seen_least;
-      uint32_t pb[4][NT][QP][2];                       // p as operands of the products with the values
-      float alpha[NT][2], psum[NT][2], vsc[NT][2];
+        bool same = true;                              // no row's maximum grew: the sums stay as they are
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float top[2] = {-INFINITY, -INFINITY};
+        for (int nt = 0; nt < NT; ++nt) same &= alpha[nt][0] == 1.f && alpha[nt][1] == 1.f;
+        if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = fmaf(s[i][nt][e], qscale[nt][e & 1], qbias[nt][e & 1]) * ks;
-            if (masked && tile * KV_TILE + 16 * (g >> 1) + 4 * i + (g & 1) + (e & 2) >= limit[nt][e & 1]) v = -INFINITY;
-            s[i][nt][e] = v;
-            top[e & 1] = fmaxf(top[e & 1], v);         // passes a NaN over: its p is one
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][nt][e] *= alpha[nt][e & 1];
+        }
+#pragma unroll
+        for (int part = 0; part < KU; ++part) {
+          const uint32_t at = wait_unit(0) + v_lane;
+#pragma unroll
+          for (int ii = 0; ii < DTU; ++ii) {
+            const int d = part * DTU + ii;
+            const uint4 wa = lds16(at + ii * 1024), wb = lds16(at + ii * 1024 + 512);
+            float x[NT][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = code_pair<EXACT>(word_of(wa, i), 0), a2 = code_pair<EXACT>(word_of(wa, i), 1);
+              const uint32_t a1 = code_pair<EXACT>(word_of(wb, i), 0), a3 = code_pair<EXACT>(word_of(wb, i), 1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int pl = 0; pl < QP; ++pl) {
+                  if (i == 0 && pl == 0) mma_h0(x[nt], a0, a1, a2, a3, pb[i][nt][pl][0], pb[i][nt][pl][1]);
+                  else                   mma_h(x[nt], a0, a1, a2, a3, pb[i][nt][pl][0], pb[i][nt][pl][1]);
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[d][nt][e] = fmaf(fmaf(x[nt][e], UP24, psum[nt][e & 1]), vsc[nt][e & 1], o[d][nt][e]);
           }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[b] = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], x));
-          const float now = fmaxf(m[nt][b], top[b]), ref = now == -INFINITY ? 0.f : now;
-          alpha[nt][b] = exp2_fast(m[nt][b] - ref);
-          m[nt][b] = now;
-          top[b] = ref;
-        }
-        float ones[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float pv[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pv[e] = exp2_fast(s[i][nt][e] - top[e & 1]);
-          uint32_t ra = half2_bits(pv[0], pv[1]), rb = half2_bits(pv[2], pv[3]);
-          pb[i][nt][0][0] = transpose8x8(ra);
-          pb[i][nt][0][1] = transpose8x8(rb);
-          mma_h(ones, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[i][nt][0][0], pb[i][nt][0][1]);
-          if (QP == 2) {
-            const float2 fa = half2_floats(ra), fb = half2_floats(rb);
-            pb[i][nt][QP - 1][0] = transpose8x8(half2_bits(pv[0] - fa.x, pv[1] - fa.y));
-            pb[i][nt][QP - 1][1] = transpose8x8(half2_bits(pv[2] - fb.x, pv[3] - fb.y));
-            mma_h(ones, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, pb[i][nt][QP - 1][0], pb[i][nt][QP - 1][1]);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          l[nt][b] = fmaf(l[nt][b], alpha[nt][b], ones[b]);
-          psum[nt][b] = EXACT ? 0.f : -128.f * ones[b];
-          vsc[nt][b] = ones[b] == 0.f ? 0.f : vs;      // a row that sees none of the tile takes nothing of it, not even a NaN
+          pass_unit(k, KU + part);
         }
       }
+      page_now = page_1; page_1 = page_2; page_2 = page_3;
+      ks = ks_next; vs = vs_next;
+    }
+    if (idx == idx_begin) ATRACE(2);
+    ATRACE(4);
+    if (!alive) {                                      // a wait ran out: the result says so
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const uint4 wa = load16(vp + d * 1024), wb = load16(vp + d * 1024 + 512);
-        float x[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t a0 = code_pair<EXACT>(word_of(wa, i), 0), a2 = code_pair<EXACT>(word_of(wa, i), 1);
-          const uint32_t a1 = code_pair<EXACT>(word_of(wb, i), 0), a3 = code_pair<EXACT>(word_of(wb, i), 1);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int pl = 0; pl < QP; ++pl) mma_h(x[nt], a0, a1, a2, a3, pb[i][nt][pl][0], pb[i][nt][pl][1]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[d][nt][e] = fmaf(fmaf(x[nt][e], UP24, psum[nt][e & 1]), vsc[nt][e & 1], o[d][nt][e] * alpha[nt][e & 1]);
-      }
+      for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fc00000);
     }
 
-    // ---- join the warps: columns' sums through shared memory ----
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int col = 8 * nt + 2 * t + b;
-        float* dst = so + (warp * NC + col) * DW;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          dst[16 * d + g] = o[d][nt][b];
-          dst[16 * d + 8 + g] = o[d][nt][2 + b];
-        }
-        if (g == 0) { sml[(warp * NC + col) * 2] = m[nt][b]; sml[(warp * NC + col) * 2 + 1] = l[nt][b]; }
-      }
-    __syncthreads();
+    // ---- out ----
     const bool whole = t_first == 0 && t_last == tiles;
-    const int first_c = attend_cta_of(item_at, S, G), last_c = attend_cta_of(item_at + tiles - 1, S, G);
-    auto finish = [&](int col, int d, float sum, float mx, float den) {
-      const int row = c0 + col, token = row_first + row / p.group, head = h * p.group + row % p.group;
-      if (d < p.D) reinterpret_cast<XT*>(p.out)[((int64_t)token * p.Hq + head) * p.D + d] = from_f32<XT>(den == 0.f ? 0.f : sum / den);
-      if (d == 0 && p.lse) p.lse[(int64_t)token * p.Hq + head] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
+    const int first_c = attend_cta_of(item_at + kPieceCost, S, G), last_c = attend_cta_of(item_at + kPieceCost + tiles - 1, S, G);
+    // where a row of the item goes: the row of (token, head)
+    auto out_row = [&](int col) {
+      const int row = c0 + col, i = p.group == 1 ? row : row / p.group;
+      return (int64_t)(row_first + i) * p.Hq + h * p.group + (row - i * p.group);
     };
-    float* slice = p.slices + ((int64_t)blockIdx.x * 2 + (idx_begin >= item_at ? 0 : 1)) * SLICE;
-    for (int i = tid; i < rows * DW; i += KA_THREADS) {
-      const int col = i / DW, d = i % DW;
-      float mx = -INFINITY, sum = 0.f, den = 0.f;
+    auto put_lse = [&](int64_t at, float mx, float den) {
+      if (p.lse) p.lse[at] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
+    };
+    auto finish4 = [&](int col, int d, const float4& sum, float mx, float den) {       // four channels
+      const int64_t at = out_row(col);
+      const float f = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
+      const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+      XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
+      if (p.vec_o) {
+        if (d < p.D) {
+          __align__(16) XT e[4];
 #pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) mx = fmaxf(mx, sml[(w * NC + col) * 2]);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) {
-        const float f = exp2_fast(sml[(w * NC + col) * 2] - ref);
-        sum = fmaf(so[(w * NC + col) * DW + d], f, sum);
-        den = fmaf(sml[(w * NC + col) * 2 + 1], f, den);
-      }
-      if (whole) {
-        finish(col, d, sum, mx, den);
+          for (int i = 0; i < 4; ++i) e[i] = from_f32<XT>(v[i]);
+          if (F32) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(e);
+          else     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+        }
       } else {
-        slice[col * DW + d] = sum;
-        if (d == 0) { slice[NC * DW + 2 * col] = mx; slice[NC * DW + 2 * col + 1] = den; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d + i < p.D) dst[i] = from_f32<XT>(v[i]);
+      }
+      if (d == 0) put_lse(at, mx, den);
+    };
+    float* slice = p.slices + ((int64_t)blockIdx.x * 2 + (idx_begin > item_at + kPieceCost ? 0 : 1)) * SLICE;
+    if (COLS) {
+      // every warp has all of its rows' tokens here
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (whole) {
+          float f[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int c = 8 * nt + 2 * t + b;
+            f[b] = l[nt][b] == 0.f ? 0.f : __fdiv_rn(1.f, l[nt][b]);
+            if (g == 0 && c < mine && p.lse) put_lse(out_row(w0 + c), m[nt][b], l[nt][b]);
+          }
+          if (F32) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int c = 8 * nt + 2 * t + b;
+              if (c < mine) {
+                XT* dst = reinterpret_cast<XT*>(p.out) + out_row(w0 + c) * p.D;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (16 * d + 8 * e + g < p.D) dst[16 * d + 8 * e + g] = from_f32<XT>(o[d][nt][2 * e + b] * f[b]);
+              }
+            }
+          } else {
+            // transposed eight by eight: two neighbouring channels of row g per lane
+            const int c = 8 * nt + g;
+            XT* dst = reinterpret_cast<XT*>(p.out) + (c < mine ? out_row(w0 + c) * p.D : 0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const XT pr[2] = {from_f32<XT>(o[d][nt][2 * e] * f[0]), from_f32<XT>(o[d][nt][2 * e + 1] * f[1])};
+                const uint32_t w = transpose8x8((uint32_t)*reinterpret_cast<const uint16_t*>(&pr[0]) | ((uint32_t)*reinterpret_cast<const uint16_t*>(&pr[1]) << 16));
+                const int ch = 16 * d + 8 * e + 2 * t;
+                if (c < mine && ch < p.D) {
+                  if (p.vec_o) *reinterpret_cast<uint32_t*>(dst + ch) = w;
+                  else {
+                    reinterpret_cast<uint16_t*>(dst)[ch] = (uint16_t)w;
+                    if (ch + 1 < p.D) reinterpret_cast<uint16_t*>(dst)[ch + 1] = (uint16_t)(w >> 16);
+                  }
+                }
+              }
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int c = 8 * nt + 2 * t + b, col = w0 + c;
+            if (c < mine) {
+#pragma unroll
+              for (int d = 0; d < DT; ++d) {
+                slice[col * DW + 16 * d + g] = o[d][nt][b];
+                slice[col * DW + 16 * d + 8 + g] = o[d][nt][2 + b];
+              }
+              if (g == 0) { slice[NC * DW + 2 * col] = m[nt][b]; slice[NC * DW + 2 * col + 1] = l[nt][b]; }
+            }
+          }
+        }
+      }
+    } else {
+      // join the warps: columns' sums through shared memory
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int col = 8 * nt + 2 * t + b;
+          float* dst = sums_of(warp) + col * DW;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            dst[16 * d + g] = o[d][nt][b];
+            dst[16 * d + 8 + g] = o[d][nt][2 + b];
+          }
+          if (g == 0) { sml[(warp * NC + col) * 2] = m[nt][b]; sml[(warp * NC + col) * 2 + 1] = l[nt][b]; }
+        }
+      __syncthreads();
+      for (int i = tid; i < rows * (DW / 4); i += KA_THREADS) {
+        const int col = i / (DW / 4), d = 4 * (i % (DW / 4));
+        float2 ml[KA_WARPS];
+        float mx = -INFINITY, den = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; ++w) { ml[w] = *reinterpret_cast<const float2*>(&sml[(w * NC + col) * 2]); mx = fmaxf(mx, ml[w].x); }
+        const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; ++w) {
+          const float f = exp2_fast(ml[w].x - ref);
+          const float4 v = *reinterpret_cast<const float4*>(sums_of(w) + col * DW + d);
+          sum.x = fmaf(v.x, f, sum.x); sum.y = fmaf(v.y, f, sum.y); sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
+          den = fmaf(ml[w].y, f, den);
+        }
+        if (whole) {
+          finish4(col, d, sum, mx, den);
+        } else {
+          *reinterpret_cast<float4*>(slice + col * DW + d) = sum;
+          if (d == 0) *reinterpret_cast<float2*>(slice + NC * DW + 2 * col) = make_float2(mx, den);
+        }
       }
     }
     if (!whole) {
@@ -411,64 +716,107 @@ kv_attend_kernel(const AttendParams p) {
       __syncthreads();
       if (s_flag) {
         __threadfence();
-        for (int i = tid; i < rows * DW; i += KA_THREADS) {
-          const int col = i / DW, d = i % DW;
-          float mx = -INFINITY, sum = 0.f, den = 0.f;
-          for (int c = first_c; c <= last_c; ++c) {    // in CTA order
-            const int64_t begins = (int64_t)c * S / G;
-            const float* src = p.slices + ((int64_t)c * 2 + (begins >= item_at ? 0 : 1)) * SLICE;
-            const float v = __ldcg(src + NC * DW + 2 * col), dv = __ldcg(src + NC * DW + 2 * col + 1), sv = __ldcg(src + col * DW + d);
-            const float now = fmaxf(mx, v), ref = now == -INFINITY ? 0.f : now;
-            const float fo = exp2_fast(mx - ref), fn = exp2_fast(v - ref);
-            sum = fmaf(sum, fo, sv * fn);
-            den = fmaf(den, fo, dv * fn);
-            mx = now;
+        // four channels of JP rows per thread, four slices at a time: 4 JP loads in flight
+        constexpr int JP = COLS ? 4 : (NC * DW / 4 + KA_THREADS - 1) / KA_THREADS, STEP = KA_THREADS * JP;
+        for (int i0 = tid; i0 < rows * (DW / 4); i0 += STEP) {
+          float mx[JP], den[JP];
+          float4 sum[JP];
+#pragma unroll
+          for (int j = 0; j < JP; ++j) { mx[j] = -INFINITY; den[j] = 0.f; sum[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
+          for (int cb = first_c; cb <= last_c; cb += 4) {          // in CTA order
+            float v[4][JP], dv[4][JP];
+            float4 sv[4][JP];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int cc = min(cb + c, last_c);
+              const float* src = p.slices + ((int64_t)cc * 2 + ((int64_t)cc * S / G > item_at + kPieceCost ? 0 : 1)) * SLICE;
+#pragma unroll
+              for (int j = 0; j < JP; ++j) {
+                const int i = min(i0 + j * KA_THREADS, rows * (DW / 4) - 1), col = i / (DW / 4);
+                v[c][j] = __ldcg(src + NC * DW + 2 * col);
+                dv[c][j] = __ldcg(src + NC * DW + 2 * col + 1);
+                sv[c][j] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (cb + c <= last_c) {
+#pragma unroll
+                for (int j = 0; j < JP; ++j) {
+                  const float now = fmaxf(mx[j], v[c][j]), ref = now == -INFINITY ? 0.f : now;
+                  const float fo = exp2_fast(mx[j] - ref), fn = exp2_fast(v[c][j] - ref);
+                  sum[j].x = fmaf(sum[j].x, fo, sv[c][j].x * fn); sum[j].y = fmaf(sum[j].y, fo, sv[c][j].y * fn);
+                  sum[j].z = fmaf(sum[j].z, fo, sv[c][j].z * fn); sum[j].w = fmaf(sum[j].w, fo, sv[c][j].w * fn);
+                  den[j] = fmaf(den[j], fo, dv[c][j] * fn);
+                  mx[j] = now;
+                }
+              }
           }
-          finish(col, d, sum, mx, den);
+#pragma unroll
+          for (int j = 0; j < JP; ++j) {
+            const int i = i0 + j * KA_THREADS, col = i / (DW / 4), d = 4 * (i % (DW / 4));
+            if (i < rows * (DW / 4)) finish4(col, d, sum[j], mx[j], den[j]);
+          }
         }
       }
     }
-    __syncthreads();
-    idx = item_at + t_last;
+    if (idx == idx_begin) ATRACE(3);
+    __syncthreads();                                   // before the rings are filled again
+    idx = tile_at + t_last;
+  }
+
+  ATRACE(5);
+  // After a wait that ran out copies may still be in flight: a bounded time to land before the shared memory is released.
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) {}
   }
 }
 
 // ------------------------------------------------------------------ host ----
-struct AttendPlan { int nt, G, smem; size_t slice_bytes; };
+struct AttendPlan { int nt, cols, G; size_t slice_bytes; };
 
 static AttendPlan plan_attend(int64_t max_new, int64_t group, int dw, int x_dtype) {
   AttendPlan pl;
   const int64_t rows = max_new * group;
-  pl.nt = (rows <= 8 || dw == 256 || x_dtype == JGQ_F32) ? 1 : 2;
-  const int nc = 8 * pl.nt;
-  pl.smem = KA_WARPS * nc * (dw + 2) * (int)sizeof(float);
-  pl.G = std::min(KA_TICKETS, 3 * sm_count());
+  const bool one = dw == 256 || x_dtype == JGQ_F32;    // more accumulators than eight rows' do not fit the registers
+  pl.cols = rows > (one ? 8 : 16);
+  pl.nt = one || rows <= (pl.cols ? 32 : 8) ? 1 : 2;
+  const int nc = 8 * pl.nt * (pl.cols ? KA_WARPS : 1);
+  pl.G = std::min(KA_TICKETS, attend_ctas(dw, pl.nt, x_dtype == JGQ_F32, pl.cols != 0) * sm_count());
   pl.slice_bytes = align_up((size_t)pl.G * 2 * nc * (dw + 2) * sizeof(float), 256);
   return pl;
 }
 
-template <typename XT, int DW, int NT>
+template <typename XT, int DW, int NT, bool COLS>
 static int launch_attend_inst(const AttendPlan& pl, const AttendParams& p, cudaStream_t s) {
-  auto kern = kv_attend_kernel<XT, DW, NT>;
+  auto kern = kv_attend_kernel<XT, DW, NT, COLS>;
+  constexpr int smem = attend_smem(DW, COLS);
   struct AttrTag {};
-  const int arc = once_per_device<AttrTag>([&]() { return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem); });
+  const int arc = once_per_device<AttrTag>([&]() {
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaGetLastError();
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
   if (arc != 0) return fail(JGQ_ERR_CUDA, "kv_attend: cannot raise the dynamic shared memory limit");
-  kern<<<(unsigned)pl.G, KA_THREADS, pl.smem, s>>>(p);
+  kern<<<(unsigned)pl.G, KA_THREADS, smem, s>>>(p);
   return check_launch("kv_attend");
+}
+
+template <typename XT, int DW>
+static int launch_attend_width(const AttendPlan& pl, const AttendParams& p, cudaStream_t s) {
+  if constexpr (!std::is_same<XT, float>::value && DW <= 128) {
+    if (pl.nt == 2) return pl.cols ? launch_attend_inst<XT, DW, 2, true>(pl, p, s) : launch_attend_inst<XT, DW, 2, false>(pl, p, s);
+  }
+  return pl.cols ? launch_attend_inst<XT, DW, 1, true>(pl, p, s) : launch_attend_inst<XT, DW, 1, false>(pl, p, s);
 }
 
 template <typename XT>
 static int launch_attend(const AttendPlan& pl, const AttendParams& p, int dw, cudaStream_t s) {
-  constexpr bool F32 = std::is_same<XT, float>::value;
-  if (dw == 64) {
-    if constexpr (!F32) { if (pl.nt == 2) return launch_attend_inst<XT, 64, 2>(pl, p, s); }
-    return launch_attend_inst<XT, 64, 1>(pl, p, s);
-  }
-  if (dw == 128) {
-    if constexpr (!F32) { if (pl.nt == 2) return launch_attend_inst<XT, 128, 2>(pl, p, s); }
-    return launch_attend_inst<XT, 128, 1>(pl, p, s);
-  }
-  return launch_attend_inst<XT, 256, 1>(pl, p, s);
+  if (dw == 64) return launch_attend_width<XT, 64>(pl, p, s);
+  if (dw == 128) return launch_attend_width<XT, 128>(pl, p, s);
+  return launch_attend_width<XT, 256>(pl, p, s);
 }
 
 }  // namespace jgq
@@ -515,6 +863,7 @@ extern "C" int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride,
   p.T = (int)tokens; p.B = (int)requests; p.W = (int)table_width; p.Hq = (int)q_heads; p.Hkv = (int)kv_heads;
   p.group = (int)(q_heads / kv_heads); p.D = (int)head_dim; p.P = page_size; p.pages = (int)pages;
   p.vec_q = aligned(q, 16) && q_token_stride * xb % 16 == 0 && q_head_stride * xb % 16 == 0;
+  p.vec_o = head_dim % 4 == 0 && aligned(out, 4 * xb);
   p.zero_rest = (flags & JGQ_KV_ZERO_REST) != 0;
   p.G = pl.G;
   p.scale = scale * 1.4426950408889634f;
