@@ -29,10 +29,10 @@ Step.__doc__ = """What `PageTable.reserve` returns: slots (int64) and positions 
 last one; cu_seqlens (int32, requests + 1), the requests' first rows; lengths (int32) with the added tokens."""
 
 
-def _cuda(t, name, device=None):
+def _cuda(t, name, device):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f'{name} must be a CUDA tensor')
-    if device is not None and t.device != device:
+    if t.get_device() != device.index:
         raise ValueError(f'{name} is on {t.device}, not on {device}')
     return t
 
@@ -55,6 +55,23 @@ def _device_of(device):
 
 def _raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _Here:
+    """`with _here(device)`: the device is current inside; nothing to do where it is already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _here(device):
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def stored_width(head_dim):
@@ -100,8 +117,8 @@ class PageTable:
             raise ValueError('max_tokens must not be negative')
         slots = torch.empty(max_tokens, dtype=torch.int64, device=d)
         small = torch.empty(max_tokens + 2 * n + 1, dtype=torch.int32, device=d)
-        positions, cu, out = small[:max_tokens], small[max_tokens:max_tokens + n + 1], small[max_tokens + n + 1:]
-        with torch.cuda.device(d):
+        positions, cu, out = small.split_with_sizes((max_tokens, n + 1, n))
+        with _here(d):
             check(lib.jgq_kv_reserve(self.block_table.data_ptr(), self.block_table.stride(0), self.max_pages, self.held.data_ptr(),
                                      self.free.data_ptr(), self.free_count.data_ptr(), self.num_pages, self.page_size,
                                      lengths.data_ptr(), added.data_ptr(), _ptr(finished), n, _ptr(slots), _ptr(positions), max_tokens,
@@ -141,6 +158,7 @@ class KVCache:
         self.num_pages, self.kv_heads, self.head_dim, self.page_size = int(num_pages), int(kv_heads), int(head_dim), int(page_size)
         self.k = torch.full((num_pages, kv_heads, page_size, w), 128, dtype=torch.uint8, device=d)
         self.v = torch.full((num_pages, kv_heads, page_size // 64, w, 64), 128, dtype=torch.uint8, device=d)
+        self._ws_bytes = {}          # workspace bytes of `attend`, a function of the sizes and the device
         self.k_scale = torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=d)
         self.v_scale = torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=d)
 
@@ -151,9 +169,11 @@ class KVCache:
             raise TypeError(f'{name} must be float32, float16 or bfloat16, not {t.dtype}')
         if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != self.head_dim:
             raise ValueError(f'{name} must have shape (tokens, {"heads" if heads is None else heads}, {self.head_dim}), not {tuple(t.shape)}')
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f'{name} requires a gradient; the cache has none (detach it)')
-        return t.detach() if t.stride(2) == 1 or t.shape[2] == 1 else t.detach().contiguous()
+        if t.requires_grad:
+            if torch.is_grad_enabled():
+                raise ValueError(f'{name} requires a gradient; the cache has none (detach it)')
+            t = t.detach()
+        return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
     def write(self, k, v, slots):
         """Quantizes row t of `k` and `v` (tokens, kv_heads, head_dim) into token slot `slots[t]` (int64; page * page_size +
@@ -166,7 +186,7 @@ class KVCache:
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f'k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ')
         slots = _vector(slots, 'slots', torch.int64, k.shape[0], self.device)
-        with torch.cuda.device(self.device):
+        with _here(self.device):
             check(lib.jgq_kv_write(_ptr(k), _ptr(v), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(slots), k.shape[0],
                                    self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                                    self.num_pages, self.page_size, self.kv_heads, self.head_dim, _raw_stream(self.device)))
@@ -179,7 +199,7 @@ class KVCache:
         pages = _vector(pages, 'pages', torch.int64, None, self.device)
         shape = (pages.shape[0], self.kv_heads, self.page_size, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
+        with _here(self.device):
             check(lib.jgq_kv_read(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages,
                                   self.page_size, self.kv_heads, self.head_dim, _ptr(pages), pages.shape[0], _ptr(k), _ptr(v), _DT[dtype],
                                   _raw_stream(self.device)))
@@ -221,8 +241,13 @@ class KVCache:
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
                 raise ValueError(f'out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}')
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=d) if return_lse else None
-        with torch.cuda.device(d):
-            need = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, _DT[q.dtype])
+        with _here(d):
+            key = (heads, most, q.dtype)
+            need = self._ws_bytes.get(key)
+            if need is None:
+                if len(self._ws_bytes) >= 1024:
+                    self._ws_bytes.clear()
+                need = self._ws_bytes[key] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, _DT[q.dtype])
             ws = _scratch(need, 'kv')
             check(lib.jgq_kv_attend(_ptr(q), _DT[q.dtype], q.stride(0), q.stride(1), _ptr(out), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(),
                                     self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages, self.page_size, _ptr(table),

@@ -89,7 +89,7 @@ def _scratch(nbytes, tag):
     graph and an eager call, ever share one."""
     dev = torch.cuda.current_device()
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    capture = lib.jgq_capture_id(stream) if torch.cuda.is_current_stream_capturing() else 0
+    capture = lib.jgq_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
     if not capture:
         return _workspace(nbytes, zeroed=True, tag=tag)
     key = (dev, stream, tag)

@@ -32,17 +32,19 @@ def _settled(w):
     return seen == w._version
 
 
-_ws_bytes = {}           # (device, M, N, K, transpose_b) -> workspace bytes: a function of the sizes and the device's SM count
+_ws_bytes = {}           # (device, M, N, K, transpose_b, group_size) -> workspace bytes: a function of the sizes and the device's SM count
 
 
-def _workspace_bytes(dev, M, N, K, transpose_b):
+def _workspace_bytes(dev, M, N, K, transpose_b, group_size=None):
     """For the current device, whose index is `dev`."""
-    key = (dev, M, N, K, transpose_b)
+    key = (dev, M, N, K, transpose_b, group_size)
     need = _ws_bytes.get(key)
     if need is None:
         if len(_ws_bytes) >= 4096:
             _ws_bytes.clear()
-        need = _ws_bytes[key] = lib.jgq_w4_matmul_workspace_bytes(M, N, K, int(transpose_b))
+        need = (lib.jgq_w4_matmul_workspace_bytes(M, N, K, int(transpose_b)) if group_size is None else
+                lib.jgq_w4_group_matmul_workspace_bytes(M, N, K, group_size, int(transpose_b)))
+        _ws_bytes[key] = need
     return need
 
 
@@ -69,6 +71,16 @@ def _launch(x, w, zero, scale, transpose_b):
     return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
 
 
+def _enqueue_groups(x, w, zero, scale, out, M, N, K, group_size, transpose_b, dev):
+    need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
+    ws = _scratch(need, 'w4g')
+    flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
+    rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
+                                 out.data_ptr(), M, N, K, group_size, flags, ws.data_ptr(), need, _raw_stream(dev))
+    if rc:
+        check(rc)
+
+
 def _launch_groups(x, w, zero, scale, group_size, transpose_b):
     """The product with a scale and a zero point per group of `group_size` rows of the weights."""
     shape = x.shape
@@ -81,15 +93,15 @@ def _launch_groups(x, w, zero, scale, group_size, transpose_b):
     Kw *= 2
     K2, out_n = (Nw, Kw) if transpose_b else (Kw, Nw)
     assert K == K2, f'Inner dim mismatch: {K} != {K2}'
-    with torch.cuda.device(x.device):
-        out = x.new_empty((M, out_n))
-        if M == 0:
-            return out.reshape(shape[:-1] + (out_n,))
-        need = lib.jgq_w4_group_matmul_workspace_bytes(M, Nw, Kw, group_size, int(transpose_b))
-        ws = _scratch(need, 'w4g')
-        flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
-        check(lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
-                                      out.data_ptr(), M, Nw, Kw, group_size, flags, ws.data_ptr(), need, _raw_stream(x.device.index)))
+    out = x.new_empty((M, out_n))
+    if M == 0:
+        return out.reshape(shape[:-1] + (out_n,))
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            _enqueue_groups(x, w, zero, scale, out, M, Nw, Kw, group_size, transpose_b, dev)
+    else:
+        _enqueue_groups(x, w, zero, scale, out, M, Nw, Kw, group_size, transpose_b, dev)
     return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
 
 
@@ -103,9 +115,10 @@ class _GroupMatmul(torch.autograd.Function):
         return _launch_groups(x, w, zero, scale, group_size, transpose_b)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, y_bar):
         w, zero, scale = ctx.saved_tensors
+        if y_bar.requires_grad and torch.is_grad_enabled():          # the gradient is to be differentiated again
+            return _GroupMatmul.apply(y_bar, w, zero, scale, ctx.group_size, not ctx.transpose_b), None, None, None, None, None
         return _launch_groups(y_bar, w, zero, scale, ctx.group_size, not ctx.transpose_b), None, None, None, None, None
 
 
@@ -166,8 +179,11 @@ def quantized_matmul(x, quantized_matrix, transpose_b=False):
     zero, scale = _on_device(zero), _on_device(scale)
     group_size = getattr(quantized_matrix, 'group_size', None)
     if group_size is not None:
-        _check_groups(w.dim(), 0, 2 * w.shape[0], w.shape[1], group_size, scale, zero)
-        if not (xd.device == w.device == zero.device == scale.device):
+        rows, channels = w.shape
+        want = (-(-2 * rows // group_size), channels)
+        if scale.shape != want or zero.shape != want:
+            _check_groups(2, 0, 2 * rows, channels, group_size, scale, zero)
+        if not (xd.get_device() == w.get_device() == zero.get_device() == scale.get_device()):
             raise ValueError(f'x is on {xd.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
         if _needs_function(xd, zero, scale):
             out = _GroupMatmul.apply(xd, w, zero, scale, group_size, bool(transpose_b))

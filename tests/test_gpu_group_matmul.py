@@ -178,6 +178,17 @@ def test_gradient_agrees_with_differences(G, M):
     assert abs(float(f(1.0) - f(-1.0)) / 2 - float((dx.double() * step.double()).sum())) <= 96 * 2.0 ** -22 * size
 
 
+def test_gradient_of_the_gradient(G):
+    """The product is linear: differentiating its gradient with respect to the incoming one is the product again."""
+    qm, w, size = matrix(G, 128, 64, 32)
+    x = torch.randn((3, 128), device='cuda', requires_grad=True)
+    dy = torch.randn((3, 64), device='cuda', requires_grad=True)
+    dx, = torch.autograd.grad(G.quantized_matmul(x, qm), x, dy, create_graph=True)
+    v = torch.randn((3, 128), device='cuda')
+    again, = torch.autograd.grad(dx, dy, v)
+    check(again, v, w, size, torch.float32)
+
+
 @pytest.mark.parametrize('M', [1, 12, 48])
 def test_two_captured_graphs_do_not_share_a_workspace(G, M):
     """Graphs captured on one stream, replayed on two at once, beside eager calls."""
