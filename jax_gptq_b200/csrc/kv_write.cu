@@ -9,11 +9,12 @@
 // Growing by powers of two keeps what a token loses when its page's scale grows below one step of the final scale,
 // however often it grows: 1/2 + 1/4 + ... of it on top of nothing but the first rounding's half step.
 //
-// HBM-bound: one CTA per run of rows in a page, head and K or V, one pass: a thread keeps 4 tokens x 16 channels in
+// HBM-bound: a CTA takes a run of rows in a page for a head's keys or values after the other, in one pass each: a thread keeps 4 tokens x 16 channels in
 // registers between the maximum and the codes.  Neighbouring threads have neighbouring channels for keys (a row's codes are
 // contiguous) and neighbouring tokens for values (a channel's are); either way a thread's 16 channels fill 32-byte sectors of the
 // rows and its stores complete ones, without shared memory.
-// A CTA looks through `chunk` rows for the runs that begin there: few rows per CTA when there are few rows.
+// A CTA looks through `chunk` rows for the runs that begin there; which rows follow on their predecessors is found once, as a
+// mask, for the chunk and what its last run may reach.  Runs of one row (a decode step) go to a warp each, without a barrier.
 #include "kv_cache.cuh"
 #include <algorithm>
 #include <cstring>
@@ -72,169 +73,298 @@ __device__ __forceinline__ float row_element(const Row16<XT>& r, int i) {      /
   }
 }
 
-// The codes of four elements, in excess 128, as a word.  rne(x / s) with the quotient rounded to fp32 is rne(x * (1 / s)) unless
-// the product comes within 1e-4 of half way between two whole numbers (its error is below 2e-5): those, and what is not
-// finite, are divided.
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float s, float inv) {
-  uint32_t b[4];
-  bool plain = true;
+// The codes of four elements, in excess 128, as a word: rne(x / s) with the quotient rounded to fp32.  x times a reciprocal
+// 2^-21 too small and one as much too large, each rounded to a whole number by adding 1.5 * 2^23 (one fused operation, the sum's
+// low byte is the number): where both give the same, the quotient and its rounding to fp32, which lie between, do too.
+// Otherwise, and where elements are not finite or the reciprocal is not normal (lo = NaN), the elements are divided.
+static __device__ __noinline__ uint32_t encode4_divided(float x0, float x1, float x2, float x3, float s) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t r = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float q = x[i] * inv, t = q + 12582912.f;            // 1.5 * 2^23: the sum's low byte is the rounded q
-    const float off = fabsf(q - (t - 12582912.f));
-    plain = plain && fabsf(q) <= 127.4f && fabsf(off - 0.5f) >= 1e-4f;
-    b[i] = __float_as_uint(t);
+    const float v = x[i] != x[i] ? 0.f : x[i];
+    r |= ((uint32_t)(int)(fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.f), 127.f) + 128.f) & 255u) << (8 * i);
   }
-  if (!plain) {
+  return r;
+}
+// bytes a .. b - 1 of a word
+static __device__ __noinline__ void store_bytes(uint8_t* dst, uint32_t c, int a, int b) {
+  for (int i = a; i < b; ++i) dst[i] = (uint8_t)(c >> (8 * i));
+}
+struct Reciprocal { float s, lo, hi; };
+__device__ __forceinline__ Reciprocal reciprocal(float s, bool finite) {
+  Reciprocal r;
+  r.s = s > 0.f ? s : 1.f;
+  const float inv = __fdiv_rn(1.f, r.s);
+  const bool ok = finite && r.s >= 1.1754943508222875e-38f && inv >= 1.1754943508222875e-38f;
+  r.lo = ok ? inv * 0.99999952316284180f : __int_as_float(0x7fc00000);
+  r.hi = inv * 1.0000004768371582f;
+  return r;
+}
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], const Reciprocal& q) {
+  uint32_t b[4], differ = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = x[i] != x[i] ? 0.f : x[i];
-      b[i] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.f), 127.f);
-    }
+  for (int i = 0; i < 4; ++i) {
+    b[i] = __float_as_uint(fmaf(x[i], q.lo, 12582912.f));
+    differ |= b[i] ^ __float_as_uint(fmaf(x[i], q.hi, 12582912.f));
   }
+  if (differ) return encode4_divided(x[0], x[1], x[2], x[3], q.s);
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) ^ 0x80808080u;
 }
 
+// The largest magnitude among four rows' elements: of their bits, two at a time for 16-bit types.  What is not finite comes out
+// on top; it is then looked for again among the finite ones.
+template <typename XT>
+__device__ __forceinline__ uint32_t top_bits(const Row16<XT>& r, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(XT); ++i) {
+    const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (sizeof(XT) == 4) top = max(top, w[j] & 0x7fffffffu);
+      else asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(w[j] & 0x7fff7fffu));
+    }
+  }
+  return top;
+}
+template <typename XT>
+__device__ __forceinline__ float top_value(uint32_t bits) {            // of the bits of one element, or of two
+  if constexpr (sizeof(XT) == 4) return __uint_as_float(bits);
+  else {
+    const uint16_t b = (uint16_t)max(bits & 0xffffu, bits >> 16);
+    return to_f32<XT>(*reinterpret_cast<const XT*>(&b));
+  }
+}
+
+// scale of a page for rows whose largest magnitude is `top`, and by how many powers of two it has grown
+__device__ __forceinline__ float page_scale(float old, float top, bool first, int& grown) {
+  const float need = __fdiv_rn(top, 127.f);
+  float s = first || !(old > 0.f) ? need : old;
+  grown = 0;
+  while (s < need && grown < 300) { s *= 2.f; ++grown; }
+  return s;
+}
+// the codes of a page, `bytes` of them, rounded to a scale 2^grown times as large
+__device__ __forceinline__ void requantize(uint8_t* base, int bytes, int grown, int thread, int threads) {
+  const float f = __uint_as_float((uint32_t)(127 - min(grown, 30)) << 23);            // from 8 on every code becomes 0
+  auto word = [&](uint32_t v) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) r |= (uint32_t)(__float2int_rn((float)((int)((v >> (8 * b)) & 255u) - 128) * f) + 128) << (8 * b);
+    return r;
+  };
+#pragma unroll 4
+  for (int i = thread; i < bytes / 16; i += threads) {
+    const uint4 w = reinterpret_cast<const uint4*>(base)[i];
+    reinterpret_cast<uint4*>(base)[i] = make_uint4(word(w.x), word(w.y), word(w.z), word(w.w));
+  }
+}
+
 template <typename XT, int DW>
-__global__ void __launch_bounds__(KW_MAX_THREADS) kv_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(KW_MAX_THREADS, sizeof(XT) == 4 ? 1 : 2) kv_write_kernel(const WriteParams p) {
   constexpr int CG = DW / 16;                              // channel groups of a row
+  constexpr int MASK = (KV_TILE + 256) / 32;               // words: a chunk and the longest run behind it
   __shared__ float s_top[KW_MAX_THREADS / 32];
-  __shared__ uint32_t s_begin[2];
-  __shared__ int s_len;
-  const int tid = threadIdx.x, h = blockIdx.y, kv = blockIdx.z, P = p.P, threads = blockDim.x;
+  __shared__ uint32_t s_follows[MASK], s_valid[KV_TILE / 32];
+  const int tid = threadIdx.x, lane = tid & 31, P = p.P, threads = blockDim.x;
+  const int page_shift = P == 64 ? 6 : P == 128 ? 7 : 8;
   const int items = P / 4 * CG;                            // four tokens x 16 channels each
-  const bool vec = (kv ? p.vec[1] : p.vec[0]) != 0;
-  const int64_t ts = kv ? p.token_stride[1] : p.token_stride[0];
-  const XT* x = reinterpret_cast<const XT*>(kv ? p.x[1] : p.x[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]);
-  uint8_t* codes = kv ? p.codes[1] : p.codes[0];
-  float* scales = kv ? p.scale[1] : p.scale[0];
   const int64_t limit = p.pages * P, t0 = (int64_t)blockIdx.x * p.chunk;
 
-  // ---- rows of the chunk that begin a run ----
-  if (tid < 64) {
-    bool begins = false;
-    if (tid < p.chunk && t0 + tid < p.T) {
-      const int64_t slot = p.slots[t0 + tid];
-      begins = slot >= 0 && slot < limit && (slot % P == 0 || t0 + tid == 0 || p.slots[t0 + tid - 1] != slot - 1);
+  // ---- which rows follow on their predecessor in its page ----
+  for (int i = tid; i < MASK * 32; i += threads) {
+    bool follows = false, valid = false;
+    const int64_t t = t0 + i;
+    if (i < p.chunk + P && t < p.T) {
+      const int64_t slot = p.slots[t];
+      valid = slot >= 0 && slot < limit;
+      follows = valid && t > 0 && (slot & (P - 1)) != 0 && p.slots[t - 1] == slot - 1;
     }
-    const uint32_t m = __ballot_sync(0xffffffffu, begins);
-    if ((tid & 31) == 0) s_begin[tid >> 5] = m;
+    const uint32_t f = __ballot_sync(0xffffffffu, follows), v = __ballot_sync(0xffffffffu, valid);
+    if (lane == 0) {
+      s_follows[i >> 5] = f;
+      if (i < KV_TILE) s_valid[i >> 5] = v;
+    }
   }
   __syncthreads();
-  uint64_t todo = s_begin[0] | ((uint64_t)s_begin[1] << 32);
-  while (todo) {
-    const int64_t t = t0 + __ffsll((long long)todo) - 1;
-    todo &= todo - 1;
-    const int64_t slot = p.slots[t], page = slot / P;
-    const int offset = (int)(slot % P);
-    float* scale_at = scales + page * p.H + h;
-    const float old = *scale_at;
-    // ---- the run: rows t .. t + len - 1 ----
-    int len = 1;
-    if (t + 1 < p.T && offset + 1 < P && p.slots[t + 1] == slot + 1) {
-      if (tid == 0) s_len = (int)min((int64_t)(P - offset), p.T - t);
-      __syncthreads();
-      for (int i = 1 + tid; i < P - offset && t + i < p.T; i += threads)
-        if (p.slots[t + i] != slot + i) { atomicMin(&s_len, i); break; }
-      __syncthreads();
-      len = s_len;
+  const uint64_t in_chunk = p.chunk == 64 ? ~0ull : (1ull << p.chunk) - 1;
+  const uint64_t begin = (s_valid[0] | ((uint64_t)s_valid[1] << 32)) & ~(s_follows[0] | ((uint64_t)s_follows[1] << 32)) & in_chunk;
+  const uint64_t next_follows = ((s_follows[0] | ((uint64_t)s_follows[1] << 32)) >> 1) | ((uint64_t)(s_follows[2] & 1u) << 63);
+
+  for (int part = blockIdx.y; part < 2 * p.H; part += gridDim.y) {         // keys, then values, of every head
+    const int h = part >> 1, kv = part & 1;
+    const bool vec = (kv ? p.vec[1] : p.vec[0]) != 0;
+    const int64_t ts = kv ? p.token_stride[1] : p.token_stride[0];
+    const XT* x = reinterpret_cast<const XT*>(kv ? p.x[1] : p.x[0]) + h * (kv ? p.head_stride[1] : p.head_stride[0]);
+    uint8_t* codes = kv ? p.codes[1] : p.codes[0];
+    float* scales = kv ? p.scale[1] : p.scale[0];
+
+    // ---- single rows, a warp each ----
+    uint64_t todo = begin & ~next_follows;
+    for (int n = 0; todo; ++n) {
+      const int i = __ffsll((long long)todo) - 1;
+      todo &= todo - 1;
+      if (n % (threads / 32) != tid / 32) continue;
+      constexpr int CPL = DW / 32;                           // channels per lane
+      const XT* row = x + (t0 + i) * ts;
+      const int d0 = lane * CPL;
+      float f[CPL], top = 0.f;
+      if (vec && d0 + CPL <= p.D) {
+        using V = typename std::conditional<sizeof(XT) * CPL == 32, uint4, typename std::conditional<sizeof(XT) * CPL == 16, uint4,
+                  typename std::conditional<sizeof(XT) * CPL == 8, uint2, uint32_t>::type>::type>::type;
+        __align__(16) XT e[CPL];
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(XT) * CPL / sizeof(V)); ++j) reinterpret_cast<V*>(e)[j] = reinterpret_cast<const V*>(row + d0)[j];
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) f[j] = to_f32<XT>(e[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) f[j] = d0 + j < p.D ? to_f32<XT>(row[d0 + j]) : 0.f;
+      }
+      const int64_t slot = p.slots[t0 + i], page = slot >> page_shift;
+      const int offset = (int)slot & (P - 1);
+      float* scale_at = scales + page * p.H + h;
+      const float old = *scale_at;
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        const float a = fabsf(f[j]);
+        if (a <= 3.402823466e38f) top = fmaxf(top, a);
+      }
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      int grown;
+      const float s = page_scale(old, top, offset == 0, grown);
+      uint8_t* base = codes + (page * p.H + h) * (int64_t)P * DW;
+      if (grown > 0) { requantize(base, P * DW, grown, lane, 32); __syncwarp(); }
+      if (lane == 0 && (grown > 0 || s != old)) *scale_at = s;
+      const Reciprocal by = reciprocal(s, false);            // few elements: divided
+#pragma unroll
+      for (int j = 0; j < CPL; j += 4) {
+        const float v[4] = {f[j], f[j + 1], CPL > 2 ? f[CPL > 2 ? j + 2 : 0] : 0.f, CPL > 2 ? f[CPL > 2 ? j + 3 : 0] : 0.f};
+        const uint32_t c = encode4_divided(v[0], v[1], v[2], v[3], by.s);
+        if (kv == 0) {
+          uint8_t* dst = base + offset * DW + d0 + j;
+          if (CPL == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c;
+          else *reinterpret_cast<uint32_t*>(dst) = c;
+        } else {
+          uint8_t* dst = base + (offset / KV_TILE) * DW * KV_TILE + (d0 + j) * KV_TILE + offset % KV_TILE;
+#pragma unroll
+          for (int b = 0; b < (CPL < 4 ? CPL : 4); ++b) dst[b * KV_TILE] = (uint8_t)(c >> (8 * b));
+        }
+      }
     }
 
-    Row16<XT> raw[4];
-    auto place = [&](int item, int& pos, int& d0) {        // first of the item's four positions in the page, and its channel
-      const int quads = P / 4;
-      pos = 4 * (kv ? item % quads : item / CG);
-      d0 = 16 * (kv ? item / quads : item % CG);
-    };
-    auto fetch = [&](int pos, int d0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = pos + i - offset;
-        if (row >= 0 && row < len) load_row16<XT>(raw[i], x + (t + row) * ts + d0, p.D - d0, vec);
-        else
-#pragma unroll
-          for (int j = 0; j < (int)sizeof(XT); ++j) raw[i].v[j] = make_uint4(0, 0, 0, 0);
+    // ---- longer runs, the whole CTA ----
+    todo = begin & next_follows;
+    while (todo) {
+      const int first = __ffsll((long long)todo) - 1;
+      todo &= todo - 1;
+      const int64_t t = t0 + first, slot = p.slots[t], page = slot >> page_shift;
+      const int offset = (int)slot & (P - 1);
+      float* scale_at = scales + page * p.H + h;
+      const float old = *scale_at;
+      int len = 1;                                           // rows t .. t + len - 1
+      for (int i = first + 1; i < MASK * 32;) {
+        const uint32_t rest = ~(s_follows[i >> 5] >> (i & 31));      // the first row that does not follow
+        const int n = rest ? __ffs(rest) - 1 : 32, room = 32 - (i & 31);
+        len += min(n, room);
+        if (n < room) break;
+        i += room;
       }
-    };
-    float top = 0.f;
-    for (int item = tid; item < items; item += threads) {
-      int pos, d0;
-      place(item, pos, d0);
-      if (pos + 4 > offset && pos < offset + len) {
-        fetch(pos, d0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = fabsf(row_element<XT>(raw[i], e));
-            if (a <= 3.402823466e38f) top = fmaxf(top, a);
-          }
-      }
-    }
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((tid & 31) == 0) s_top[tid >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, s_top[w]);
-    const float need = __fdiv_rn(top, 127.f);
-    const bool begins = offset == 0 || !(old > 0.f);
-    float s = begins ? need : old;
-    int grown = 0;
-    while (s < need && grown < 300) { s *= 2.f; ++grown; }
-    uint8_t* base = codes + (page * p.H + h) * (int64_t)P * DW;
-    if (grown > 0) {
-      const float f = __uint_as_float((uint32_t)(127 - min(grown, 30)) << 23);        // 2^-grown; from 8 on every code becomes 0
-      for (int i = tid; i < P * DW / 16; i += threads) {
-        uint4 w = reinterpret_cast<const uint4*>(base)[i];
-        auto requantized = [&](uint32_t v) {
-          uint32_t r = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b) r |= (uint32_t)(__float2int_rn((float)((int)((v >> (8 * b)) & 255u) - 128) * f) + 128) << (8 * b);
-          return r;
-        };
-        reinterpret_cast<uint4*>(base)[i] = make_uint4(requantized(w.x), requantized(w.y), requantized(w.z), requantized(w.w));
-      }
-      __syncthreads();
-    }
-    if (tid == 0) *scale_at = s;
-    const float by = s > 0.f ? s : 1.f, inv = __fdiv_rn(1.f, by);
+      len = min(len, P - offset);
 
-    for (int item = tid; item < items; item += threads) {
-      int pos, d0;
-      place(item, pos, d0);
-      if (pos + 4 <= offset || pos >= offset + len) continue;
-      if (items > threads) fetch(pos, d0);                 // one item per thread is still there
-      if (kv == 0) {
+      Row16<XT> raw[4];
+      auto place = [&](int item, int& pos, int& d0) {        // first of the item's four positions in the page, and its channel
+        const int quads = P / 4;
+        pos = 4 * (kv ? item & (quads - 1) : item / CG);
+        d0 = 16 * (kv ? item >> (page_shift - 2) : item % CG);
+      };
+      auto fetch = [&](int pos, int d0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = pos + i - offset;
-          if (row >= 0 && row < len) {
-            uint32_t c[4];
+          if (row >= 0 && row < len) load_row16<XT>(raw[i], x + (t + row) * ts + d0, p.D - d0, vec);
+          else
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float v[4] = {row_element<XT>(raw[i], 4 * j), row_element<XT>(raw[i], 4 * j + 1), row_element<XT>(raw[i], 4 * j + 2), row_element<XT>(raw[i], 4 * j + 3)};
-              c[j] = encode4(v, by, inv);
-            }
-            *reinterpret_cast<uint4*>(base + (pos + i) * DW + d0) = make_uint4(c[0], c[1], c[2], c[3]);
-          }
+            for (int j = 0; j < (int)sizeof(XT); ++j) raw[i].v[j] = make_uint4(0, 0, 0, 0);
         }
-      } else {
-        uint8_t* dst = base + (pos / KV_TILE) * DW * KV_TILE + d0 * KV_TILE + pos % KV_TILE;
-        const bool all = pos >= offset && pos + 4 <= offset + len;
+      };
+      uint32_t bits = 0;
+      for (int item = tid; item < items; item += threads) {
+        int pos, d0;
+        place(item, pos, d0);
+        if (pos + 4 > offset && pos < offset + len) {
+          fetch(pos, d0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float v[4] = {row_element<XT>(raw[0], e), row_element<XT>(raw[1], e), row_element<XT>(raw[2], e), row_element<XT>(raw[3], e)};
-          const uint32_t c = encode4(v, by, inv);
-          if (all) {
-            *reinterpret_cast<uint32_t*>(dst + e * KV_TILE) = c;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (pos + i >= offset && pos + i < offset + len) dst[e * KV_TILE + i] = (uint8_t)(c >> (8 * i));
+          for (int i = 0; i < 4; ++i) bits = top_bits<XT>(raw[i], bits);
+        }
+      }
+      float top = top_value<XT>(bits);
+      bool finite = top <= 3.402823466e38f;
+      if (!__syncthreads_and(finite)) {
+        top = 0.f;
+        finite = false;
+#pragma unroll 1
+        for (int item = tid; item < items; item += threads) {
+          int pos, d0;
+          place(item, pos, d0);
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const int row = pos + i - offset;
+            if (row < 0 || row >= len) continue;
+            for (int e = 0; e < 16 && d0 + e < p.D; ++e) {
+              const float a = fabsf(to_f32<XT>(x[(t + row) * ts + d0 + e]));
+              if (a <= 3.402823466e38f) top = fmaxf(top, a);
+            }
           }
         }
       }
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) s_top[tid >> 5] = top;
+      __syncthreads();
+      for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, s_top[w]);
+      int grown;
+      const float s = page_scale(old, top, offset == 0, grown);
+      uint8_t* base = codes + (page * p.H + h) * (int64_t)P * DW;
+      if (grown > 0) {
+        requantize(base, P * DW, grown, tid, threads);
+        __syncthreads();
+      }
+      if (tid == 0) *scale_at = s;
+      const Reciprocal by = reciprocal(s, finite);
+
+      for (int item = tid; item < items; item += threads) {
+        int pos, d0;
+        place(item, pos, d0);
+        if (pos + 4 <= offset || pos >= offset + len) continue;
+        if (items > threads) fetch(pos, d0);                 // one item per thread is still there
+        if (kv == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = pos + i - offset;
+            if (row >= 0 && row < len) {
+              uint32_t c[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float v[4] = {row_element<XT>(raw[i], 4 * j), row_element<XT>(raw[i], 4 * j + 1), row_element<XT>(raw[i], 4 * j + 2), row_element<XT>(raw[i], 4 * j + 3)};
+                c[j] = encode4(v, by);
+              }
+              *reinterpret_cast<uint4*>(base + (pos + i) * DW + d0) = make_uint4(c[0], c[1], c[2], c[3]);
+            }
+          }
+        } else {
+          uint8_t* dst = base + (pos / KV_TILE) * DW * KV_TILE + d0 * KV_TILE + pos % KV_TILE;
+          const bool all = pos >= offset && pos + 4 <= offset + len;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float v[4] = {row_element<XT>(raw[0], e), row_element<XT>(raw[1], e), row_element<XT>(raw[2], e), row_element<XT>(raw[3], e)};
+            const uint32_t c = encode4(v, by);
+            if (all) *reinterpret_cast<uint32_t*>(dst + e * KV_TILE) = c;
+            else     store_bytes(dst + e * KV_TILE, c, max(0, offset - pos), min(4, offset + len - pos));
+          }
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -297,7 +427,9 @@ __global__ void __launch_bounds__(DW) kv_read_kernel(const ReadParams p) {
 
 template <typename XT>
 static int launch_write(const WriteParams& p, int dw, cudaStream_t s) {
-  const dim3 grid((unsigned)cdiv(p.T, p.chunk), (unsigned)p.H, 2);
+  // a CTA takes several heads where that leaves some waves of CTAs: what a chunk's rows are is then found once for them
+  const int64_t x = cdiv(p.T, p.chunk);
+  const dim3 grid((unsigned)x, (unsigned)std::max<int64_t>(1, std::min<int64_t>(2 * p.H, 32 * (int64_t)sm_count() / x)));
   const int threads = std::min(KW_MAX_THREADS, dw * p.P / KV_TILE);
   if (dw == 64)       kv_write_kernel<XT, 64><<<grid, threads, 0, s>>>(p);
   else if (dw == 128) kv_write_kernel<XT, 128><<<grid, threads, 0, s>>>(p);
@@ -348,9 +480,9 @@ extern "C" int jgq_kv_write(const void* k_new, const void* v_new, int dtype, int
   p.H = (int)kv_heads; p.D = (int)head_dim; p.P = page_size;
   for (int i = 0; i < 2; ++i)
     p.vec[i] = head_dim % 8 == 0 && aligned(p.x[i], 16) && p.token_stride[i] * xb % 16 == 0 && p.head_stride[i] * xb % 16 == 0;
-  // rows looked through by a CTA: one while that makes no more than some thousand CTAs, up to a tile's 64
-  p.chunk = 1;
-  while (p.chunk < KV_TILE && cdiv(tokens, p.chunk) * kv_heads * 2 > 4096) p.chunk *= 2;
+  // rows looked through by a CTA: two while that makes no more than some thousand CTAs, up to a tile's 64
+  p.chunk = 2;
+  while (p.chunk < KV_TILE && cdiv(tokens, p.chunk) * kv_heads * 2 > 2048) p.chunk *= 2;
   cudaStream_t s = (cudaStream_t)stream;
   const int dw = kv_width(head_dim);
   if (dtype == JGQ_F32) return launch_write<float>(p, dw, s);
