@@ -31,8 +31,7 @@
 // items (its first and its last), so two slices per CTA are all the scratch there is.
 // Where the rows of a sequence make several row tiles, the earlier ones see fewer tokens: tile counts are a linear function
 // rounded down, whose sums have a closed form (floor_sum).
-#include "kv_cache.cuh"
-#include "umma.cuh"
+#include "kv_attend.cuh"
 #include "trace.cuh"
 #include <algorithm>
 #include <cstring>
@@ -45,56 +44,6 @@ JGQ_TRACE_DEFINE(attend, 8 * 1024)
 namespace jgq {
 
 constexpr int KA_WARPS = 4, KA_THREADS = 32 * KA_WARPS;
-constexpr int KA_TICKETS = 4096;                       // int32 tickets at the front of the workspace, zero between launches
-
-struct AttendParams {
-  const void* q; void* out; float* lse;
-  const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
-  const int32_t* table; const int32_t* lengths; const int32_t* cu;
-  int64_t q_token, q_head;     // strides of q in elements
-  int64_t table_stride;
-  int32_t* tickets; float* slices;
-  int T, B, W, Hq, Hkv, group, D, P, pages;
-  int vec_q, vec_o;            // 16-byte loads of q, stores of four channels are legal
-  int zero_rest;               // rows behind the last sequence are zeroed
-  int G;                       // CTAs
-  float scale;                 // of the scores, times log2(e)
-};
-
-__device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 units in the last place; 2^-inf = 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void mma_h(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_h0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // d = a b
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 half2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ uint4 lds16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(umma::smem_u32(bar)) : "memory");
-}
 
 // two codes of a word as f16: as subnormals with their excess, or exact
 template <bool EXACT>
@@ -105,54 +54,6 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int upper) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-__device__ __forceinline__ int attend_cta_of(int64_t idx, int64_t S, int G) {
-  return (int)(((idx + 1) * G + S - 1) / S) - 1;     // the c with c S / G <= idx < (c + 1) S / G
-}
-
-__device__ __forceinline__ int seq_rows(const AttendParams& p, int r) {
-  if (!p.cu) return 1;
-  const int a = max(0, min(p.cu[r], p.T)), b = max(0, min(p.cu[r + 1], p.T));
-  return max(0, b - a);
-}
-__device__ __forceinline__ int seq_len(const AttendParams& p, int r) {
-  return (int)min((int64_t)max(0, p.lengths[r]), (int64_t)p.W * p.P);
-}
-
-// sum over i < n of floor((a i + b) / m); a, b >= 0
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t sum = 0;
-  while (n > 0) {
-    if (a >= m) { sum += n * (n - 1) / 2 * (a / m); a %= m; }
-    if (b >= m) { sum += n * (b / m); b %= m; }
-    const int64_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;                                         // the lattice points below the line, counted along the other axis
-    b = y % m;
-    const int64_t t = a; a = m; m = t;
-  }
-  return sum;
-}
-
-// a sequence's part of the list: row tiles per head, and units of row tile c: floor((a c + b) / m), COST in front and a tile each
-struct SeqWork {
-  int n, L, ct;
-  int64_t m, a, b;
-};
-template <int NC, int COST>
-__device__ __forceinline__ SeqWork seq_work(const AttendParams& p, int r) {
-  SeqWork w;
-  w.n = seq_rows(p, r);
-  w.L = seq_len(p, r);
-  w.ct = (w.n * p.group + NC - 1) / NC;
-  w.m = 1; w.a = 0; w.b = COST + max(1, (w.L + KV_TILE - 1) / KV_TILE);
-  if (w.ct > 1 && w.L >= w.n) {                        // what the last row of row tile c sees, in tokens times group, rounded up
-    w.m = (int64_t)KV_TILE * p.group;
-    w.a = NC;
-    w.b = (int64_t)(w.L - w.n) * p.group + NC + p.group - 1 + w.m - 1 + COST * w.m;
-  }
-  return w;
-}
 
 __host__ __device__ constexpr int attend_unit(int dw) { return dw == 64 ? 4096 : 8192; }      // bytes
 __host__ __device__ constexpr int attend_slots(int dw, bool cols) { return cols ? (dw == 64 ? 8 : 6) : (dw == 64 ? 4 : dw == 128 ? 2 : 3); }   // units per ring
@@ -178,7 +79,6 @@ kv_attend_kernel(const AttendParams p) {
   constexpr int UNIT = attend_unit(DW), NSLOT = attend_slots(DW, COLS);
   constexpr int UPT = 2 * 64 * DW / UNIT, KU = UPT / 2;                // units per tile; of keys
   constexpr int DTU = DT / KU;                         // channel tiles per unit of values
-  constexpr int SLICE = NC * (DW + 2);                 // floats: sums, then (max, sum) per row
   constexpr float UP24 = EXACT ? 1.f : 16777216.f;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint64_t* full_all = reinterpret_cast<uint64_t*>(smem_raw);          // [rings][NSLOT]
@@ -201,53 +101,10 @@ kv_attend_kernel(const AttendParams p) {
     s_abort = 0;
     fence_barrier_init();
   }
-  auto units = [&](int r) {                            // work of a sequence
-    const SeqWork w = seq_work<NC, kPieceCost>(p, r);
-    return w.n > 0 ? (int64_t)p.Hkv * (w.a ? floor_sum(w.ct, w.m, w.a, w.b) : w.ct * w.b) : 0;
-  };
-
-  // ---- this CTA's range ----
-  const int per = (p.B + KA_THREADS - 1) / KA_THREADS;
-  {
-    int64_t sum = 0;
-    for (int r = tid * per; r < min(p.B, (tid + 1) * per); ++r) sum += units(r);
-    int64_t inc = sum;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) s_pre[warp] = inc;
-    __syncthreads();
-    int64_t before = 0;
-    for (int w = 0; w < warp; ++w) before += s_pre[w];
-    __syncthreads();
-    s_pre[tid + 1] = before + inc;
-    if (tid == 0) s_pre[0] = 0;
-    __syncthreads();
-  }
-  const int64_t S = s_pre[KA_THREADS];
-  if (p.zero_rest && p.cu) {                           // rows behind the last sequence
-    const int64_t first = max(0, min(p.cu[p.B], p.T)), count = (p.T - first) * p.Hq * p.D;
-    XT* o = reinterpret_cast<XT*>(p.out) + first * p.Hq * p.D;
-    for (int64_t i = blockIdx.x * (int64_t)KA_THREADS + tid; i < count; i += (int64_t)gridDim.x * KA_THREADS) o[i] = from_f32<XT>(0.f);
-    if (p.lse)
-      for (int64_t i = first * p.Hq + blockIdx.x * (int64_t)KA_THREADS + tid; i < (int64_t)p.T * p.Hq; i += (int64_t)gridDim.x * KA_THREADS) p.lse[i] = -INFINITY;
-  }
-  const int G = (int)min((int64_t)p.G, (S + kPieceCost + KA_WARPS - 1) / (kPieceCost + KA_WARPS));
-  if ((int)blockIdx.x >= G) return;
-  const int64_t idx_begin = (int64_t)blockIdx.x * S / G, idx_end = ((int64_t)blockIdx.x + 1) * S / G;
-  if (s_pre[tid] <= idx_begin && idx_begin < s_pre[tid + 1]) {
-    int64_t at = s_pre[tid];
-    for (int r = tid * per;; ++r) {
-      const int64_t u = units(r);
-      if (idx_begin < at + u) { s_found[0] = r; s_found[1] = at; break; }
-      at += u;
-    }
-  }
   __syncthreads();
-  int r = (int)s_found[0];
-  int64_t seq_at = s_found[1];                         // first unit of the sequence
-
+  attend_zero_rest<XT, KA_THREADS>(p);
+  AttendRange rg = attend_range<NC, kPieceCost, KA_THREADS>(p, kPieceCost + KA_WARPS, s_pre, s_found);
+  if ((int)blockIdx.x >= rg.G) return;
   uint64_t* full = full_all + (COLS ? 0 : warp * NSLOT);
   const uint32_t ring = smem_u32(ring_all) + (COLS ? 0 : warp * NSLOT * UNIT);
   int slot = 0;                                        // of the ring's next unit, and the parity its arrival has
@@ -257,36 +114,10 @@ kv_attend_kernel(const AttendParams p) {
   const int page_shift = p.P == 64 ? 0 : p.P == 128 ? 1 : 2;          // tiles per page
 
   // ---- pieces: the part of one item (sequence, head, row tile) in this range ----
-  for (int64_t idx = idx_begin; idx < idx_end;) {
-    int64_t u = units(r);
-    while (idx >= seq_at + u) { seq_at += u; ++r; u = units(r); }
-    const SeqWork wk = seq_work<NC, kPieceCost>(p, r);
-    const int n = wk.n, L = wk.L;
-    const int64_t per_head = u / p.Hkv;
-    const int h = (int)((idx - seq_at) / per_head);
-    int64_t in_head = (idx - seq_at) - h * per_head;
-    int row_tile, tiles;
-    if (wk.a) {                                        // the row tile by bisection in the sums
-      int lo = 0, hi = wk.ct;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (floor_sum(mid, wk.m, wk.a, wk.b) <= in_head) lo = mid; else hi = mid;
-      }
-      row_tile = lo;
-      in_head -= floor_sum(lo, wk.m, wk.a, wk.b);
-      tiles = (int)((wk.a * lo + wk.b) / wk.m) - kPieceCost;
-    } else {
-      row_tile = (int)(in_head / wk.b);
-      in_head -= row_tile * wk.b;
-      tiles = (int)wk.b - kPieceCost;
-    }
-    const int c0 = row_tile * NC;
-    const int64_t item_at = idx - in_head;
-    const int64_t tile_at = item_at + kPieceCost;
-    const int t_first = (int)max((int64_t)0, idx - tile_at), t_last = (int)max((int64_t)0, min((int64_t)tiles, idx_end - tile_at));
-    if (t_last <= t_first) { idx = idx_end; break; }   // the item's tiles begin behind this range
-    const int row_first = p.cu ? max(0, min(p.cu[r], p.T)) : r;
-    const int rows = min(NC, n * p.group - c0);        // rows of q of this item
+  for (int64_t idx = rg.begin; idx < rg.end;) {
+    const AttendPiece pc = attend_piece<NC, kPieceCost>(p, rg, idx);
+    if (pc.t_last <= pc.t_first) break;                // the item's tiles begin behind this range
+    const int n = pc.n, L = pc.L, h = pc.h, c0 = pc.c0, rows = pc.rows, row_first = pc.row_first, t_first = pc.t_first, t_last = pc.t_last;
     const int w0 = COLS ? 8 * NT * warp : 0;           // this warp's first one
     const int mine = COLS ? max(0, min(8 * NT, rows - w0)) : rows;
     // tokens that the first and the last of this warp's rows see, and the last of the item's
@@ -298,7 +129,7 @@ kv_attend_kernel(const AttendParams p) {
     // ---- the ring: unit i of this piece's tiles ----
     const int t_begin = COLS ? t_first : t_first + warp, t_step = COLS ? 1 : KA_WARPS;
     const int my_tiles = t_begin < t_end ? (t_end - t_begin + t_step - 1) / t_step : 0;
-    const int32_t* row_of_table = p.table + (int64_t)r * p.table_stride;
+    const int32_t* row_of_table = p.table + (int64_t)rg.r * p.table_stride;
     auto page_of = [&](int k) { return k < my_tiles ? row_of_table[(t_begin + k * t_step) >> page_shift] : -1; };
     auto issue = [&](int to, int k, int part, int page) {         // part `part` of tile k, on that page, into a slot; one lane
       const int tile = t_begin + k * t_step;
@@ -567,7 +398,7 @@ kv_attend_kernel(const AttendParams p) {
       page_now = page_1; page_1 = page_2; page_2 = page_3;
       ks = ks_next; vs = vs_next;
     }
-    if (idx == idx_begin) ATRACE(2);
+    if (idx == rg.begin) ATRACE(2);
     ATRACE(4);
     if (!alive) {                                      // a wait ran out: the result says so
 #pragma unroll
@@ -575,37 +406,8 @@ kv_attend_kernel(const AttendParams p) {
     }
 
     // ---- out ----
-    const bool whole = t_first == 0 && t_last == tiles;
-    const int first_c = attend_cta_of(item_at + kPieceCost, S, G), last_c = attend_cta_of(item_at + kPieceCost + tiles - 1, S, G);
-    // where a row of the item goes: the row of (token, head)
-    auto out_row = [&](int col) {
-      const int row = c0 + col, i = p.group == 1 ? row : row / p.group;
-      return (int64_t)(row_first + i) * p.Hq + h * p.group + (row - i * p.group);
-    };
-    auto put_lse = [&](int64_t at, float mx, float den) {
-      if (p.lse) p.lse[at] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
-    };
-    auto finish4 = [&](int col, int d, const float4& sum, float mx, float den) {       // four channels
-      const int64_t at = out_row(col);
-      const float f = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
-      const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
-      XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
-      if (p.vec_o) {
-        if (d < p.D) {
-          __align__(16) XT e[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[i] = from_f32<XT>(v[i]);
-          if (F32) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(e);
-          else     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d + i < p.D) dst[i] = from_f32<XT>(v[i]);
-      }
-      if (d == 0) put_lse(at, mx, den);
-    };
-    float* slice = p.slices + ((int64_t)blockIdx.x * 2 + (idx_begin > item_at + kPieceCost ? 0 : 1)) * SLICE;
+    const bool whole = t_first == 0 && t_last == pc.tiles;
+    float* slice = attend_slice<NC, DW>(p, rg, blockIdx.x, pc);
     if (COLS) {
       // every warp has all of its rows' tokens here
 #pragma unroll
@@ -616,14 +418,14 @@ kv_attend_kernel(const AttendParams p) {
           for (int b = 0; b < 2; ++b) {
             const int c = 8 * nt + 2 * t + b;
             f[b] = l[nt][b] == 0.f ? 0.f : __fdiv_rn(1.f, l[nt][b]);
-            if (g == 0 && c < mine && p.lse) put_lse(out_row(w0 + c), m[nt][b], l[nt][b]);
+            if (g == 0 && c < mine && p.lse) attend_put_lse(p, attend_out_row(p, pc, w0 + c), m[nt][b], l[nt][b]);
           }
           if (F32) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               const int c = 8 * nt + 2 * t + b;
               if (c < mine) {
-                XT* dst = reinterpret_cast<XT*>(p.out) + out_row(w0 + c) * p.D;
+                XT* dst = reinterpret_cast<XT*>(p.out) + attend_out_row(p, pc, w0 + c) * p.D;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -634,7 +436,7 @@ kv_attend_kernel(const AttendParams p) {
           } else {
             // transposed eight by eight: two neighbouring channels of row g per lane
             const int c = 8 * nt + g;
-            XT* dst = reinterpret_cast<XT*>(p.out) + (c < mine ? out_row(w0 + c) * p.D : 0);
+            XT* dst = reinterpret_cast<XT*>(p.out) + (c < mine ? attend_out_row(p, pc, w0 + c) * p.D : 0);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -698,7 +500,7 @@ kv_attend_kernel(const AttendParams p) {
           den = fmaf(ml[w].y, f, den);
         }
         if (whole) {
-          finish4(col, d, sum, mx, den);
+          attend_finish4<XT>(p, pc, col, d, sum, mx, den);
         } else {
           *reinterpret_cast<float4*>(slice + col * DW + d) = sum;
           if (d == 0) *reinterpret_cast<float2*>(slice + NC * DW + 2 * col) = make_float2(mx, den);
@@ -706,63 +508,12 @@ kv_attend_kernel(const AttendParams p) {
       }
     }
     if (!whole) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const int old = atomicAdd(&p.tickets[first_c], 1);
-        s_flag = old == last_c - first_c;
-        if (s_flag) p.tickets[first_c] = 0;            // ready for the next launch
-      }
-      __syncthreads();
-      if (s_flag) {
-        __threadfence();
-        // four channels of JP rows per thread, four slices at a time: 4 JP loads in flight
-        constexpr int JP = COLS ? 4 : (NC * DW / 4 + KA_THREADS - 1) / KA_THREADS, STEP = KA_THREADS * JP;
-        for (int i0 = tid; i0 < rows * (DW / 4); i0 += STEP) {
-          float mx[JP], den[JP];
-          float4 sum[JP];
-#pragma unroll
-          for (int j = 0; j < JP; ++j) { mx[j] = -INFINITY; den[j] = 0.f; sum[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
-          for (int cb = first_c; cb <= last_c; cb += 4) {          // in CTA order
-            float v[4][JP], dv[4][JP];
-            float4 sv[4][JP];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int cc = min(cb + c, last_c);
-              const float* src = p.slices + ((int64_t)cc * 2 + ((int64_t)cc * S / G > item_at + kPieceCost ? 0 : 1)) * SLICE;
-#pragma unroll
-              for (int j = 0; j < JP; ++j) {
-                const int i = min(i0 + j * KA_THREADS, rows * (DW / 4) - 1), col = i / (DW / 4);
-                v[c][j] = __ldcg(src + NC * DW + 2 * col);
-                dv[c][j] = __ldcg(src + NC * DW + 2 * col + 1);
-                sv[c][j] = __ldcg(reinterpret_cast<const float4*>(src) + i);
-              }
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (cb + c <= last_c) {
-#pragma unroll
-                for (int j = 0; j < JP; ++j) {
-                  const float now = fmaxf(mx[j], v[c][j]), ref = now == -INFINITY ? 0.f : now;
-                  const float fo = exp2_fast(mx[j] - ref), fn = exp2_fast(v[c][j] - ref);
-                  sum[j].x = fmaf(sum[j].x, fo, sv[c][j].x * fn); sum[j].y = fmaf(sum[j].y, fo, sv[c][j].y * fn);
-                  sum[j].z = fmaf(sum[j].z, fo, sv[c][j].z * fn); sum[j].w = fmaf(sum[j].w, fo, sv[c][j].w * fn);
-                  den[j] = fmaf(den[j], fo, dv[c][j] * fn);
-                  mx[j] = now;
-                }
-              }
-          }
-#pragma unroll
-          for (int j = 0; j < JP; ++j) {
-            const int i = i0 + j * KA_THREADS, col = i / (DW / 4), d = 4 * (i % (DW / 4));
-            if (i < rows * (DW / 4)) finish4(col, d, sum[j], mx[j], den[j]);
-          }
-        }
-      }
+      const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, NC, DW, KA_THREADS, COLS ? 4 : (NC * DW / 4 + KA_THREADS - 1) / KA_THREADS>(p, rg, pc, first_c, last_c);
     }
-    if (idx == idx_begin) ATRACE(3);
+    if (idx == rg.begin) ATRACE(3);
     __syncthreads();                                   // before the rings are filled again
-    idx = tile_at + t_last;
+    idx = pc.tile_at + t_last;
   }
 
   ATRACE(5);
@@ -775,7 +526,7 @@ kv_attend_kernel(const AttendParams p) {
 }
 
 // ------------------------------------------------------------------ host ----
-struct AttendPlan { int nt, cols, G; size_t slice_bytes; };
+struct AttendPlan { int nt, cols, G; size_t slice_bytes; PromptPlan prompt; };
 
 static AttendPlan plan_attend(int64_t max_new, int64_t group, int dw, int x_dtype) {
   AttendPlan pl;
@@ -786,6 +537,8 @@ static AttendPlan plan_attend(int64_t max_new, int64_t group, int dw, int x_dtyp
   const int nc = 8 * pl.nt * (pl.cols ? KA_WARPS : 1);
   pl.G = std::min(KA_TICKETS, attend_ctas(dw, pl.nt, x_dtype == JGQ_F32, pl.cols != 0) * sm_count());
   pl.slice_bytes = align_up((size_t)pl.G * 2 * nc * (dw + 2) * sizeof(float), 256);
+  pl.prompt = plan_kv_prompt(rows, dw, x_dtype);
+  if (pl.prompt.use) pl.slice_bytes = pl.prompt.slice_bytes;
   return pl;
 }
 
@@ -864,10 +617,12 @@ extern "C" int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride,
   p.group = (int)(q_heads / kv_heads); p.D = (int)head_dim; p.P = page_size; p.pages = (int)pages;
   p.vec_q = aligned(q, 16) && q_token_stride * xb % 16 == 0 && q_head_stride * xb % 16 == 0;
   p.vec_o = head_dim % 4 == 0 && aligned(out, 4 * xb);
+  p.vec_o8 = head_dim % 8 == 0 && aligned(out, 16);
   p.zero_rest = (flags & JGQ_KV_ZERO_REST) != 0;
-  p.G = pl.G;
+  p.G = pl.prompt.use ? pl.prompt.G : pl.G;
   p.scale = scale * 1.4426950408889634f;
   cudaStream_t s = (cudaStream_t)stream;
+  if (pl.prompt.use) return launch_kv_prompt(pl.prompt, p, dw, q_dtype, s);
   if (q_dtype == JGQ_F32) return launch_attend<float>(pl, p, dw, s);
   if (q_dtype == JGQ_F16) return launch_attend<__half>(pl, p, dw, s);
   return launch_attend<__nv_bfloat16>(pl, p, dw, s);

@@ -1,0 +1,316 @@
+// What the attention kernels over the paged cache share: parameters, the cut of the work, small device helpers.
+#pragma once
+#include "kv_cache.cuh"
+#include "umma.cuh"
+#include <type_traits>
+
+namespace jgq {
+
+constexpr int KA_TICKETS = 4096;                       // int32 tickets at the front of the workspace, zero between launches
+
+struct AttendParams {
+  const void* q; void* out; float* lse;
+  const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
+  const int32_t* table; const int32_t* lengths; const int32_t* cu;
+  int64_t q_token, q_head;     // strides of q in elements
+  int64_t table_stride;
+  int32_t* tickets; float* slices;
+  int T, B, W, Hq, Hkv, group, D, P, pages;
+  int vec_q, vec_o, vec_o8;    // 16-byte loads of q, stores of four and of eight channels are legal
+  int zero_rest;               // rows behind the last sequence are zeroed
+  int G;                       // CTAs
+  float scale;                 // of the scores, times log2(e)
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 units in the last place; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_h(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_h0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // d = a b
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(umma::smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ int attend_cta_of(int64_t idx, int64_t S, int G) {
+  return (int)(((idx + 1) * G + S - 1) / S) - 1;     // the c with c S / G <= idx < (c + 1) S / G
+}
+
+__device__ __forceinline__ int seq_rows(const AttendParams& p, int r) {
+  if (!p.cu) return 1;
+  const int a = max(0, min(p.cu[r], p.T)), b = max(0, min(p.cu[r + 1], p.T));
+  return max(0, b - a);
+}
+__device__ __forceinline__ int seq_len(const AttendParams& p, int r) {
+  return (int)min((int64_t)max(0, p.lengths[r]), (int64_t)p.W * p.P);
+}
+
+// sum over i < n of floor((a i + b) / m); a, b >= 0
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t sum = 0;
+  while (n > 0) {
+    if (a >= m) { sum += n * (n - 1) / 2 * (a / m); a %= m; }
+    if (b >= m) { sum += n * (b / m); b %= m; }
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;                                         // the lattice points below the line, counted along the other axis
+    b = y % m;
+    const int64_t t = a; a = m; m = t;
+  }
+  return sum;
+}
+
+// a sequence's part of the list: row tiles per head, and units of row tile c: floor((a c + b) / m), COST in front and a tile each
+struct SeqWork {
+  int n, L, ct;
+  int64_t m, a, b;
+};
+template <int NC, int COST>
+__device__ __forceinline__ SeqWork seq_work(const AttendParams& p, int r) {
+  SeqWork w;
+  w.n = seq_rows(p, r);
+  w.L = seq_len(p, r);
+  w.ct = (w.n * p.group + NC - 1) / NC;
+  w.m = 1; w.a = 0; w.b = COST + max(1, (w.L + KV_TILE - 1) / KV_TILE);
+  if (w.ct > 1 && w.L >= w.n) {                        // what the last row of row tile c sees, in tokens times group, rounded up
+    w.m = (int64_t)KV_TILE * p.group;
+    w.a = NC;
+    w.b = (int64_t)(w.L - w.n) * p.group + NC + p.group - 1 + w.m - 1 + COST * w.m;
+  }
+  return w;
+}
+
+template <int NC, int COST>
+__device__ __forceinline__ int64_t seq_units(const AttendParams& p, int r) {
+  const SeqWork w = seq_work<NC, COST>(p, r);
+  return w.n > 0 ? (int64_t)p.Hkv * (w.a ? floor_sum(w.ct, w.m, w.a, w.b) : w.ct * w.b) : 0;
+}
+
+// The list of all units cut into equal contiguous ranges, one per CTA, `least` units at least.
+struct AttendRange {
+  int64_t S, begin, end;       // units in all, this CTA's
+  int G;                       // CTAs that have a range; this one if blockIdx.x < G
+  int r;                       // the sequence `begin` lies in, and its first unit
+  int64_t seq_at;
+};
+// Every thread sums up a run of consecutive sequences; s_pre: THREADS + 1 words, s_found: 2.
+template <int NC, int COST, int THREADS>
+__device__ __forceinline__ AttendRange attend_range(const AttendParams& p, int least, int64_t* s_pre, int64_t* s_found) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (p.B + THREADS - 1) / THREADS;
+  AttendRange g;
+  int64_t sum = 0;
+  for (int r = tid * per; r < min(p.B, (tid + 1) * per); ++r) sum += seq_units<NC, COST>(p, r);
+  int64_t inc = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) s_pre[warp] = inc;
+  __syncthreads();
+  int64_t before = 0;
+  for (int w = 0; w < warp; ++w) before += s_pre[w];
+  __syncthreads();
+  s_pre[tid + 1] = before + inc;
+  if (tid == 0) s_pre[0] = 0;
+  __syncthreads();
+  g.S = s_pre[THREADS];
+  g.G = (int)min((int64_t)p.G, (g.S + least - 1) / least);
+  g.begin = g.end = g.seq_at = 0;
+  g.r = 0;
+  if ((int)blockIdx.x >= g.G) return g;
+  g.begin = (int64_t)blockIdx.x * g.S / g.G;
+  g.end = ((int64_t)blockIdx.x + 1) * g.S / g.G;
+  if (s_pre[tid] <= g.begin && g.begin < s_pre[tid + 1]) {
+    int64_t at = s_pre[tid];
+    for (int r = tid * per;; ++r) {
+      const int64_t u = seq_units<NC, COST>(p, r);
+      if (g.begin < at + u) { s_found[0] = r; s_found[1] = at; break; }
+      at += u;
+    }
+  }
+  __syncthreads();
+  g.r = (int)s_found[0];
+  g.seq_at = s_found[1];
+  return g;
+}
+
+// The piece of the item (sequence, kv head, NC rows of q) at unit idx of a range.
+struct AttendPiece {
+  int n, L, h, c0, rows;       // rows of the sequence, tokens, kv head, first row of q, rows of q
+  int row_first;               // the sequence's first row among all
+  int t_first, t_last, tiles;  // tiles of the piece, and of the item
+  int64_t tile_at;             // unit of the item's tile 0
+};
+template <int NC, int COST>
+__device__ __forceinline__ AttendPiece attend_piece(const AttendParams& p, AttendRange& g, int64_t idx) {
+  AttendPiece e;
+  int64_t u = seq_units<NC, COST>(p, g.r);
+  while (idx >= g.seq_at + u) { g.seq_at += u; ++g.r; u = seq_units<NC, COST>(p, g.r); }
+  const SeqWork wk = seq_work<NC, COST>(p, g.r);
+  const int64_t per_head = u / p.Hkv;
+  e.n = wk.n; e.L = wk.L;
+  e.h = (int)((idx - g.seq_at) / per_head);
+  int64_t in_head = (idx - g.seq_at) - e.h * per_head;
+  int row_tile;
+  if (wk.a) {                                          // the row tile by bisection in the sums
+    int lo = 0, hi = wk.ct;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (floor_sum(mid, wk.m, wk.a, wk.b) <= in_head) lo = mid; else hi = mid;
+    }
+    row_tile = lo;
+    in_head -= floor_sum(lo, wk.m, wk.a, wk.b);
+    e.tiles = (int)((wk.a * lo + wk.b) / wk.m) - COST;
+  } else {
+    row_tile = (int)(in_head / wk.b);
+    in_head -= row_tile * wk.b;
+    e.tiles = (int)wk.b - COST;
+  }
+  e.c0 = row_tile * NC;
+  e.rows = min(NC, e.n * p.group - e.c0);
+  e.row_first = p.cu ? max(0, min(p.cu[g.r], p.T)) : g.r;
+  e.tile_at = idx - in_head + COST;
+  e.t_first = (int)max((int64_t)0, idx - e.tile_at);
+  e.t_last = (int)max((int64_t)0, min((int64_t)e.tiles, g.end - e.tile_at));
+  return e;
+}
+
+// rows of q behind the last sequence become zero
+template <typename XT, int THREADS>
+__device__ __forceinline__ void attend_zero_rest(const AttendParams& p) {
+  if (!p.zero_rest || !p.cu) return;
+  const int64_t first = max(0, min(p.cu[p.B], p.T)), count = (p.T - first) * p.Hq * p.D, at = blockIdx.x * (int64_t)THREADS + threadIdx.x;
+  XT* o = reinterpret_cast<XT*>(p.out) + first * p.Hq * p.D;
+  for (int64_t i = at; i < count; i += (int64_t)gridDim.x * THREADS) o[i] = from_f32<XT>(0.f);
+  if (p.lse)
+    for (int64_t i = first * p.Hq + at; i < (int64_t)p.T * p.Hq; i += (int64_t)gridDim.x * THREADS) p.lse[i] = -INFINITY;
+}
+
+// where row `col` of an item goes: the row of (token, head)
+__device__ __forceinline__ int64_t attend_out_row(const AttendParams& p, const AttendPiece& e, int col) {
+  const int row = e.c0 + col, i = p.group == 1 ? row : row / p.group;
+  return (int64_t)(e.row_first + i) * p.Hq + e.h * p.group + (row - i * p.group);
+}
+__device__ __forceinline__ void attend_put_lse(const AttendParams& p, int64_t at, float mx, float den) {
+  if (p.lse) p.lse[at] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
+}
+// four channels of a row's result
+template <typename XT>
+__device__ __forceinline__ void attend_finish4(const AttendParams& p, const AttendPiece& piece, int col, int d, const float4& sum, float mx, float den) {
+  const int64_t at = attend_out_row(p, piece, col);
+  const float f = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
+  const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+  XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
+  if (p.vec_o) {
+    if (d < p.D) {
+      __align__(16) XT e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = from_f32<XT>(v[i]);
+      if constexpr (sizeof(XT) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(e);
+      else                           *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < p.D) dst[i] = from_f32<XT>(v[i]);
+  }
+  if (d == 0) attend_put_lse(p, at, mx, den);
+}
+
+// A CTA shares at most two items, its first (the one its range begins inside of) and its last: slice 0 and slice 1.
+// A slice holds the sums [NC][DW] relative to the row's maximum, then (maximum, sum of exponentials) per row.
+template <int NC, int DW>
+__device__ __forceinline__ float* attend_slice(const AttendParams& p, const AttendRange& g, int cta, const AttendPiece& e) {
+  return p.slices + ((int64_t)cta * 2 + ((int64_t)cta * g.S / g.G > e.tile_at ? 0 : 1)) * (NC * (DW + 2));
+}
+// After a CTA's slice of an item is written (all threads): true in the CTA that is the last one; the tickets are left zero.
+__device__ __forceinline__ bool attend_last(const AttendParams& p, int first_c, int last_c, int* s_flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int old = atomicAdd(&p.tickets[first_c], 1);
+    *s_flag = old == last_c - first_c;
+    if (*s_flag) p.tickets[first_c] = 0;               // ready for the next launch
+  }
+  __syncthreads();
+  const bool last = *s_flag != 0;
+  if (last) __threadfence();
+  return last;
+}
+// The slices of an item added in CTA order: four channels of JP rows per thread, four slices at a time: 4 JP loads in flight.
+template <typename XT, int NC, int DW, int THREADS, int JP>
+__device__ __forceinline__ void attend_join(const AttendParams& p, const AttendRange& g, const AttendPiece& e, int first_c, int last_c) {
+  const int count = e.rows * (DW / 4);
+  for (int i0 = threadIdx.x; i0 < count; i0 += THREADS * JP) {
+    float mx[JP], den[JP];
+    float4 sum[JP];
+#pragma unroll
+    for (int j = 0; j < JP; ++j) { mx[j] = -INFINITY; den[j] = 0.f; sum[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    for (int cb = first_c; cb <= last_c; cb += 4) {
+      float v[4][JP], dv[4][JP];
+      float4 sv[4][JP];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float* src = attend_slice<NC, DW>(p, g, min(cb + c, last_c), e);
+#pragma unroll
+        for (int j = 0; j < JP; ++j) {
+          const int i = min(i0 + j * THREADS, count - 1), col = i / (DW / 4);
+          v[c][j] = __ldcg(src + NC * DW + 2 * col);
+          dv[c][j] = __ldcg(src + NC * DW + 2 * col + 1);
+          sv[c][j] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (cb + c <= last_c) {
+#pragma unroll
+          for (int j = 0; j < JP; ++j) {
+            const float now = fmaxf(mx[j], v[c][j]), ref = now == -INFINITY ? 0.f : now;
+            const float fo = exp2_fast(mx[j] - ref), fn = exp2_fast(v[c][j] - ref);
+            sum[j].x = fmaf(sum[j].x, fo, sv[c][j].x * fn); sum[j].y = fmaf(sum[j].y, fo, sv[c][j].y * fn);
+            sum[j].z = fmaf(sum[j].z, fo, sv[c][j].z * fn); sum[j].w = fmaf(sum[j].w, fo, sv[c][j].w * fn);
+            den[j] = fmaf(den[j], fo, dv[c][j] * fn);
+            mx[j] = now;
+          }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < JP; ++j) {
+      const int i = i0 + j * THREADS;
+      if (i < count) attend_finish4<XT>(p, e, i / (DW / 4), 4 * (i % (DW / 4)), sum[j], mx[j], den[j]);
+    }
+  }
+}
+
+// the prompt kernel (kv_prompt.cu): 128 rows of q per item, 16-bit types, rows of 64 or 128 channels
+struct PromptPlan { int use, G; size_t slice_bytes; };
+PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype);
+int launch_kv_prompt(const PromptPlan& pl, const AttendParams& p, int dw, int q_dtype, cudaStream_t s);
+
+}  // namespace jgq

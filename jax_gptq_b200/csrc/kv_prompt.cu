@@ -1,0 +1,468 @@
+// Attention over the paged 8-bit cache for many rows per sequence (prompts and chunks of them): tcgen05.
+//
+// An item is 128 rows of q (tokens x heads of one kv head's group) of a sequence and kv head; its tiles are 64 tokens.
+//   S = Q K^T     M = 128 rows, N = 64 tokens:  Q and the tile's keys in shared memory, S in tensor memory (two buffers)
+//   P             softmax warps read S (one row per thread), write p as f16 over it
+//   O += P V      M = 128 rows, N = DW channels: P out of tensor memory, the tile's values [channel][token] in shared memory
+// The codes become f16 whole numbers (exact); q is f16 after a power of two per row (exact for f16, and for bf16 down to
+// 2^-24 of the row's largest element).  Scales meet fp32 numbers: the keys' in the scores, the values' in the exponent,
+//   p' = 2^(score - reference + log2(v_scale 2^-w)),
+// so that p' is rounded once; w follows the exponent of v_scale (kept while v_scale stays below 2^(w + 5)).  The row's reference is
+// raised only when a score passes it by 8 (p' then stays below 2^13), O is rescaled then, by the row's thread.
+// The sum of exponentials is that of p' before its rounding, divided by v_scale 2^-w.
+//
+// Per tile and CTA: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  Two CTAs
+// share an SM: while one's softmax warps work, the other's products run.
+//
+// Roles (256 threads): warps 0-3 softmax and output, warp 4 bulk copies of the raw codes (ring of four units), warp 5 issues
+// the MMAs, warp 6 turns the keys' codes into an operand, warp 7 the values' (128-byte swizzle; [token][64 channels] twice, [channel][64 tokens]).
+// The work is cut into equal ranges as in kv_attend.cu, with the same slices and tickets.  Waits are bounded: a row whose
+// wait ran out becomes NaN.
+#include "kv_attend.cuh"
+#include "trace.cuh"
+#include <algorithm>
+#include <cstring>
+
+namespace jgq {
+
+constexpr int KP_ROWS = 128, KP_THREADS = 256;
+constexpr int KP_COST = 6;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
+constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
+constexpr int KP_TMEM = 256;                           // columns: S and P 2 x 64, O DW
+constexpr float KP_LAZY = 8.f;                         // log2 by which a score may pass its row's reference
+constexpr int KP_LAZY_V = 5;                           // and log2 by which v_scale may pass 2^w
+
+__host__ __device__ constexpr int kp_unit(int dw) { return 64 * dw; }
+__host__ __device__ constexpr int kp_smem(int dw) { return 1024 + 1024 + KP_ROWS * dw * 2 + 2 * 64 * dw * 2 + KP_RAW * kp_unit(dw); }
+
+// D[tmem] (+)= A[tmem] B[smem], f16
+__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// two codes as f16 whole numbers; the values' are masked and signed
+__device__ __forceinline__ uint32_t code_pair_f16(uint32_t w, uint32_t sel) {
+  uint32_t r = __byte_perm(w, 0x64646464u, sel);       // 1024 + byte
+  const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__float2half_rn(1152.f)));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename XT, int DW>
+__global__ void __launch_bounds__(KP_THREADS, 2)
+kv_prompt_kernel(const AttendParams p) {
+  using namespace umma;
+  constexpr int UNIT = kp_unit(DW), KB = DW / 64;      // 64-channel blocks of a row
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base);
+  uint64_t* raw_full = bars, *raw_empty = bars + KP_RAW;
+  uint64_t *k_full = bars + 2 * KP_RAW, *k_empty = k_full + 1, *v_full = k_full + 2, *v_empty = k_full + 3;
+  uint64_t *s_full = k_full + 4, *p_full = s_full + 2, *o_done = p_full + 2;           // two of each, for even and odd tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint8_t* q_smem = base + 1024;                       // [KB][128 rows][128 bytes], swizzled
+  uint8_t* k_smem = q_smem + KP_ROWS * DW * 2;         // [KB][64 tokens][128 bytes]
+  uint8_t* v_smem = k_smem + 64 * DW * 2;              // [DW channels][128 bytes]
+  uint8_t* raw = v_smem + 64 * DW * 2;
+  __shared__ int64_t s_pre[KP_THREADS + 1];
+  __shared__ int64_t s_found[2];
+  __shared__ int s_flag, s_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = &s_abort;
+  if (tid == 0) {
+    for (int i = 0; i < KP_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 1); }
+    mbar_init(k_full, 1); mbar_init(k_empty, 1); mbar_init(v_full, 1); mbar_init(v_empty, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+    s_abort = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  attend_zero_rest<XT, KP_THREADS>(p);
+  AttendRange rg = attend_range<KP_ROWS, KP_COST, KP_THREADS>(p, 2 * KP_COST, s_pre, s_found);
+  if ((int)blockIdx.x >= rg.G) return;
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, KP_TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;
+  const int page_shift = p.P == 64 ? 0 : p.P == 128 ? 1 : 2;
+  uint32_t done = 0;                                   // tiles of earlier pieces: every role's barriers count on from them
+  bool ok = true;
+
+  for (int64_t idx = rg.begin; idx < rg.end;) {
+    const AttendPiece pc = attend_piece<KP_ROWS, KP_COST>(p, rg, idx);
+    if (pc.t_last <= pc.t_first) break;                // the item's tiles begin behind this range
+    const int n = pc.n, L = pc.L, h = pc.h;
+    const int seen_item = max(0, L - n + (pc.c0 + pc.rows - 1) / p.group + 1);
+    const int t_end = min(pc.t_last, (seen_item + KV_TILE - 1) / KV_TILE);
+    const int nt = max(0, t_end - pc.t_first);         // tiles of this piece
+    const int32_t* row_of_table = p.table + (int64_t)rg.r * p.table_stride;
+    auto block_of = [&](int tile, bool& bad) {         // page and head of a tile
+      const int page = row_of_table[tile >> page_shift];
+      bad = page < 0 || page >= p.pages;
+      return (int64_t)(bad ? 0 : page) * p.Hkv + h;
+    };
+
+    // ---- q into shared memory: thread = row, two threads a row ----
+    float q_factor = 0.f;                              // of the scores of row tid (softmax warps)
+    {
+      const int row = tid & 127, half = tid >> 7;      // channels half DW / 2 ..
+      const bool live = row < pc.rows;
+      const int gr = pc.c0 + (live ? row : 0), i = p.group == 1 ? gr : gr / p.group;
+      const XT* src = reinterpret_cast<const XT*>(p.q) + (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head;
+      // the largest element of the whole row, by both threads
+      float big = 0.f;
+      auto load8 = [&](float (&f)[8], int d) {
+        if (live && p.vec_q && d + 8 <= p.D) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src + d);
+          const XT* e = reinterpret_cast<const XT*>(&v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = to_f32<XT>(e[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = (live && d + j < p.D) ? to_f32<XT>(src[d + j]) : 0.f;
+        }
+      };
+#pragma unroll 4
+      for (int d = 0; d < DW; d += 8) {
+        float f[8];
+        load8(f, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(f[j]));
+      }
+      // a power of two brings the row's largest element to [2^13, 2^14): f16 then holds what bf16 says down to 2^-27 of it
+      const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
+      const float up = __uint_as_float((267u - e) << 23), down = __uint_as_float((e - 13u) << 23);
+      const float sign = p.scale < 0.f ? -1.f : 1.f;   // the factor of the scores is positive: a row's maximum is that of its products
+      q_factor = down * fabsf(p.scale);
+#pragma unroll 4
+      for (int d = half * (DW / 2); d < (half + 1) * (DW / 2); d += 8) {
+        float f[8];
+        load8(f, d);
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = half2_bits(f[2 * j] * up * sign, f[2 * j + 1] * up * sign);
+        sts16(smem_u32(q_smem) + (d >> 6) * (KP_ROWS * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+
+    if (warp == 4) {
+      // ===================== raw codes =====================
+      if (lane == 0) {
+        bool bad;
+        int64_t block = nt > 0 ? block_of(pc.t_first, bad) : 0;
+        for (int k = 0; k < nt && ok; ++k) {
+          const int tile = pc.t_first + k;
+          const int64_t next = k + 1 < nt ? block_of(tile + 1, bad) : 0;      // one ahead
+          const int64_t at = ((block << page_shift) + (tile & ((1 << page_shift) - 1))) * (int64_t)UNIT;
+          for (int part = 0; part < 2 && ok; ++part) {
+            const uint32_t u = 2 * (done + k) + part, slot = u % KP_RAW;
+            if (u >= KP_RAW) ok = mbar_wait(&raw_empty[slot], (u / KP_RAW + 1) & 1, abort_flag);
+            if (!ok) break;
+            mbar_expect_tx(&raw_full[slot], UNIT);
+            bulk_load(smem_u32(raw) + slot * UNIT, (part ? p.v : p.k) + at, UNIT, &raw_full[slot]);
+          }
+          block = next;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    } else if (warp == 5) {
+      // ===================== MMAs =====================
+      const uint32_t idesc_s = make_idesc_f16(0, 0, 0, KP_ROWS, 64), idesc_o = make_idesc_f16(0, 0, 0, KP_ROWS, DW);
+      const uint64_t dq = make_desc_sw128(smem_u32(q_smem), 16, 1024), dk = make_desc_sw128(smem_u32(k_smem), 16, 1024);
+      const uint64_t dv = make_desc_sw128(smem_u32(v_smem), 16, 1024);
+      for (int k = 0; k <= nt && ok; ++k) {
+        if (k < nt) {                                  // scores of tile k
+          const uint32_t c = done + k, b = c & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(k_full, c & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int k16 = 0; k16 < 4; ++k16)
+                mma_f16_ss(tmem + 64 * b, dq + (uint32_t)((kb * KP_ROWS * 128 + k16 * 32) >> 4), dk + (uint32_t)((kb * 64 * 128 + k16 * 32) >> 4), idesc_s,
+                           kb > 0 || k16 > 0 ? 1u : 0u);
+            mma_commit(k_empty);
+            mma_commit(&s_full[b]);
+          }
+          __syncwarp();
+        }
+        if (k > 0) {                                   // outputs of tile k - 1
+          const uint32_t c = done + k - 1, b = c & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(v_full, c & 1, abort_flag) && mbar_wait(&p_full[b], (c >> 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k16 = 0; k16 < 4; ++k16)
+              mma_f16_ts(tmem_o, tmem + 64 * b + 8 * k16, dv + (uint32_t)((k16 * 32) >> 4), idesc_o, k > 1 || k16 > 0 ? 1u : 0u);
+            mma_commit(v_empty);
+            mma_commit(&o_done[b]);
+          }
+          __syncwarp();
+        }
+      }
+    } else if (warp >= 6) {
+      // ===================== codes into operands: warp 6 the keys, warp 7 the values =====================
+      const int part = warp - 6;
+      uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
+      for (int k = 0; k < nt && ok; ++k) {
+        const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW;
+        float vs = 1.f;
+        bool bad;
+        if (part) vs = p.v_scale[block_of(pc.t_first + k, bad)];
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[slot], (u / KP_RAW) & 1, abort_flag));
+        if (ok && c > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty, (c + 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        // values of a zero scale are zero, of a negative one negative
+        const uint32_t keep = vs == 0.f ? 0u : 0xffffffffu, flip = vs < 0.f ? 0x80008000u : 0u;
+        const uint32_t from = smem_u32(raw) + slot * UNIT, to = smem_u32(part ? v_smem : k_smem);
+#pragma unroll 4
+        for (int i = lane; i < UNIT / 16; i += 32) {
+          const uint4 v = lds16(from + i * 16);
+          // 16 codes: two 16-byte pieces of the operand
+          const int row = part ? i >> 2 : i / (DW / 16), col = part ? i & 3 : i % (DW / 16);      // row of codes, piece of it
+          const uint32_t at = to + (part ? 0 : (col >> 2) * (64 * 128)) + row * 128;
+          const uint32_t c0 = ((2 * (col & 3)) ^ (row & 7)) << 4, c1 = ((2 * (col & 3) + 1) ^ (row & 7)) << 4;
+          auto h = [&](uint32_t w, uint32_t sel) { return (code_pair_f16(w, sel) & keep) ^ flip; };
+          sts16(at + c0, h(v.x, 0x4140), h(v.x, 0x4342), h(v.y, 0x4140), h(v.y, 0x4342));
+          sts16(at + c1, h(v.z, 0x4140), h(v.z, 0x4342), h(v.w, 0x4140), h(v.w, 0x4342));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(full); mbar_arrive(&raw_empty[slot]); }
+      }
+    } else {
+      // ===================== softmax (thread = row), output =====================
+      const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+      const int limit = tid < pc.rows ? L - n + (p.group == 1 ? pc.c0 + tid : (pc.c0 + tid) / p.group) + 1 : 0;
+      const int least = max(0, L - n + (pc.c0 + min(32 * warp, pc.rows - 1)) / p.group + 1);        // what the warp's first row sees
+      const bool partial = 32 * warp + 32 > pc.rows;
+      float ref = -INFINITY, l = 0.f;
+      int w = -1000;                                   // none yet
+      bool bad;
+      int64_t block = nt > 0 ? block_of(pc.t_first, bad) : 0;
+      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : p.k_scale[block]) : 0.f, vs = nt > 0 ? p.v_scale[block] : 0.f;
+      for (int k = 0; k < nt; ++k) {
+        const uint32_t c = done + k, b = c & 1;
+        const int tile = pc.t_first + k;
+        float ks_next = 0.f, vs_next = 0.f;
+        if (k + 1 < nt) {
+          block = block_of(tile + 1, bad);
+          ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+          vs_next = p.v_scale[block];
+        }
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (c >> 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s0[32], s1[32];
+        tmem_ld_32x32(tmem + 64 * b + lanes, s0);
+        tmem_ld_32x32(tmem + 64 * b + 32 + lanes, s1);
+        tmem_ld_wait();
+        const bool masked = partial || (tile + 1) * KV_TILE > least;
+        const int seen = limit - tile * KV_TILE;       // columns of the tile that this row sees
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= seen) s0[i] = 0xff800000u;
+            if (32 + i >= seen) s1[i] = 0xff800000u;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+        const float f = q_factor * ks;                 // not negative
+        top = top == -INFINITY ? top : top * f;
+        // the reference of the row, and the exponent taken off v_scale
+        const float av = fabsf(vs);
+        const int ev = av > 0.f ? (int)(__float_as_uint(av) >> 23) - 127 : w;
+        int w_now = w;
+        if (ev > w + KP_LAZY_V || w == -1000) w_now = ev == -1000 ? w : ev;
+        const float now = top > ref + KP_LAZY || ref == -INFINITY ? fmaxf(top, ref) : ref;
+        if (__any_sync(0xffffffffu, l > 0.f && (now != ref || w_now != w))) {
+          // O is complete up to tile k - 1 once that product is done
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[b ^ 1], ((c - 1) >> 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const float down = (ref == -INFINITY ? 1.f : exp2_fast(ref - now)), alpha = down * exp2_fast((float)max(w - w_now, -200));
+          if (ref != -INFINITY) l *= down;
+#pragma unroll
+          for (int d = 0; d < DW; d += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(tmem_o + d + lanes, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32(tmem_o + d + lanes, o);
+          }
+          tmem_st_wait();
+        }
+        ref = now;
+        w = w_now;
+        // p' = 2^(score - ref + log2(|v_scale| 2^-w)); a zero scale counts as 2^w (its values are zero)
+        const float unit = av == 0.f ? 1.f : w == -1000 ? av : av * __uint_as_float((uint32_t)(min(max(127 - w, 1), 254)) << 23);
+        const float add = (ref == -INFINITY ? 0.f : -ref) + log2f(unit);
+        float sum = 0.f;
+        uint32_t ph[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a = exp2_fast(fmaf(__uint_as_float(s0[2 * i]), f, add)), e = exp2_fast(fmaf(__uint_as_float(s0[2 * i + 1]), f, add));
+          float a1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i]), f, add)), e1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i + 1]), f, add));
+          if (masked) {                                // not even a NaN of the scales reaches a row that does not see the token
+            if (2 * i >= seen) a = 0.f;
+            if (2 * i + 1 >= seen) e = 0.f;
+            if (2 * i + 32 >= seen) a1 = 0.f;
+            if (2 * i + 33 >= seen) e1 = 0.f;
+          }
+          sum += (a + e) + (a1 + e1);
+          ph[i] = half2_bits(a, e);
+          ph[16 + i] = half2_bits(a1, e1);
+        }
+        tmem_st_32x32(tmem + 64 * b + lanes, ph);
+        tmem_st_wait();
+        if (sum != 0.f) l += sum * __fdiv_rn(1.f, unit);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+        ks = ks_next; vs = vs_next;
+      }
+
+      // ---- out ----
+      const bool whole = pc.t_first == 0 && pc.t_last == pc.tiles;
+      float* slice = attend_slice<KP_ROWS, DW>(p, rg, blockIdx.x, pc);
+      const uint32_t c_last = done + nt - 1;
+      if (ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[c_last & 1], (c_last >> 1) & 1, abort_flag));
+      tc_fence_after();
+      if (!ok) l = __int_as_float(0x7fc00000);
+      const float scale_o = w == -1000 ? 0.f : exp2_fast((float)w);
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      const int64_t at = tid < pc.rows ? attend_out_row(p, pc, tid) : 0;
+      if (tid < pc.rows) {
+        if (whole) attend_put_lse(p, at, ref, l);
+        else { slice[KP_ROWS * DW + 2 * tid] = ref; slice[KP_ROWS * DW + 2 * tid + 1] = l; }
+      }
+#pragma unroll
+      for (int d = 0; d < DW; d += 32) {
+        uint32_t o[32];
+        if (ok && nt > 0) {
+          tmem_ld_32x32(tmem_o + d + lanes, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (tid < pc.rows) {
+          if (whole) {
+            XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
+            XT v[32];
+            // a row whose sum is NaN is NaN in every channel
+            const float f = inv * scale_o;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = from_f32<XT>(l == 0.f ? 0.f : (w == -1000 ? l * 0.f : __uint_as_float(o[i]) * f));
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              if (p.vec_o8 && d + i + 8 <= p.D) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  u[j] = (uint32_t)*reinterpret_cast<const uint16_t*>(&v[i + 2 * j]) | ((uint32_t)*reinterpret_cast<const uint16_t*>(&v[i + 2 * j + 1]) << 16);
+                *reinterpret_cast<uint4*>(dst + i) = make_uint4(u[0], u[1], u[2], u[3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (d + i + j < p.D) dst[i + j] = v[i + j];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(slice + tid * DW + d + i) =
+                  make_float4(__uint_as_float(o[i]) * scale_o, __uint_as_float(o[i + 1]) * scale_o, __uint_as_float(o[i + 2]) * scale_o, __uint_as_float(o[i + 3]) * scale_o);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+    done += nt;
+    if (!(pc.t_first == 0 && pc.t_last == pc.tiles)) {
+      const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, 2>(p, rg, pc, first_c, last_c);
+    }
+    __syncthreads();                                   // before Q and O are written again
+    tc_fence_after();
+    ok = *abort_flag == 0;
+    idx = pc.tile_at + pc.t_last;
+  }
+
+  // After a wait that ran out copies may still be in flight: a bounded time to land before the shared memory is released.
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20000000LL) {}
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, KP_TMEM);
+  }
+}
+
+// ------------------------------------------------------------------ host ----
+PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype) {
+  PromptPlan pl;
+  memset(&pl, 0, sizeof(pl));
+  if (rows <= 64 || dw > 128 || q_dtype == JGQ_F32) return pl;
+  pl.use = 1;
+  pl.G = std::min(KA_TICKETS, 2 * sm_count());
+  pl.slice_bytes = align_up((size_t)pl.G * 2 * KP_ROWS * (dw + 2) * sizeof(float), 256);
+  return pl;
+}
+
+template <typename XT, int DW>
+static int launch_prompt_inst(const PromptPlan& pl, const AttendParams& p, cudaStream_t s) {
+  auto kern = kv_prompt_kernel<XT, DW>;
+  struct AttrTag {};
+  const int arc = once_per_device<AttrTag>([&]() {
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaGetLastError();
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem(DW));
+  });
+  if (arc != 0) return fail(JGQ_ERR_CUDA, "kv_attend: cannot raise the dynamic shared memory limit");
+  kern<<<(unsigned)pl.G, KP_THREADS, kp_smem(DW), s>>>(p);
+  return check_launch("kv_prompt");
+}
+
+int launch_kv_prompt(const PromptPlan& pl, const AttendParams& p, int dw, int q_dtype, cudaStream_t s) {
+  if (q_dtype == JGQ_F16) return dw == 64 ? launch_prompt_inst<__half, 64>(pl, p, s) : launch_prompt_inst<__half, 128>(pl, p, s);
+  return dw == 64 ? launch_prompt_inst<__nv_bfloat16, 64>(pl, p, s) : launch_prompt_inst<__nv_bfloat16, 128>(pl, p, s);
+}
+
+}  // namespace jgq
