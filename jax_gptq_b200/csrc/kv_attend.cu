@@ -114,8 +114,10 @@ kv_attend_kernel(const AttendParams p) {
   const int page_shift = p.P == 64 ? 0 : p.P == 128 ? 1 : 2;          // tiles per page
 
   // ---- pieces: the part of one item (sequence, head, row tile) in this range ----
-  for (int64_t idx = rg.begin; idx < rg.end;) {
-    const AttendPiece pc = attend_piece<NC, kPieceCost>(p, rg, idx);
+  AttendCursor<NC, kPieceCost> cursor;
+  cursor.find(p, rg);
+  for (int64_t idx = rg.begin; idx < rg.end; cursor.next(p, rg)) {
+    const AttendPiece pc = cursor.piece(p, rg, idx);
     if (pc.t_last <= pc.t_first) break;                // the item's tiles begin behind this range
     const int n = pc.n, L = pc.L, h = pc.h, c0 = pc.c0, rows = pc.rows, row_first = pc.row_first, t_first = pc.t_first, t_last = pc.t_last;
     const int w0 = COLS ? 8 * NT * warp : 0;           // this warp's first one

@@ -71,18 +71,23 @@ __device__ __forceinline__ int seq_len(const AttendParams& p, int r) {
 }
 
 // sum over i < n of floor((a i + b) / m); a, b >= 0
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+template <typename T>
+__device__ __forceinline__ int64_t floor_sum_of(T n, T m, T a, T b) {
   int64_t sum = 0;
   while (n > 0) {
-    if (a >= m) { sum += n * (n - 1) / 2 * (a / m); a %= m; }
-    if (b >= m) { sum += n * (b / m); b %= m; }
-    const int64_t y = a * n + b;
+    if (a >= m) { const T q = a / m; sum += (int64_t)n * (n - 1) / 2 * q; a -= q * m; }
+    if (b >= m) { const T q = b / m; sum += (int64_t)n * q; b -= q * m; }
+    const T y = a * n + b;
     if (y < m) break;
     n = y / m;                                         // the lattice points below the line, counted along the other axis
-    b = y % m;
-    const int64_t t = a; a = m; m = t;
+    b = y - n * m;
+    const T t = a; a = m; m = t;
   }
   return sum;
+}
+// (quotients of 64 bits take five times as long: 32 where they do; n and m only shrink)
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  return a * n + b < (1ll << 31) && n < 65536 && m < 65536 ? floor_sum_of<uint32_t>((uint32_t)n, (uint32_t)m, (uint32_t)a, (uint32_t)b) : floor_sum_of<int64_t>(n, m, a, b);
 }
 
 // a sequence's part of the list: row tiles per head, and units of row tile c: floor((a c + b) / m), COST in front and a tile each
@@ -167,39 +172,69 @@ struct AttendPiece {
   int t_first, t_last, tiles;  // tiles of the piece, and of the item
   int64_t tile_at;             // unit of the item's tile 0
 };
+// Where a range stands: set to its first item, then moved from item to item.
 template <int NC, int COST>
-__device__ __forceinline__ AttendPiece attend_piece(const AttendParams& p, AttendRange& g, int64_t idx) {
-  AttendPiece e;
-  int64_t u = seq_units<NC, COST>(p, g.r);
-  while (idx >= g.seq_at + u) { g.seq_at += u; ++g.r; u = seq_units<NC, COST>(p, g.r); }
-  const SeqWork wk = seq_work<NC, COST>(p, g.r);
-  const int64_t per_head = u / p.Hkv;
-  e.n = wk.n; e.L = wk.L;
-  e.h = (int)((idx - g.seq_at) / per_head);
-  int64_t in_head = (idx - g.seq_at) - e.h * per_head;
-  int row_tile;
-  if (wk.a) {                                          // the row tile by bisection in the sums
-    int lo = 0, hi = wk.ct;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (floor_sum(mid, wk.m, wk.a, wk.b) <= in_head) lo = mid; else hi = mid;
-    }
-    row_tile = lo;
-    in_head -= floor_sum(lo, wk.m, wk.a, wk.b);
-    e.tiles = (int)((wk.a * lo + wk.b) / wk.m) - COST;
-  } else {
-    row_tile = (int)(in_head / wk.b);
-    in_head -= row_tile * wk.b;
-    e.tiles = (int)wk.b - COST;
+struct AttendCursor {
+  SeqWork wk;
+  int h, row_tile, units;      // item and its units
+  int64_t at;                  // its first unit
+  int row_first;
+
+  __device__ __forceinline__ void open(const AttendParams& p, const AttendRange& g) {
+    wk = seq_work<NC, COST>(p, g.r);
+    row_first = p.cu ? max(0, min(p.cu[g.r], p.T)) : g.r;
   }
-  e.c0 = row_tile * NC;
-  e.rows = min(NC, e.n * p.group - e.c0);
-  e.row_first = p.cu ? max(0, min(p.cu[g.r], p.T)) : g.r;
-  e.tile_at = idx - in_head + COST;
-  e.t_first = (int)max((int64_t)0, idx - e.tile_at);
-  e.t_last = (int)max((int64_t)0, min((int64_t)e.tiles, g.end - e.tile_at));
-  return e;
-}
+  __device__ __forceinline__ int units_of(int c) const { return wk.a == 0 ? (int)wk.b : (int)((wk.a * c + wk.b) / wk.m); }
+  // whole warps: the lanes look for the row tile together
+  __device__ __forceinline__ void find(const AttendParams& p, const AttendRange& g) {
+    open(p, g);
+    const int64_t per_head = wk.a ? floor_sum(wk.ct, wk.m, wk.a, wk.b) : wk.ct * wk.b;
+    h = (int)((g.begin - g.seq_at) / per_head);
+    const int64_t in_head = g.begin - g.seq_at - h * per_head;
+    int64_t before;
+    if (wk.a) {
+      int lo = 0, hi = wk.ct;                          // sums up to lo are at most in_head, up to hi more
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, c = min(hi, lo + ((threadIdx.x & 31) + 1) * step);
+        const uint32_t m = __ballot_sync(0xffffffffu, c >= hi || floor_sum(c, wk.m, wk.a, wk.b) > in_head);
+        const int first = __ffs(m) - 1;                // the last lane's c is hi: there is one
+        hi = min(hi, lo + (first + 1) * step);
+        lo += first * step;
+      }
+      row_tile = lo;
+      before = floor_sum(lo, wk.m, wk.a, wk.b);
+    } else {
+      row_tile = (int)(in_head / wk.b);
+      before = row_tile * wk.b;
+    }
+    at = g.seq_at + h * per_head + before;
+    units = units_of(row_tile);
+  }
+  __device__ __forceinline__ void next(const AttendParams& p, AttendRange& g) {
+    at += units;
+    if (++row_tile == wk.ct) {
+      row_tile = 0;
+      if (++h == p.Hkv) {
+        h = 0;
+        do { ++g.r; } while (g.r < p.B && seq_rows(p, g.r) == 0);
+        if (g.r < p.B) open(p, g);
+      }
+    }
+    units = units_of(row_tile);
+  }
+  __device__ __forceinline__ AttendPiece piece(const AttendParams& p, const AttendRange& g, int64_t idx) const {
+    AttendPiece e;
+    e.n = wk.n; e.L = wk.L; e.h = h;
+    e.c0 = row_tile * NC;
+    e.rows = min(NC, e.n * p.group - e.c0);
+    e.row_first = row_first;
+    e.tiles = units - COST;
+    e.tile_at = at + COST;
+    e.t_first = (int)max((int64_t)0, idx - e.tile_at);
+    e.t_last = (int)max((int64_t)0, min((int64_t)e.tiles, g.end - e.tile_at));
+    return e;
+  }
+};
 
 // rows of q behind the last sequence become zero
 template <typename XT, int THREADS>

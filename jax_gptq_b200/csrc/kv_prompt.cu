@@ -14,8 +14,9 @@
 // Per tile and CTA: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  Two CTAs
 // share an SM: while one's softmax warps work, the other's products run.
 //
-// Roles (256 threads): warps 0-3 softmax and output, warp 4 bulk copies of the raw codes (ring of four units), warp 5 issues
-// the MMAs, warp 6 turns the keys' codes into an operand, warp 7 the values' (128-byte swizzle; [token][64 channels] twice, [channel][64 tokens]).
+// Roles (320 threads): warps 0-3 softmax and output, warp 4 bulk copies of the raw codes (ring of four units), warp 5 issues
+// the MMAs, warps 6 and 7 turn the keys' codes into an operand, 8 and 9 the values' (128-byte swizzle; [token][64 channels]
+// twice, [channel][64 tokens]).  A row's 64 scores are read twice, 32 at a time, which keeps a thread below 96 registers.
 // The work is cut into equal ranges as in kv_attend.cu, with the same slices and tickets.  Waits are bounded: a row whose
 // wait ran out becomes NaN.
 #include "kv_attend.cuh"
@@ -23,9 +24,14 @@
 #include <algorithm>
 #include <cstring>
 
+// measurement builds, per CTA: 0 entry, 1 range known, 2 first piece's q staged, 3 its tiles done, 4 last piece's tiles done, 5 exit,
+// 6 tiles of the CTA
+JGQ_TRACE_DEFINE(prompt, 8 * 1024)
+#define PTRACE(i) JGQ_TRACE_CTA(prompt, i, 1024)
+
 namespace jgq {
 
-constexpr int KP_ROWS = 128, KP_THREADS = 256;
+constexpr int KP_ROWS = 128, KP_THREADS = 320;
 constexpr int KP_COST = 6;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
 constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
 constexpr int KP_TMEM = 256;                           // columns: S and P 2 x 64, O DW
@@ -53,6 +59,14 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
         "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -84,13 +98,15 @@ kv_prompt_kernel(const AttendParams p) {
   uint8_t* raw = v_smem + 64 * DW * 2;
   __shared__ int64_t s_pre[KP_THREADS + 1];
   __shared__ int64_t s_found[2];
+  __shared__ float s_factor[KP_ROWS];                  // of a row's scores
   __shared__ int s_flag, s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &s_abort;
+  PTRACE(0);
   if (tid == 0) {
-    for (int i = 0; i < KP_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 1); }
-    mbar_init(k_full, 1); mbar_init(k_empty, 1); mbar_init(v_full, 1); mbar_init(v_empty, 1);
+    for (int i = 0; i < KP_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2); }
+    mbar_init(k_full, 2); mbar_init(k_empty, 1); mbar_init(v_full, 2); mbar_init(v_empty, 1);
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
     s_abort = 0;
     fence_barrier_init();
@@ -99,6 +115,7 @@ kv_prompt_kernel(const AttendParams p) {
   attend_zero_rest<XT, KP_THREADS>(p);
   AttendRange rg = attend_range<KP_ROWS, KP_COST, KP_THREADS>(p, 2 * KP_COST, s_pre, s_found);
   if ((int)blockIdx.x >= rg.G) return;
+  PTRACE(1);
   if (warp == 5) {
     tmem_alloc(tmem_slot, KP_TMEM);
     tmem_relinquish();
@@ -111,8 +128,10 @@ kv_prompt_kernel(const AttendParams p) {
   uint32_t done = 0;                                   // tiles of earlier pieces: every role's barriers count on from them
   bool ok = true;
 
-  for (int64_t idx = rg.begin; idx < rg.end;) {
-    const AttendPiece pc = attend_piece<KP_ROWS, KP_COST>(p, rg, idx);
+  AttendCursor<KP_ROWS, KP_COST> cursor;
+  cursor.find(p, rg);
+  for (int64_t idx = rg.begin; idx < rg.end; cursor.next(p, rg)) {
+    const AttendPiece pc = cursor.piece(p, rg, idx);
     if (pc.t_last <= pc.t_first) break;                // the item's tiles begin behind this range
     const int n = pc.n, L = pc.L, h = pc.h;
     const int seen_item = max(0, L - n + (pc.c0 + pc.rows - 1) / p.group + 1);
@@ -125,50 +144,56 @@ kv_prompt_kernel(const AttendParams p) {
       return (int64_t)(bad ? 0 : page) * p.Hkv + h;
     };
 
-    // ---- q into shared memory: thread = row, two threads a row ----
-    float q_factor = 0.f;                              // of the scores of row tid (softmax warps)
+    // ---- q into shared memory: a warp per row, four rows at a time ----
     {
-      const int row = tid & 127, half = tid >> 7;      // channels half DW / 2 ..
-      const bool live = row < pc.rows;
-      const int gr = pc.c0 + (live ? row : 0), i = p.group == 1 ? gr : gr / p.group;
-      const XT* src = reinterpret_cast<const XT*>(p.q) + (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head;
-      // the largest element of the whole row, by both threads
-      float big = 0.f;
-      auto load8 = [&](float (&f)[8], int d) {
-        if (live && p.vec_q && d + 8 <= p.D) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src + d);
-          const XT* e = reinterpret_cast<const XT*>(&v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = to_f32<XT>(e[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = (live && d + j < p.D) ? to_f32<XT>(src[d + j]) : 0.f;
-        }
-      };
-#pragma unroll 4
-      for (int d = 0; d < DW; d += 8) {
-        float f[8];
-        load8(f, d);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(f[j]));
-      }
-      // a power of two brings the row's largest element to [2^13, 2^14): f16 then holds what bf16 says down to 2^-27 of it
-      const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
-      const float up = __uint_as_float((267u - e) << 23), down = __uint_as_float((e - 13u) << 23);
+      constexpr int CPL = DW / 32;                     // channels per lane
       const float sign = p.scale < 0.f ? -1.f : 1.f;   // the factor of the scores is positive: a row's maximum is that of its products
-      q_factor = down * fabsf(p.scale);
-#pragma unroll 4
-      for (int d = half * (DW / 2); d < (half + 1) * (DW / 2); d += 8) {
-        float f[8];
-        load8(f, d);
-        uint32_t w[4];
+      const int d0 = lane * CPL;
+      for (int row0 = warp; row0 < KP_ROWS; row0 += 4 * (KP_THREADS / 32)) {
+        float f[4][CPL];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = half2_bits(f[2 * j] * up * sign, f[2 * j + 1] * up * sign);
-        sts16(smem_u32(q_smem) + (d >> 6) * (KP_ROWS * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
+        for (int r = 0; r < 4; ++r) {
+          const int row = row0 + r * (KP_THREADS / 32), gr = pc.c0 + row, i = p.group == 1 ? gr : gr / p.group;
+          const bool live = row < pc.rows;
+          const XT* src = reinterpret_cast<const XT*>(p.q) + (live ? (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head : 0);
+          if (live && p.vec_q && d0 + CPL <= p.D) {
+            using V = typename std::conditional<CPL == 4, uint2, uint32_t>::type;
+            const V v = *reinterpret_cast<const V*>(src + d0);
+            const XT* e = reinterpret_cast<const XT*>(&v);
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) f[r][j] = to_f32<XT>(e[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) f[r][j] = (live && d0 + j < p.D) ? to_f32<XT>(src[d0 + j]) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = row0 + r * (KP_THREADS / 32);
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < CPL; ++j) big = fmaxf(big, fabsf(f[r][j]));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          // a power of two brings the row's largest element to [2^13, 2^14): f16 then holds what bf16 says down to 2^-27 of it
+          const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
+          const float up = __uint_as_float((267u - e) << 23) * sign, down = __uint_as_float((e - 13u) << 23);
+          if (row < KP_ROWS) {
+            const uint32_t at = smem_u32(q_smem) + (d0 >> 6) * (KP_ROWS * 128) + row * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2;
+            const uint32_t w0 = half2_bits(f[r][0] * up, f[r][1] * up);
+            if constexpr (CPL == 4) {
+              asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(w0), "r"(half2_bits(f[r][2] * up, f[r][3] * up)) : "memory");
+            } else {
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w0) : "memory");
+            }
+            if (lane == 0) s_factor[row] = down * fabsf(p.scale);
+          }
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
+    if (idx == rg.begin) PTRACE(2);
 
     if (warp == 4) {
       // ===================== raw codes =====================
@@ -229,9 +254,16 @@ kv_prompt_kernel(const AttendParams p) {
         }
       }
     } else if (warp >= 6) {
-      // ===================== codes into operands: warp 6 the keys, warp 7 the values =====================
-      const int part = warp - 6;
+      // ===================== codes into operands: warps 6 and 7 the keys, 8 and 9 the values =====================
+      const int part = (warp - 6) >> 1, half = warp & 1;
       uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
+      // lane's 16-byte piece i = lane + 32 j: row and chunk of the operand; the row's low bits, which swizzle, follow j's parity at most
+      constexpr int KP = DW / 16;                      // pieces per row of keys
+      const int row0 = part ? lane >> 2 : lane / KP, col = part ? lane & 3 : lane % KP;
+      const uint32_t to = smem_u32(part ? v_smem : k_smem) + (part ? 0 : (col >> 2) * (64 * 128)) + row0 * 128;
+      const uint32_t row_step = part ? 8 * 128 : (32 / KP) * 128, odd = !part && KP == 8 ? 64u : 0u;
+      const uint32_t c0 = ((2 * (col & 3)) ^ (row0 & 7)) << 4, c1 = c0 ^ 16;
+      constexpr int STEPS = UNIT / 16 / 32;            // of both warps
       for (int k = 0; k < nt && ok; ++k) {
         const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW;
         float vs = 1.f;
@@ -241,19 +273,22 @@ kv_prompt_kernel(const AttendParams p) {
         if (ok && c > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty, (c + 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        // values of a zero scale are zero, of a negative one negative
-        const uint32_t keep = vs == 0.f ? 0u : 0xffffffffu, flip = vs < 0.f ? 0x80008000u : 0u;
-        const uint32_t from = smem_u32(raw) + slot * UNIT, to = smem_u32(part ? v_smem : k_smem);
-#pragma unroll 4
-        for (int i = lane; i < UNIT / 16; i += 32) {
-          const uint4 v = lds16(from + i * 16);
-          // 16 codes: two 16-byte pieces of the operand
-          const int row = part ? i >> 2 : i / (DW / 16), col = part ? i & 3 : i % (DW / 16);      // row of codes, piece of it
-          const uint32_t at = to + (part ? 0 : (col >> 2) * (64 * 128)) + row * 128;
-          const uint32_t c0 = ((2 * (col & 3)) ^ (row & 7)) << 4, c1 = ((2 * (col & 3) + 1) ^ (row & 7)) << 4;
-          auto h = [&](uint32_t w, uint32_t sel) { return (code_pair_f16(w, sel) & keep) ^ flip; };
-          sts16(at + c0, h(v.x, 0x4140), h(v.x, 0x4342), h(v.y, 0x4140), h(v.y, 0x4342));
-          sts16(at + c1, h(v.z, 0x4140), h(v.z, 0x4342), h(v.w, 0x4140), h(v.w, 0x4342));
+        const uint32_t from = smem_u32(raw) + slot * UNIT + lane * 16;
+        auto expand = [&](auto f) {
+#pragma unroll
+          for (int jj = 0; jj < STEPS / 2; ++jj) {
+            const int j = half * (STEPS / 2) + jj;
+            const uint4 v = lds16(from + j * 512);
+            const uint32_t at = to + j * row_step, x = (j & 1) ? odd : 0u;
+            sts16(at + (c0 ^ x), f(v.x, 0x4140), f(v.x, 0x4342), f(v.y, 0x4140), f(v.y, 0x4342));
+            sts16(at + (c1 ^ x), f(v.z, 0x4140), f(v.z, 0x4342), f(v.w, 0x4140), f(v.w, 0x4342));
+          }
+        };
+        if (vs > 0.f) {
+          expand([](uint32_t w, uint32_t sel) { return code_pair_f16(w, sel); });
+        } else {                                       // values of a zero scale are zero, of a negative one negative
+          const uint32_t keep = vs == 0.f ? 0u : 0xffffffffu, flip = vs < 0.f ? 0x80008000u : 0u;
+          expand([=](uint32_t w, uint32_t sel) { return (code_pair_f16(w, sel) & keep) ^ flip; });
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -262,6 +297,7 @@ kv_prompt_kernel(const AttendParams p) {
     } else {
       // ===================== softmax (thread = row), output =====================
       const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+      const float q_factor = s_factor[tid];
       const int limit = tid < pc.rows ? L - n + (p.group == 1 ? pc.c0 + tid : (pc.c0 + tid) / p.group) + 1 : 0;
       const int least = max(0, L - n + (pc.c0 + min(32 * warp, pc.rows - 1)) / p.group + 1);        // what the warp's first row sees
       const bool partial = 32 * warp + 32 > pc.rows;
@@ -282,22 +318,23 @@ kv_prompt_kernel(const AttendParams p) {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (c >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        uint32_t s0[32], s1[32];
-        tmem_ld_32x32(tmem + 64 * b + lanes, s0);
-        tmem_ld_32x32(tmem + 64 * b + 32 + lanes, s1);
-        tmem_ld_wait();
         const bool masked = partial || (tile + 1) * KV_TILE > least;
         const int seen = limit - tile * KV_TILE;       // columns of the tile that this row sees
-        if (masked) {
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i >= seen) s0[i] = 0xff800000u;
-            if (32 + i >= seen) s1[i] = 0xff800000u;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t sc[32];
+          tmem_ld_32x32(tmem + 64 * b + 32 * half + lanes, sc);
+          tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * half + i >= seen) sc[i] = 0xff800000u;
           }
-        }
-        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+          for (int i = 0; i < 32; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(sc[i]));
+        }
+        float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
         const float f = q_factor * ks;                 // not negative
         top = top == -INFINITY ? top : top * f;
         // the reference of the row, and the exponent taken off v_scale
@@ -329,24 +366,26 @@ kv_prompt_kernel(const AttendParams p) {
         // p' = 2^(score - ref + log2(|v_scale| 2^-w)); a zero scale counts as 2^w (its values are zero)
         const float unit = av == 0.f ? 1.f : w == -1000 ? av : av * __uint_as_float((uint32_t)(min(max(127 - w, 1), 254)) << 23);
         const float add = (ref == -INFINITY ? 0.f : -ref) + log2f(unit);
-        float sum = 0.f;
-        uint32_t ph[32];
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a = exp2_fast(fmaf(__uint_as_float(s0[2 * i]), f, add)), e = exp2_fast(fmaf(__uint_as_float(s0[2 * i + 1]), f, add));
-          float a1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i]), f, add)), e1 = exp2_fast(fmaf(__uint_as_float(s1[2 * i + 1]), f, add));
-          if (masked) {                                // not even a NaN of the scales reaches a row that does not see the token
-            if (2 * i >= seen) a = 0.f;
-            if (2 * i + 1 >= seen) e = 0.f;
-            if (2 * i + 32 >= seen) a1 = 0.f;
-            if (2 * i + 33 >= seen) e1 = 0.f;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t sc[32], ph[16];
+          tmem_ld_32x32(tmem + 64 * b + 32 * half + lanes, sc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a = exp2_fast(fmaf(__uint_as_float(sc[2 * i]), f, add)), e = exp2_fast(fmaf(__uint_as_float(sc[2 * i + 1]), f, add));
+            if (masked) {                              // not even a NaN of the scales reaches a row that does not see the token
+              if (32 * half + 2 * i >= seen) a = 0.f;
+              if (32 * half + 2 * i + 1 >= seen) e = 0.f;
+            }
+            sum4[i & 3] += a + e;
+            ph[i] = half2_bits(a, e);
           }
-          sum += (a + e) + (a1 + e1);
-          ph[i] = half2_bits(a, e);
-          ph[16 + i] = half2_bits(a1, e1);
+          tmem_st_32x16(tmem + 64 * b + 16 * half + lanes, ph);        // over scores that have been read
         }
-        tmem_st_32x32(tmem + 64 * b + lanes, ph);
         tmem_st_wait();
+        const float sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
         if (sum != 0.f) l += sum * __fdiv_rn(1.f, unit);
         tc_fence_before();
         __syncwarp();
@@ -354,6 +393,8 @@ kv_prompt_kernel(const AttendParams p) {
         ks = ks_next; vs = vs_next;
       }
 
+      if (idx == rg.begin) PTRACE(3);
+      PTRACE(4);
       // ---- out ----
       const bool whole = pc.t_first == 0 && pc.t_last == pc.tiles;
       float* slice = attend_slice<KP_ROWS, DW>(p, rg, blockIdx.x, pc);
@@ -413,7 +454,7 @@ kv_prompt_kernel(const AttendParams p) {
     done += nt;
     if (!(pc.t_first == 0 && pc.t_last == pc.tiles)) {
       const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
-      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, 2>(p, rg, pc, first_c, last_c);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, 3>(p, rg, pc, first_c, last_c);
     }
     __syncthreads();                                   // before Q and O are written again
     tc_fence_after();
@@ -421,6 +462,10 @@ kv_prompt_kernel(const AttendParams p) {
     idx = pc.tile_at + pc.t_last;
   }
 
+  PTRACE(5);
+#ifdef JGQ_TRACE
+  if (threadIdx.x == 0 && blockIdx.x < 1024) g_trace_prompt[8 * blockIdx.x + 6] = done;
+#endif
   // After a wait that ran out copies may still be in flight: a bounded time to land before the shared memory is released.
   __syncthreads();
   if (*abort_flag) {
