@@ -1,6 +1,7 @@
 // Attention over the paged 8-bit cache for many rows per sequence (prompts and chunks of them): tcgen05.
 //
-// An item is 128 rows of q (tokens x heads of one kv head's group) of a sequence and kv head; its tiles are 64 tokens.
+// An item is 128 NG rows of q (tokens x heads of one kv head's group) of a sequence and kv head; its tiles are 64 tokens.
+// NG = 1: two CTAs share an SM; NG = 2, for 256 rows and more: one CTA, whose two groups of 128 rows share the expanded codes.
 //   S = Q K^T     M = 128 rows, N = 64 tokens:  Q and the tile's keys in shared memory, S in tensor memory (two buffers)
 //   P             softmax warps read S (one row per thread), write p as f16 over it
 //   O += P V      M = 128 rows, N = DW channels: P out of tensor memory, the tile's values [channel][token] in shared memory
@@ -11,12 +12,13 @@
 // raised only when a score passes it by 8 (p' then stays below 2^13), O is rescaled then, by the row's thread.
 // The sum of exponentials is that of p' before its rounding, divided by v_scale 2^-w.
 //
-// Per tile and CTA: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  Two CTAs
-// share an SM: while one's softmax warps work, the other's products run.
+// Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  While one
+// group's (or CTA's) softmax warps work, the other's products run.
 //
-// Roles (320 threads): warps 0-3 softmax and output, warp 4 bulk copies of the raw codes (ring of four units), warp 5 issues
-// the MMAs, warps 6 and 7 turn the keys' codes into an operand, 8 and 9 the values' (128-byte swizzle; [token][64 channels]
-// twice, [channel][64 tokens]).  A row's 64 scores are read twice, 32 at a time, which keeps a thread below 96 registers.
+// Roles: warps 0 .. 4 NG - 1 softmax, then one warp for bulk copies of the raw codes (ring of four units), one that issues the MMAs,
+// two (NG = 2: one) that turn the keys' codes into an operand, as many for the values' (128-byte swizzle; [token][64 channels]
+// twice, [channel][64 tokens]).  With NG = 1 a row's 64 scores are read twice, 32 at a time, which keeps a thread below 96 registers.
+// All warps write the outputs, by way of shared memory, so that rows go out whole.
 // The work is cut into equal ranges as in kv_attend.cu, with the same slices and tickets.  Waits are bounded: a row whose
 // wait ran out becomes NaN.
 #include "kv_attend.cuh"
@@ -31,15 +33,18 @@ JGQ_TRACE_DEFINE(prompt, 8 * 1024)
 
 namespace jgq {
 
-constexpr int KP_ROWS = 128, KP_THREADS = 320;
+// 10 warps, or 12: three per scheduler, which leaves a thread 168 registers
+constexpr int kp_threads(int ng) { return ng == 1 ? 320 : 384; }
 constexpr int KP_COST = 6;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
 constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
-constexpr int KP_TMEM = 256;                           // columns: S and P 2 x 64, O DW
+constexpr int KP_TMEM = 256;                           // columns per group: S and P 2 x 64, O DW
 constexpr float KP_LAZY = 8.f;                         // log2 by which a score may pass its row's reference
 constexpr int KP_LAZY_V = 5;                           // and log2 by which v_scale may pass 2^w
 
 __host__ __device__ constexpr int kp_unit(int dw) { return 64 * dw; }
-__host__ __device__ constexpr int kp_smem(int dw) { return 1024 + 1024 + KP_ROWS * dw * 2 + 2 * 64 * dw * 2 + KP_RAW * kp_unit(dw); }
+// q, NG buffers of expanded keys and of values, the ring; the outputs of 128 rows take their place at the end of a piece
+__host__ __device__ constexpr int kp_operands(int dw, int ng) { return 128 * ng * dw * 2 + 2 * ng * 64 * dw * 2 + KP_RAW * kp_unit(dw); }
+__host__ __device__ constexpr int kp_smem(int dw, int ng) { return 1024 + 1024 + kp_operands(dw, ng); }
 
 // D[tmem] (+)= A[tmem] B[smem], f16
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -80,34 +85,41 @@ __device__ __forceinline__ uint32_t code_pair_f16(uint32_t w, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename XT, int DW>
-__global__ void __launch_bounds__(KP_THREADS, 2)
+template <typename XT, int DW, int NG>
+__global__ void __launch_bounds__(kp_threads(NG), NG == 1 ? 2 : 1)
 kv_prompt_kernel(const AttendParams p) {
   using namespace umma;
+  constexpr int KP_THREADS = NG == 1 ? 320 : 384, KP_ROWS = 128 * NG, WARPS = KP_THREADS / 32;
   constexpr int UNIT = kp_unit(DW), KB = DW / 64;      // 64-channel blocks of a row
+  constexpr int W_COPY = 4 * NG, W_MMA = W_COPY + 1, W_EXPAND = W_COPY + 2;
+  constexpr int EW = (WARPS - W_EXPAND) / 2;           // warps per operand
+  constexpr int OST = DW + 4;                          // floats per row of staged outputs
+  static_assert(128 * OST * 4 <= kp_operands(DW, NG), "the outputs of 128 rows fit the operands' place");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base);
   uint64_t* raw_full = bars, *raw_empty = bars + KP_RAW;
-  uint64_t *k_full = bars + 2 * KP_RAW, *k_empty = k_full + 1, *v_full = k_full + 2, *v_empty = k_full + 3;
-  uint64_t *s_full = k_full + 4, *p_full = s_full + 2, *o_done = p_full + 2;           // two of each, for even and odd tiles
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
-  uint8_t* q_smem = base + 1024;                       // [KB][128 rows][128 bytes], swizzled
-  uint8_t* k_smem = q_smem + KP_ROWS * DW * 2;         // [KB][64 tokens][128 bytes]
-  uint8_t* v_smem = k_smem + 64 * DW * 2;              // [DW channels][128 bytes]
-  uint8_t* raw = v_smem + 64 * DW * 2;
+  uint64_t *k_full = bars + 2 * KP_RAW, *k_empty = k_full + NG, *v_full = k_empty + NG, *v_empty = v_full + NG;       // per buffer
+  uint64_t *s_full = v_empty + NG, *p_full = s_full + 2 * NG, *o_done = p_full + 2 * NG;         // per group, for even and odd tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2 * NG);
+  uint8_t* q_smem = base + 1024;                       // [NG][KB][128 rows][128 bytes], swizzled
+  uint8_t* k_smem = q_smem + KP_ROWS * DW * 2;         // [NG buffers][KB][64 tokens][128 bytes]
+  uint8_t* v_smem = k_smem + NG * 64 * DW * 2;         // [NG buffers][DW channels][128 bytes]
+  uint8_t* raw = v_smem + NG * 64 * DW * 2;
+  float* staged = reinterpret_cast<float*>(q_smem);
   __shared__ int64_t s_pre[KP_THREADS + 1];
   __shared__ int64_t s_found[2];
   __shared__ float s_factor[KP_ROWS];                  // of a row's scores
+  __shared__ float2 s_ml[KP_ROWS];                     // a row's reference and sum, when its piece is done
   __shared__ int s_flag, s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &s_abort;
   PTRACE(0);
   if (tid == 0) {
-    for (int i = 0; i < KP_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 2); }
-    mbar_init(k_full, 2); mbar_init(k_empty, 1); mbar_init(v_full, 2); mbar_init(v_empty, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < KP_RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], EW); }
+    for (int i = 0; i < NG; ++i) { mbar_init(&k_full[i], EW); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], EW); mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < 2 * NG; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
     s_abort = 0;
     fence_barrier_init();
   }
@@ -116,18 +128,19 @@ kv_prompt_kernel(const AttendParams p) {
   AttendRange rg = attend_range<KP_ROWS, KP_COST, KP_THREADS>(p, 2 * KP_COST, s_pre, s_found);
   if ((int)blockIdx.x >= rg.G) return;
   PTRACE(1);
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, KP_TMEM);
+  if (warp == W_MMA) {
+    tmem_alloc(tmem_slot, NG * KP_TMEM);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;
+  const uint32_t tmem = *tmem_slot;
   const int page_shift = p.P == 64 ? 0 : p.P == 128 ? 1 : 2;
   uint32_t done = 0;                                   // tiles of earlier pieces: every role's barriers count on from them
   bool ok = true;
 
+  constexpr bool KEEP = NG == 2;
   AttendCursor<KP_ROWS, KP_COST> cursor;
   cursor.find(p, rg);
   for (int64_t idx = rg.begin; idx < rg.end; cursor.next(p, rg)) {
@@ -144,16 +157,18 @@ kv_prompt_kernel(const AttendParams p) {
       return (int64_t)(bad ? 0 : page) * p.Hkv + h;
     };
 
-    // ---- q into shared memory: a warp per row, four rows at a time ----
+    // ---- q into shared memory: a warp per row, seven rows at a time ----
     {
       constexpr int CPL = DW / 32;                     // channels per lane
       const float sign = p.scale < 0.f ? -1.f : 1.f;   // the factor of the scores is positive: a row's maximum is that of its products
       const int d0 = lane * CPL;
-      for (int row0 = warp; row0 < KP_ROWS; row0 += 4 * (KP_THREADS / 32)) {
-        float f[4][CPL];
+      constexpr int QR = 7;
+#pragma unroll 1
+      for (int row0 = warp; row0 < KP_ROWS; row0 += QR * WARPS) {
+        float f[QR][CPL];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = row0 + r * (KP_THREADS / 32), gr = pc.c0 + row, i = p.group == 1 ? gr : gr / p.group;
+        for (int r = 0; r < QR; ++r) {
+          const int row = row0 + r * WARPS, gr = pc.c0 + row, i = p.group == 1 ? gr : gr / p.group;
           const bool live = row < pc.rows;
           const XT* src = reinterpret_cast<const XT*>(p.q) + (live ? (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head : 0);
           if (live && p.vec_q && d0 + CPL <= p.D) {
@@ -168,8 +183,8 @@ kv_prompt_kernel(const AttendParams p) {
           }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = row0 + r * (KP_THREADS / 32);
+        for (int r = 0; r < QR; ++r) {
+          const int row = row0 + r * WARPS;
           float big = 0.f;
 #pragma unroll
           for (int j = 0; j < CPL; ++j) big = fmaxf(big, fabsf(f[r][j]));
@@ -179,7 +194,7 @@ kv_prompt_kernel(const AttendParams p) {
           const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
           const float up = __uint_as_float((267u - e) << 23) * sign, down = __uint_as_float((e - 13u) << 23);
           if (row < KP_ROWS) {
-            const uint32_t at = smem_u32(q_smem) + (d0 >> 6) * (KP_ROWS * 128) + row * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2;
+            const uint32_t at = smem_u32(q_smem) + ((row >> 7) * KB + (d0 >> 6)) * (128 * 128) + (row & 127) * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2;
             const uint32_t w0 = half2_bits(f[r][0] * up, f[r][1] * up);
             if constexpr (CPL == 4) {
               asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(w0), "r"(half2_bits(f[r][2] * up, f[r][3] * up)) : "memory");
@@ -195,7 +210,9 @@ kv_prompt_kernel(const AttendParams p) {
     __syncthreads();
     if (idx == rg.begin) PTRACE(2);
 
-    if (warp == 4) {
+    float ref = -INFINITY, l = 0.f;                    // of a softmax thread's row
+    int w = -1000;                                     // exponent taken off v_scale, none yet
+    if (warp == W_COPY) {
       // ===================== raw codes =====================
       if (lane == 0) {
         bool bad;
@@ -206,7 +223,7 @@ kv_prompt_kernel(const AttendParams p) {
           const int64_t at = ((block << page_shift) + (tile & ((1 << page_shift) - 1))) * (int64_t)UNIT;
           for (int part = 0; part < 2 && ok; ++part) {
             const uint32_t u = 2 * (done + k) + part, slot = u % KP_RAW;
-            if (u >= KP_RAW) ok = mbar_wait(&raw_empty[slot], (u / KP_RAW + 1) & 1, abort_flag);
+            if (u >= KP_RAW) ok = mbar_wait_suspended(&raw_empty[slot], (u / KP_RAW + 1) & 1, abort_flag);
             if (!ok) break;
             mbar_expect_tx(&raw_full[slot], UNIT);
             bulk_load(smem_u32(raw) + slot * UNIT, (part ? p.v : p.k) + at, UNIT, &raw_full[slot]);
@@ -215,47 +232,57 @@ kv_prompt_kernel(const AttendParams p) {
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-    } else if (warp == 5) {
+    } else if (warp == W_MMA) {
       // ===================== MMAs =====================
-      const uint32_t idesc_s = make_idesc_f16(0, 0, 0, KP_ROWS, 64), idesc_o = make_idesc_f16(0, 0, 0, KP_ROWS, DW);
-      const uint64_t dq = make_desc_sw128(smem_u32(q_smem), 16, 1024), dk = make_desc_sw128(smem_u32(k_smem), 16, 1024);
-      const uint64_t dv = make_desc_sw128(smem_u32(v_smem), 16, 1024);
+      const uint32_t idesc_s = make_idesc_f16(0, 0, 0, 128, 64), idesc_o = make_idesc_f16(0, 0, 0, 128, DW);
+      const uint64_t dq = make_desc_sw128(smem_u32(q_smem), 16, 1024), dk0 = make_desc_sw128(smem_u32(k_smem), 16, 1024);
+      const uint64_t dv0 = make_desc_sw128(smem_u32(v_smem), 16, 1024);
       for (int k = 0; k <= nt && ok; ++k) {
         if (k < nt) {                                  // scores of tile k
-          const uint32_t c = done + k, b = c & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(k_full, c & 1, abort_flag));
+          const uint32_t c = done + k, b = c & 1, buf = c % NG;
+          ok = __all_sync(0xffffffffu, mbar_wait_suspended(&k_full[buf], (c / NG) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
+            const uint64_t dk = dk0 + (uint32_t)((buf * 64 * DW * 2) >> 4);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int grp = 0; grp < NG; ++grp) {
 #pragma unroll
-              for (int k16 = 0; k16 < 4; ++k16)
-                mma_f16_ss(tmem + 64 * b, dq + (uint32_t)((kb * KP_ROWS * 128 + k16 * 32) >> 4), dk + (uint32_t)((kb * 64 * 128 + k16 * 32) >> 4), idesc_s,
-                           kb > 0 || k16 > 0 ? 1u : 0u);
-            mma_commit(k_empty);
-            mma_commit(&s_full[b]);
+              for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int k16 = 0; k16 < 4; ++k16)
+                  mma_f16_ss(tmem + grp * KP_TMEM + 64 * b, dq + (uint32_t)(((grp * KB + kb) * 128 * 128 + k16 * 32) >> 4),
+                             dk + (uint32_t)((kb * 64 * 128 + k16 * 32) >> 4), idesc_s, kb > 0 || k16 > 0 ? 1u : 0u);
+              if (grp == NG - 1) mma_commit(&k_empty[buf]);
+              mma_commit(&s_full[2 * grp + b]);
+            }
           }
           __syncwarp();
         }
         if (k > 0) {                                   // outputs of tile k - 1
-          const uint32_t c = done + k - 1, b = c & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(v_full, c & 1, abort_flag) && mbar_wait(&p_full[b], (c >> 1) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
+          const uint32_t c = done + k - 1, b = c & 1, buf = c % NG;
+          ok = __all_sync(0xffffffffu, mbar_wait_suspended(&v_full[buf], (c / NG) & 1, abort_flag));
 #pragma unroll
-            for (int k16 = 0; k16 < 4; ++k16)
-              mma_f16_ts(tmem_o, tmem + 64 * b + 8 * k16, dv + (uint32_t)((k16 * 32) >> 4), idesc_o, k > 1 || k16 > 0 ? 1u : 0u);
-            mma_commit(v_empty);
-            mma_commit(&o_done[b]);
+          for (int grp = 0; grp < NG; ++grp) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&p_full[2 * grp + b], (c >> 1) & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t dv = dv0 + (uint32_t)((buf * 64 * DW * 2) >> 4);
+#pragma unroll
+              for (int k16 = 0; k16 < 4; ++k16)
+                mma_f16_ts(tmem + grp * KP_TMEM + 128, tmem + grp * KP_TMEM + 64 * b + 8 * k16, dv + (uint32_t)((k16 * 32) >> 4), idesc_o,
+                           k > 1 || k16 > 0 ? 1u : 0u);
+              if (grp == NG - 1) mma_commit(&v_empty[buf]);
+              mma_commit(&o_done[2 * grp + b]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
-    } else if (warp >= 6) {
-      // ===================== codes into operands: warps 6 and 7 the keys, 8 and 9 the values =====================
-      const int part = (warp - 6) >> 1, half = warp & 1;
+    } else if (warp >= W_EXPAND) {
+      // ===================== codes into operands: one or two warps each for keys and values =====================
+      const int part = (warp - W_EXPAND) / EW, half = (warp - W_EXPAND) % EW;
       uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
       // lane's 16-byte piece i = lane + 32 j: row and chunk of the operand; the row's low bits, which swizzle, follow j's parity at most
       constexpr int KP = DW / 16;                      // pieces per row of keys
@@ -265,21 +292,21 @@ kv_prompt_kernel(const AttendParams p) {
       const uint32_t c0 = ((2 * (col & 3)) ^ (row0 & 7)) << 4, c1 = c0 ^ 16;
       constexpr int STEPS = UNIT / 16 / 32;            // of both warps
       for (int k = 0; k < nt && ok; ++k) {
-        const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW;
+        const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW, buf = c % NG;
         float vs = 1.f;
         bool bad;
         if (part) vs = p.v_scale[block_of(pc.t_first + k, bad)];
-        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[slot], (u / KP_RAW) & 1, abort_flag));
-        if (ok && c > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty, (c + 1) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait_suspended(&raw_full[slot], (u / KP_RAW) & 1, abort_flag));
+        if (ok && c >= NG) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&empty[buf], (c / NG + 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t from = smem_u32(raw) + slot * UNIT + lane * 16;
         auto expand = [&](auto f) {
 #pragma unroll
-          for (int jj = 0; jj < STEPS / 2; ++jj) {
-            const int j = half * (STEPS / 2) + jj;
+          for (int jj = 0; jj < STEPS / EW; ++jj) {
+            const int j = half * (STEPS / EW) + jj;
             const uint4 v = lds16(from + j * 512);
-            const uint32_t at = to + j * row_step, x = (j & 1) ? odd : 0u;
+            const uint32_t at = to + buf * (64 * DW * 2) + j * row_step, x = (j & 1) ? odd : 0u;
             sts16(at + (c0 ^ x), f(v.x, 0x4140), f(v.x, 0x4342), f(v.y, 0x4140), f(v.y, 0x4342));
             sts16(at + (c1 ^ x), f(v.z, 0x4140), f(v.z, 0x4342), f(v.w, 0x4140), f(v.w, 0x4342));
           }
@@ -292,17 +319,16 @@ kv_prompt_kernel(const AttendParams p) {
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) { mbar_arrive(full); mbar_arrive(&raw_empty[slot]); }
+        if (lane == 0) { mbar_arrive(&full[buf]); mbar_arrive(&raw_empty[slot]); }
       }
     } else {
-      // ===================== softmax (thread = row), output =====================
-      const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+      // ===================== softmax (thread = row) =====================
+      const int grp = warp >> 2;
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, tmem_s = tmem + grp * KP_TMEM + lanes, tmem_o = tmem_s + 128;
       const float q_factor = s_factor[tid];
       const int limit = tid < pc.rows ? L - n + (p.group == 1 ? pc.c0 + tid : (pc.c0 + tid) / p.group) + 1 : 0;
       const int least = max(0, L - n + (pc.c0 + min(32 * warp, pc.rows - 1)) / p.group + 1);        // what the warp's first row sees
       const bool partial = 32 * warp + 32 > pc.rows;
-      float ref = -INFINITY, l = 0.f;
-      int w = -1000;                                   // none yet
       bool bad;
       int64_t block = nt > 0 ? block_of(pc.t_first, bad) : 0;
       float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : p.k_scale[block]) : 0.f, vs = nt > 0 ? p.v_scale[block] : 0.f;
@@ -315,24 +341,32 @@ kv_prompt_kernel(const AttendParams p) {
           ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
           vs_next = p.v_scale[block];
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (c >> 1) & 1, abort_flag));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&s_full[2 * grp + b], (c >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const bool masked = partial || (tile + 1) * KV_TILE > least;
         const int seen = limit - tile * KV_TILE;       // columns of the tile that this row sees
         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t sc[KEEP ? 2 : 1][32];                 // NG = 2: both halves stay in registers
+        if (KEEP) {
+          tmem_ld_32x32(tmem_s + 64 * b, sc[0]);
+          tmem_ld_32x32(tmem_s + 64 * b + 32, sc[KEEP ? 1 : 0]);
+          tmem_ld_wait();
+        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t sc[32];
-          tmem_ld_32x32(tmem + 64 * b + 32 * half + lanes, sc);
-          tmem_ld_wait();
+          uint32_t (&v)[32] = sc[KEEP ? half : 0];
+          if (!KEEP) {
+            tmem_ld_32x32(tmem_s + 64 * b + 32 * half, v);
+            tmem_ld_wait();
+          }
           if (masked) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (32 * half + i >= seen) sc[i] = 0xff800000u;
+              if (32 * half + i >= seen) v[i] = 0xff800000u;
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(sc[i]));
+          for (int i = 0; i < 32; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(v[i]));
         }
         float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
         const float f = q_factor * ks;                 // not negative
@@ -345,7 +379,7 @@ kv_prompt_kernel(const AttendParams p) {
         const float now = top > ref + KP_LAZY || ref == -INFINITY ? fmaxf(top, ref) : ref;
         if (__any_sync(0xffffffffu, l > 0.f && (now != ref || w_now != w))) {
           // O is complete up to tile k - 1 once that product is done
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[b ^ 1], ((c - 1) >> 1) & 1, abort_flag));
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&o_done[2 * grp + (b ^ 1)], ((c - 1) >> 1) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const float down = (ref == -INFINITY ? 1.f : exp2_fast(ref - now)), alpha = down * exp2_fast((float)max(w - w_now, -200));
@@ -353,11 +387,11 @@ kv_prompt_kernel(const AttendParams p) {
 #pragma unroll
           for (int d = 0; d < DW; d += 32) {
             uint32_t o[32];
-            tmem_ld_32x32(tmem_o + d + lanes, o);
+            tmem_ld_32x32(tmem_o + d, o);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32(tmem_o + d + lanes, o);
+            tmem_st_32x32(tmem_o + d, o);
           }
           tmem_st_wait();
         }
@@ -369,12 +403,15 @@ kv_prompt_kernel(const AttendParams p) {
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t sc[32], ph[16];
-          tmem_ld_32x32(tmem + 64 * b + 32 * half + lanes, sc);
-          tmem_ld_wait();
+          uint32_t (&v)[32] = sc[KEEP ? half : 0];
+          uint32_t ph[16];
+          if (!KEEP) {
+            tmem_ld_32x32(tmem_s + 64 * b + 32 * half, v);
+            tmem_ld_wait();
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float a = exp2_fast(fmaf(__uint_as_float(sc[2 * i]), f, add)), e = exp2_fast(fmaf(__uint_as_float(sc[2 * i + 1]), f, add));
+            float a = exp2_fast(fmaf(__uint_as_float(v[2 * i]), f, add)), e = exp2_fast(fmaf(__uint_as_float(v[2 * i + 1]), f, add));
             if (masked) {                              // not even a NaN of the scales reaches a row that does not see the token
               if (32 * half + 2 * i >= seen) a = 0.f;
               if (32 * half + 2 * i + 1 >= seen) e = 0.f;
@@ -382,79 +419,70 @@ kv_prompt_kernel(const AttendParams p) {
             sum4[i & 3] += a + e;
             ph[i] = half2_bits(a, e);
           }
-          tmem_st_32x16(tmem + 64 * b + 16 * half + lanes, ph);        // over scores that have been read
+          tmem_st_32x16(tmem_s + 64 * b + 16 * half, ph);        // over scores that have been read
         }
         tmem_st_wait();
         const float sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
         if (sum != 0.f) l += sum * __fdiv_rn(1.f, unit);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) mbar_arrive(&p_full[2 * grp + b]);
         ks = ks_next; vs = vs_next;
       }
 
       if (idx == rg.begin) PTRACE(3);
       PTRACE(4);
-      // ---- out ----
-      const bool whole = pc.t_first == 0 && pc.t_last == pc.tiles;
-      float* slice = attend_slice<KP_ROWS, DW>(p, rg, blockIdx.x, pc);
-      const uint32_t c_last = done + nt - 1;
-      if (ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[c_last & 1], (c_last >> 1) & 1, abort_flag));
-      tc_fence_after();
-      if (!ok) l = __int_as_float(0x7fc00000);
-      const float scale_o = w == -1000 ? 0.f : exp2_fast((float)w);
-      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-      const int64_t at = tid < pc.rows ? attend_out_row(p, pc, tid) : 0;
-      if (tid < pc.rows) {
-        if (whole) attend_put_lse(p, at, ref, l);
-        else { slice[KP_ROWS * DW + 2 * tid] = ref; slice[KP_ROWS * DW + 2 * tid + 1] = l; }
-      }
-#pragma unroll
-      for (int d = 0; d < DW; d += 32) {
-        uint32_t o[32];
-        if (ok && nt > 0) {
-          tmem_ld_32x32(tmem_o + d + lanes, o);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
-        }
-        if (tid < pc.rows) {
-          if (whole) {
-            XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
-            XT v[32];
-            // a row whose sum is NaN is NaN in every channel
-            const float f = inv * scale_o;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = from_f32<XT>(l == 0.f ? 0.f : (w == -1000 ? l * 0.f : __uint_as_float(o[i]) * f));
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              if (p.vec_o8 && d + i + 8 <= p.D) {
-                uint32_t u[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  u[j] = (uint32_t)*reinterpret_cast<const uint16_t*>(&v[i + 2 * j]) | ((uint32_t)*reinterpret_cast<const uint16_t*>(&v[i + 2 * j + 1]) << 16);
-                *reinterpret_cast<uint4*>(dst + i) = make_uint4(u[0], u[1], u[2], u[3]);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (d + i + j < p.D) dst[i + j] = v[i + j];
-              }
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(slice + tid * DW + d + i) =
-                  make_float4(__uint_as_float(o[i]) * scale_o, __uint_as_float(o[i + 1]) * scale_o, __uint_as_float(o[i + 2]) * scale_o, __uint_as_float(o[i + 3]) * scale_o);
-          }
-        }
-      }
-      tc_fence_before();
     }
     done += nt;
-    if (!(pc.t_first == 0 && pc.t_last == pc.tiles)) {
+
+    // ---- out: 128 rows at a time by way of shared memory ----
+    const bool whole = pc.t_first == 0 && pc.t_last == pc.tiles;
+    float* slice = attend_slice<KP_ROWS, DW>(p, rg, blockIdx.x, pc);
+    const uint32_t c_last = done - 1;
+    if (warp < 4 * NG && ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&o_done[2 * (warp >> 2) + (c_last & 1)], (c_last >> 1) & 1, abort_flag));
+    if (!ok) l = __int_as_float(0x7fc00000);
+    if (warp < 4 * NG) s_ml[tid] = make_float2(ref, l);
+    const float scale_o = w == -1000 ? 0.f : exp2_fast((float)w);
+    for (int g0 = 0; g0 < NG && 128 * g0 < pc.rows; ++g0) {
+      __syncthreads();                                 // the operands have been read, the rows before have left
+      if (warp >> 2 == g0 && warp < 4 * NG) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int d = 0; d < DW; d += 32) {
+          uint32_t o[32];
+          if (ok && nt > 0) {
+            tmem_ld_32x32(tmem + g0 * KP_TMEM + 128 + ((uint32_t)(32 * (warp & 3)) << 16) + d, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          float4* dst = reinterpret_cast<float4*>(staged + (tid & 127) * OST + d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])};
+            dst[i] = w == -1000 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[0] * scale_o, v[1] * scale_o, v[2] * scale_o, v[3] * scale_o);
+          }
+        }
+        tc_fence_before();
+      }
+      __syncthreads();
+      const int rows = min(128, pc.rows - 128 * g0);
+      for (int i = tid; i < rows * (DW / 4); i += KP_THREADS) {
+        const int row = i / (DW / 4), d = 4 * (i % (DW / 4)), col = 128 * g0 + row;
+        const float4 v = *reinterpret_cast<const float4*>(staged + row * OST + d);
+        const float2 ml = s_ml[col];
+        if (whole) {
+          attend_finish4<XT>(p, pc, col, d, v, ml.x, ml.y);
+        } else {
+          *reinterpret_cast<float4*>(slice + col * DW + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(slice + KP_ROWS * DW + 2 * col) = ml;
+        }
+      }
+    }
+    if (!whole) {
       const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
-      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, 3>(p, rg, pc, first_c, last_c);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, NG == 1 ? 2 : 4>(p, rg, pc, first_c, last_c);
     }
     __syncthreads();                                   // before Q and O are written again
     tc_fence_after();
@@ -474,9 +502,9 @@ kv_prompt_kernel(const AttendParams p) {
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == W_MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem, KP_TMEM);
+    tmem_dealloc(tmem, NG * KP_TMEM);
   }
 }
 
@@ -486,28 +514,34 @@ PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype) {
   memset(&pl, 0, sizeof(pl));
   if (rows <= 64 || dw > 128 || q_dtype == JGQ_F32) return pl;
   pl.use = 1;
-  pl.G = std::min(KA_TICKETS, 2 * sm_count());
-  pl.slice_bytes = align_up((size_t)pl.G * 2 * KP_ROWS * (dw + 2) * sizeof(float), 256);
+  pl.groups = rows >= 256 ? 2 : 1;
+  pl.G = std::min(KA_TICKETS, (pl.groups == 2 ? 1 : 2) * sm_count());
+  pl.slice_bytes = align_up((size_t)pl.G * 2 * 128 * pl.groups * (dw + 2) * sizeof(float), 256);
   return pl;
 }
 
-template <typename XT, int DW>
+template <typename XT, int DW, int NG>
 static int launch_prompt_inst(const PromptPlan& pl, const AttendParams& p, cudaStream_t s) {
-  auto kern = kv_prompt_kernel<XT, DW>;
+  auto kern = kv_prompt_kernel<XT, DW, NG>;
   struct AttrTag {};
   const int arc = once_per_device<AttrTag>([&]() {
     cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     cudaGetLastError();
-    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem(DW));
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem(DW, NG));
   });
   if (arc != 0) return fail(JGQ_ERR_CUDA, "kv_attend: cannot raise the dynamic shared memory limit");
-  kern<<<(unsigned)pl.G, KP_THREADS, kp_smem(DW), s>>>(p);
+  kern<<<(unsigned)pl.G, kp_threads(NG), kp_smem(DW, NG), s>>>(p);
   return check_launch("kv_prompt");
 }
 
+template <typename XT>
+static int launch_prompt(const PromptPlan& pl, const AttendParams& p, int dw, cudaStream_t s) {
+  if (dw == 64) return pl.groups == 2 ? launch_prompt_inst<XT, 64, 2>(pl, p, s) : launch_prompt_inst<XT, 64, 1>(pl, p, s);
+  return pl.groups == 2 ? launch_prompt_inst<XT, 128, 2>(pl, p, s) : launch_prompt_inst<XT, 128, 1>(pl, p, s);
+}
+
 int launch_kv_prompt(const PromptPlan& pl, const AttendParams& p, int dw, int q_dtype, cudaStream_t s) {
-  if (q_dtype == JGQ_F16) return dw == 64 ? launch_prompt_inst<__half, 64>(pl, p, s) : launch_prompt_inst<__half, 128>(pl, p, s);
-  return dw == 64 ? launch_prompt_inst<__nv_bfloat16, 64>(pl, p, s) : launch_prompt_inst<__nv_bfloat16, 128>(pl, p, s);
+  return q_dtype == JGQ_F16 ? launch_prompt<__half>(pl, p, dw, s) : launch_prompt<__nv_bfloat16>(pl, p, dw, s);
 }
 
 }  // namespace jgq

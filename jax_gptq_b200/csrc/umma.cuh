@@ -64,6 +64,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// mbar_wait for warps that share their scheduler with working ones: a poll suspends the thread until the phase completes or
+// 20 us have passed, so that waiting takes no issue slots.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint32_t at = smem_u32(bar);
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > kWaitBudgetCycles) { *abort = 1; return false; }
+  }
+}
+
 // For waits that last as long as a whole tile: sleeps between polls, so that the warps that are working keep the
 // issue slots.
 __device__ __forceinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
