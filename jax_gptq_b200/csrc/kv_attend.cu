@@ -511,7 +511,7 @@ kv_attend_kernel(const AttendParams p) {
     }
     if (!whole) {
       const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
-      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, NC, DW, KA_THREADS, COLS ? 4 : (NC * DW / 4 + KA_THREADS - 1) / KA_THREADS>(p, rg, pc, first_c, last_c);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, NC, DW, KA_THREADS, COLS ? 8 : (NC * DW / 4 + KA_THREADS - 1) / KA_THREADS, COLS ? 2 : 4>(p, rg, pc, first_c, last_c);
     }
     if (idx == rg.begin) ATRACE(3);
     __syncthreads();                                   // before the rings are filled again

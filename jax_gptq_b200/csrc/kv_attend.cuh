@@ -47,11 +47,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ uint4 lds16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
+// An ordinary load: behind the wait that goes before it, but free to move among products and other loads.
+__device__ __forceinline__ uint4 lds16(uint32_t at) { return *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(at)); }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(umma::smem_u32(bar)) : "memory");
@@ -255,11 +252,9 @@ __device__ __forceinline__ int64_t attend_out_row(const AttendParams& p, const A
 __device__ __forceinline__ void attend_put_lse(const AttendParams& p, int64_t at, float mx, float den) {
   if (p.lse) p.lse[at] = den == 0.f ? -INFINITY : (mx + log2f(den)) * 0.6931471805599453f;
 }
-// four channels of a row's result
+// four channels of a row's result: sums times f, to row `at` of the output
 template <typename XT>
-__device__ __forceinline__ void attend_finish4(const AttendParams& p, const AttendPiece& piece, int col, int d, const float4& sum, float mx, float den) {
-  const int64_t at = attend_out_row(p, piece, col);
-  const float f = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
+__device__ __forceinline__ void attend_store4(const AttendParams& p, int64_t at, int d, const float4& sum, float f) {
   const float v[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
   XT* dst = reinterpret_cast<XT*>(p.out) + at * p.D + d;
   if (p.vec_o) {
@@ -275,6 +270,11 @@ __device__ __forceinline__ void attend_finish4(const AttendParams& p, const Atte
     for (int i = 0; i < 4; ++i)
       if (d + i < p.D) dst[i] = from_f32<XT>(v[i]);
   }
+}
+template <typename XT>
+__device__ __forceinline__ void attend_finish4(const AttendParams& p, const AttendPiece& piece, int col, int d, const float4& sum, float mx, float den) {
+  const int64_t at = attend_out_row(p, piece, col);
+  attend_store4<XT>(p, at, d, sum, den == 0.f ? 0.f : __fdiv_rn(1.f, den));
   if (d == 0) attend_put_lse(p, at, mx, den);
 }
 
@@ -298,8 +298,8 @@ __device__ __forceinline__ bool attend_last(const AttendParams& p, int first_c, 
   if (last) __threadfence();
   return last;
 }
-// The slices of an item added in CTA order: four channels of JP rows per thread, four slices at a time: 4 JP loads in flight.
-template <typename XT, int NC, int DW, int THREADS, int JP>
+// The slices of an item added in CTA order: four channels of JP rows per thread, SL slices at a time: SL JP loads in flight.
+template <typename XT, int NC, int DW, int THREADS, int JP, int SL>
 __device__ __forceinline__ void attend_join(const AttendParams& p, const AttendRange& g, const AttendPiece& e, int first_c, int last_c) {
   const int count = e.rows * (DW / 4);
   for (int i0 = threadIdx.x; i0 < count; i0 += THREADS * JP) {
@@ -307,11 +307,11 @@ __device__ __forceinline__ void attend_join(const AttendParams& p, const AttendR
     float4 sum[JP];
 #pragma unroll
     for (int j = 0; j < JP; ++j) { mx[j] = -INFINITY; den[j] = 0.f; sum[j] = make_float4(0.f, 0.f, 0.f, 0.f); }
-    for (int cb = first_c; cb <= last_c; cb += 4) {
-      float v[4][JP], dv[4][JP];
-      float4 sv[4][JP];
+    for (int cb = first_c; cb <= last_c; cb += SL) {
+      float v[SL][JP], dv[SL][JP];
+      float4 sv[SL][JP];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < SL; ++c) {
         const float* src = attend_slice<NC, DW>(p, g, min(cb + c, last_c), e);
 #pragma unroll
         for (int j = 0; j < JP; ++j) {
@@ -322,7 +322,7 @@ __device__ __forceinline__ void attend_join(const AttendParams& p, const AttendR
         }
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < SL; ++c)
         if (cb + c <= last_c) {
 #pragma unroll
           for (int j = 0; j < JP; ++j) {

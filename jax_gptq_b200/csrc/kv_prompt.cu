@@ -10,7 +10,7 @@
 //   p' = 2^(score - reference + log2(v_scale 2^-w)),
 // so that p' is rounded once; w follows the exponent of v_scale (kept while v_scale stays below 2^(w + 5)).  The row's reference is
 // raised only when a score passes it by 8 (p' then stays below 2^13), O is rescaled then, by the row's thread.
-// The sum of exponentials is that of p' before its rounding, divided by v_scale 2^-w.
+// The sum of exponentials is that of p' before its rounding, times 2^w / v_scale (two units of 2^-23 off at most, as 2^x is).
 //
 // Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  While one
 // group's (or CTA's) softmax warps work, the other's products run.
@@ -35,7 +35,7 @@ namespace jgq {
 
 // 10 warps, or 12: three per scheduler, which leaves a thread 168 registers
 constexpr int kp_threads(int ng) { return ng == 1 ? 320 : 384; }
-constexpr int KP_COST = 6;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
+constexpr int KP_COST = 9;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
 constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
 constexpr int KP_TMEM = 256;                           // columns per group: S and P 2 x 64, O DW
 constexpr float KP_LAZY = 8.f;                         // log2 by which a score may pass its row's reference
@@ -110,7 +110,9 @@ kv_prompt_kernel(const AttendParams p) {
   __shared__ int64_t s_pre[KP_THREADS + 1];
   __shared__ int64_t s_found[2];
   __shared__ float s_factor[KP_ROWS];                  // of a row's scores
-  __shared__ float2 s_ml[KP_ROWS];                     // a row's reference and sum, when its piece is done
+  __shared__ float2 s_ml[KP_ROWS];                     // a row's reference and sum, when its piece is done,
+  __shared__ float s_inv[KP_ROWS];                     // what its outputs are multiplied by,
+  __shared__ int64_t s_row[KP_ROWS];                   // and where they go
   __shared__ int s_flag, s_abort;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -157,52 +159,55 @@ kv_prompt_kernel(const AttendParams p) {
       return (int64_t)(bad ? 0 : page) * p.Hkv + h;
     };
 
-    // ---- q into shared memory: a warp per row, seven rows at a time ----
+    // ---- q into shared memory: a warp per row, all of a warp's rows requested at once ----
     {
-      constexpr int CPL = DW / 32;                     // channels per lane
+      constexpr int CPL = DW / 32, QR = (KP_ROWS + WARPS - 1) / WARPS;         // channels per lane, rows per warp
       const float sign = p.scale < 0.f ? -1.f : 1.f;   // the factor of the scores is positive: a row's maximum is that of its products
       const int d0 = lane * CPL;
-      constexpr int QR = 7;
-#pragma unroll 1
-      for (int row0 = warp; row0 < KP_ROWS; row0 += QR * WARPS) {
-        float f[QR][CPL];
+      using V = typename std::conditional<CPL == 4, uint2, uint32_t>::type;
+      V raw_q[QR];
 #pragma unroll
-        for (int r = 0; r < QR; ++r) {
-          const int row = row0 + r * WARPS, gr = pc.c0 + row, i = p.group == 1 ? gr : gr / p.group;
-          const bool live = row < pc.rows;
-          const XT* src = reinterpret_cast<const XT*>(p.q) + (live ? (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head : 0);
-          if (live && p.vec_q && d0 + CPL <= p.D) {
-            using V = typename std::conditional<CPL == 4, uint2, uint32_t>::type;
-            const V v = *reinterpret_cast<const V*>(src + d0);
-            const XT* e = reinterpret_cast<const XT*>(&v);
+      for (int r = 0; r < QR; ++r) {
+        const int row = warp + r * WARPS, gr = pc.c0 + row, i = p.group == 1 ? gr : gr / p.group;
+        const bool live = row < pc.rows;
+        const XT* src = reinterpret_cast<const XT*>(p.q) + (live ? (int64_t)(pc.row_first + i) * p.q_token + (int64_t)(h * p.group + gr - i * p.group) * p.q_head : 0);
+        raw_q[r] = V{};
+        if (live && p.vec_q && d0 + CPL <= p.D) {
+          raw_q[r] = *reinterpret_cast<const V*>(src + d0);
+        } else if (live) {
+          XT e[CPL];
 #pragma unroll
-            for (int j = 0; j < CPL; ++j) f[r][j] = to_f32<XT>(e[j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < CPL; ++j) f[r][j] = (live && d0 + j < p.D) ? to_f32<XT>(src[d0 + j]) : 0.f;
-          }
+          for (int j = 0; j < CPL; ++j) e[j] = d0 + j < p.D ? src[d0 + j] : from_f32<XT>(0.f);
+          raw_q[r] = *reinterpret_cast<const V*>(e);
         }
+      }
 #pragma unroll
-        for (int r = 0; r < QR; ++r) {
-          const int row = row0 + r * WARPS;
+      for (int r = 0; r < QR; ++r) {
+        const int row = warp + r * WARPS;
+        const XT* e = reinterpret_cast<const XT*>(&raw_q[r]);
+        uint32_t w[CPL / 2];
+        float down = 1.f;
+        if constexpr (std::is_same<XT, __half>::value) {
+#pragma unroll
+          for (int j = 0; j < CPL / 2; ++j) w[j] = reinterpret_cast<const uint32_t*>(&raw_q[r])[j] ^ (sign < 0.f ? 0x80008000u : 0u);
+        } else {
+          // a power of two brings the row's largest element to [2^13, 2^14): f16 then holds what bf16 says down to 2^-27 of it
           float big = 0.f;
 #pragma unroll
-          for (int j = 0; j < CPL; ++j) big = fmaxf(big, fabsf(f[r][j]));
+          for (int j = 0; j < CPL; ++j) big = fmaxf(big, fabsf(to_f32<XT>(e[j])));
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          // a power of two brings the row's largest element to [2^13, 2^14): f16 then holds what bf16 says down to 2^-27 of it
-          const uint32_t e = min(max(__float_as_uint(big) >> 23, 14u), 254u);
-          const float up = __uint_as_float((267u - e) << 23) * sign, down = __uint_as_float((e - 13u) << 23);
-          if (row < KP_ROWS) {
-            const uint32_t at = smem_u32(q_smem) + ((row >> 7) * KB + (d0 >> 6)) * (128 * 128) + (row & 127) * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2;
-            const uint32_t w0 = half2_bits(f[r][0] * up, f[r][1] * up);
-            if constexpr (CPL == 4) {
-              asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(w0), "r"(half2_bits(f[r][2] * up, f[r][3] * up)) : "memory");
-            } else {
-              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w0) : "memory");
-            }
-            if (lane == 0) s_factor[row] = down * fabsf(p.scale);
-          }
+          const uint32_t x = min(max(__float_as_uint(big) >> 23, 14u), 254u);
+          const float up = __uint_as_float((267u - x) << 23) * sign;
+          down = __uint_as_float((x - 13u) << 23);
+#pragma unroll
+          for (int j = 0; j < CPL / 2; ++j) w[j] = half2_bits(to_f32<XT>(e[2 * j]) * up, to_f32<XT>(e[2 * j + 1]) * up);
+        }
+        if (row < KP_ROWS) {
+          const uint32_t at = smem_u32(q_smem) + ((row >> 7) * KB + (d0 >> 6)) * (128 * 128) + (row & 127) * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2;
+          if constexpr (CPL == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(w[0]), "r"(w[CPL / 2 - 1]) : "memory");
+          else                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w[0]) : "memory");
+          if (lane == 0) s_factor[row] = down * fabsf(p.scale);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -290,25 +295,32 @@ kv_prompt_kernel(const AttendParams p) {
       const uint32_t to = smem_u32(part ? v_smem : k_smem) + (part ? 0 : (col >> 2) * (64 * 128)) + row0 * 128;
       const uint32_t row_step = part ? 8 * 128 : (32 / KP) * 128, odd = !part && KP == 8 ? 64u : 0u;
       const uint32_t c0 = ((2 * (col & 3)) ^ (row0 & 7)) << 4, c1 = c0 ^ 16;
-      constexpr int STEPS = UNIT / 16 / 32;            // of both warps
+      constexpr int STEPS = UNIT / 16 / 32;            // of the operand's warps together
+      float vs_next = 1.f;
+      if (part && nt > 0) { bool bad; vs_next = p.v_scale[block_of(pc.t_first, bad)]; }
       for (int k = 0; k < nt && ok; ++k) {
         const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW, buf = c % NG;
-        float vs = 1.f;
-        bool bad;
-        if (part) vs = p.v_scale[block_of(pc.t_first + k, bad)];
+        const float vs = vs_next;                      // one tile ahead
+        if (part && k + 1 < nt) { bool bad; vs_next = p.v_scale[block_of(pc.t_first + k + 1, bad)]; }
         ok = __all_sync(0xffffffffu, mbar_wait_suspended(&raw_full[slot], (u / KP_RAW) & 1, abort_flag));
         if (ok && c >= NG) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&empty[buf], (c / NG + 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t from = smem_u32(raw) + slot * UNIT + lane * 16;
+        constexpr int BATCH = STEPS / EW < 8 ? STEPS / EW : 8;      // loads ahead of the stores that they must not pass
         auto expand = [&](auto f) {
 #pragma unroll
-          for (int jj = 0; jj < STEPS / EW; ++jj) {
-            const int j = half * (STEPS / EW) + jj;
-            const uint4 v = lds16(from + j * 512);
-            const uint32_t at = to + buf * (64 * DW * 2) + j * row_step, x = (j & 1) ? odd : 0u;
-            sts16(at + (c0 ^ x), f(v.x, 0x4140), f(v.x, 0x4342), f(v.y, 0x4140), f(v.y, 0x4342));
-            sts16(at + (c1 ^ x), f(v.z, 0x4140), f(v.z, 0x4342), f(v.w, 0x4140), f(v.w, 0x4342));
+          for (int j0 = 0; j0 < STEPS / EW; j0 += BATCH) {
+            uint4 v[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) v[i] = lds16(from + (half * (STEPS / EW) + j0 + i) * 512);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              const int j = half * (STEPS / EW) + j0 + i;
+              const uint32_t at = to + buf * (64 * DW * 2) + j * row_step, x = (j & 1) ? odd : 0u;
+              sts16(at + (c0 ^ x), f(v[i].x, 0x4140), f(v[i].x, 0x4342), f(v[i].y, 0x4140), f(v[i].y, 0x4342));
+              sts16(at + (c1 ^ x), f(v[i].z, 0x4140), f(v[i].z, 0x4342), f(v[i].w, 0x4140), f(v[i].w, 0x4342));
+            }
           }
         };
         if (vs > 0.f) {
@@ -331,7 +343,7 @@ kv_prompt_kernel(const AttendParams p) {
       const bool partial = 32 * warp + 32 > pc.rows;
       bool bad;
       int64_t block = nt > 0 ? block_of(pc.t_first, bad) : 0;
-      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : p.k_scale[block]) : 0.f, vs = nt > 0 ? p.v_scale[block] : 0.f;
+      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : p.k_scale[block]) : 0.f, vs = nt > 0 ? fabsf(p.v_scale[block]) : 0.f, lv = log2f(vs);
       for (int k = 0; k < nt; ++k) {
         const uint32_t c = done + k, b = c & 1;
         const int tile = pc.t_first + k;
@@ -339,7 +351,7 @@ kv_prompt_kernel(const AttendParams p) {
         if (k + 1 < nt) {
           block = block_of(tile + 1, bad);
           ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
-          vs_next = p.v_scale[block];
+          vs_next = fabsf(p.v_scale[block]);
         }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&s_full[2 * grp + b], (c >> 1) & 1, abort_flag));
         if (!ok) break;
@@ -372,8 +384,7 @@ kv_prompt_kernel(const AttendParams p) {
         const float f = q_factor * ks;                 // not negative
         top = top == -INFINITY ? top : top * f;
         // the reference of the row, and the exponent taken off v_scale
-        const float av = fabsf(vs);
-        const int ev = av > 0.f ? (int)(__float_as_uint(av) >> 23) - 127 : w;
+        const int ev = vs > 0.f ? (int)(__float_as_uint(vs) >> 23) - 127 : w;
         int w_now = w;
         if (ev > w + KP_LAZY_V || w == -1000) w_now = ev == -1000 ? w : ev;
         const float now = top > ref + KP_LAZY || ref == -INFINITY ? fmaxf(top, ref) : ref;
@@ -397,9 +408,8 @@ kv_prompt_kernel(const AttendParams p) {
         }
         ref = now;
         w = w_now;
-        // p' = 2^(score - ref + log2(|v_scale| 2^-w)); a zero scale counts as 2^w (its values are zero)
-        const float unit = av == 0.f ? 1.f : w == -1000 ? av : av * __uint_as_float((uint32_t)(min(max(127 - w, 1), 254)) << 23);
-        const float add = (ref == -INFINITY ? 0.f : -ref) + log2f(unit);
+        // p' = 2^(score - ref + log2(|v_scale|) - w); a zero scale counts as 2^w (its values are zero)
+        const float shift = vs == 0.f ? 0.f : lv - (w == -1000 ? 0.f : (float)w), add = (ref == -INFINITY ? 0.f : -ref) + shift;
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -423,11 +433,11 @@ kv_prompt_kernel(const AttendParams p) {
         }
         tmem_st_wait();
         const float sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-        if (sum != 0.f) l += sum * __fdiv_rn(1.f, unit);
+        if (sum != 0.f) l = fmaf(sum, exp2_fast(-shift), l);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * grp + b]);
-        ks = ks_next; vs = vs_next;
+        ks = ks_next; vs = vs_next; lv = log2f(vs);
       }
 
       if (idx == rg.begin) PTRACE(3);
@@ -441,7 +451,11 @@ kv_prompt_kernel(const AttendParams p) {
     const uint32_t c_last = done - 1;
     if (warp < 4 * NG && ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&o_done[2 * (warp >> 2) + (c_last & 1)], (c_last >> 1) & 1, abort_flag));
     if (!ok) l = __int_as_float(0x7fc00000);
-    if (warp < 4 * NG) s_ml[tid] = make_float2(ref, l);
+    if (warp < 4 * NG) {
+      s_ml[tid] = make_float2(ref, l);
+      s_inv[tid] = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      s_row[tid] = attend_out_row(p, pc, min(tid, pc.rows - 1));
+    }
     const float scale_o = w == -1000 ? 0.f : exp2_fast((float)w);
     for (int g0 = 0; g0 < NG && 128 * g0 < pc.rows; ++g0) {
       __syncthreads();                                 // the operands have been read, the rows before have left
@@ -471,18 +485,18 @@ kv_prompt_kernel(const AttendParams p) {
       for (int i = tid; i < rows * (DW / 4); i += KP_THREADS) {
         const int row = i / (DW / 4), d = 4 * (i % (DW / 4)), col = 128 * g0 + row;
         const float4 v = *reinterpret_cast<const float4*>(staged + row * OST + d);
-        const float2 ml = s_ml[col];
         if (whole) {
-          attend_finish4<XT>(p, pc, col, d, v, ml.x, ml.y);
+          attend_store4<XT>(p, s_row[col], d, v, s_inv[col]);
+          if (d == 0 && p.lse) attend_put_lse(p, s_row[col], s_ml[col].x, s_ml[col].y);
         } else {
           *reinterpret_cast<float4*>(slice + col * DW + d) = v;
-          if (d == 0) *reinterpret_cast<float2*>(slice + KP_ROWS * DW + 2 * col) = ml;
+          if (d == 0) *reinterpret_cast<float2*>(slice + KP_ROWS * DW + 2 * col) = s_ml[col];
         }
       }
     }
     if (!whole) {
       const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
-      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, NG == 1 ? 2 : 4>(p, rg, pc, first_c, last_c);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join<XT, KP_ROWS, DW, KP_THREADS, NG == 1 ? 3 : 4, 2>(p, rg, pc, first_c, last_c);
     }
     __syncthreads();                                   // before Q and O are written again
     tc_fence_after();
