@@ -55,10 +55,10 @@ int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_
                 swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-int encode_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
-                       uint32_t box_cols, uint32_t box_rows) {
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, cols, rows, row_stride_bytes, box_cols, box_rows,
-                CU_TENSOR_MAP_SWIZZLE_NONE);
+int encode_tmap_2d_zs(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
+  const bool f32 = dtype == JGQ_F32;
+  return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, base, cols, rows,
+                cols * (f32 ? 4 : 2), box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace jgq

@@ -231,7 +231,7 @@ int encode_tmap_2d_b16(CUtensorMap* map, const void* base, uint64_t cols, uint64
                        uint32_t box_cols, uint32_t box_rows);
 int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
                       uint32_t box_cols, uint32_t box_rows, int swizzle128);
-int encode_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
-                       uint32_t box_cols, uint32_t box_rows);      // not swizzled
+// rows of f32 or f16 scales, not swizzled
+int encode_tmap_2d_zs(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows);
 
 }  // namespace jgq

@@ -37,8 +37,8 @@
 // 2304 28.5 -> 12.3 us against two passes of it.
 //
 // Scales per group of the contraction (FU > 0): a warp keeps the sums of the current group apart and, where the group ends,
-// adds scale * (sum - zero * sum_k x) to totals, in fp32.  The scales and zero points of the next group are requested
-// when the current one begins.  FU is the number of 32-index units between two looks for a group's end: 4 where groups
+// adds scale * (sum - zero * sum_k x) to totals, in fp32.  The scales and zero points of a stage's groups come by TMA with its
+// box (requested one group ahead by each lane instead, 8192 x 28672 took 44 us with groups of 128, 100 with 32).  FU is the number of 32-index units between two looks for a group's end: 4 where groups
 // are multiples of 128, else 1.  A slice then holds the totals alone.  fp32 activations take three planes here (all 24
 // bits), and codes other than f16's enter as code - 8, which halves what the zero point takes off again.
 //
@@ -62,6 +62,7 @@ namespace jgq {
 
 constexpr int GV_NST = 3;                      // boxes in flight per CTA
 constexpr int GV_THREADS = WWARPS * 32;
+constexpr int GV_MAX_SMEM = 200 * 1024;
 constexpr int GV_TICKET_BYTES = W4_TICKET_REGION;   // one ticket per (channel group, warp): 1024 groups
 __host__ __device__ constexpr int gemv_xs_tokens(int nt) { return nt > 16 ? nt : 16; }      // sum_k x slots per slice
 
@@ -75,7 +76,8 @@ struct GemvParams {
   int maxc;                    // slice slots per group
   int early;                   // 1: weights may be fetched before the stream's previous kernel has finished
   int group;                   // contraction indices per group
-  int zs_f16;                  // scale and zero point are f16 (with groups; without, a template parameter says so)
+  int zs_bytes;                // of a scale or zero point (with groups; without, a template parameter says what they are)
+  int zs_rows;                 // groups that a stage may touch
 };
 
 __device__ __forceinline__ int gemv_cta_of(int64_t idx, int64_t S, int G) {
@@ -158,7 +160,8 @@ __host__ __device__ constexpr int gemv_ctas(int nt, int planes) { return nt * pl
 template <typename XT, int FU> __host__ __device__ constexpr int gemv_planes() { return std::is_same<XT, float>::value ? (FU ? 3 : 2) : 1; }
 template <typename XT, int NT, typename ZST, int FU>
 __global__ void __launch_bounds__(GV_THREADS, gemv_ctas(NT, gemv_planes<XT, FU>()))
-w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
+w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap smap, const __grid_constant__ CUtensorMap zmap,
+               const GemvParams p) {
   using namespace umma;
   using T = GemvType<XT>;
   constexpr int PL = gemv_planes<XT, FU>();
@@ -173,7 +176,9 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
   constexpr int XWARP = NT * PL * XROW;            // planes one after the other
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* xs_all = ring + GV_NST * STAGE_BYTES;   // [warp][token row][PAIRS] operand pairs, then one row of zeros
+  uint8_t* zs_ring = ring + GV_NST * STAGE_BYTES;  // with groups: per stage scales [zs_rows][128], then zero points
+  const int zs_half = GROUPED ? p.zs_rows * WCOLS * p.zs_bytes : 0;
+  uint8_t* xs_all = zs_ring + GV_NST * 2 * zs_half;   // [warp][token row][PAIRS] operand pairs, then one row of zeros
   __shared__ __align__(8) uint64_t full_bar[GV_NST];
   __shared__ int issued[GV_NST];
   __shared__ int done[GV_NST];
@@ -193,8 +198,13 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     const int gg = g_begin + lin / p.spc, ss = lin % p.spc;
     const int slot = j % GV_NST;
     issued[slot] = j;
-    mbar_expect_tx(&full_bar[slot], STAGE_BYTES);
+    mbar_expect_tx(&full_bar[slot], STAGE_BYTES + 2 * zs_half);
     tma_load_2d(ring + slot * STAGE_BYTES, &wmap, gg * WCOLS, ss * ROWS, &full_bar[slot]);
+    if (GROUPED) {
+      const int row = ss * (2 * ROWS) / p.group;
+      tma_load_2d(zs_ring + slot * 2 * zs_half, &smap, gg * WCOLS, row, &full_bar[slot]);
+      tma_load_2d(zs_ring + slot * 2 * zs_half + zs_half, &zmap, gg * WCOLS, row, &full_bar[slot]);
+    }
   };
 
   GTRACE(0);
@@ -203,6 +213,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     s_abort = 0;
     fence_barrier_init();
     prefetch_tensormap(&wmap);
+    if (GROUPED) { prefetch_tensormap(&smap); prefetch_tensormap(&zmap); }
   }
   // the row of zeros that lanes of absent token rows read
   for (int i = threadIdx.x; i < XROW / 4; i += GV_THREADS)
@@ -233,9 +244,8 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
       }
   };
   clear_acc();
-  // with groups: totals of this lane's channels and tokens, scale and zero point of the current group and of the next
+  // with groups: totals of this lane's channels and tokens
   float tot[GROUPED ? NG : 1][2][4];
-  uint4 zs_now[2], zs_next[2];
   auto clear_tot = [&]() {
 #pragma unroll
     for (int q = 0; q < (GROUPED ? NG : 1); ++q)
@@ -243,40 +253,28 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
       for (int i = 0; i < 4; ++i) { tot[q][0][i] = 0.f; tot[q][1][i] = 0.f; }
   };
   clear_tot();
-  // (ordinary loads, as for the activations below) the four channels of a lane: 16 bytes of fp32 or 8 of f16, behind the matrix nothing
-  auto fetch_zs = [&](uint4 (&zs)[2], int cgr, int64_t k) {
-    const int n0 = cgr * WCOLS + 32 * warp + 4 * g;
-    zs[0] = zs[1] = make_uint4(0, 0, 0, 0);
-    if (n0 < p.N && k < p.K) {
-      const int64_t at = (k / p.group) * p.N + n0;
-      if (p.zs_f16) {
-        const uint2 a = *reinterpret_cast<const uint2*>((const __half*)p.scale + at), b = *reinterpret_cast<const uint2*>((const __half*)p.zero + at);
-        zs[0].x = a.x; zs[0].y = a.y; zs[1].x = b.x; zs[1].y = b.y;
-      } else {
-        zs[0] = *reinterpret_cast<const uint4*>((const float*)p.scale + at);
-        zs[1] = *reinterpret_cast<const uint4*>((const float*)p.zero + at);
-      }
-    }
-  };
-  auto zs_values = [&](const uint4& v, float (&f)[4]) {
-    if (p.zs_f16) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-    } else {
-      f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
-    }
-  };
-  // the sums since the last call, which belong to one group, into the totals
-  auto finish_group = [&]() {
+  // the sums since the last call, which belong to the group in row `row` of stage `slot`'s scales, into the totals
+  auto finish_group = [&](int slot, int row) {
     float sc[4], z[4];
-    zs_values(zs_now[0], sc);
-    zs_values(zs_now[1], z);
+    const uint8_t* at = zs_ring + slot * 2 * zs_half + (row * WCOLS + 32 * warp + 4 * g) * p.zs_bytes;
+    if (p.zs_bytes == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + zs_half);
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+      const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), d = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+      sc[0] = a.x; sc[1] = a.y; sc[2] = b.x; sc[3] = b.y;
+      z[0] = c.x; z[1] = c.y; z[2] = d.x; z[3] = d.y;
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + zs_half);
+      sc[0] = a.x; sc[1] = a.y; sc[2] = a.z; sc[3] = a.w;
+      z[0] = b.x; z[1] = b.y; z[2] = b.z; z[3] = b.w;
+    }
 #pragma unroll
     for (int q = 0; q < (GROUPED ? NG : 1); ++q)
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                  // channel 2 tile + i / 2 of the four, token 2 t + i % 2
+          if (NT == 1 && (i & 1)) continue;            // one token row: column 0 alone
           const int c = 2 * tile + (i >> 1);
           const float v = ACCS == 2 ? fmaf(acc[q][tile][ACCS - 1][i], 0.0625f, acc[q][tile][0][i]) : acc[q][tile][0][i];
           tot[q][tile][i] = fmaf(sc[c], fmaf(-(CENTRED ? z[c] - 8.f : z[c]), accx[q][i & 1], v * T::UP), tot[q][tile][i]);
@@ -301,13 +299,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
   constexpr uint32_t ones = T::ONES;
 
   int gid = g_begin, st = st_begin;
-  int64_t group_end = 0;               // contraction index behind the current group
-  if (GROUPED) {
-    const int64_t k = (int64_t)st * (2 * ROWS);
-    group_end = (k / p.group + 1) * p.group;
-    fetch_zs(zs_now, gid, k);
-    fetch_zs(zs_next, gid, group_end);
-  }
+  int group_now = GROUPED ? st * (2 * ROWS) / p.group : 0, group_end = GROUPED ? (group_now + 1) * p.group : 0;      // current group, and the index behind it
   bool alive = true;
   for (int s = 0; s < nstage; ++s) {
     const int cg = gid;
@@ -372,12 +364,18 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     __syncwarp();
     if (alive) {
       const uint32_t tile = ring_u32 + slot * STAGE_BYTES;
-      auto steps = [&](int sl) {                     // ACCS steps of 16 contraction indices
+      auto words = [&](uint32_t (&w)[ACCS][2], int sl) {       // of ACCS steps of 16 contraction indices
+#pragma unroll
+        for (int h = 0; h < ACCS; ++h) {
+          w[h][0] = lds32(tile + (sl + h) * (8 * WCOLS) + off0);
+          w[h][1] = lds32(tile + (sl + h) * (8 * WCOLS) + off1);
+        }
+      };
+      auto steps = [&](const uint32_t (&w)[ACCS][2], int sl) {
         uint32_t a0[ACCS][4], a1[ACCS][4];         // per step: low nibbles, then high nibbles, of the two channel tiles
 #pragma unroll
         for (int h = 0; h < ACCS; ++h) {
-          const uint32_t w1 = lds32(tile + (sl + h) * (8 * WCOLS) + off0);
-          const uint32_t w2 = lds32(tile + (sl + h) * (8 * WCOLS) + off1);
+          const uint32_t w1 = w[h][0], w2 = w[h][1];
           T::template expand<CENTRED>(__byte_perm(w1, w2, 0x4400), __byte_perm(w1, w2, 0x5511), a0[h]);
           T::template expand<CENTRED>(__byte_perm(w1, w2, 0x6622), __byte_perm(w1, w2, 0x7733), a1[h]);
         }
@@ -404,21 +402,53 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
       };
       if constexpr (!GROUPED) {
 #pragma unroll
-        for (int sl = 0; sl < STEPS; sl += ACCS) steps(sl);
+        for (int sl = 0; sl < STEPS; sl += ACCS) {
+          uint32_t w[ACCS][2];
+          words(w, sl);
+          steps(w, sl);
+        }
       } else {
-        int64_t k = (int64_t)st * (2 * ROWS);
+        int k = st * (2 * ROWS);
+        const int first = k / p.group;                 // the stage's row 0 of scales
+        bool pending = false;
+        // the words of the next CB steps are read before the products of these
+        constexpr int CB = FU >= 2 ? 4 : 2, CN = CB / ACCS;
+        uint32_t w[2][CN][ACCS][2];
+        auto chunk_words = [&](uint32_t (&c)[CN][ACCS][2], int sl) {
+#pragma unroll
+          for (int i = 0; i < CN; ++i) words(c[i], sl + i * ACCS);
+        };
+        auto chunk_steps = [&](const uint32_t (&c)[CN][ACCS][2], int sl) {
+#pragma unroll
+          for (int i = 0; i < CN; ++i) steps(c[i], sl + i * ACCS);
+        };
+        chunk_words(w[0], 0);
 #pragma unroll 1
         for (int s0 = 0; s0 < STEPS; s0 += 2 * FU) {
+          if constexpr (2 * FU == 2 * CB) {
+            chunk_words(w[1], s0 + CB);
+            chunk_steps(w[0], s0);
+            if (s0 + 2 * CB < STEPS) chunk_words(w[0], s0 + 2 * CB);
+            chunk_steps(w[1], s0 + CB);
+          } else {
+            static_assert(2 * FU == CB, "a look for the group's end per chunk, or per two");
+            if (s0 + CB < STEPS) chunk_words(w[1], s0 + CB);
+            chunk_steps(w[0], s0);
 #pragma unroll
-          for (int sl = 0; sl < 2 * FU; sl += ACCS) steps(s0 + sl);
+            for (int i = 0; i < CN; ++i)
+#pragma unroll
+              for (int h = 0; h < ACCS; ++h) { w[0][i][h][0] = w[1][i][h][0]; w[0][i][h][1] = w[1][i][h][1]; }
+          }
           k += 32 * FU;
-          if (k == group_end && s0 + 2 * FU <= STEPS) {
-            finish_group();
-            zs_now[0] = zs_next[0]; zs_now[1] = zs_next[1];
+          pending = k != group_end;
+          if (!pending) {
+            finish_group(slot, group_now - first);
+            ++group_now;
             group_end += p.group;
-            fetch_zs(zs_next, gid, group_end);
           }
         }
+        // the channel group's last stage, or this CTA's: what its last group has so far
+        if (pending && (st == p.spc - 1 || s == nstage - 1)) finish_group(slot, group_now - first);
       }
       __syncwarp();
       if (lane == 0) {
@@ -439,7 +469,6 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     const bool last_of_group = (st_now == p.spc - 1) || (s == nstage - 1);
     if (!last_of_group) continue;
     if (s == nstage - 1) GTRACE(3);
-    if (GROUPED) finish_group();                     // what the last group has here (none: sums of zero)
 
     // ---- flush this warp's 32 channels of group cg ----
     // lane (g, t): tokens 2t and 2t+1; channels n0 .. n0+3 = (tile 0 row g, tile 0 row g+8, tile 1 row g, tile 1 row g+8)
@@ -533,11 +562,8 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
     clear_acc();
     if (GROUPED) {                                   // the next channel group begins at contraction index 0
       clear_tot();
+      group_now = 0;
       group_end = p.group;
-      if (s + 1 < nstage) {
-        fetch_zs(zs_now, gid, 0);
-        fetch_zs(zs_next, gid, group_end);
-      }
     }
   }
 
@@ -557,10 +583,13 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const GemvParams p) {
 
 // ------------------------------------------------------------------ host ----
 
-GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped) {
+// groups of scales that a stage of `span` contraction indices may touch
+static int gemv_zs_rows(int span, int group) { return group % span == 0 ? 1 : span % group == 0 ? span / group : span / group + 2; }
+
+GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int group, int zs_bytes) {
   GemvPlan pl;
   memset(&pl, 0, sizeof(pl));
-  const int planes = x_dtype == JGQ_F32 ? (grouped ? 3 : 2) : 1;
+  const int planes = x_dtype == JGQ_F32 ? (group ? 3 : 2) : 1;
   if (M < 1 || M > (planes > 1 ? 16 : 32) || N % 16 != 0 || K % 8 != 0) return pl;
   pl.ncg = (int)cdiv(N, WCOLS);
   if (pl.ncg * WWARPS > GV_TICKET_BYTES / (int)sizeof(int)) return pl;
@@ -570,7 +599,8 @@ GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped)
   pl.spc = (int)cdiv(K / 2, pl.rows);
   pl.S = (int64_t)pl.ncg * pl.spc;
   const int xrow = (pl.rows / 2) * 8 + 32;
-  pl.smem_bytes = GV_NST * pl.rows * WCOLS + 1024 + (WWARPS * pl.nt * planes + 1) * xrow;
+  pl.zs_rows = group ? gemv_zs_rows(2 * pl.rows, group) : 0;
+  pl.smem_bytes = GV_NST * (pl.rows * WCOLS + 2 * pl.zs_rows * WCOLS * zs_bytes) + 1024 + (WWARPS * pl.nt * planes + 1) * xrow;
   const int by_smem = (227 * 1024) / (pl.smem_bytes + 1024 + 128);
   const int per_sm = std::max(1, std::min(gemv_ctas(pl.nt, planes), by_smem));
   pl.G = (int)std::min<int64_t>(per_sm * (int64_t)sm_count(), std::max<int64_t>(1, pl.S / 2));   // one resident wave
@@ -582,11 +612,11 @@ GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped)
 }
 
 template <typename XT, int NT, typename ZST, int FU>
-static int launch_gemv_inst(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, cudaStream_t s) {
+static int launch_gemv_inst(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, const CUtensorMap& smap, const CUtensorMap& zmap, cudaStream_t s) {
   auto kern = w4_gemv_kernel<XT, NT, ZST, FU>;
   struct AttrTag {};
-  const int arc = once_per_device<AttrTag>([&]() {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem_bytes);
+  const int arc = once_per_device<AttrTag>([&]() {         // with groups the size varies: as much as any call may want
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FU ? GV_MAX_SMEM : pl.smem_bytes);
     cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);   // a hint: all of it as shared memory
     cudaGetLastError();
     return (int)e;
@@ -603,22 +633,22 @@ static int launch_gemv_inst(const GemvPlan& pl, const GemvParams& p, const CUten
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, wmap, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, wmap, smap, zmap, p);
   note_launches(1);
   if (e != cudaSuccess) { cudaGetLastError(); return fail(JGQ_ERR_CUDA, "w4_gemv: %s", cudaGetErrorString(e)); }
   return JGQ_OK;
 }
 
 template <typename XT, typename ZST, int FU>
-static int launch_gemv_type(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, cudaStream_t s) {
+static int launch_gemv_type(const GemvPlan& pl, const GemvParams& p, const CUtensorMap& wmap, const CUtensorMap& smap, const CUtensorMap& zmap, cudaStream_t s) {
   switch (pl.nt) {
-    case 1:  return launch_gemv_inst<XT, 1, ZST, FU>(pl, p, wmap, s);
-    case 2:  return launch_gemv_inst<XT, 2, ZST, FU>(pl, p, wmap, s);
-    case 4:  return launch_gemv_inst<XT, 4, ZST, FU>(pl, p, wmap, s);
-    case 8:  return launch_gemv_inst<XT, 8, ZST, FU>(pl, p, wmap, s);
-    case 16: return launch_gemv_inst<XT, 16, ZST, FU>(pl, p, wmap, s);
+    case 1:  return launch_gemv_inst<XT, 1, ZST, FU>(pl, p, wmap, smap, zmap, s);
+    case 2:  return launch_gemv_inst<XT, 2, ZST, FU>(pl, p, wmap, smap, zmap, s);
+    case 4:  return launch_gemv_inst<XT, 4, ZST, FU>(pl, p, wmap, smap, zmap, s);
+    case 8:  return launch_gemv_inst<XT, 8, ZST, FU>(pl, p, wmap, smap, zmap, s);
+    case 16: return launch_gemv_inst<XT, 16, ZST, FU>(pl, p, wmap, smap, zmap, s);
     default:
-      if constexpr (GemvType<XT>::PLANES == 1) return launch_gemv_inst<XT, 32, ZST, FU>(pl, p, wmap, s);
+      if constexpr (GemvType<XT>::PLANES == 1) return launch_gemv_inst<XT, 32, ZST, FU>(pl, p, wmap, smap, zmap, s);
       return fail(JGQ_ERR_ARG, "w4_gemv: bad plan");
   }
 }
@@ -638,18 +668,25 @@ int launch_w4_gemv(const GemvPlan& pl, const void* x, int x_dtype, const uint8_t
   p.early = settled ? 1 : 0;
   if (group > 0) {
     p.group = group;
-    p.zs_f16 = zs_dtype == JGQ_F16;
-#define JGQ_GEMV(XT) return group % 128 == 0 ? launch_gemv_type<XT, float, 4>(pl, p, wmap, s) : launch_gemv_type<XT, float, 1>(pl, p, wmap, s)
+    p.zs_bytes = dtype_size(zs_dtype);
+    p.zs_rows = pl.zs_rows;
+    CUtensorMap smap, zmap;
+    const uint64_t groups = (uint64_t)cdiv(K, group);
+    int zrc = encode_tmap_2d_zs(&smap, scale, zs_dtype, (uint64_t)N, groups, WCOLS, (uint32_t)pl.zs_rows);
+    if (!zrc) zrc = encode_tmap_2d_zs(&zmap, zero, zs_dtype, (uint64_t)N, groups, WCOLS, (uint32_t)pl.zs_rows);
+    if (zrc) return zrc;
+#define JGQ_GEMV(XT) return group % 128 == 0 ? launch_gemv_type<XT, float, 4>(pl, p, wmap, smap, zmap, s) : launch_gemv_type<XT, float, 1>(pl, p, wmap, smap, zmap, s)
     if (x_dtype == JGQ_F16) { JGQ_GEMV(__half); }
     if (x_dtype == JGQ_BF16) { JGQ_GEMV(__nv_bfloat16); }
     JGQ_GEMV(float);
 #undef JGQ_GEMV
   }
+  const CUtensorMap &smap = wmap, &zmap = wmap;            // not used
   const bool zf = zs_dtype == JGQ_F32;
-  if (x_dtype == JGQ_F16) return zf ? launch_gemv_type<__half, float, 0>(pl, p, wmap, s) : launch_gemv_type<__half, __half, 0>(pl, p, wmap, s);
+  if (x_dtype == JGQ_F16) return zf ? launch_gemv_type<__half, float, 0>(pl, p, wmap, smap, zmap, s) : launch_gemv_type<__half, __half, 0>(pl, p, wmap, smap, zmap, s);
   if (x_dtype == JGQ_BF16)
-    return zf ? launch_gemv_type<__nv_bfloat16, float, 0>(pl, p, wmap, s) : launch_gemv_type<__nv_bfloat16, __half, 0>(pl, p, wmap, s);
-  return zf ? launch_gemv_type<float, float, 0>(pl, p, wmap, s) : launch_gemv_type<float, __half, 0>(pl, p, wmap, s);
+    return zf ? launch_gemv_type<__nv_bfloat16, float, 0>(pl, p, wmap, smap, zmap, s) : launch_gemv_type<__nv_bfloat16, __half, 0>(pl, p, wmap, smap, zmap, s);
+  return zf ? launch_gemv_type<float, float, 0>(pl, p, wmap, smap, zmap, s) : launch_gemv_type<float, __half, 0>(pl, p, wmap, smap, zmap, s);
 }
 
 }  // namespace jgq

@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(256) w4_group_join_kernel(const float* __restr
 // ---- which kernel ----
 // Up to 32 rows, forward: the decode kernel (fp32 activations in passes of 16 rows).
 constexpr int64_t kGroupDecodeRows = 32, kGroupPassRows = 16;
-static bool group_decodes(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b) {
-  return !transpose_b && M <= kGroupDecodeRows && plan_w4_gemv(x_dtype == JGQ_F32 ? std::min(M, kGroupPassRows) : M, N, K, x_dtype, 1).use;
+static bool group_decodes(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b, int group) {
+  return !transpose_b && M <= kGroupDecodeRows && plan_w4_gemv(x_dtype == JGQ_F32 ? std::min(M, kGroupPassRows) : M, N, K, x_dtype, group).use;
 }
 // 16-bit activations, more rows or transposed: CTA pairs.
 static PairPlan group_pairs(int64_t M, int64_t N, int64_t K, int x_dtype, int transpose_b, int group) {
@@ -362,11 +362,12 @@ extern "C" size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int6
   const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
   size_t bytes = W4_TICKET_REGION + pl.xsum_bytes + pl.part_bytes;
   for (int dt : {JGQ_F32, JGQ_F16, JGQ_BF16}) {
-    if (group_decodes(M, N, K, dt, transpose_b))
-      for (int64_t rows : {std::min(M, kGroupPassRows), M}) {
-        const GemvPlan gp = plan_w4_gemv(rows, N, K, dt, 1);
-        if (gp.use) bytes = std::max(bytes, gp.ws_bytes);
-      }
+    if (group_decodes(M, N, K, dt, transpose_b, group_size))
+      for (int64_t rows : {std::min(M, kGroupPassRows), M})
+        for (int zb : {2, 4}) {
+          const GemvPlan gp = plan_w4_gemv(rows, N, K, dt, group_size, zb);
+          if (gp.use) bytes = std::max(bytes, gp.ws_bytes);
+        }
     const PairPlan pp = group_pairs(M, N, K, dt, transpose_b, group_size);
     if (pp.use) bytes = std::max(bytes, pp.ws_bytes);
   }
@@ -393,12 +394,12 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   JGQ_REQUIRE(ws && ws_bytes >= need, JGQ_ERR_WORKSPACE, "w4_group_matmul: workspace %zu < %zu bytes", ws_bytes, need);
   JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_group_matmul: workspace must be 256-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
-  if (group_decodes(M, N, K, x_dtype, transpose_b) && aligned(packed, 16) && aligned(x, 16) && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) &&
-      aligned(scale, 4 * zb) && aligned(zero, 4 * zb)) {
+  if (group_decodes(M, N, K, x_dtype, transpose_b, group_size) && aligned(packed, 16) && aligned(x, 16) && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) &&
+      aligned(scale, 16) && aligned(zero, 16)) {
     const int64_t step = x_dtype == JGQ_F32 ? kGroupPassRows : M;
     for (int64_t r0 = 0; r0 < M; r0 += step) {
       const int64_t rows = std::min(step, M - r0);
-      const int rc = launch_w4_gemv(plan_w4_gemv(rows, N, K, x_dtype, 1), (const char*)x + (size_t)r0 * K * xb, x_dtype, packed, zero, scale,
+      const int rc = launch_w4_gemv(plan_w4_gemv(rows, N, K, x_dtype, group_size, (int)zb), (const char*)x + (size_t)r0 * K * xb, x_dtype, packed, zero, scale,
                                     zs_dtype, (char*)out + (size_t)r0 * N * xb, rows, N, K, group_size, ws, (flags & JGQ_W4_WEIGHTS_SETTLED) != 0, s);
       if (rc) return rc;
     }

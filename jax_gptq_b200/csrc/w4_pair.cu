@@ -672,9 +672,9 @@ static int launch_pair_groups(const PairPlan& pl, PairParams& p, const void* x, 
   const uint64_t depth = (uint64_t)(transpose_b ? N : K);
   rc = encode_tmap_2d_b16(&xm, x, depth, (uint64_t)M, depth * 2, P_STAGE_K, (uint32_t)pl.nt / 2);
   if (rc) return rc;
-  rc = encode_tmap_2d_f32(&am, a, (uint64_t)N, (uint64_t)groups, (uint64_t)N * 4, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
+  rc = encode_tmap_2d_zs(&am, a, JGQ_F32, (uint64_t)N, (uint64_t)groups, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
   if (rc) return rc;
-  rc = encode_tmap_2d_f32(&bm, b, (uint64_t)N, (uint64_t)groups, (uint64_t)N * 4, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
+  rc = encode_tmap_2d_zs(&bm, b, JGQ_F32, (uint64_t)N, (uint64_t)groups, transpose_b ? P_STAGE_K : 128, (uint32_t)p.tab_rows);
   if (rc) return rc;
   if (transpose_b) return launch_pair_inst<XT, float, FMT, true, true>(pl, p, wmap, xm, am, bm, s);
   return launch_pair_inst<XT, float, FMT, false, true>(pl, p, wmap, xm, am, bm, s);

@@ -52,9 +52,10 @@ struct GemvPlan {
   size_t part_bytes;     // slices in the workspace (after the ticket region)
   size_t ws_bytes;       // tickets + slices
   int smem_bytes;        // dynamic shared memory per CTA
+  int zs_rows;           // with groups: those that a stage may touch
 };
-// group: contraction indices per scale (0: one per channel); grouped: whether there are such
-GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int grouped = 0);
+// group: contraction indices per scale (0: one per channel), of zs_bytes each
+GemvPlan plan_w4_gemv(int64_t M, int64_t N, int64_t K, int x_dtype, int group = 0, int zs_bytes = 4);
 int launch_w4_gemv(const GemvPlan& pl, const void* x, int x_dtype, const uint8_t* packed, const void* zero, const void* scale,
                    int zs_dtype, void* out, int64_t M, int64_t N, int64_t K, int group, void* ws, int settled, cudaStream_t s);
 
