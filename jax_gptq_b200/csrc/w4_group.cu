@@ -9,8 +9,8 @@
 //
 // General kernel: mma.sync with the weights as the 16-row operand, always as exact codes; what depends on the
 // group is applied to fp32 numbers, so nothing but the sums is rounded:
-//   forward      the sums of one group are finished with  total += scale * (sum - zero * xsum[m, group])  before the next
-//                group's begin; xsum comes from a small kernel in front;
+//   forward      the sums of one group are finished with  total += scale * (sum - zero * sum_k x[m, k])  before the next
+//                group's begin; the activations are summed up while they are staged;
 //   transposed   scale varies along the contraction, the group along the rows: a tile's rows lie in one group, the
 //                activations are multiplied with that group's scales while they are staged (products in fp32, split into
 //                bf16 planes), and sum_n x scale zero is summed up beside it.
@@ -18,7 +18,8 @@
 // sums truncate, so they are handed to fp32 totals at the latest every 128 indices (28672 in one chain: relative error 3.7e-5).
 // 16-bit activations enter the forward product as they are; x * scale as two bf16 planes (16 bits of the product, below
 // the result's own rounding); fp32 activations as three (all 24 bits).
-// A long contraction with few tiles is split; the slices are added in order by the kernel behind.
+// A long contraction with few tiles is split; the CTA that draws a tile's last ticket adds the slices in order (with more tiles
+// than tickets a kernel behind does).
 #include "w4_common.cuh"
 #include "w4_plans.cuh"
 #include <algorithm>
@@ -38,8 +39,8 @@ template <typename XT, bool TB> struct GroupType {                 // operand ty
 
 struct GroupParams {
   const void* x; const uint8_t* packed; const void* zero; const void* scale; void* out;
-  const float* xsum;           // forward: [M][groups]
   float* part;                 // [splits][M][rows] when the contraction is split
+  int32_t* tickets;            // one per tile, zero between launches; null: no tile is joined here
   int64_t M, N, K;
   int64_t rows, depth;         // weight rows of the product (N or K) and its contraction length (K or N)
   int group, groups;
@@ -77,20 +78,6 @@ template <> __device__ __forceinline__ uint32_t pair_bits<__nv_bfloat16>(float a
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// sums of the activations per group: xsum[m][i] = sum of x[m, i g .. i g + g - 1]; one warp per (row, group)
-template <typename XT>
-__global__ void __launch_bounds__(256) w4_group_xsum_kernel(const XT* __restrict__ x, float* __restrict__ xsum, int64_t M, int64_t K, int group, int groups) {
-  const int64_t item = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (item >= M * groups) return;
-  const int64_t m = item / groups, i = item % groups;
-  const int64_t k0 = i * group, k1 = min(K, k0 + group);
-  float s = 0.f;
-  for (int64_t k = k0 + lane; k < k1; k += 32) s += to_f32<XT>(x[m * K + k]);
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) xsum[item] = s;
-}
-
 // BM: weight rows per tile (32 or 64; in the transposed product a tile lies in one group)
 template <typename XT, typename ZST, bool TB, int BM>
 __global__ void __launch_bounds__(WG_THREADS)
@@ -104,7 +91,8 @@ w4_group_kernel(const GroupParams p) {
   constexpr int WORDS = BM * WG_KC / 8 / WG_THREADS;   // 4-byte words of codes per thread and stage
   __shared__ __align__(16) CT sa[2][AROWS * ASTRIDE];
   __shared__ __align__(16) CT sx[2][PL][WG_TOK * WG_XSTRIDE];
-  __shared__ float scz[WG_TOK];
+  __shared__ float scz[WG_TOK], sxs[2][WG_TOK];        // transposed: sum_n x scale zero; forward: a group's sums of x
+  __shared__ int s_last;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int wm = (warp % WM) * 32, wn = (warp / WM) * (WG_TOK / WN);
@@ -113,8 +101,11 @@ w4_group_kernel(const GroupParams p) {
   const int64_t c_begin = (int64_t)blockIdx.z * p.chunks_per_split, c_end = min(chunks, c_begin + p.chunks_per_split);
   const int64_t tb_group = TB ? row0 / p.group : 0;
 
+  // what a stage needs is requested a stage ahead (two ahead: 30 registers more, a CTA per SM less, up to 40 % slower)
   uint32_t wreg[WORDS];
-  float xreg[16], cz = 0.f;
+  __align__(16) XT xraw[16];                        // as loaded: first touched when they are staged
+  float s_lane = 0.f, z_lane = 0.f, cz = 0.f, xs = 0.f;
+  ZST s_raw, z_raw;                                    // transposed: scale and zero point of index `lane` of the stage
   const int xt = tid >> 1, xh = (tid & 1) * 16;        // this thread's token of the tile and half of the stage's indices
   const XT* xrow = reinterpret_cast<const XT*>(p.x) + (tok0 + xt) * p.depth;
   const bool xlive = tok0 + xt < p.M;
@@ -130,37 +121,58 @@ w4_group_kernel(const GroupParams p) {
       uint32_t w = 0;
       if (2 * br < p.K && n < p.N) {
         const uint8_t* src = p.packed + br * p.N + n;
-        if (p.vec_w) w = *reinterpret_cast<const uint32_t*>(src);       // N % 4 == 0: the word is inside the row
-        else
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (n + b < p.N) w |= (uint32_t)src[b] << (8 * b);
+        if (p.vec_w) {
+          w = *reinterpret_cast<const uint32_t*>(src);       // N % 4 == 0: the word is inside the row
+        } else {                                             // out of the one or two aligned words that hold its bytes
+          const uintptr_t at = reinterpret_cast<uintptr_t>(src);
+          const uint32_t shift = 8 * (uint32_t)(at & 3), left = (uint32_t)min((int64_t)4, p.N - n);
+          const uint32_t* lo = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+          const uint32_t w0 = lo[0], w1 = shift / 8 + left > 4 ? lo[1] : 0u;
+          w = __funnelshift_r(w0, w1, shift) & (0xffffffffu >> (8 * (4 - left)));
+        }
       }
       wreg[u] = w;
     }
     const int64_t d = d0 + xh;
     if (xlive && p.vec_x && d + 16 <= p.depth) {
-      __align__(16) XT e[16];
 #pragma unroll
-      for (int v = 0; v < (int)sizeof(XT); ++v) reinterpret_cast<uint4*>(e)[v] = reinterpret_cast<const uint4*>(xrow + d)[v];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) xreg[i] = to_f32<XT>(e[i]);
+      for (int v = 0; v < (int)sizeof(XT); ++v) reinterpret_cast<uint4*>(xraw)[v] = reinterpret_cast<const uint4*>(xrow + d)[v];
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) xreg[i] = (xlive && d + i < p.depth) ? to_f32<XT>(xrow[d + i]) : 0.f;
+      for (int i = 0; i < 16; ++i) xraw[i] = (xlive && d + i < p.depth) ? xrow[d + i] : from_f32<XT>(0.f);
     }
-    if (TB) {                                          // times this tile's scales; sum_n x scale zero beside it
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const bool in = d + i < p.depth;
-        const int64_t o = tb_group * p.N + (in ? d + i : 0);
-        xreg[i] = in ? __fmul_rn(xreg[i], zs_to_f32<ZST>(p.scale, o)) : 0.f;
-        cz = fmaf(xreg[i], zs_to_f32<ZST>(p.zero, o) - 8.f, cz);
-      }
+    if (TB) {
+      const bool in = d0 + lane < p.depth;
+      const int64_t o = tb_group * p.N + (in ? d0 + lane : 0);
+      s_raw = in ? reinterpret_cast<const ZST*>(p.scale)[o] : from_f32<ZST>(0.f);
+      z_raw = in ? reinterpret_cast<const ZST*>(p.zero)[o] : from_f32<ZST>(0.f);
     }
   };
-  auto stage = [&](int buf) {
+  auto stage = [&](int buf, int64_t c) {
     CT* a = sa[buf];
+    float xreg[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) xreg[i] = to_f32<XT>(xraw[i]);
+    if (TB) {                                          // times this tile's scales; sum_n x scale zero beside it
+      s_lane = to_f32<ZST>(s_raw);
+      z_lane = to_f32<ZST>(z_raw) - 8.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        xreg[i] = __fmul_rn(xreg[i], __shfl_sync(0xffffffffu, s_lane, xh + i));
+        cz = fmaf(xreg[i], __shfl_sync(0xffffffffu, z_lane, xh + i), cz);
+      }
+    }
+    if (!TB) {
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s4[i & 3] += xreg[i];
+      xs += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      if (c + 1 == c_end || (c + 1) * WG_KC % p.group == 0) {          // the group, or what of it lies in this slice, is complete
+        xs += __shfl_xor_sync(0xffffffffu, xs, 1);
+        if ((tid & 1) == 0) sxs[buf][xt] = xs;
+        xs = 0.f;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < WORDS; ++u) {
       const int i = tid + WG_THREADS * u;
@@ -202,9 +214,8 @@ w4_group_kernel(const GroupParams p) {
       for (int e = 0; e < 4; ++e) { acc[i][j][e] = 0.f; total[i][j][e] = 0.f; }
 
   // The sums since the last call, all of one group (transposed: of any), into the totals.  Where the group ends, or the
-  // slice, the zero point's part: a group that two slices share gives it to the one it begins in.
-  auto hand_over = [&](int64_t grp, bool ends) {
-    const bool begins = grp * p.group >= c_begin * WG_KC;
+  // slice, the zero point's part.
+  auto hand_over = [&](int64_t grp, bool ends, int buf) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -216,9 +227,8 @@ w4_group_kernel(const GroupParams p) {
         for (int j = 0; j < NTW; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int64_t m = tok0 + wn + 8 * j + 2 * q + e;
             float v = acc[i][j][2 * h + e];
-            if (!TB && ends && begins && m < p.M) v = fmaf(-z, p.xsum[m * p.groups + grp], v);
+            if (!TB && ends) v = fmaf(-z, sxs[buf][wn + 8 * j + 2 * q + e], v);
             total[i][j][2 * h + e] = TB ? total[i][j][2 * h + e] + v : fmaf(s, v, total[i][j][2 * h + e]);
             acc[i][j][2 * h + e] = 0.f;
           }
@@ -227,7 +237,7 @@ w4_group_kernel(const GroupParams p) {
 
   if (c_begin < c_end) {
     fetch(c_begin);
-    stage(0);
+    stage(0, c_begin);
   }
   __syncthreads();
   for (int64_t c = c_begin; c < c_end; ++c) {
@@ -260,9 +270,9 @@ w4_group_kernel(const GroupParams p) {
     {
       const int64_t k = (c + 1) * WG_KC;
       const bool ends = c + 1 == c_end || (!TB && k % p.group == 0);
-      if (ends || k % 128 == 0) hand_over(TB ? 0 : c * WG_KC / p.group, ends);
+      if (ends || k % 128 == 0) hand_over(TB ? 0 : c * WG_KC / p.group, ends, buf);
     }
-    if (c + 1 < c_end) stage(buf ^ 1);
+    if (c + 1 < c_end) stage(buf ^ 1, c + 1);
     __syncthreads();
   }
   if (TB) {
@@ -288,6 +298,41 @@ w4_group_kernel(const GroupParams p) {
           else reinterpret_cast<XT*>(p.out)[m * p.rows + r] = from_f32<XT>(v);
         }
     }
+  if (p.splits > 1 && p.tickets) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      int32_t* ticket = p.tickets + blockIdx.y * gridDim.x + blockIdx.x;
+      s_last = atomicAdd(ticket, 1) == p.splits - 1;
+      if (s_last) *ticket = 0;                         // ready for the next launch
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const int rows = (int)min((int64_t)BM, p.rows - row0), toks = (int)min((int64_t)WG_TOK, p.M - tok0);
+    const int64_t slice = p.M * p.rows;
+    constexpr int E = 16;                              // elements of a thread whose slices are requested together
+    for (int i0 = tid; i0 < toks * BM; i0 += E * WG_THREADS) {
+      int64_t at[E];
+      float sum[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = i0 + e * WG_THREADS, t = i / BM, r = i % BM;
+        at[e] = t < toks && r < rows ? (tok0 + t) * p.rows + row0 + r : -1;
+        sum[e] = 0.f;
+      }
+      for (int z = 0; z < p.splits; ++z) {
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = at[e] >= 0 ? __ldcg(p.part + z * slice + at[e]) : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] += v[e];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at[e] >= 0) reinterpret_cast<XT*>(p.out)[at[e]] = from_f32<XT>(sum[e]);
+    }
+  }
 }
 
 // the slices of a split contraction, added in order
@@ -312,7 +357,7 @@ static PairPlan group_pairs(int64_t M, int64_t N, int64_t K, int x_dtype, int tr
   return plan_w4_pair(M, N, K, x_dtype, transpose_b, group);
 }
 
-struct GroupPlan { int bm, tiles, mtiles, splits, chunks_per_split; size_t xsum_bytes, part_bytes; };
+struct GroupPlan { int bm, tiles, mtiles, splits, chunks_per_split; size_t part_bytes; };
 
 static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int transpose_b) {
   GroupPlan pl;
@@ -323,28 +368,23 @@ static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int tran
   // a transposed tile lies in one group; narrower tiles where the wide ones leave most SMs without one
   while (pl.bm > 32 && ((transpose_b && group % pl.bm != 0) || cdiv(rows, pl.bm) * pl.mtiles < sm_count() / 2)) pl.bm /= 2;
   pl.tiles = (int)cdiv(rows, pl.bm);
-  const int64_t want = std::max<int64_t>(1, 3 * (int64_t)sm_count() / ((int64_t)pl.tiles * pl.mtiles));
-  const int64_t splits = std::min<int64_t>({want, cdiv(chunks, 8), 64});       // at least eight stages each
+  // one resident wave of CTAs, of six stages at least
+  const int64_t want = std::max<int64_t>(1, 4 * (int64_t)sm_count() / ((int64_t)pl.tiles * pl.mtiles));
+  const int64_t splits = std::min<int64_t>({want, cdiv(chunks, 6), 32});
   pl.chunks_per_split = (int)cdiv(chunks, splits);
   pl.splits = (int)cdiv(chunks, pl.chunks_per_split);
-  pl.xsum_bytes = transpose_b ? 0 : align_up((size_t)M * cdiv(K, group) * sizeof(float), 256);
   pl.part_bytes = pl.splits > 1 ? align_up((size_t)pl.splits * M * rows * sizeof(float), 256) : 0;
   return pl;
 }
 
 template <typename XT, typename ZST, bool TB>
 static int launch_group(const GroupPlan& pl, GroupParams& p, uint8_t* ws, cudaStream_t s) {
-  if (!TB) {
-    float* xsum = reinterpret_cast<float*>(ws);
-    w4_group_xsum_kernel<XT><<<(unsigned)cdiv(p.M * p.groups, 8), 256, 0, s>>>((const XT*)p.x, xsum, p.M, p.K, p.group, p.groups);
-    JGQ_LAUNCHED();
-    p.xsum = xsum;
-  }
-  p.part = reinterpret_cast<float*>(ws + pl.xsum_bytes);
+  p.part = reinterpret_cast<float*>(ws + W4_TICKET_REGION);
+  p.tickets = (int64_t)pl.tiles * pl.mtiles <= W4_TICKET_REGION / 4 ? reinterpret_cast<int32_t*>(ws) : nullptr;
   const dim3 grid((unsigned)pl.tiles, (unsigned)pl.mtiles, (unsigned)pl.splits);
   if (pl.bm == 64) w4_group_kernel<XT, ZST, TB, 64><<<grid, WG_THREADS, 0, s>>>(p);
   else             w4_group_kernel<XT, ZST, TB, 32><<<grid, WG_THREADS, 0, s>>>(p);
-  if (pl.splits > 1) {
+  if (pl.splits > 1 && !p.tickets) {
     JGQ_LAUNCHED();
     const int64_t count = p.M * p.rows;
     w4_group_join_kernel<XT><<<(unsigned)std::min<int64_t>(cdiv(count, 256), 8 * (int64_t)sm_count()), 256, 0, s>>>(p.part, (XT*)p.out, count, pl.splits);
@@ -360,7 +400,7 @@ extern "C" size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int6
   if (M <= 0 || N <= 0 || K <= 0 || group_size <= 0) return 0;
   // over all activation types, and over the kernels that the alignment of the pointers chooses between
   const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
-  size_t bytes = W4_TICKET_REGION + pl.xsum_bytes + pl.part_bytes;
+  size_t bytes = W4_TICKET_REGION + pl.part_bytes;
   for (int dt : {JGQ_F32, JGQ_F16, JGQ_BF16}) {
     if (group_decodes(M, N, K, dt, transpose_b, group_size))
       for (int64_t rows : {std::min(M, kGroupPassRows), M})
@@ -418,7 +458,7 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   p.chunks_per_split = pl.chunks_per_split; p.splits = pl.splits;
   p.vec_w = N % 4 == 0 && aligned(packed, 4);
   p.vec_x = p.depth * xb % 16 == 0 && aligned(x, 16);
-  uint8_t* w = (uint8_t*)ws + W4_TICKET_REGION;
+  uint8_t* w = (uint8_t*)ws;
   const bool zf = zs_dtype == JGQ_F32;
 #define JGQ_GROUP(XT)                                                                                                      \
   return transpose_b ? (zf ? launch_group<XT, float, true>(pl, p, w, s) : launch_group<XT, __half, true>(pl, p, w, s))       \
