@@ -17,7 +17,9 @@
 //     (movmatrix) per 16 tokens.  The score tiles' token order is chosen so that these are the tokens of a value load.
 //   * sum(p) for denominator and excess comes from MMAs with ones, of the very p that the products use (rounded to f16:
 //     half a step of 2^-11, as an f16 result is).
-//   * running maximum and sum per row (in log2 units), fp32 accumulators; scales meet fp32 numbers only.
+//   * running maximum and sum per row (in log2 units), fp32 accumulators; scales meet fp32 numbers only.  p is rounded relative
+//     to its tile's maximum, which joins the others in fp32: the weights of a tile keep their precision however faint it
+//     is, which counts where its values are larger than others by orders of magnitude.
 //
 // Keys and values of 64 tokens are contiguous: they come by bulk copies in units of 8 KB (DW = 64: 4 KB), a ring of NSLOT
 // units ahead of their use.
@@ -253,7 +255,7 @@ kv_attend_kernel(const AttendParams p) {
     if (my_tiles > 0) {
       const bool bad = page_now < 0 || page_now >= p.pages;            // no such page: the result is NaN
       const int64_t block = (int64_t)(bad ? 0 : page_now) * p.Hkv + h;
-      ks = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+      ks = bad ? __int_as_float(0x7fc00000) : attend_key_scale(p.k_scale[block]);
       vs = p.v_scale[block];
     }
     for (int k = 0; k < my_tiles; ++k) {
@@ -264,7 +266,7 @@ kv_attend_kernel(const AttendParams p) {
       if (k + 1 < my_tiles) {
         const bool bad = page_1 < 0 || page_1 >= p.pages;
         const int64_t block = (int64_t)(bad ? 0 : page_1) * p.Hkv + h;
-        ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+        ks_next = bad ? __int_as_float(0x7fc00000) : attend_key_scale(p.k_scale[block]);
         vs_next = p.v_scale[block];
       }
       if (COLS && tile * KV_TILE >= seen_most) {       // nothing for this warp's rows
@@ -313,7 +315,7 @@ kv_attend_kernel(const AttendParams p) {
         float alpha[NT][2], psum[NT][2], vsc[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float top[2] = {-INFINITY, -INFINITY};
+          float top[2] = {-INFINITY, -INFINITY}, down[2];
           const float fs[2] = {qscale[nt][0] * ks, qscale[nt][1] * ks}, fb[2] = {qbias[nt][0] * ks, qbias[nt][1] * ks};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -330,8 +332,9 @@ kv_attend_kernel(const AttendParams p) {
             for (int x = 4; x < 32; x <<= 1) top[b] = fmaxf(top[b], __shfl_xor_sync(0xffffffffu, top[b], x));
             const float now = fmaxf(m[nt][b], top[b]), ref = now == -INFINITY ? 0.f : now;
             alpha[nt][b] = exp2_fast(m[nt][b] - ref);
+            down[b] = exp2_fast(top[b] - ref);
             m[nt][b] = now;
-            top[b] = ref;
+            if (top[b] == -INFINITY) top[b] = 0.f;
           }
           float ones[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -352,9 +355,9 @@ kv_attend_kernel(const AttendParams p) {
           }
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            l[nt][b] = fmaf(l[nt][b], alpha[nt][b], ones[b]);
+            l[nt][b] = fmaf(l[nt][b], alpha[nt][b], ones[b] * down[b]);
             psum[nt][b] = EXACT ? 0.f : -128.f * ones[b];
-            vsc[nt][b] = ones[b] == 0.f ? 0.f : vs;      // a row that sees none of the tile takes nothing of it, not even a NaN
+            vsc[nt][b] = ones[b] == 0.f ? 0.f : vs * down[b];      // a row that sees none of the tile takes nothing of it, not even a NaN
           }
         }
         bool same = true;                              // no row's maximum grew: the sums stay as they are

@@ -27,6 +27,8 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 units in the
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// a page's scale of keys: infinity spoils its page's scores as NaN does (it could pass for a token that is masked)
+__device__ __forceinline__ float attend_key_scale(float s) { return s + (s - s); }
 __device__ __forceinline__ void mma_h(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])

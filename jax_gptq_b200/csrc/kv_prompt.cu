@@ -7,10 +7,11 @@
 //   O += P V      M = 128 rows, N = DW channels: P out of tensor memory, the tile's values [channel][token] in shared memory
 // The codes become f16 whole numbers (exact); q is f16 after a power of two per row (exact for f16, and for bf16 down to
 // 2^-24 of the row's largest element).  Scales meet fp32 numbers: the keys' in the scores, the values' in the exponent,
-//   p' = 2^(score - reference + log2(v_scale 2^-w)),
-// so that p' is rounded once; w follows the exponent of v_scale (kept while v_scale stays below 2^(w + 5)).  The row's reference is
-// raised only when a score passes it by 8 (p' then stays below 2^13), O is rescaled then, by the row's thread.
-// The sum of exponentials is that of p' before its rounding, times 2^w / v_scale (two units of 2^-23 off at most, as 2^x is).
+//   p' = 2^(score + log2(v_scale) - reference),
+// so that p' is rounded once, and finest where p v_scale is largest, whatever the scales of the pages are.  The row's reference is
+// raised only when score + log2(v_scale) passes it by 12 (p' then stays below 2^12), O is rescaled then, by the row's thread.
+// The sum of exponentials has a reference of its own, the running maximum of the scores: it takes p' before the rounding, 64 of
+// them at a time, times 2^(reference - log2(v_scale) - maximum) (two units of 2^-23 off at most, as 2^x is).
 //
 // Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit).  While one
 // group's (or CTA's) softmax warps work, the other's products run.
@@ -38,8 +39,8 @@ constexpr int kp_threads(int ng) { return ng == 1 ? 320 : 384; }
 constexpr int KP_COST = 9;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
 constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
 constexpr int KP_TMEM = 256;                           // columns per group: S and P 2 x 64, O DW
-constexpr float KP_LAZY = 8.f;                         // log2 by which a score may pass its row's reference
-constexpr int KP_LAZY_V = 5;                           // and log2 by which v_scale may pass 2^w
+constexpr float KP_LAZY = 12.f;                        // log2 by which p v_scale may pass its row's reference
+constexpr float KP_FAINT = 60.f;                       // log2 below which it is as good as nothing beside the reference
 
 __host__ __device__ constexpr int kp_unit(int dw) { return 64 * dw; }
 // q, NG buffers of expanded keys and of values, the ring; the outputs of 128 rows take their place at the end of a piece
@@ -110,7 +111,7 @@ kv_prompt_kernel(const AttendParams p) {
   __shared__ int64_t s_pre[KP_THREADS + 1];
   __shared__ int64_t s_found[2];
   __shared__ float s_factor[KP_ROWS];                  // of a row's scores
-  __shared__ float2 s_ml[KP_ROWS];                     // a row's reference and sum, when its piece is done,
+  __shared__ float2 s_ml[KP_ROWS];                     // a row's maximum and sum, when its piece is done,
   __shared__ float s_inv[KP_ROWS];                     // what its outputs are multiplied by,
   __shared__ int64_t s_row[KP_ROWS];                   // and where they go
   __shared__ int s_flag, s_abort;
@@ -215,8 +216,7 @@ kv_prompt_kernel(const AttendParams p) {
     __syncthreads();
     if (idx == rg.begin) PTRACE(2);
 
-    float ref = -INFINITY, l = 0.f;                    // of a softmax thread's row
-    int w = -1000;                                     // exponent taken off v_scale, none yet
+    float ref = -INFINITY, m = -INFINITY, l = 0.f;     // of a softmax thread's row: references of O and of l
     if (warp == W_COPY) {
       // ===================== raw codes =====================
       if (lane == 0) {
@@ -343,14 +343,14 @@ kv_prompt_kernel(const AttendParams p) {
       const bool partial = 32 * warp + 32 > pc.rows;
       bool bad;
       int64_t block = nt > 0 ? block_of(pc.t_first, bad) : 0;
-      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : p.k_scale[block]) : 0.f, vs = nt > 0 ? fabsf(p.v_scale[block]) : 0.f, lv = log2f(vs);
+      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : attend_key_scale(p.k_scale[block])) : 0.f, vs = nt > 0 ? fabsf(p.v_scale[block]) : 0.f, lv = log2f(vs);
       for (int k = 0; k < nt; ++k) {
         const uint32_t c = done + k, b = c & 1;
         const int tile = pc.t_first + k;
         float ks_next = 0.f, vs_next = 0.f;
         if (k + 1 < nt) {
           block = block_of(tile + 1, bad);
-          ks_next = bad ? __int_as_float(0x7fc00000) : p.k_scale[block];
+          ks_next = bad ? __int_as_float(0x7fc00000) : attend_key_scale(p.k_scale[block]);
           vs_next = fabsf(p.v_scale[block]);
         }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&s_full[2 * grp + b], (c >> 1) & 1, abort_flag));
@@ -383,18 +383,18 @@ kv_prompt_kernel(const AttendParams p) {
         float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
         const float f = q_factor * ks;                 // not negative
         top = top == -INFINITY ? top : top * f;
-        // the reference of the row, and the exponent taken off v_scale
-        const int ev = vs > 0.f ? (int)(__float_as_uint(vs) >> 23) - 127 : w;
-        int w_now = w;
-        if (ev > w + KP_LAZY_V || w == -1000) w_now = ev == -1000 ? w : ev;
-        const float now = top > ref + KP_LAZY || ref == -INFINITY ? fmaxf(top, ref) : ref;
-        if (__any_sync(0xffffffffu, l > 0.f && (now != ref || w_now != w))) {
+        if (top > m) {
+          l *= exp2_fast(m - top);
+          m = top;
+        }
+        const float most = top == -INFINITY || vs == 0.f ? -INFINITY : top + lv;      // values of a zero scale are zero, whatever p' is
+        const float now = most > ref + KP_LAZY || ref == -INFINITY ? fmaxf(most, ref) : ref;
+        if (__any_sync(0xffffffffu, ref != -INFINITY && now != ref)) {
           // O is complete up to tile k - 1 once that product is done
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&o_done[2 * grp + (b ^ 1)], ((c - 1) >> 1) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
-          const float down = (ref == -INFINITY ? 1.f : exp2_fast(ref - now)), alpha = down * exp2_fast((float)max(w - w_now, -200));
-          if (ref != -INFINITY) l *= down;
+          const float alpha = ref == -INFINITY ? 1.f : exp2_fast(ref - now);
 #pragma unroll
           for (int d = 0; d < DW; d += 32) {
             uint32_t o[32];
@@ -407,9 +407,8 @@ kv_prompt_kernel(const AttendParams p) {
           tmem_st_wait();
         }
         ref = now;
-        w = w_now;
-        // p' = 2^(score - ref + log2(|v_scale|) - w); a zero scale counts as 2^w (its values are zero)
-        const float shift = vs == 0.f ? 0.f : lv - (w == -1000 ? 0.f : (float)w), add = (ref == -INFINITY ? 0.f : -ref) + shift;
+        // p' = 2^(score + lv - ref) = 2^(score - m - back)
+        const float back = vs == 0.f || ref == -INFINITY ? 0.f : fminf(ref - lv - m, KP_FAINT), add = (m == -INFINITY ? 0.f : -m - back) + (vs - vs);       // NaN for scales that are not finite
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -433,7 +432,7 @@ kv_prompt_kernel(const AttendParams p) {
         }
         tmem_st_wait();
         const float sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-        if (sum != 0.f) l = fmaf(sum, exp2_fast(-shift), l);
+        if (sum != 0.f) l = fmaf(sum, exp2_fast(back), l);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * grp + b]);
@@ -452,11 +451,11 @@ kv_prompt_kernel(const AttendParams p) {
     if (warp < 4 * NG && ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&o_done[2 * (warp >> 2) + (c_last & 1)], (c_last >> 1) & 1, abort_flag));
     if (!ok) l = __int_as_float(0x7fc00000);
     if (warp < 4 * NG) {
-      s_ml[tid] = make_float2(ref, l);
+      s_ml[tid] = make_float2(m, l);
       s_inv[tid] = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
       s_row[tid] = attend_out_row(p, pc, min(tid, pc.rows - 1));
     }
-    const float scale_o = w == -1000 ? 0.f : exp2_fast((float)w);
+    const float scale_o = exp2_fast(ref - m);
     for (int g0 = 0; g0 < NG && 128 * g0 < pc.rows; ++g0) {
       __syncthreads();                                 // the operands have been read, the rows before have left
       if (warp >> 2 == g0 && warp < 4 * NG) {
@@ -475,7 +474,7 @@ kv_prompt_kernel(const AttendParams p) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])};
-            dst[i] = w == -1000 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[0] * scale_o, v[1] * scale_o, v[2] * scale_o, v[3] * scale_o);
+            dst[i] = ref == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[0] * scale_o, v[1] * scale_o, v[2] * scale_o, v[3] * scale_o);
           }
         }
         tc_fence_before();
