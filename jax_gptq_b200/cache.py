@@ -38,7 +38,9 @@ def _cuda(t, name, device):
 
 
 def _vector(t, name, dtype, n, device):
-    t = _cuda(t, name, device)
+    if type(t) is torch.Tensor and t.dtype == dtype and t.get_device() == device.index and t.dim() == 1 and (n is None or t.numel() == n) and t.is_contiguous():
+        return t
+    t = _cuda(t, name, device)                       # what is wrong, or a copy
     if t.dtype != dtype:
         raise TypeError(f'{name} must be {dtype}, not {t.dtype}')
     if t.dim() != 1 or (n is not None and t.shape[0] != n):
@@ -53,25 +55,18 @@ def _device_of(device):
     return torch.device('cuda', torch.cuda.current_device()) if d.index is None else d
 
 
-def _raw_stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-class _Here:
-    """`with _here(device)`: the device is current inside; nothing to do where it is already."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def _here(device):
-    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+def _launch(index, call, *args):
+    """`call` with the current stream of device `index`, on which it runs, behind its arguments."""
+    if _current_device() == index:
+        rc = call(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, _raw_stream(index))
+    if rc:
+        check(rc)
 
 
 def stored_width(head_dim):
@@ -118,11 +113,9 @@ class PageTable:
         slots = torch.empty(max_tokens, dtype=torch.int64, device=d)
         small = torch.empty(max_tokens + 2 * n + 1, dtype=torch.int32, device=d)
         positions, cu, out = small.split_with_sizes((max_tokens, n + 1, n))
-        with _here(d):
-            check(lib.jgq_kv_reserve(self.block_table.data_ptr(), self.block_table.stride(0), self.max_pages, self.held.data_ptr(),
-                                     self.free.data_ptr(), self.free_count.data_ptr(), self.num_pages, self.page_size,
-                                     lengths.data_ptr(), added.data_ptr(), _ptr(finished), n, _ptr(slots), _ptr(positions), max_tokens,
-                                     cu.data_ptr(), out.data_ptr(), self.status.data_ptr(), _raw_stream(d)))
+        _launch(d.index, lib.jgq_kv_reserve, self.block_table.data_ptr(), self.block_table.stride(0), self.max_pages, self.held.data_ptr(),
+                self.free.data_ptr(), self.free_count.data_ptr(), self.num_pages, self.page_size, lengths.data_ptr(), added.data_ptr(),
+                _ptr(finished), n, slots.data_ptr(), positions.data_ptr(), max_tokens, cu.data_ptr(), out.data_ptr(), self.status.data_ptr())
         return Step(slots, positions, cu, out)
 
     def release(self, finished):
@@ -164,16 +157,17 @@ class KVCache:
 
     def _rows(self, t, name, heads):
         """(tensor with a contiguous last axis, dtype code) of (tokens, heads, head_dim) rows."""
-        t = _cuda(t, name, self.device)
+        if type(t) is not torch.Tensor or t.get_device() != self.device.index:
+            t = _cuda(t, name, self.device)
         if t.dtype not in _DT:
             raise TypeError(f'{name} must be float32, float16 or bfloat16, not {t.dtype}')
-        if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != self.head_dim:
+        if t.dim() != 3 or (heads is not None and t.size(1) != heads) or t.size(2) != self.head_dim:
             raise ValueError(f'{name} must have shape (tokens, {"heads" if heads is None else heads}, {self.head_dim}), not {tuple(t.shape)}')
         if t.requires_grad:
             if torch.is_grad_enabled():
                 raise ValueError(f'{name} requires a gradient; the cache has none (detach it)')
             t = t.detach()
-        return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+        return t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
 
     def write(self, k, v, slots):
         """Quantizes row t of `k` and `v` (tokens, kv_heads, head_dim) into token slot `slots[t]` (int64; page * page_size +
@@ -186,10 +180,9 @@ class KVCache:
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f'k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ')
         slots = _vector(slots, 'slots', torch.int64, k.shape[0], self.device)
-        with _here(self.device):
-            check(lib.jgq_kv_write(_ptr(k), _ptr(v), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(slots), k.shape[0],
-                                   self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                                   self.num_pages, self.page_size, self.kv_heads, self.head_dim, _raw_stream(self.device)))
+        _launch(self.device.index, lib.jgq_kv_write, k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                slots.data_ptr(), k.shape[0], self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.num_pages, self.page_size, self.kv_heads, self.head_dim)
 
     def read(self, pages, dtype=torch.float32):
         """Keys and values of the pages `pages` (int64), each (len(pages), kv_heads, page_size, head_dim) in `dtype`; NaN
@@ -198,11 +191,10 @@ class KVCache:
             raise TypeError(f'dtype must be float32, float16 or bfloat16, not {dtype}')
         pages = _vector(pages, 'pages', torch.int64, None, self.device)
         shape = (pages.shape[0], self.kv_heads, self.page_size, self.head_dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
-        with _here(self.device):
-            check(lib.jgq_kv_read(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages,
-                                  self.page_size, self.kv_heads, self.head_dim, _ptr(pages), pages.shape[0], _ptr(k), _ptr(v), _DT[dtype],
-                                  _raw_stream(self.device)))
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty(shape, dtype=dtype, device=self.device)
+        _launch(self.device.index, lib.jgq_kv_read, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.num_pages, self.page_size, self.kv_heads, self.head_dim, pages.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), _DT[dtype])
         return k, v
 
     def attend(self, q, block_table, lengths, cu_seqlens=None, max_new=None, scale=None, out=None, return_lse=False):
@@ -219,15 +211,15 @@ class KVCache:
         d = self.device
         if block_table.dim() != 2 or block_table.dtype != torch.int32:
             raise ValueError('block_table must be a 2-D int32 tensor')
-        table = _cuda(block_table, 'block_table', d)
+        table = block_table if type(block_table) is torch.Tensor and block_table.get_device() == d.index else _cuda(block_table, 'block_table', d)
         if table.stride(1) != 1 and table.shape[1] > 1:
             table = table.contiguous()
-        n, heads = table.shape[0], q.shape[1]
+        n, heads = table.size(0), q.size(1)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f'{heads} query heads are no multiple of {self.kv_heads} kv heads')
         lengths = _vector(lengths, 'lengths', torch.int32, n, d)
         if cu_seqlens is None:
-            if q.shape[0] != n:
+            if q.size(0) != n:
                 raise ValueError(f'{q.shape[0]} rows of q for {n} requests without cu_seqlens')
             most = 1
         else:
@@ -235,23 +227,31 @@ class KVCache:
             most = max(1, q.shape[0] if max_new is None else int(max_new))
         fresh = out is None
         if fresh:
-            out = torch.empty(q.shape, dtype=q.dtype, device=d)
+            out = q.new_empty(q.shape)
         else:
             _cuda(out, 'out', d)
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
                 raise ValueError(f'out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}')
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=d) if return_lse else None
-        with _here(d):
-            key = (heads, most, q.dtype)
-            need = self._ws_bytes.get(key)
-            if need is None:
-                if len(self._ws_bytes) >= 1024:
-                    self._ws_bytes.clear()
-                need = self._ws_bytes[key] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, _DT[q.dtype])
-            ws = _scratch(need, 'kv')
-            check(lib.jgq_kv_attend(_ptr(q), _DT[q.dtype], q.stride(0), q.stride(1), _ptr(out), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(),
-                                    self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages, self.page_size, _ptr(table),
-                                    table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(cu_seqlens), q.shape[0], n, most,
-                                    heads, self.kv_heads, self.head_dim, float(self.head_dim ** -0.5 if scale is None else scale),
-                                    _lib.KV_ZERO_REST if fresh else 0, ws.data_ptr(), need, _raw_stream(d)))
+        if _current_device() == d.index:
+            self._attend(q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh)
+        else:
+            with torch.cuda.device(d):
+                self._attend(q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh)
         return (out, lse) if return_lse else out
+
+    def _attend(self, q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh):
+        code, index = _DT[q.dtype], self.device.index
+        need = self._ws_bytes.get((heads, most, code))
+        if need is None:
+            if len(self._ws_bytes) >= 1024:
+                self._ws_bytes.clear()
+            need = self._ws_bytes[heads, most, code] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, code)
+        stream = _raw_stream(index)
+        rc = lib.jgq_kv_attend(q.data_ptr(), code, q.stride(0), q.stride(1), out.data_ptr(), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(),
+                               self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages, self.page_size, table.data_ptr(),
+                               table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(cu_seqlens), q.shape[0], n, most,
+                               heads, self.kv_heads, self.head_dim, float(self.head_dim ** -0.5 if scale is None else scale),
+                               _lib.KV_ZERO_REST if fresh else 0, _scratch(need, 'kv', index, stream), need, stream)
+        if rc:
+            check(rc)

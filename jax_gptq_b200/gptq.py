@@ -80,24 +80,27 @@ def _workspace(nbytes, zeroed=False, tag='ws'):
     return buf
 
 
-_capture_ws = {}
+_scratch_ws, _capture_ws = {}, {}
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
-def _scratch(nbytes, tag):
-    """A zeroed workspace of the current device and stream for kernels that leave their tickets zero.  While the stream is
-    being captured the buffer belongs to that capture (allocated and cleared inside it, once), so that no two graphs, and no
-    graph and an eager call, ever share one."""
-    dev = torch.cuda.current_device()
-    stream = torch._C._cuda_getCurrentRawStream(dev)
-    capture = lib.jgq_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
-    if not capture:
-        return _workspace(nbytes, zeroed=True, tag=tag)
+def _scratch(nbytes, tag, dev, stream):
+    """Address of a zeroed workspace of the current device `dev` and its current stream for kernels that leave their tickets
+    zero.  While the stream is being captured the buffer belongs to that capture (allocated and cleared inside it, once), so that
+    no two graphs, and no graph and an eager call, ever share one."""
     key = (dev, stream, tag)
+    if not _capturing():
+        have = _scratch_ws.get(key)
+        if have is None or have[0] < nbytes:
+            buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=torch.device('cuda', dev))
+            have = _scratch_ws[key] = (buf.numel(), buf.data_ptr(), buf)
+        return have[1]
+    capture = lib.jgq_capture_id(stream)
     owner, buf = _capture_ws.get(key, (0, None))
     if owner != capture or buf.numel() < nbytes:
         buf = torch.zeros(int(nbytes), dtype=torch.uint8, device=torch.device('cuda', dev))
         _capture_ws[key] = (capture, buf)
-    return buf
+    return buf.data_ptr()
 
 
 _ELEMENT_SIZE = {torch.float32: 4, torch.float64: 8, torch.float16: 2, torch.bfloat16: 2, torch.uint8: 1,

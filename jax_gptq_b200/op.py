@@ -73,18 +73,19 @@ def _launch(x, w, zero, scale, transpose_b):
 
 def _enqueue_groups(x, w, zero, scale, out, M, N, K, group_size, transpose_b, dev):
     need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
-    ws = _scratch(need, 'w4g')
+    stream = _raw_stream(dev)
     flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
     rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
-                                 out.data_ptr(), M, N, K, group_size, flags, ws.data_ptr(), need, _raw_stream(dev))
+                                 out.data_ptr(), M, N, K, group_size, flags, _scratch(need, 'w4g', dev, stream), need, stream)
     if rc:
         check(rc)
 
 
 def _launch_groups(x, w, zero, scale, group_size, transpose_b):
     """The product with a scale and a zero point per group of `group_size` rows of the weights."""
-    shape = x.shape
-    if len(shape) > 2:
+    shape = None
+    if x.dim() != 2:
+        shape = x.shape
         x = x.reshape(-1, shape[-1])
     if not x.is_contiguous():
         x = x.contiguous()
@@ -94,15 +95,14 @@ def _launch_groups(x, w, zero, scale, group_size, transpose_b):
     K2, out_n = (Nw, Kw) if transpose_b else (Kw, Nw)
     assert K == K2, f'Inner dim mismatch: {K} != {K2}'
     out = x.new_empty((M, out_n))
-    if M == 0:
-        return out.reshape(shape[:-1] + (out_n,))
-    dev = x.get_device()
-    if dev != _current_device():
-        with torch.cuda.device(dev):
+    if M:
+        dev = x.get_device()
+        if dev == _current_device():
             _enqueue_groups(x, w, zero, scale, out, M, Nw, Kw, group_size, transpose_b, dev)
-    else:
-        _enqueue_groups(x, w, zero, scale, out, M, Nw, Kw, group_size, transpose_b, dev)
-    return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
+        else:
+            with torch.cuda.device(dev):
+                _enqueue_groups(x, w, zero, scale, out, M, Nw, Kw, group_size, transpose_b, dev)
+    return out if shape is None else out.reshape(shape[:-1] + (out_n,))
 
 
 class _GroupMatmul(torch.autograd.Function):
@@ -153,13 +153,28 @@ def _needs_function(x, zero, scale):
             or (torch.is_grad_enabled() and (x.requires_grad or zero.requires_grad or scale.requires_grad)))
 
 
+def _group_matmul(x, w, zero, scale, group_size, transpose_b):
+    """`quantized_matmul` of contiguous CUDA tensors with groups, of the types that the kernels take."""
+    rows, channels = w.shape
+    want = (-(-2 * rows // group_size), channels)
+    if scale.shape != want or zero.shape != want:
+        _check_groups(2, 0, 2 * rows, channels, group_size, scale, zero)
+    if not (x.get_device() == w.get_device() == zero.get_device() == scale.get_device()):
+        raise ValueError(f'x is on {x.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
+    if _needs_function(x, zero, scale):
+        return _GroupMatmul.apply(x, w, zero, scale, group_size, transpose_b)
+    return _launch_groups(x, w, zero, scale, group_size, transpose_b)
+
+
 def quantized_matmul(x, quantized_matrix, transpose_b=False):
     """x @ dequant(quantized_matrix) (or its transpose); result in x's dtype.  A matrix with a ``group_size`` has a scale and
     a zero point per group of rows and channel, one without per channel."""
-    as_np = _is_np(x)
-    xd = x if type(x) is torch.Tensor and x.is_cuda else _to_dev(x)
-    if xd.dtype not in _DT:
-        xd = xd.to(torch.float32)
+    if type(x) is torch.Tensor and x.is_cuda and x.dtype in _DT:
+        as_np, xd = False, x
+    else:
+        as_np, xd = _is_np(x), _to_dev(x)
+        if xd.dtype not in _DT:
+            xd = xd.to(torch.float32)
     if getattr(quantized_matrix, 'bits', 4) == 3:
         # 3-bit storage: expanded once to the nibble layout the kernels read and kept with the matrix
         cached = getattr(quantized_matrix, '_int4', None)
@@ -179,17 +194,7 @@ def quantized_matmul(x, quantized_matrix, transpose_b=False):
     zero, scale = _on_device(zero), _on_device(scale)
     group_size = getattr(quantized_matrix, 'group_size', None)
     if group_size is not None:
-        rows, channels = w.shape
-        want = (-(-2 * rows // group_size), channels)
-        if scale.shape != want or zero.shape != want:
-            _check_groups(2, 0, 2 * rows, channels, group_size, scale, zero)
-        if not (xd.get_device() == w.get_device() == zero.get_device() == scale.get_device()):
-            raise ValueError(f'x is on {xd.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
-        if _needs_function(xd, zero, scale):
-            out = _GroupMatmul.apply(xd, w, zero, scale, group_size, bool(transpose_b))
-        else:
-            out = _launch_groups(xd, w, zero, scale, group_size, bool(transpose_b))
-        return _out(out, as_np)
+        return _out(_group_matmul(xd, w, zero, scale, group_size, bool(transpose_b)), as_np)
     if _needs_function(xd, zero, scale):
         out = _QuantizedMatmul.apply(xd, w, zero, scale, bool(transpose_b))
     else:
