@@ -18,8 +18,10 @@
 // sums truncate, so they are handed to fp32 totals at the latest every 128 indices (28672 in one chain: relative error 3.7e-5).
 // 16-bit activations enter the forward product as they are; x * scale as two bf16 planes (16 bits of the product, below
 // the result's own rounding); fp32 activations as three (all 24 bits).
-// A long contraction with few tiles is split; the CTA that draws a tile's last ticket adds the slices in order (with more tiles
-// than tickets a kernel behind does).
+// A long contraction with few tiles is split; the CTA that draws a tile's last ticket adds the slices in order.
+//
+// Bound by the legacy tensor path and what feeds it (three planes of fp32 activations): 1024 x 4096 x 4096 fp32 502 us, 205
+// TFLOP/s executed; transposed 554.  Small ones by latency: 137 x 272 x 909 fp32 13.5 us, transposed 14.8.
 #include "w4_common.cuh"
 #include "w4_plans.cuh"
 #include <algorithm>
@@ -40,7 +42,7 @@ template <typename XT, bool TB> struct GroupType {                 // operand ty
 struct GroupParams {
   const void* x; const uint8_t* packed; const void* zero; const void* scale; void* out;
   float* part;                 // [splits][M][rows] when the contraction is split
-  int32_t* tickets;            // one per tile, zero between launches; null: no tile is joined here
+  int32_t* tickets;            // one per tile of a split contraction, zero between launches
   int64_t M, N, K;
   int64_t rows, depth;         // weight rows of the product (N or K) and its contraction length (K or N)
   int group, groups;
@@ -298,7 +300,7 @@ w4_group_kernel(const GroupParams p) {
           else reinterpret_cast<XT*>(p.out)[m * p.rows + r] = from_f32<XT>(v);
         }
     }
-  if (p.splits > 1 && p.tickets) {
+  if (p.splits > 1) {
     __threadfence();
     __syncthreads();
     if (tid == 0) {
@@ -335,16 +337,6 @@ w4_group_kernel(const GroupParams p) {
   }
 }
 
-// the slices of a split contraction, added in order
-template <typename XT>
-__global__ void __launch_bounds__(256) w4_group_join_kernel(const float* __restrict__ part, XT* __restrict__ out, int64_t count, int splits) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
-    float s = 0.f;
-    for (int z = 0; z < splits; ++z) s += part[z * count + i];
-    out[i] = from_f32<XT>(s);
-  }
-}
-
 // ------------------------------------------------------------------ host ----
 // ---- which kernel ----
 // Up to 32 rows, forward: the decode kernel (fp32 activations in passes of 16 rows).
@@ -369,7 +361,8 @@ static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int tran
   while (pl.bm > 32 && ((transpose_b && group % pl.bm != 0) || cdiv(rows, pl.bm) * pl.mtiles < sm_count() / 2)) pl.bm /= 2;
   pl.tiles = (int)cdiv(rows, pl.bm);
   // one resident wave of CTAs, of six stages at least
-  const int64_t want = std::max<int64_t>(1, 4 * (int64_t)sm_count() / ((int64_t)pl.tiles * pl.mtiles));
+  const int64_t tiles = (int64_t)pl.tiles * pl.mtiles;
+  const int64_t want = tiles > W4_TICKET_REGION / 4 ? 1 : std::max<int64_t>(1, 4 * (int64_t)sm_count() / tiles);
   const int64_t splits = std::min<int64_t>({want, cdiv(chunks, 6), 32});
   pl.chunks_per_split = (int)cdiv(chunks, splits);
   pl.splits = (int)cdiv(chunks, pl.chunks_per_split);
@@ -380,15 +373,10 @@ static GroupPlan plan_group(int64_t M, int64_t N, int64_t K, int group, int tran
 template <typename XT, typename ZST, bool TB>
 static int launch_group(const GroupPlan& pl, GroupParams& p, uint8_t* ws, cudaStream_t s) {
   p.part = reinterpret_cast<float*>(ws + W4_TICKET_REGION);
-  p.tickets = (int64_t)pl.tiles * pl.mtiles <= W4_TICKET_REGION / 4 ? reinterpret_cast<int32_t*>(ws) : nullptr;
+  p.tickets = reinterpret_cast<int32_t*>(ws);
   const dim3 grid((unsigned)pl.tiles, (unsigned)pl.mtiles, (unsigned)pl.splits);
   if (pl.bm == 64) w4_group_kernel<XT, ZST, TB, 64><<<grid, WG_THREADS, 0, s>>>(p);
   else             w4_group_kernel<XT, ZST, TB, 32><<<grid, WG_THREADS, 0, s>>>(p);
-  if (pl.splits > 1 && !p.tickets) {
-    JGQ_LAUNCHED();
-    const int64_t count = p.M * p.rows;
-    w4_group_join_kernel<XT><<<(unsigned)std::min<int64_t>(cdiv(count, 256), 8 * (int64_t)sm_count()), 256, 0, s>>>(p.part, (XT*)p.out, count, pl.splits);
-  }
   return check_launch("w4_group_matmul");
 }
 

@@ -42,6 +42,8 @@
 // what its own rounding does.  The tables come from a small kernel in front and reach the expanding warps by TMA beside the
 // raw bytes.  For f16, f is the power of two that brings the largest weight of an output channel (transposed: of a
 // group) to [2^13, 2^14); the epilogue takes it off again.  One plane of activations in both directions, in their own order.
+// Tiles that leave half the pairs idle are shared along the contraction; a pair's fp32 sums go to the workspace, and the last
+// CTA of a tile joins them in order (64 rows, bf16, 11008 x 4096: 103 -> 39 us; 256 rows: 112 -> 49; transposed, 4096 x 11008: 99 -> 37).
 //
 // Measured (replayed over rotating weights): forward, 2048 x 4096 x 11008, bf16: 291 us on the single-CTA kernel, 177 with a
 // tile per pair and launch, 152 now, 1.22 PFLOP/s (of 1.67 measured with cuBLAS in a burst; 175 us in a loop of calls that
@@ -90,12 +92,15 @@ struct PairParams {
   uint32_t emask_lo, emask_hi, emagic;
   const float* inv;            // with groups: what the epilogue multiplies by, per channel (transposed: per group); null: nothing
   int group, tab_rows;         // contraction-axis indices per group, groups per stage's table (transposed: per 128 rows)
+  int splits;                  // with groups: pairs that share a tile along the contraction; above 1, a pair has one item
+  float* slices; int* tickets; // their sums [tile][split][CTA of the pair][token][128 rows], and a ticket per tile and CTA of the pair
 };
 
 struct PairItem { int rp, m0, nh; };            // row pair, first token, tiles taken together (1 or 2)
 __device__ __forceinline__ PairItem pair_item(const PairParams& p, int t) {
   PairItem s;
   s.nh = 1;
+  if (p.splits > 1) t /= p.splits;
   if (t < p.twos) {
     s.rp = t % p.nrp; s.m0 = 512 * (t / p.nrp); s.nh = 2;
   } else if (t < p.twos + p.halves) {
@@ -163,7 +168,13 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
   const int pair = blockIdx.x >> 1;
   const bool misaligned = (smem_u32(smem) & 1023u) != 0u;       // never, but nothing may be loaded then: the outputs become NaN
   const int w_end = misaligned ? 0 : p.items;                    // items pair, pair + G, ...
-  const int nst = p.nst, x_st = p.x_st;
+  const int x_st = p.x_st;
+  int nst = p.nst, st0 = 0;                                      // stages of an item, from st0 on
+  if (GR && p.splits > 1) {
+    const int s = pair % p.splits;
+    st0 = (int)((int64_t)s * p.nst / p.splits);
+    nst = (int)((int64_t)(s + 1) * p.nst / p.splits) - st0;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < P_RAW_ST; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], P_DQ_WARPS / P_A_ST); }
@@ -205,10 +216,10 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(&raw_full[rs], P_RAW_BYTES + 2 * tab);
-          if (TB) tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, st * P_STAGE_K, row0 / 2, &raw_full[rs]);
-          else    tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, row0, st * (P_STAGE_K / 2), &raw_full[rs]);
+          if (TB) tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, (st0 + st) * P_STAGE_K, row0 / 2, &raw_full[rs]);
+          else    tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, row0, (st0 + st) * (P_STAGE_K / 2), &raw_full[rs]);
           if (GR) {
-            const int cx = TB ? st * P_STAGE_K : row0, cy = (TB ? row0 : st * P_STAGE_K) / p.group;
+            const int cx = TB ? (st0 + st) * P_STAGE_K : row0, cy = (TB ? row0 : (st0 + st) * P_STAGE_K) / p.group;
             tma_load_2d(tab_ring + rs * P_TAB_BYTES, &xmap1, cx, cy, &raw_full[rs]);
             tma_load_2d(tab_ring + rs * P_TAB_BYTES + P_TAB_BYTES / 2, &zmap, cx, cy, &raw_full[rs]);
           }
@@ -239,7 +250,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           const uint32_t bar = x_full0 + (uint32_t)(xs * 8);
           for (int b = 0; b < nblk; ++b)
             tma_load_2d_pair(x_ring + xs * p.x_slot + b * p.x_blk, (p.planes == 2 && b == 1) ? &xmap1 : &xmap0,
-                             st * P_STAGE_K, sg.m0 + (p.planes == 2 ? 0 : 256 * b) + (p.nt >> 1) * (int)rank, bar);
+                             (st0 + st) * P_STAGE_K, sg.m0 + (p.planes == 2 ? 0 : 256 * b) + (p.nt >> 1) * (int)rank, bar);
         }
         __syncwarp();
         ++issued;
@@ -345,8 +356,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         if constexpr (GR) {
           // the 32 contraction-axis indices from here on lie in one group: all of a forward warp's, half of a transposed one's
           if (u == 0 || (TB && u == 2)) {
-            const int k = TB ? row0 + 16 * (u0 + u) : st * P_STAGE_K + 8 * u0;
-            const int first = (TB ? row0 : st * P_STAGE_K) / p.group;
+            const int k = TB ? row0 + 16 * (u0 + u) : (st0 + st) * P_STAGE_K + 8 * u0;
+            const int first = (TB ? row0 : (st0 + st) * P_STAGE_K) / p.group;
             const uint32_t at_tab = smem_u32(tab_ring + rs * P_TAB_BYTES) + (uint32_t)((k / p.group - first) * (TB ? P_STAGE_K : 128) * 4 +
                                                                                       (TB ? lane & 3 : lane & 7) * 64);
 #pragma unroll
@@ -454,6 +465,13 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0x7fc00000u;
           }
+          if (GR && p.splits > 1) {
+            float* dst = p.slices + ((int64_t)(2 * t + (int)rank) * p.nt + c) * 128 + 32 * q + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i < ntok) dst[i * 128] = __uint_as_float(v[i]);
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             float o;
@@ -493,6 +511,68 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     }
   }
 
+  // ===================== tiles shared along the contraction: the last of their CTAs joins the sums, in order =====================
+  if constexpr (GR) {
+    if (p.splits > 1) {
+      const int tile = pair / p.splits;
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const int got = atomicAdd(p.tickets + 2 * tile + (int)rank, 1);
+        if (got == p.splits - 1) p.tickets[2 * tile + (int)rank] = 0;
+        tmem_slot[2] = got == p.splits - 1;
+      }
+      __syncthreads();
+      if (tmem_slot[2]) {
+        __threadfence();
+        const PairItem it = pair_item(p, pair);
+        const int ntok = (int)min((int64_t)p.nt, p.M - it.m0), row_base = it.rp * 256 + 128 * (int)rank;
+        const int64_t ld = TB ? p.K : p.N, next = (int64_t)2 * p.nt * 128;
+        const float* src = p.slices + (int64_t)(2 * tile * p.splits + (int)rank) * p.nt * 128;
+        const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
+        constexpr int B = 4;                          // pieces of four rows on their way at once
+        static_assert(P_THREADS % 32 == 0, "a thread's rows are the same in all its pieces");
+        const int row = row_base + 4 * (int)(threadIdx.x & 31);
+        float f[4] = {1.f, 1.f, 1.f, 1.f};            // groups of the transposed product are multiples of 32 rows
+        if (p.inv && row < p.rows) {
+          f[0] = p.inv[TB ? row / p.group : row];
+#pragma unroll
+          for (int x = 1; x < 4; ++x) f[x] = TB ? f[0] : row + x < p.rows ? p.inv[row + x] : 1.f;
+        }
+        for (int i0 = threadIdx.x; i0 < ntok * 32; i0 += P_THREADS * B) {
+          float4 sum[B];
+#pragma unroll
+          for (int j = 0; j < B; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (int s = 0; s < p.splits; ++s) {
+            float4 v[B];
+#pragma unroll
+            for (int j = 0; j < B; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(src + s * next) + min(i0 + j * P_THREADS, ntok * 32 - 1));
+#pragma unroll
+            for (int j = 0; j < B; ++j) { sum[j].x += v[j].x; sum[j].y += v[j].y; sum[j].z += v[j].z; sum[j].w += v[j].w; }
+          }
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            const int i = i0 + j * P_THREADS;
+            if (i >= ntok * 32 || row >= p.rows) continue;
+            const float o[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
+            XT* dst = reinterpret_cast<XT*>(p.out) + (int64_t)(it.m0 + (i >> 5)) * ld + row;
+            XT e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = from_f32<XT>(o[x] * f[x]);
+            if (sizeof(XT) == 2 && wide && row + 4 <= p.rows) {
+              *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (row + x < p.rows) dst[x] = e[x];
+            }
+          }
+        }
+      }
+    }
+  }
+
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();            // the partner may still signal this CTA's barriers or read its shared memory until here
@@ -524,6 +604,16 @@ PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpos
   pl.cols = (int)(pl.planes == 2 ? 0 : cols / 2 * 2);
   pl.items = (int)(pl.twos + pl.halves + odd);
   pl.G = std::min(pairs, pl.items);
+  pl.splits = 1;
+  // With groups, tiles that leave half the pairs idle are shared along the contraction, eight stages at least per pair:
+  // the slices of a tile (128 KB per CTA and split at most) cost less than the stages they save.
+  const int64_t share = group > 0 ? std::min<int64_t>(std::min<int64_t>(pairs / tiles, 8), cdiv(pl.depth, P_STAGE_K) / 8) : 1;
+  if (share > 1) {
+    pl.splits = (int)share;
+    pl.twos = pl.halves = pl.cols = 0;
+    pl.items = pl.G = (int)(tiles * share);
+    pl.slice_bytes = (size_t)pl.items * 2 * pl.nt * 128 * sizeof(float);
+  }
   // Estimate of the forward product (see w4_pair_choice): per round the stages and the outputs of a tile, more with its
   // tokens; 0.68 us a stage for two tiles at once.
   const double nst = (double)cdiv(pl.depth, P_STAGE_K), nt = pl.nt, two = 0.68 * nst + 4.0;
@@ -537,7 +627,7 @@ PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpos
     pl.plane_bytes = align_up((size_t)cdiv(K, group) * N * sizeof(float), 256);
     pl.tok_bytes = align_up((size_t)std::max<int64_t>(N, cdiv(K, group)) * sizeof(float), 256);
   }
-  pl.ws_bytes = W4_TICKET_REGION + pl.tok_bytes + 2 * pl.plane_bytes;
+  pl.ws_bytes = W4_TICKET_REGION + pl.tok_bytes + 2 * pl.plane_bytes + pl.slice_bytes;
   pl.use = 1;
   return pl;
 }
@@ -663,6 +753,8 @@ static int launch_pair_groups(const PairPlan& pl, PairParams& p, const void* x, 
   int rc = check_launch("w4_group_tables");
   if (rc) return rc;
   p.inv = FACTOR ? inv : nullptr;
+  p.tickets = (int*)ws;
+  p.slices = (float*)(ws + W4_TICKET_REGION + pl.tok_bytes + 2 * pl.plane_bytes);
   p.group = group;
   p.tab_rows = transpose_b ? (group % 128 == 0 ? 1 : 4) : (group % P_STAGE_K == 0 ? 1 : 2);
   CUtensorMap wmap, xm, am, bm;
@@ -687,6 +779,7 @@ int launch_w4_pair(const PairPlan& pl, const void* x, int x_dtype, const uint8_t
   p.nst = (int)cdiv(pl.depth, P_STAGE_K);
   p.items = pl.items; p.twos = pl.twos; p.halves = pl.halves; p.cols = pl.cols; p.G = pl.G;
   p.nt = pl.nt;
+  p.splits = pl.splits;
   p.x_blk = pl.nt / 2 * P_STAGE_K * 2;
   p.x_slot = (pl.planes == 2 || pl.twos > 0) ? 2 * p.x_blk : p.x_blk;
   p.x_st = std::min(P_MAX_XST, P_XRING_BYTES / p.x_slot);

@@ -70,6 +70,22 @@ def test_product_and_gradient(G, M, K, N, group, x):
     check(dx, dy, w.T, size.T, dtype)
 
 
+@pytest.mark.parametrize('M,K,N,group', [(33, 5002, 272, 96), (40, 11008, 256, 32), (64, 2998, 1008, 64), (96, 1030, 4096, 128), (130, 4096, 4112, 128),
+                                         (257, 3000, 528, 32), (300, 2050, 2064, 160), (512, 8200, 256, 8224), (700, 1536, 1536, 64)])
+@pytest.mark.parametrize('x', ['f16', 'bf16'])
+def test_tiles_shared_along_the_contraction(G, M, K, N, group, x):
+    """Few tiles and a long contraction in either direction: odd numbers of stages per slice, groups that straddle the slices,
+    rows that are no multiple of four, token columns that are not full; the same bits every time."""
+    dtype = DT[x]
+    qm, w, size = matrix(G, K, N, group, seed=1)
+    gen = torch.Generator(device='cuda').manual_seed(K)
+    xs, dy = (torch.randn((M, d), generator=gen, device='cuda').to(dtype) for d in (K, N))
+    for a, flip in ((xs, False), (dy, True)):
+        got = G.quantized_matmul(a, qm, transpose_b=flip)
+        check(got, a, w.T if flip else w, size.T if flip else size, dtype)
+        assert torch.equal(G.quantized_matmul(a, qm, transpose_b=flip), got)
+
+
 @pytest.mark.parametrize('M', [1, 7, 40, 260])
 @pytest.mark.parametrize('x', ['f16', 'bf16', 'f32'])
 def test_scales_over_many_magnitudes_and_fractional_zero_points(G, M, x):
