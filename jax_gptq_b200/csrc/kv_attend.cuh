@@ -16,6 +16,7 @@ struct AttendParams {
   int64_t table_stride;
   int32_t* tickets; float* slices;
   int T, B, W, Hq, Hkv, group, D, P, pages;
+  int q_map;                   // prompts: rows of q come by TMA
   int vec_q, vec_o, vec_o8;    // 16-byte loads of q, stores of four and of eight channels are legal
   int zero_rest;               // rows behind the last sequence are zeroed
   int G;                       // CTAs
@@ -345,9 +346,75 @@ __device__ __forceinline__ void attend_join(const AttendParams& p, const AttendR
   }
 }
 
+// The same for many rows: a thread first finds a row's maximum and sum over all slices, then the sums are added with weights of
+// known size.  `at`: the rows' places in the output (shared memory), `ml`, `inv`: room for them.
+template <typename XT, int NC, int DW, int THREADS, int JP, int SL>
+__device__ __forceinline__ void attend_join_rows(const AttendParams& p, const AttendRange& g, const AttendPiece& e, int first_c, int last_c,
+                                                 const int64_t* at, float2* ml, float* inv) {
+  __syncthreads();                                     // the rows' places are known, and nothing reads ml and inv any more
+  for (int col = threadIdx.x; col < e.rows; col += THREADS) {
+    float mx = -INFINITY, den = 0.f;
+    for (int cb = first_c; cb <= last_c; cb += SL) {
+      float2 v[SL];
+#pragma unroll
+      for (int c = 0; c < SL; ++c) v[c] = __ldcg(reinterpret_cast<const float2*>(attend_slice<NC, DW>(p, g, min(cb + c, last_c), e) + NC * DW) + col);
+#pragma unroll
+      for (int c = 0; c < SL; ++c)
+        if (cb + c <= last_c) {
+          const float now = fmaxf(mx, v[c].x), ref = now == -INFINITY ? 0.f : now;
+          den = fmaf(den, exp2_fast(mx - ref), v[c].y * exp2_fast(v[c].x - ref));
+          mx = now;
+        }
+    }
+    ml[col] = make_float2(mx == -INFINITY ? 0.f : mx, den);
+    inv[col] = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
+    if (p.lse) attend_put_lse(p, at[col], mx, den);
+  }
+  __syncthreads();
+  const int count = e.rows * (DW / 4);
+  for (int i0 = threadIdx.x; i0 < count; i0 += THREADS * JP) {
+    float4 sum[JP];
+    float ref[JP];
+#pragma unroll
+    for (int j = 0; j < JP; ++j) {
+      sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      ref[j] = ml[min(i0 + j * THREADS, count - 1) / (DW / 4)].x;
+    }
+    for (int cb = first_c; cb <= last_c; cb += SL) {
+      float w[SL][JP];
+      float4 sv[SL][JP];
+#pragma unroll
+      for (int c = 0; c < SL; ++c) {
+        const float* src = attend_slice<NC, DW>(p, g, min(cb + c, last_c), e);
+#pragma unroll
+        for (int j = 0; j < JP; ++j) {
+          const int i = min(i0 + j * THREADS, count - 1);
+          w[c][j] = __ldcg(src + NC * DW + 2 * (i / (DW / 4)));
+          sv[c][j] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < SL; ++c)
+        if (cb + c <= last_c) {
+#pragma unroll
+          for (int j = 0; j < JP; ++j) {
+            const float f = exp2_fast(w[c][j] - ref[j]);
+            sum[j].x = fmaf(sv[c][j].x, f, sum[j].x); sum[j].y = fmaf(sv[c][j].y, f, sum[j].y);
+            sum[j].z = fmaf(sv[c][j].z, f, sum[j].z); sum[j].w = fmaf(sv[c][j].w, f, sum[j].w);
+          }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < JP; ++j) {
+      const int i = i0 + j * THREADS, col = i / (DW / 4);
+      if (i < count) attend_store4<XT>(p, at[col], 4 * (i % (DW / 4)), sum[j], inv[col]);
+    }
+  }
+}
+
 // the prompt kernel (kv_prompt.cu): 128 or 256 rows of q per item, 16-bit types, rows of 64 or 128 channels
 struct PromptPlan { int use, groups, G; size_t slice_bytes; };
 PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype);
-int launch_kv_prompt(const PromptPlan& pl, const AttendParams& p, int dw, int q_dtype, cudaStream_t s);
+int launch_kv_prompt(const PromptPlan& pl, AttendParams& p, int dw, int q_dtype, cudaStream_t s);
 
 }  // namespace jgq

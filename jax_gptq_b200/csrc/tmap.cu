@@ -55,6 +55,22 @@ int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_
                 swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+int encode_tmap_3d_b16(CUtensorMap* map, const void* base, const uint64_t (&dims)[3], uint64_t stride1, uint64_t stride2,
+                       uint32_t box0, uint32_t box1, uint32_t box2) {
+  EncodeTiledFn fn = encoder();
+  if (!fn) return fail(JGQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  if (!aligned(base, 16) || stride1 % 16 != 0 || stride2 % 16 != 0)
+    return fail(JGQ_ERR_ALIGN, "TMA needs a 16-byte aligned base and strides");
+  cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
+  cuuint64_t strides[2] = {stride1, stride2};
+  cuuint32_t box[3] = {box0, box1, box2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), d, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(JGQ_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return JGQ_OK;
+}
+
 int encode_tmap_2d_zs(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
   const bool f32 = dtype == JGQ_F32;
   return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, f32 ? 4 : 2, base, cols, rows,

@@ -104,6 +104,12 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       ::"r"(smem_u32(smem_dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -231,6 +237,9 @@ int encode_tmap_2d_b16(CUtensorMap* map, const void* base, uint64_t cols, uint64
                        uint32_t box_cols, uint32_t box_rows);
 int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
                       uint32_t box_cols, uint32_t box_rows, int swizzle128);
+// [d2][d1][d0] of 16-bit elements, strides in bytes; 128-byte swizzle (box0 = 64 elements)
+int encode_tmap_3d_b16(CUtensorMap* map, const void* base, const uint64_t (&dims)[3], uint64_t stride1, uint64_t stride2,
+                       uint32_t box0, uint32_t box1, uint32_t box2);
 // rows of f32 or f16 scales, not swizzled
 int encode_tmap_2d_zs(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t rows, uint32_t box_cols, uint32_t box_rows);
 
