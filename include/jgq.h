@@ -231,7 +231,7 @@ int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed,
  *     k (pages, kv_heads, page_size, DW)      v (pages, kv_heads, page_size / 64, DW, 64)      value = (byte - 128) * scale
  * jgq_kv_write: row t of k_new, v_new (tokens, kv_heads, head_dim; strides in elements, the last axis contiguous) goes to
  *     slot slots[t] = page * page_size + offset; a slot outside the cache is passed over.  The rows of one page must be
- *     consecutive rows with ascending slots (as jgq_kv_reserve makes them).  A page's scale is set when its first token is
+ *     consecutive rows with consecutive ascending slots (as jgq_kv_reserve makes them).  A page's scale is set when its first token is
  *     written and grows by powers of two when later tokens need it; the codes that are there are then rounded again.
  * jgq_kv_read: out (count, kv_heads, page_size, head_dim) of the pages index[i]; NaN where there is no such page.
  * jgq_kv_attend: q (tokens, q_heads, head_dim; strides in elements), out and lse (tokens, q_heads[, head_dim]) contiguous, lse

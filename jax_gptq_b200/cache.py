@@ -173,7 +173,8 @@ class KVCache:
         """Quantizes row t of `k` and `v` (tokens, kv_heads, head_dim) into token slot `slots[t]` (int64; page * page_size +
         offset; negative or outside the cache: nowhere).
 
-        The rows of one page must be consecutive, with ascending slots, as `PageTable.reserve` gives them.  Where a
+        The rows of one page must be consecutive rows whose slots follow one another without a gap, as `PageTable.reserve` gives
+        them (runs of one page that lie apart in one call spoil each other's codes; two calls do not).  Where a
         page's first token is written its scale is set anew; later tokens that need more make it grow by a power of two,
         and the codes that are there are rounded to it.  NaN is stored as 0, infinities as the largest code."""
         k, v = self._rows(k, 'k', self.kv_heads), self._rows(v, 'v', self.kv_heads)

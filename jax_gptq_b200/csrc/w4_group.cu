@@ -391,7 +391,7 @@ extern "C" size_t jgq_w4_group_matmul_workspace_bytes(int64_t M, int64_t N, int6
   size_t bytes = W4_TICKET_REGION + pl.part_bytes;
   for (int dt : {JGQ_F32, JGQ_F16, JGQ_BF16}) {
     if (group_decodes(M, N, K, dt, transpose_b, group_size))
-      for (int64_t rows : {std::min(M, kGroupPassRows), M})
+      for (int64_t rows : {M, std::min(M, kGroupPassRows), M % kGroupPassRows})
         for (int zb : {2, 4}) {
           const GemvPlan gp = plan_w4_gemv(rows, N, K, dt, group_size, zb);
           if (gp.use) bytes = std::max(bytes, gp.ws_bytes);
@@ -418,25 +418,38 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   JGQ_REQUIRE(x && packed && zero && scale && out, JGQ_ERR_ARG, "w4_group_matmul: null pointer");
   const size_t zb = dtype_size(zs_dtype), xb = dtype_size(x_dtype);
   JGQ_REQUIRE(aligned(x, xb) && aligned(out, xb) && aligned(zero, zb) && aligned(scale, zb), JGQ_ERR_ALIGN, "w4_group_matmul: a pointer is not aligned to its element");
-  const size_t need = jgq_w4_group_matmul_workspace_bytes(M, N, K, group_size, transpose_b);
-  JGQ_REQUIRE(ws && ws_bytes >= need, JGQ_ERR_WORKSPACE, "w4_group_matmul: workspace %zu < %zu bytes", ws_bytes, need);
+  // the kernel's own need: the entry point for it, which is asked once, covers every kernel and takes a microsecond
+  auto fits = [&](size_t need) {
+    return ws && ws_bytes >= need ? (int)JGQ_OK : fail(JGQ_ERR_WORKSPACE, "w4_group_matmul: workspace %zu < %zu bytes", ws_bytes, need);
+  };
+  int rc = fits(W4_TICKET_REGION);
+  if (rc) return rc;
   JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_group_matmul: workspace must be 256-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
-  if (group_decodes(M, N, K, x_dtype, transpose_b, group_size) && aligned(packed, 16) && aligned(x, 16) && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) &&
-      aligned(scale, 16) && aligned(zero, 16)) {
-    const int64_t step = x_dtype == JGQ_F32 ? kGroupPassRows : M;
-    for (int64_t r0 = 0; r0 < M; r0 += step) {
-      const int64_t rows = std::min(step, M - r0);
-      const int rc = launch_w4_gemv(plan_w4_gemv(rows, N, K, x_dtype, group_size, (int)zb), (const char*)x + (size_t)r0 * K * xb, x_dtype, packed, zero, scale,
-                                    zs_dtype, (char*)out + (size_t)r0 * N * xb, rows, N, K, group_size, ws, (flags & JGQ_W4_WEIGHTS_SETTLED) != 0, s);
-      if (rc) return rc;
+  const bool dense = aligned(packed, 16) && aligned(x, 16);
+  if (!transpose_b && M <= kGroupDecodeRows && dense && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) && aligned(scale, 16) && aligned(zero, 16)) {
+    const int64_t step = x_dtype == JGQ_F32 ? std::min(M, kGroupPassRows) : M;
+    const GemvPlan whole = plan_w4_gemv(step, N, K, x_dtype, group_size, (int)zb);
+    if (whole.use) {
+      const int64_t rest = M % step;                   // one pass, or two of fp32 activations
+      const GemvPlan last = rest ? plan_w4_gemv(rest, N, K, x_dtype, group_size, (int)zb) : whole;
+      rc = fits(std::max(whole.ws_bytes, last.ws_bytes));
+      for (int64_t r0 = 0; r0 < M && !rc; r0 += step) {
+        const int64_t rows = std::min(step, M - r0);
+        rc = launch_w4_gemv(rows == step ? whole : last, (const char*)x + (size_t)r0 * K * xb, x_dtype, packed, zero, scale, zs_dtype,
+                            (char*)out + (size_t)r0 * N * xb, rows, N, K, group_size, ws, (flags & JGQ_W4_WEIGHTS_SETTLED) != 0, s);
+      }
+      return rc;
     }
-    return JGQ_OK;
   }
   const PairPlan pp = group_pairs(M, N, K, x_dtype, transpose_b, group_size);
-  if (pp.use && aligned(packed, 16) && aligned(x, 16))
-    return launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, transpose_b, group_size, ws, s);
+  if (pp.use && dense) {
+    rc = fits(pp.ws_bytes);
+    return rc ? rc : launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, transpose_b, group_size, ws, s);
+  }
   const GroupPlan pl = plan_group(M, N, K, group_size, transpose_b);
+  rc = fits(W4_TICKET_REGION + pl.part_bytes);
+  if (rc) return rc;
   GroupParams p;
   memset(&p, 0, sizeof(p));
   p.x = x; p.packed = packed; p.zero = zero; p.scale = scale; p.out = out;

@@ -32,6 +32,12 @@ def _settled(w):
     return seen == w._version
 
 
+def _settled_groups(w, zero, scale):
+    """The same for weights with groups, whose scales and zero points are fetched together with the first weight tiles: all three
+    unchanged since a matmul before this one."""
+    return _settled(w) & _settled(zero) & _settled(scale)               # each is to be noted
+
+
 _ws_bytes = {}           # (device, M, N, K, transpose_b, group_size) -> workspace bytes: a function of the sizes and the device's SM count
 
 
@@ -72,9 +78,11 @@ def _launch(x, w, zero, scale, transpose_b):
 
 
 def _enqueue_groups(x, w, zero, scale, out, M, N, K, group_size, transpose_b, dev):
-    need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
+    need = _ws_bytes.get((dev, M, N, K, transpose_b, group_size))
+    if need is None:
+        need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
     stream = _raw_stream(dev)
-    flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
+    flags = _lib.W4_TRANSPOSE_B if transpose_b else _lib.W4_WEIGHTS_SETTLED if _settled_groups(w, zero, scale) else 0
     rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
                                  out.data_ptr(), M, N, K, group_size, flags, _scratch(need, 'w4g', dev, stream), need, stream)
     if rc:
@@ -183,7 +191,9 @@ def quantized_matmul(x, quantized_matrix, transpose_b=False):
             cached = to_int4_layout(quantized_matrix)
             quantized_matrix._int4 = cached
         quantized_matrix = cached
-    w = _on_device(quantized_matrix.int_weight)
+    w = quantized_matrix.int_weight
+    if not (type(w) is torch.Tensor and w.is_cuda and w.is_contiguous()):
+        w = _on_device(w)
     if w.dim() != 2 or quantized_matrix.contraction_axis != 0:
         raise ValueError('quantized_matmul expects a 2-D QuantizedMatrix packed along axis 0')
     zero, scale = quantized_matrix.zero, quantized_matrix.scale
@@ -191,7 +201,8 @@ def quantized_matmul(x, quantized_matrix, transpose_b=False):
         zero, scale = _to_dev(zero), _to_dev(scale)
         if zero.dtype not in _ZS or zero.dtype != scale.dtype:
             zero, scale = zero.to(torch.float32), scale.to(torch.float32)
-    zero, scale = _on_device(zero), _on_device(scale)
+    if not (zero.is_cuda and scale.is_cuda and zero.is_contiguous() and scale.is_contiguous()):
+        zero, scale = _on_device(zero), _on_device(scale)
     group_size = getattr(quantized_matrix, 'group_size', None)
     if group_size is not None:
         return _out(_group_matmul(xd, w, zero, scale, group_size, bool(transpose_b)), as_np)

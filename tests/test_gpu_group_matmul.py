@@ -340,3 +340,26 @@ def test_gptq_many_with_groups(G):
         _, _, wide = g.gptq(W, xs, group_size=128, return_packed=True)
         for got, ref in ((a, one), (b, one), (c, wide)):
             assert torch.equal(got.int_weight, ref.int_weight) and torch.equal(got.scale, ref.scale) and got.group_size == ref.group_size
+
+
+@pytest.mark.parametrize('M,K,N,group', [(1, 4096, 4096, 128), (5, 272, 909, 32), (17, 4096, 512, 32), (24, 2048, 1024, 64), (32, 8192, 272, 128), (40, 11008, 256, 32),
+                                         (130, 4096, 528, 128), (300, 512, 2064, 96), (700, 384, 1040, 32)])
+@pytest.mark.parametrize('x', ['f16', 'bf16', 'f32'])
+def test_a_workspace_of_the_stated_size_is_enough(G, M, K, N, group, x):
+    """Both directions, also with a pointer that keeps the call from the kernels that want alignment; nothing behind it changes."""
+    lib, code = G._lib.lib, {'f16': G._lib.F16, 'bf16': G._lib.BF16, 'f32': G._lib.F32}[x]
+    qm, w, size = matrix(G, K, N, group)
+    stream = torch.cuda.current_stream().cuda_stream
+    for flags, depth, rows in ((0, K, N), (1, N, K)):
+        xs = torch.randn((M, depth), device='cuda').to(DT[x])
+        off = torch.empty(xs.numel() + 1, dtype=xs.dtype, device='cuda')[1:].view_as(xs).copy_(xs)
+        need = lib.jgq_w4_group_matmul_workspace_bytes(M, N, K, group, flags)
+        for a in (xs, off):
+            ws = torch.zeros(need + 4096, dtype=torch.uint8, device='cuda')
+            ws[need:] = 171
+            out = torch.empty((M, rows), dtype=xs.dtype, device='cuda')
+            rc = lib.jgq_w4_group_matmul(a.data_ptr(), code, qm.int_weight.data_ptr(), qm.zero.data_ptr(), qm.scale.data_ptr(), G._lib.F32, out.data_ptr(),
+                                         M, N, K, group, flags, ws.data_ptr(), need, stream)
+            assert rc == 0, lib.jgq_last_error()
+            check(out, xs, w.T if flags else w, size.T if flags else size, DT[x])
+            assert bool((ws[need:] == 171).all()) and not bool(ws[:16384].any())

@@ -226,3 +226,25 @@ def test_a_captured_chunk_replayed_with_other_lengths(G, new):
         for q, o in zip(qs, outs):
             assert torch.equal(o, cache.attend(q, table, lengths, cu_seqlens=cu, max_new=new))
             assert bool((o[rows[-1]:] == 0).all())
+
+
+@pytest.mark.parametrize('x', ['f16', 'bf16', 'f32'])
+@pytest.mark.parametrize('new', [1, 30, 100, 300])
+@pytest.mark.parametrize('Hq,H,D', [(4, 4, 64), (8, 1, 128), (2, 2, 256)])
+def test_a_workspace_of_the_stated_size_is_enough(G, x, new, Hq, H, D):
+    """Sequences that many blocks share; nothing behind the workspace changes, its tickets are left zero."""
+    lib, code = G._lib.lib, {'f16': G._lib.F16, 'bf16': G._lib.BF16, 'f32': G._lib.F32}[x]
+    lengths = [5000, new, 3000]
+    cache, table, gen = filled(G, lengths, H, D, 64, new)
+    q = torch.randn((3 * new, Hq, D), generator=gen, device='cuda').to(DT[x])
+    n, cu = i32(lengths), i32([0, new, 2 * new, 3 * new])
+    need = lib.jgq_kv_attend_workspace_bytes(Hq, H, D, new, code)
+    ws = torch.zeros(need + 4096, dtype=torch.uint8, device='cuda')
+    ws[need:] = 171
+    out = torch.empty_like(q)
+    rc = lib.jgq_kv_attend(q.data_ptr(), code, q.stride(0), q.stride(1), out.data_ptr(), 0, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+                           cache.v_scale.data_ptr(), cache.num_pages, 64, table.data_ptr(), table.stride(0), table.shape[1], n.data_ptr(), cu.data_ptr(),
+                           3 * new, 3, new, Hq, H, D, D ** -0.5, 0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.jgq_last_error()
+    assert torch.equal(out, cache.attend(q, table, n, cu_seqlens=cu, max_new=new))
+    assert bool((ws[need:] == 171).all()) and not bool(ws[:16384].any())

@@ -28,6 +28,21 @@ def test_grouped_entry_points_refuse(jlib):  # noqa: F811
     assert lib.jgq_gptq_quantize_groups(256, 256, 256, 256, 100, 8, 32, 32, 15, 256, F32, None, 256, ws, None) == -1
 
 
+def test_scales_that_changed_are_not_fetched_early(jlib):  # noqa: F811
+    """The decode kernel may read weights, scales and zero points ahead of the stream's previous kernel only if none of them
+    changed since the matmul before."""
+    import torch
+    from jax_gptq_b200.op import _settled_groups
+    w, zero, scale = torch.zeros((64, 16), dtype=torch.uint8), torch.zeros((4, 16)), torch.ones((4, 16))
+    assert not _settled_groups(w, zero, scale) and _settled_groups(w, zero, scale)
+    for changed in (w, zero, scale):
+        changed.add_(1)
+        assert not _settled_groups(w, zero, scale) and _settled_groups(w, zero, scale)
+    scale[0].mul_(2)                                                     # through a view
+    assert not _settled_groups(w, zero, scale) and _settled_groups(w, zero, scale)
+    assert not _settled_groups(w, zero, scale.clone()) and not _settled_groups(w, zero.clone(), scale)
+
+
 def test_cache_entry_points_refuse(jlib):  # noqa: F811
     lib, F16 = jlib.lib, jlib.F16
 
@@ -91,3 +106,18 @@ def test_group_parts_cover_every_row():
             for j in range(n):
                 rows += [(r0 + j * per + x, i + j) for x in range(per)]
         assert rows == [(k, k // g) for k in range(K)]
+
+
+def test_grouped_workspaces(jlib):  # noqa: F811
+    """Workspaces without room for the tickets, none at all and misaligned ones are refused, whichever kernel the call is for."""
+    lib = jlib.lib
+    for M in (1, 5, 16, 17, 31, 32, 33, 200):
+        for K, N in ((4096, 4096), (272, 909), (11008, 256), (256, 8192)):
+            for g in (32, 128):
+                for flags in (0, 1):
+                    need = lib.jgq_w4_group_matmul_workspace_bytes(M, N, K, g, flags)
+                    assert need >= 16384
+                    for xd in (jlib.F32, jlib.F16, jlib.BF16):
+                        call = lambda ws, n: lib.jgq_w4_group_matmul(256, xd, 256, 256, 256, jlib.F32, 256, M, N, K, g, flags, ws, n, None)
+                        assert call(256, 16383) == -3 and call(None, need) == -3
+                        assert call(8, need) == -2
