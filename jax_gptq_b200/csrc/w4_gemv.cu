@@ -38,7 +38,8 @@
 //
 // Scales per group of the contraction (FU > 0): a warp keeps the sums of the current group apart and, where the group ends,
 // adds scale * (sum - zero * sum_k x) to totals, in fp32.  The scales and zero points of a stage's groups come by TMA with its
-// box (requested one group ahead by each lane instead, 8192 x 28672 took 44 us with groups of 128, 100 with 32).  FU is the number of 32-index units between two looks for a group's end: 4 where groups
+// box (requested one group ahead by each lane instead, 8192 x 28672 took 100 us with groups of 32; f16, one row, now: 36 us with groups
+// of 128, 47 of 64, 55 of 32; 29 without groups).  FU is the number of 32-index units between two looks for a group's end: 4 where groups
 // are multiples of 128, else 1.  A slice then holds the totals alone.  fp32 activations take three planes here (all 24
 // bits), and codes other than f16's enter as code - 8, which halves what the zero point takes off again.
 //
@@ -158,15 +159,20 @@ __host__ __device__ constexpr int gemv_ctas(int nt, int planes) { return nt * pl
 // rows are further such groups fed from the same expanded weights.  ROWS: byte rows per stage (64 or 128).
 // FU: see above; 0: one scale per channel.
 template <typename XT, int FU> __host__ __device__ constexpr int gemv_planes() { return std::is_same<XT, float>::value ? (FU ? 3 : 2) : 1; }
+// bf16 activations of few rows, with groups: they enter as f16, like codes without conversion, after a power of two per row and stage
+// that brings the largest to [2^13, 2^14) (what they say down to 2^-39 of it); a stage's sums are therefore finished with it.
+// 8192 x 28672, groups of 128, one row: 48 -> 38 us, four rows 54 -> 48 (eight: no gain, every warp stages every row).
+template <typename XT, int NT, int FU> __host__ __device__ constexpr bool gemv_scaled() { return FU > 0 && NT <= 4 && std::is_same<XT, __nv_bfloat16>::value; }
 template <typename XT, int NT, typename ZST, int FU>
 __global__ void __launch_bounds__(GV_THREADS, gemv_ctas(NT, gemv_planes<XT, FU>()))
 w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap smap, const __grid_constant__ CUtensorMap zmap,
                const GemvParams p) {
   using namespace umma;
-  using T = GemvType<XT>;
+  constexpr bool SCALED = gemv_scaled<XT, NT, FU>();
+  using T = GemvType<typename std::conditional<SCALED, __half, XT>::type>;
   constexpr int PL = gemv_planes<XT, FU>();
   constexpr bool GROUPED = FU > 0;
-  constexpr bool CENTRED = GROUPED && !std::is_same<XT, __half>::value;
+  constexpr bool CENTRED = GROUPED && !std::is_same<XT, __half>::value && !SCALED;
   constexpr int ROWS = gemv_rows(NT, PL);
   constexpr int STAGE_BYTES = ROWS * WCOLS;
   constexpr int STEPS = ROWS / 8;                  // 8 byte rows (16 contraction indices) per MMA step
@@ -253,6 +259,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
       for (int i = 0; i < 4; ++i) { tot[q][0][i] = 0.f; tot[q][1][i] = 0.f; }
   };
   clear_tot();
+  float down[SCALED ? NT : 1];                   // what takes the power of two of a stage's activations off again, per row
   // the sums since the last call, which belong to the group in row `row` of stage `slot`'s scales, into the totals
   auto finish_group = [&](int slot, int row) {
     float sc[4], z[4];
@@ -277,7 +284,9 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           if (NT == 1 && (i & 1)) continue;            // one token row: column 0 alone
           const int c = 2 * tile + (i >> 1);
           const float v = ACCS == 2 ? fmaf(acc[q][tile][ACCS - 1][i], 0.0625f, acc[q][tile][0][i]) : acc[q][tile][0][i];
-          tot[q][tile][i] = fmaf(sc[c], fmaf(-(CENTRED ? z[c] - 8.f : z[c]), accx[q][i & 1], v * T::UP), tot[q][tile][i]);
+          float sum = fmaf(-(CENTRED ? z[c] - 8.f : z[c]), accx[q][i & 1], v * T::UP);
+          if constexpr (SCALED) sum *= NT == 1 ? down[0] : NT == 2 ? down[i & 1] : t == 0 ? down[i & 1] : down[NT == 4 ? 2 + (i & 1) : 0];
+          tot[q][tile][i] = fmaf(sc[c], sum, tot[q][tile][i]);
         }
     clear_acc();
   };
@@ -324,6 +333,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&full_bar[slot], (s / GV_NST) & 1, abort_flag));
     if (s == 0) GTRACE(2);
     __syncwarp();                          // the previous stage's operand pairs have been read by every lane
+    float up = 1.f;
 #pragma unroll
     for (int r = 0; r < NT; ++r)
 #pragma unroll
@@ -349,8 +359,24 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           sts64(dst + NT * XROW, lo[0], lo[1]);
           if (PL == 3) sts64(dst + 2 * NT * XROW, least[0], least[1]);
         } else {
-          const uint32_t ev = __byte_perm(xv[r][h].x, xv[r][h].y, 0x5410);
-          const uint32_t od = __byte_perm(xv[r][h].x, xv[r][h].y, 0x7632);
+          uint32_t ev, od;
+          if constexpr (SCALED) {
+            if (h == 0) {
+              uint32_t top = 0;
+#pragma unroll
+              for (int j = 0; j < ROWS / 64; ++j) top = __vmaxu2(top, __vmaxu2(xv[r][j].x & 0x7fff7fffu, xv[r][j].y & 0x7fff7fffu));
+              const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)) >> 7, 14u), 254u);
+              up = __uint_as_float((267u - e) << 23);
+              down[r] = __uint_as_float((e - 13u) << 23);
+            }
+            const __half2 a = __floats2half2_rn(__uint_as_float(xv[r][h].x << 16) * up, __uint_as_float(xv[r][h].y << 16) * up);
+            const __half2 b = __floats2half2_rn(__uint_as_float(xv[r][h].x & 0xffff0000u) * up, __uint_as_float(xv[r][h].y & 0xffff0000u) * up);
+            ev = *reinterpret_cast<const uint32_t*>(&a);
+            od = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            ev = __byte_perm(xv[r][h].x, xv[r][h].y, 0x5410);
+            od = __byte_perm(xv[r][h].x, xv[r][h].y, 0x7632);
+          }
           if constexpr (ACCS == 2) {
             // pair `lane & 3` of step lane / 4: 8 bytes per pair for two steps
             const uint32_t dst2 = xs_warp + r * XROW + h * 128 + (lane >> 3) * 32 + (lane & 3) * 8 + ((lane >> 2) & 1) * 4;
@@ -448,7 +474,7 @@ w4_gemv_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           }
         }
         // the channel group's last stage, or this CTA's: what its last group has so far
-        if (pending && (st == p.spc - 1 || s == nstage - 1)) finish_group(slot, group_now - first);
+        if (pending && (SCALED || st == p.spc - 1 || s == nstage - 1)) finish_group(slot, group_now - first);
       }
       __syncwarp();
       if (lane == 0) {

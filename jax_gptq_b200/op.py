@@ -35,7 +35,10 @@ def _settled(w):
 def _settled_groups(w, zero, scale):
     """The same for weights with groups, whose scales and zero points are fetched together with the first weight tiles: all three
     unchanged since a matmul before this one."""
-    return _settled(w) & _settled(zero) & _settled(scale)               # each is to be noted
+    try:
+        return _settled(w) & _settled(zero) & _settled(scale)           # each is to be noted
+    except RuntimeError:                                                # tensors made in inference mode have no version
+        return False
 
 
 _ws_bytes = {}           # (device, M, N, K, transpose_b, group_size) -> workspace bytes: a function of the sizes and the device's SM count

@@ -363,3 +363,28 @@ def test_a_workspace_of_the_stated_size_is_enough(G, M, K, N, group, x):
             assert rc == 0, lib.jgq_last_error()
             check(out, xs, w.T if flags else w, size.T if flags else size, DT[x])
             assert bool((ws[need:] == 171).all()) and not bool(ws[:16384].any())
+
+
+@pytest.mark.parametrize('M', [1, 40])
+def test_in_inference_mode(G, M):
+    with torch.inference_mode():
+        qm, w, size = matrix(G, 256, 64, 64)
+        xs = torch.randn((M, 256), device='cuda').half()
+        for _ in range(2):
+            check(G.quantized_matmul(xs, qm), xs, w, size, torch.float16)
+
+
+def test_scales_changed_just_before_a_call(G):
+    """Decode products with scales and zero points that a kernel on the same stream has just written."""
+    qm, w, size = matrix(G, 4096, 2048, 64)
+    xs = torch.randn((1, 4096), device='cuda').half() / 8
+    base, ones = G.quantized_matmul(xs, qm), torch.ones_like(qm.scale)
+    scale = qm.scale.clone()
+    for i in range(30):
+        for _ in range(i % 3):
+            G.quantized_matmul(xs, qm)
+        f = 2.0 ** ((i % 7) - 3)
+        torch.mul(scale, ones * f, out=qm.scale)
+        assert torch.equal(G.quantized_matmul(xs, qm), (base.float() * f).half()) or f < 1      # subnormals round
+        if f < 1:
+            assert float((G.quantized_matmul(xs, qm).float() - base.float() * f).abs().max()) <= float(base.abs().max()) * f * 2.0 ** -10

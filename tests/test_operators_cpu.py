@@ -41,6 +41,9 @@ def test_scales_that_changed_are_not_fetched_early(jlib):  # noqa: F811
     scale[0].mul_(2)                                                     # through a view
     assert not _settled_groups(w, zero, scale) and _settled_groups(w, zero, scale)
     assert not _settled_groups(w, zero, scale.clone()) and not _settled_groups(w, zero.clone(), scale)
+    with torch.inference_mode():                                         # no version counter: never early
+        made = torch.ones((4, 16))
+    assert not _settled_groups(w, zero, made) and not _settled_groups(w, zero, made)
 
 
 def test_cache_entry_points_refuse(jlib):  # noqa: F811
