@@ -42,8 +42,11 @@
 // what its own rounding does.  The tables come from a small kernel in front and reach the expanding warps by TMA beside the
 // raw bytes.  For f16, f is the power of two that brings the largest weight of an output channel (transposed: of a
 // group) to [2^13, 2^14); the epilogue takes it off again.  One plane of activations in both directions, in their own order.
-// Tiles that leave half the pairs idle are shared along the contraction; a pair's fp32 sums go to the workspace, and the last
-// CTA of a tile joins them in order (64 rows, bf16, 11008 x 4096: 103 -> 39 us; 256 rows: 112 -> 49; transposed, 4096 x 11008: 99 -> 37).
+// What leaves half the pairs idle is cut along the contraction: a pair's fp32 sums go to the workspace in units of 32 rows x 32 (or
+// 64) tokens with a ticket each, and the warp that brings a unit's last part adds the parts in order; parts begin with different
+// units, so that the joins are spread (one join per CTA: 5 to 10 us more at 256 tokens).  64 rows, bf16, 11008 x 4096: 103 -> 37 us;
+// 256 rows: 112 -> 47; 1024 rows: 120 -> 96; transposed, 4096 x 11008, 64 rows: 99 -> 37.
+// 2048 rows, 4096 x 11008, groups of 128: 162 us (152 without groups); 1024 rows, 11008 x 4096, groups of 64, both directions: 196.
 //
 // Measured (replayed over rotating weights): forward, 2048 x 4096 x 11008, bf16: 291 us on the single-CTA kernel, 177 with a
 // tile per pair and launch, 152 now, 1.22 PFLOP/s (of 1.67 measured with cuBLAS in a burst; 175 us in a loop of calls that
@@ -92,15 +95,24 @@ struct PairParams {
   uint32_t emask_lo, emask_hi, emagic;
   const float* inv;            // with groups: what the epilogue multiplies by, per channel (transposed: per group); null: nothing
   int group, tab_rows;         // contraction-axis indices per group, groups per stage's table (transposed: per 128 rows)
-  int splits;                  // with groups: pairs that share a tile along the contraction; above 1, a pair has one item
-  float* slices; int* tickets; // their sums [tile][split][CTA of the pair][token][128 rows], and a ticket per tile and CTA of the pair
+  // with groups: items from `whole` on are cut into `splits` along the contraction; a pair has at most one such, its last
+  int whole, splits;
+  float* slices; int* tickets; // their sums [item][CTA of the pair][tile][32 tokens][32 rows][8][row][4 tokens], and a ticket per unit
+  int unit;                    // of 32 rows x this many tokens, 32 or 64
 };
 
-struct PairItem { int rp, m0, nh; };            // row pair, first token, tiles taken together (1 or 2)
+struct PairItem { int rp, m0, nh, st0, nst; };  // row pair, first token, tiles taken together (1 or 2), stages
 __device__ __forceinline__ PairItem pair_item(const PairParams& p, int t) {
   PairItem s;
   s.nh = 1;
-  if (p.splits > 1) t /= p.splits;
+  s.st0 = 0;
+  s.nst = p.nst;
+  if (p.splits > 1 && t >= p.whole) {
+    const int c = (t - p.whole) % p.splits;
+    t = p.whole + (t - p.whole) / p.splits;
+    s.st0 = (int)((int64_t)c * p.nst / p.splits);
+    s.nst = (int)((int64_t)(c + 1) * p.nst / p.splits) - s.st0;
+  }
   if (t < p.twos) {
     s.rp = t % p.nrp; s.m0 = 512 * (t / p.nrp); s.nh = 2;
   } else if (t < p.twos + p.halves) {
@@ -169,12 +181,6 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
   const bool misaligned = (smem_u32(smem) & 1023u) != 0u;       // never, but nothing may be loaded then: the outputs become NaN
   const int w_end = misaligned ? 0 : p.items;                    // items pair, pair + G, ...
   const int x_st = p.x_st;
-  int nst = p.nst, st0 = 0;                                      // stages of an item, from st0 on
-  if (GR && p.splits > 1) {
-    const int s = pair % p.splits;
-    st0 = (int)((int64_t)s * p.nst / p.splits);
-    nst = (int)((int64_t)(s + 1) * p.nst / p.splits) - st0;
-  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < P_RAW_ST; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], P_DQ_WARPS / P_A_ST); }
@@ -211,15 +217,15 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     for (int t = pair; t < w_end && ok; t += p.G) {
       const PairItem sg = pair_item(p, t);
       const int row0 = sg.rp * 256 + 128 * (int)rank;
-      for (int st = 0; st < nst; ++st) {
+      for (int st = 0; st < sg.nst; ++st) {
         if (issued >= P_RAW_ST) ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[rs], rph ^ 1, abort_flag));
         if (!ok) break;
         if (lane == 0) {
           mbar_expect_tx(&raw_full[rs], P_RAW_BYTES + 2 * tab);
-          if (TB) tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, (st0 + st) * P_STAGE_K, row0 / 2, &raw_full[rs]);
-          else    tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, row0, (st0 + st) * (P_STAGE_K / 2), &raw_full[rs]);
+          if (TB) tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, (sg.st0 + st) * P_STAGE_K, row0 / 2, &raw_full[rs]);
+          else    tma_load_2d(raw_ring + rs * P_RAW_BYTES, &wmap, row0, (sg.st0 + st) * (P_STAGE_K / 2), &raw_full[rs]);
           if (GR) {
-            const int cx = TB ? (st0 + st) * P_STAGE_K : row0, cy = (TB ? row0 : (st0 + st) * P_STAGE_K) / p.group;
+            const int cx = TB ? (sg.st0 + st) * P_STAGE_K : row0, cy = (TB ? row0 : (sg.st0 + st) * P_STAGE_K) / p.group;
             tma_load_2d(tab_ring + rs * P_TAB_BYTES, &xmap1, cx, cy, &raw_full[rs]);
             tma_load_2d(tab_ring + rs * P_TAB_BYTES + P_TAB_BYTES / 2, &zmap, cx, cy, &raw_full[rs]);
           }
@@ -242,7 +248,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     for (int t = pair; t < w_end && ok; t += p.G) {
       const PairItem sg = pair_item(p, t);
       const int nblk = p.planes == 2 ? 2 : sg.nh;
-      for (int st = 0; st < nst; ++st) {
+      for (int st = 0; st < sg.nst; ++st) {
         if (issued >= x_st) ok = __all_sync(0xffffffffu, mbar_wait(&x_empty[xs], xph ^ 1, abort_flag));
         if (!ok) break;
         if (lane == 0) {
@@ -250,7 +256,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           const uint32_t bar = x_full0 + (uint32_t)(xs * 8);
           for (int b = 0; b < nblk; ++b)
             tma_load_2d_pair(x_ring + xs * p.x_slot + b * p.x_blk, (p.planes == 2 && b == 1) ? &xmap1 : &xmap0,
-                             (st0 + st) * P_STAGE_K, sg.m0 + (p.planes == 2 ? 0 : 256 * b) + (p.nt >> 1) * (int)rank, bar);
+                             (sg.st0 + st) * P_STAGE_K, sg.m0 + (p.planes == 2 ? 0 : 256 * b) + (p.nt >> 1) * (int)rank, bar);
         }
         __syncwarp();
         ++issued;
@@ -281,7 +287,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
           if (use + h >= 2)
             ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[(use + h) & 1], ((uint32_t)((use + h) >> 1) & 1u) ^ 1u, abort_flag));
         tc_fence_after();
-        for (int st = 0; st < nst && ok; ++st) {
+        for (int st = 0; st < sg.nst && ok; ++st) {
           ok = __all_sync(0xffffffffu, mbar_wait(&x_full[xs], xph, abort_flag) && mbar_wait_cluster(&a_full[as], aph, abort_flag));
           if (!ok) break;
           tc_fence_after();
@@ -298,7 +304,7 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             }
             mma_commit_pair(my_a + (uint32_t)(as * 8)); mma_commit_pair(peer_a + (uint32_t)(as * 8));
             mma_commit_pair(my_x + (uint32_t)(xs * 8)); mma_commit_pair(peer_x + (uint32_t)(xs * 8));
-            if (st + 1 == nst)
+            if (st + 1 == sg.nst)
               for (int h = 0; h < sg.nh; ++h) {
                 const uint32_t o = (uint32_t)(((use + h) & 1) * 8);
                 mma_commit_pair(my_acc + o); mma_commit_pair(peer_acc + o);
@@ -322,9 +328,13 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     bool ok = true;
     int rs = as;
     uint32_t rph = 0, aph = 0;
-    int row0 = 0, st = as, t_now = pair - p.G;         // with groups: the tile's first row, and where in its item the stage is
-    if (GR) st += nst;                                 // (the first step takes the first item)
-    const int total = pair < w_end ? (w_end - 1 - pair) / p.G * nst + nst : 0;      // stages of all items
+    // with groups: the tile's first row, and where in its item the stage is (the first step takes the first item)
+    int row0 = 0, st = as + p.nst, t_now = pair - p.G;
+    PairItem sg;
+    sg.st0 = 0;
+    sg.nst = p.nst;
+    const int before = pair < w_end ? (w_end - 1 - pair) / p.G : 0;                 // items but the last
+    const int total = pair < w_end ? before * p.nst + pair_item(p, pair + before * p.G).nst : 0;      // stages of all items
     for (int i = as; i < total; i += P_A_ST) {
       ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[rs], rph, abort_flag));
       if (!ok) break;
@@ -343,10 +353,11 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
       }
       uint8_t* at = a_ring + as * P_A_BYTES;
       if (GR) {
-        while (st >= nst) {
-          st -= nst;
+        while (st >= sg.nst) {
+          st -= sg.nst;
           t_now += p.G;
-          row0 = pair_item(p, t_now).rp * 256 + 128 * (int)rank;
+          sg = pair_item(p, t_now);
+          row0 = sg.rp * 256 + 128 * (int)rank;
         }
       }
       float ta[GR ? 16 : 1], tb[GR ? 16 : 1];          // the tables' entries of this lane's 16 channels
@@ -356,8 +367,8 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         if constexpr (GR) {
           // the 32 contraction-axis indices from here on lie in one group: all of a forward warp's, half of a transposed one's
           if (u == 0 || (TB && u == 2)) {
-            const int k = TB ? row0 + 16 * (u0 + u) : (st0 + st) * P_STAGE_K + 8 * u0;
-            const int first = (TB ? row0 : (st0 + st) * P_STAGE_K) / p.group;
+            const int k = TB ? row0 + 16 * (u0 + u) : (sg.st0 + st) * P_STAGE_K + 8 * u0;
+            const int first = (TB ? row0 : (sg.st0 + st) * P_STAGE_K) / p.group;
             const uint32_t at_tab = smem_u32(tab_ring + rs * P_TAB_BYTES) + (uint32_t)((k / p.group - first) * (TB ? P_STAGE_K : 128) * 4 +
                                                                                       (TB ? lane & 3 : lane & 7) * 64);
 #pragma unroll
@@ -439,6 +450,91 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
       if (!GR && !TB && row < p.rows) { sc = zs_to_f32<ZST>(p.scale, row); zr = zs_to_f32<ZST>(p.zero, row); }
       const int piece = lane % LT, n_left = p.rows - row32 - piece * V;
       const bool wide = n_left >= V && (ld * (int64_t)sizeof(XT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+      // 32 tokens of this warp's rows, from m on, by way of its buffer
+      auto emit = [&](int64_t m, int count) {
+        __syncwarp();
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += TPW) {
+          const int i = i0 + lane / LT;
+          if (i < count) {
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + i * P_OUT_STRIDE + piece * 16);
+            XT* dst = reinterpret_cast<XT*>(p.out) + (m + i) * ld + row32 + piece * V;
+            if (wide) {
+              *reinterpret_cast<uint4*>(dst) = w;
+            } else {
+              const XT* e = reinterpret_cast<const XT*>(&w);
+#pragma unroll
+              for (int x = 0; x < V; ++x)
+                if (x < n_left) dst[x] = e[x];
+            }
+          }
+        }
+        __syncwarp();
+      };
+      if constexpr (GR) {
+        if (p.splits > 1 && t >= p.whole) {
+          // The sums of this pair's part go to the workspace, 32 rows x 64 tokens at a time; the warp that brings a unit's last
+          // part adds all of them in order.  The parts begin with different units, so that the joins are spread.
+          const bool done = __all_sync(0xffffffffu, mbar_wait_long(&acc_full[2], 0u, abort_flag));
+          tc_fence_after();
+          const int part = (t - p.whole) % p.splits, first = t - part, units_h = (p.nt + p.unit - 1) / p.unit, units = it.nh * units_h;
+          const int64_t tile_floats = (int64_t)p.nt * 128, part_floats = 2 * it.nh * tile_floats;
+          float4* base = reinterpret_cast<float4*>(p.slices + (first - p.whole) * part_floats + (int64_t)rank * it.nh * tile_floats) + 256 * q + lane;
+          int* ticket0 = p.tickets + (((first - p.whole) / p.splits * 2 + (int)rank) * 4 + q) * units;
+          for (int n = share; n < units; n += 3) {
+            const int unit = (n + part * units / p.splits) % units, h = unit / units_h, c0 = unit % units_h * p.unit, m0 = it.m0 + 256 * h;
+            const int ntok = (int)min((int64_t)p.nt, p.M - m0), c_end = min(c0 + p.unit, ntok);
+            float4* tile = base + h * (tile_floats / 4);
+#pragma unroll 1
+            for (int c = c0; c < c_end; c += 32) {
+              uint32_t v[32];
+              if (done) {
+                tmem_ld_32x32(tmem_acc + (uint32_t)(256 * h) + ((uint32_t)(32 * q) << 16) + (uint32_t)c, v);
+                tmem_ld_wait();
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0x7fc00000u;
+              }
+              float4* dst = tile + part * (part_floats / 4) + c * 32;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[32 * i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            }
+            __threadfence();
+            __syncwarp();
+            int last = 0;
+            if (lane == 0) {
+              last = atomicAdd(ticket0 + unit, 1) == p.splits - 1;
+              if (last) ticket0[unit] = 0;               // ready for the next launch
+            }
+            if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+            __threadfence();
+#pragma unroll 1
+            for (int c = c0; c < c_end; c += 32) {
+              float4 sum[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              const float4* src = tile + c * 32;
+#pragma unroll 2
+              for (int k = 0; k < p.splits; ++k, src += part_floats / 4) {
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __ldcg(src + 32 * i);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { sum[i].x += v[i].x; sum[i].y += v[i].y; sum[i].z += v[i].z; sum[i].w += v[i].w; }
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float4 v = sum[i / 4];
+                *reinterpret_cast<XT*>(buf + i * P_OUT_STRIDE + lrow * (int)sizeof(XT)) = from_f32<XT>((i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w) * sc);
+              }
+              emit(m0 + c, ntok - c);
+            }
+          }
+          tc_fence_before();
+          continue;
+        }
+      }
       for (int h = 0; h < it.nh; ++h, ++use) {
         const int b = use & 1, m0 = it.m0 + 256 * h;
         // A helper has not followed acc_full's phases and could take an earlier one for the last: it waits for the end.
@@ -465,13 +561,6 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0x7fc00000u;
           }
-          if (GR && p.splits > 1) {
-            float* dst = p.slices + ((int64_t)(2 * t + (int)rank) * p.nt + c) * 128 + 32 * q + lane;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c + i < ntok) dst[i * 128] = __uint_as_float(v[i]);
-            continue;
-          }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             float o;
@@ -485,90 +574,11 @@ w4_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             }
             *reinterpret_cast<XT*>(buf + i * P_OUT_STRIDE + lrow * (int)sizeof(XT)) = from_f32<XT>(o);
           }
-          __syncwarp();
-#pragma unroll
-          for (int i0 = 0; i0 < 32; i0 += TPW) {
-            const int i = i0 + lane / LT;
-            if (c + i < ntok) {
-              const uint4 w = *reinterpret_cast<const uint4*>(buf + i * P_OUT_STRIDE + piece * 16);
-              XT* dst = reinterpret_cast<XT*>(p.out) + (int64_t)(m0 + c + i) * ld + row32 + piece * V;
-              if (wide) {
-                *reinterpret_cast<uint4*>(dst) = w;
-              } else {
-                const XT* e = reinterpret_cast<const XT*>(&w);
-#pragma unroll
-                for (int x = 0; x < V; ++x)
-                  if (x < n_left) dst[x] = e[x];
-              }
-            }
-          }
-          __syncwarp();
+          emit(m0 + c, ntok - c);
         }
         tc_fence_before();
         __syncwarp();
         if (!helper && lane == 0) mbar_arrive_cluster(acc_empty0 + (uint32_t)(b * 8));
-      }
-    }
-  }
-
-  // ===================== tiles shared along the contraction: the last of their CTAs joins the sums, in order =====================
-  if constexpr (GR) {
-    if (p.splits > 1) {
-      const int tile = pair / p.splits;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const int got = atomicAdd(p.tickets + 2 * tile + (int)rank, 1);
-        if (got == p.splits - 1) p.tickets[2 * tile + (int)rank] = 0;
-        tmem_slot[2] = got == p.splits - 1;
-      }
-      __syncthreads();
-      if (tmem_slot[2]) {
-        __threadfence();
-        const PairItem it = pair_item(p, pair);
-        const int ntok = (int)min((int64_t)p.nt, p.M - it.m0), row_base = it.rp * 256 + 128 * (int)rank;
-        const int64_t ld = TB ? p.K : p.N, next = (int64_t)2 * p.nt * 128;
-        const float* src = p.slices + (int64_t)(2 * tile * p.splits + (int)rank) * p.nt * 128;
-        const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0;
-        constexpr int B = 4;                          // pieces of four rows on their way at once
-        static_assert(P_THREADS % 32 == 0, "a thread's rows are the same in all its pieces");
-        const int row = row_base + 4 * (int)(threadIdx.x & 31);
-        float f[4] = {1.f, 1.f, 1.f, 1.f};            // groups of the transposed product are multiples of 32 rows
-        if (p.inv && row < p.rows) {
-          f[0] = p.inv[TB ? row / p.group : row];
-#pragma unroll
-          for (int x = 1; x < 4; ++x) f[x] = TB ? f[0] : row + x < p.rows ? p.inv[row + x] : 1.f;
-        }
-        for (int i0 = threadIdx.x; i0 < ntok * 32; i0 += P_THREADS * B) {
-          float4 sum[B];
-#pragma unroll
-          for (int j = 0; j < B; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-          for (int s = 0; s < p.splits; ++s) {
-            float4 v[B];
-#pragma unroll
-            for (int j = 0; j < B; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(src + s * next) + min(i0 + j * P_THREADS, ntok * 32 - 1));
-#pragma unroll
-            for (int j = 0; j < B; ++j) { sum[j].x += v[j].x; sum[j].y += v[j].y; sum[j].z += v[j].z; sum[j].w += v[j].w; }
-          }
-#pragma unroll
-          for (int j = 0; j < B; ++j) {
-            const int i = i0 + j * P_THREADS;
-            if (i >= ntok * 32 || row >= p.rows) continue;
-            const float o[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
-            XT* dst = reinterpret_cast<XT*>(p.out) + (int64_t)(it.m0 + (i >> 5)) * ld + row;
-            XT e[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) e[x] = from_f32<XT>(o[x] * f[x]);
-            if (sizeof(XT) == 2 && wide && row + 4 <= p.rows) {
-              *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
-            } else {
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                if (row + x < p.rows) dst[x] = e[x];
-            }
-          }
-        }
       }
     }
   }
@@ -605,14 +615,33 @@ PairPlan plan_w4_pair(int64_t M, int64_t N, int64_t K, int x_dtype, int transpos
   pl.items = (int)(pl.twos + pl.halves + odd);
   pl.G = std::min(pairs, pl.items);
   pl.splits = 1;
-  // With groups, tiles that leave half the pairs idle are shared along the contraction, eight stages at least per pair:
-  // the slices of a tile (128 KB per CTA and split at most) cost less than the stages they save.
-  const int64_t share = group > 0 ? std::min<int64_t>(std::min<int64_t>(pairs / tiles, 8), cdiv(pl.depth, P_STAGE_K) / 8) : 1;
-  if (share > 1) {
-    pl.splits = (int)share;
-    pl.twos = pl.halves = pl.cols = 0;
-    pl.items = pl.G = (int)(tiles * share);
-    pl.slice_bytes = (size_t)pl.items * 2 * pl.nt * 128 * sizeof(float);
+  pl.whole = pl.items;
+  // With groups, what whole rounds of pairs leave may be cut along the contraction, eight stages at least per part: into single
+  // tiles if there are no whole rounds, or into blocks of two (one set of expanded weights).  In us, from measurements: a stage of one
+  // tile 0.55, of two 0.75; sums out and joined 3 to 9 for single tiles, 18 for blocks; outputs of tiles that are not cut 3.
+  // 4096 x 4096, 512 rows: single tiles 38, blocks 41, not cut 48; 11008 x 4096: 73, 64, 112; 1024 x 2048, 2048 rows: blocks 33, not cut 21.
+  if (group > 0) {
+    const double nst = (double)cdiv(pl.depth, P_STAGE_K);
+    const int64_t most = std::min<int64_t>(8, cdiv(pl.depth, P_STAGE_K) / 8);
+    const int64_t by_tile = blocks == left ? std::min<int64_t>(pairs / tiles, most) : 1;
+    const int64_t by_block = odd == 0 && left > 0 ? std::min<int64_t>(pairs / left, most) : 1;
+    double us = halve ? 0.55 * nst + 3 : 0.75 * nst + 3;
+    auto cut = [&](int nh, int64_t share, int64_t first, int64_t units) {
+      pl.splits = (int)share;
+      pl.whole = (int)first;
+      pl.twos = nh == 2 ? (int)blocks : 0;
+      pl.halves = 0;
+      pl.cols = nh == 2 ? (int)cols : 0;
+      pl.items = (int)(first + units * share);
+      pl.G = std::min(pairs, pl.items);
+      pl.unit = units * 8 * nh * (pl.nt / 32) <= W4_TICKET_REGION / 4 ? 32 : 64;      // a ticket each
+      pl.slice_bytes = (size_t)(units * share) * 2 * nh * pl.nt * 128 * sizeof(float);
+    };
+    if (by_tile > 1 && 0.55 * nst / by_tile + 3 + 6 * pl.nt / 256.0 < us) {
+      us = 0.55 * nst / by_tile + 3 + 6 * pl.nt / 256.0;
+      cut(1, by_tile, 0, tiles);
+    }
+    if (by_block > 1 && 0.75 * nst / by_block + 18 < us) cut(2, by_block, blocks - left, left);
   }
   // Estimate of the forward product (see w4_pair_choice): per round the stages and the outputs of a tile, more with its
   // tokens; 0.68 us a stage for two tiles at once.
@@ -779,7 +808,7 @@ int launch_w4_pair(const PairPlan& pl, const void* x, int x_dtype, const uint8_t
   p.nst = (int)cdiv(pl.depth, P_STAGE_K);
   p.items = pl.items; p.twos = pl.twos; p.halves = pl.halves; p.cols = pl.cols; p.G = pl.G;
   p.nt = pl.nt;
-  p.splits = pl.splits;
+  p.whole = pl.whole; p.splits = pl.splits; p.unit = pl.unit;
   p.x_blk = pl.nt / 2 * P_STAGE_K * 2;
   p.x_slot = (pl.planes == 2 || pl.twos > 0) ? 2 * p.x_blk : p.x_blk;
   p.x_st = std::min(P_MAX_XST, P_XRING_BYTES / p.x_slot);

@@ -39,7 +39,7 @@ struct PairPlan {
   int use; int planes; int rows; int depth; int nrp; int nt; int items; int twos; int halves; int cols; int64_t Np;
   size_t plane_bytes; size_t tok_bytes; size_t ws_bytes;
   int G;                            // pairs
-  int splits; size_t slice_bytes;   // with groups: pairs that share a tile, and their sums
+  int whole, splits, unit; size_t slice_bytes;      // with groups: items that are not cut along the contraction, pairs that share another one, their sums
   double us;                        // estimate
 };
 // group: contraction indices per scale (0: one per channel); not for fp32 activations
