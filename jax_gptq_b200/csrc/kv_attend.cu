@@ -27,7 +27,7 @@
 // Work: the list of all (sequence, kv head, NC rows of q, 64-token tile) is cut into equal contiguous ranges, one per CTA; the
 // ranges follow from the lengths on the device.  Two ways to share a CTA's piece of an item among its four warps:
 //   few rows (NC = 8 NT): the warps take tiles in turn, each with a ring of its own, and are joined through shared memory;
-//   COLS (NC = 32 NT): every warp has 8 NT rows of its own and all walk the same tiles in one ring, refilled by the warp
+//   COLS (NC = 32): every warp has eight rows of its own and all walk the same tiles in one ring, refilled by the warp
 //   that is the last to have read a unit.  A warp passes over tiles that none of its rows sees.
 // An item that several CTAs share is joined by the one that draws the last ticket, in CTA order.  A CTA shares at most two
 // items (its first and its last), so two slices per CTA are all the scratch there is.
@@ -538,7 +538,7 @@ static AttendPlan plan_attend(int64_t max_new, int64_t group, int dw, int x_dtyp
   const int64_t rows = max_new * group;
   const bool one = dw == 256 || x_dtype == JGQ_F32;    // more accumulators than eight rows' do not fit the registers
   pl.cols = rows > (one ? 8 : 16);
-  pl.nt = one || rows <= (pl.cols ? 32 : 8) ? 1 : 2;
+  pl.nt = !one && rows > 8 && !pl.cols ? 2 : 1;
   const int nc = 8 * pl.nt * (pl.cols ? KA_WARPS : 1);
   pl.G = std::min(KA_TICKETS, attend_ctas(dw, pl.nt, x_dtype == JGQ_F32, pl.cols != 0) * sm_count());
   pl.slice_bytes = align_up((size_t)pl.G * 2 * nc * (dw + 2) * sizeof(float), 256);
@@ -565,7 +565,7 @@ static int launch_attend_inst(const AttendPlan& pl, const AttendParams& p, cudaS
 template <typename XT, int DW>
 static int launch_attend_width(const AttendPlan& pl, const AttendParams& p, cudaStream_t s) {
   if constexpr (!std::is_same<XT, float>::value && DW <= 128) {
-    if (pl.nt == 2) return pl.cols ? launch_attend_inst<XT, DW, 2, true>(pl, p, s) : launch_attend_inst<XT, DW, 2, false>(pl, p, s);
+    if (pl.nt == 2) return launch_attend_inst<XT, DW, 2, false>(pl, p, s);
   }
   return pl.cols ? launch_attend_inst<XT, DW, 1, true>(pl, p, s) : launch_attend_inst<XT, DW, 1, false>(pl, p, s);
 }

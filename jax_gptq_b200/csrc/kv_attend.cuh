@@ -412,8 +412,8 @@ __device__ __forceinline__ void attend_join_rows(const AttendParams& p, const At
   }
 }
 
-// the prompt kernel (kv_prompt.cu): 128 or 256 rows of q per item, 16-bit types, rows of 64 or 128 channels
-struct PromptPlan { int use, groups, G; size_t slice_bytes; };
+// the prompt kernel (kv_prompt.cu): 256 rows of q per item, 16-bit types, rows of 64 or 128 channels
+struct PromptPlan { int use, G; size_t slice_bytes; };
 PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype);
 int launch_kv_prompt(const PromptPlan& pl, AttendParams& p, int dw, int q_dtype, cudaStream_t s);
 

@@ -1,7 +1,8 @@
 // Attention over the paged 8-bit cache for many rows per sequence (prompts and chunks of them): tcgen05.
 //
-// An item is 128 NG rows of q (tokens x heads of one kv head's group) of a sequence and kv head; its tiles are 64 tokens.
-// NG = 1: two CTAs share an SM; NG = 2, for 256 rows and more: one CTA, whose two groups of 128 rows share the expanded codes.
+// An item is 256 rows of q (tokens x heads of one kv head's group) of a sequence and kv head, two groups of 128 (the second may be
+// empty), which share the expanded codes; its tiles are 64 tokens.  One CTA per SM.  (With 128 rows per item and two CTAs per SM,
+// 160 rows of 64 sequences took 165 us for 132, 100 rows of 4 long ones 84 for 62; 70 rows of 32 shorter ones 69 for 75.)
 //   S = Q K^T     M = 128 rows, N = 64 tokens:  Q and the tile's keys in shared memory, S in tensor memory (two buffers)
 //   P             softmax warps read S (one row per thread), write p as f16 over it
 //   O += P V      M = 128 rows, N = DW channels: P out of tensor memory, the tile's values [channel][token] in shared memory
@@ -16,13 +17,12 @@
 // rounding, 64 of them at a time, times 2^(reference - log2(v_scale) - maximum) (two units of 2^-23 off at most, as 2^x is).
 //
 // Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit, which bounds
-// the softmax warps: 1600 clocks of a tile's 2650 go by between the first score and the last p' of 256 rows).  While one
-// group's (or CTA's) softmax warps work, the other's products run.
+// the softmax warps: 1600 clocks of a tile's 2650 go by between the first score and the last p' of 256 rows).
 // Measured: four chunks of 512 rows, 32 heads of 128, up to 4096 tokens (f16): 95 us, 36 GFLOP; 2048 rows, 16384 tokens, 32 / 8 heads
 // (bf16): 640 us, 0.8 PFLOP/s.  Copies of the softmax loop cost more than a second pass over a tile: with three of them 109 and 684 us.
 //
-// Roles: warps 0 .. 4 NG - 1 softmax, then one warp for copies (q; a ring of four units of raw codes), one that issues the MMAs,
-// two (NG = 2: four; with one 118 us instead of 101) that turn the keys' codes into an operand, two for the values' (128-byte
+// Roles: warps 0 .. 7 softmax, then one warp for copies (q; a ring of four units of raw codes), one that issues the MMAs,
+// four (with one 118 us instead of 101) that turn the keys' codes into an operand, two for the values' (128-byte
 // swizzle; [token][64 channels] twice, [channel][64 tokens]).  Page numbers are read two tiles ahead, scales one: in front of a tile
 // they cost 500 clocks.  All warps write the outputs, by way of shared memory, so that rows go out whole.
 // The work is cut into equal ranges as in kv_attend.cu, with the same slices and tickets.  Waits are bounded: a row whose
@@ -39,8 +39,8 @@ JGQ_TRACE_DEFINE(prompt, 8 * 1024)
 
 namespace jgq {
 
-// 10 warps, two CTAs per SM; or 16
-__host__ __device__ constexpr int kp_threads(int ng) { return ng == 1 ? 320 : 512; }
+constexpr int NG = 2;                                  // groups of 128 rows, and buffers of expanded codes
+constexpr int KP_THREADS = 512, KP_ROWS = 128 * NG;
 constexpr int KP_COST = 5;                             // what an item takes beside its tiles, in tiles (see kv_attend.cu)
 constexpr int KP_RAW = 4;                              // raw units (keys or values of a tile) in the ring
 constexpr int KP_TMEM = 256;                           // columns per group: S and P 2 x 64, O DW
@@ -48,9 +48,9 @@ constexpr float KP_LAZY = 12.f;                        // log2 by which p v_scal
 constexpr float KP_FAINT = 60.f;                       // log2 below which it is as good as nothing beside the reference
 
 __host__ __device__ constexpr int kp_unit(int dw) { return 64 * dw; }
-// q, NG buffers of expanded keys and of values, the ring; the outputs of 128 rows take their place at the end of a piece
-__host__ __device__ constexpr int kp_operands(int dw, int ng) { return 128 * ng * dw * 2 + 2 * ng * 64 * dw * 2 + KP_RAW * kp_unit(dw); }
-__host__ __device__ constexpr int kp_smem(int dw, int ng) { return 1024 + 1024 + kp_operands(dw, ng); }
+// q, two buffers of expanded keys and of values, the ring; the outputs take their place at the end of a piece
+__host__ __device__ constexpr int kp_operands(int dw) { return KP_ROWS * dw * 2 + 2 * NG * 64 * dw * 2 + KP_RAW * kp_unit(dw); }
+__host__ __device__ constexpr int kp_smem(int dw) { return 1024 + 1024 + kp_operands(dw); }
 
 // D[tmem] (+)= A[tmem] B[smem], f16
 __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -99,18 +99,18 @@ __device__ __forceinline__ uint32_t code_pair_bf16(uint32_t w, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename XT, int DW, int NG>
-__global__ void __launch_bounds__(kp_threads(NG), NG == 1 ? 2 : 1)
+template <typename XT, int DW>
+__global__ void __launch_bounds__(KP_THREADS, 1)
 kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p) {
   using namespace umma;
-  constexpr int KP_THREADS = kp_threads(NG), KP_ROWS = 128 * NG, WARPS = KP_THREADS / 32;
+  constexpr int WARPS = KP_THREADS / 32;
   constexpr int UNIT = kp_unit(DW), KB = DW / 64;      // 64-channel blocks of a row
   constexpr int W_COPY = 4 * NG, W_MMA = W_COPY + 1, W_EXPAND = W_COPY + 2;
-  constexpr int EWK = NG == 1 ? 2 : 4, EWV = 2;        // warps that expand keys, and values
+  constexpr int EWK = 4, EWV = 2;        // warps that expand keys, and values
   static_assert(W_EXPAND + EWK + EWV == WARPS, "every warp has a role");
   constexpr bool BF = std::is_same<XT, __nv_bfloat16>::value;
   constexpr int OST = DW + 4;                          // floats per row of staged outputs
-  static_assert(KP_ROWS * OST * 4 <= kp_operands(DW, NG), "the outputs fit the operands' place");
+  static_assert(KP_ROWS * OST * 4 <= kp_operands(DW), "the outputs fit the operands' place");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base);
@@ -170,6 +170,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
     const int seen_item = max(0, L - n + (pc.c0 + pc.rows - 1) / p.group + 1);
     const int t_end = min(pc.t_last, (seen_item + KV_TILE - 1) / KV_TILE);
     const int nt = max(0, t_end - pc.t_first);         // tiles of this piece
+    const bool two = pc.rows > 128;                    // the second group has rows; otherwise its barriers alone go on
     const int32_t* row_of_table = p.table + (int64_t)rg.r * p.table_stride;
     // A tile's scales lie behind its page number: numbers are read two tiles ahead, scales one, so that no warp waits for both.
     auto page_of = [&](int k) { return k < nt ? row_of_table[(pc.t_first + k) >> page_shift] : 0; };
@@ -219,8 +220,8 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
       // ===================== raw codes =====================
       if (lane == 0) {
         if (p.q_map && nt > 0) {                       // rows behind the item's are loaded too, and masked
-          mbar_expect_tx(q_full, KP_ROWS * DW * 2);
-          for (int grp = 0; grp < NG; ++grp)
+          mbar_expect_tx(q_full, (two ? 2 : 1) * 128 * DW * 2);
+          for (int grp = 0; grp < (two ? 2 : 1); ++grp)
             for (int kb = 0; kb < KB; ++kb)
               tma_load_3d(smem_u32(q_smem) + (grp * KB + kb) * (128 * 128), &qmap, 64 * kb, h * p.group, pc.row_first + (pc.c0 + 128 * grp) / p.group, q_full);
         }
@@ -258,6 +259,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
             const uint64_t dk = dk0 + (uint32_t)((buf * 64 * DW * 2) >> 4);
 #pragma unroll
             for (int grp = 0; grp < NG; ++grp) {
+              if (grp == 0 || two)
 #pragma unroll
               for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -280,6 +282,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
             tc_fence_after();
             if (elect_one()) {
               const uint64_t dv = dv0 + (uint32_t)((buf * 64 * DW * 2) >> 4);
+              if (grp == 0 || two)
 #pragma unroll
               for (int k16 = 0; k16 < 4; ++k16)
                 mma_f16_ts(tmem + grp * KP_TMEM + 128, tmem + grp * KP_TMEM + 64 * b + 8 * k16, dv + (uint32_t)((k16 * 32) >> 4), idesc_o,
@@ -368,6 +371,10 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&s_full[2 * grp + b], (c >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
+        if (grp > 0 && !two) {
+          if (lane == 0) mbar_arrive(&p_full[2 * grp + b]);
+          continue;
+        }
         const bool masked = partial || (tile + 1) * KV_TILE > least;
         const int seen = limit - tile * KV_TILE;       // columns of the tile that this row sees
         const float f = q_factor * ks;                 // not negative
@@ -507,7 +514,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
     }
     if (!whole) {
       const int first_c = attend_cta_of(pc.tile_at, rg.S, rg.G), last_c = attend_cta_of(pc.tile_at + pc.tiles - 1, rg.S, rg.G);
-      if (attend_last(p, first_c, last_c, &s_flag)) attend_join_rows<XT, KP_ROWS, DW, KP_THREADS, NG == 1 ? 3 : 4, 2>(p, rg, pc, first_c, last_c, s_row, s_ml, s_inv);
+      if (attend_last(p, first_c, last_c, &s_flag)) attend_join_rows<XT, KP_ROWS, DW, KP_THREADS, 4, 2>(p, rg, pc, first_c, last_c, s_row, s_ml, s_inv);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the next writers of the staged outputs' place are copies
     __syncthreads();                                   // before Q and O are written again
@@ -538,32 +545,32 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
 PromptPlan plan_kv_prompt(int64_t rows, int dw, int q_dtype) {
   PromptPlan pl;
   memset(&pl, 0, sizeof(pl));
-  if (rows <= 64 || dw > 128 || q_dtype == JGQ_F32) return pl;
+  // 40 rows of 32 sequences, bf16: 67 us here, 63 on mma.sync; of 4 long ones 61 and 66; 64 rows: 71 and 70, 53 and 68; 32 rows: 52 and 52, 46
+  // and 44 (kv_attend.cu, with 32 rows per item)
+  if (rows <= 32 || dw > 128 || q_dtype == JGQ_F32) return pl;
   pl.use = 1;
-  pl.groups = rows >= 256 ? 2 : 1;
-  pl.G = std::min(KA_TICKETS, (pl.groups == 2 ? 1 : 2) * sm_count());
-  pl.slice_bytes = align_up((size_t)pl.G * 2 * 128 * pl.groups * (dw + 2) * sizeof(float), 256);
+  pl.G = std::min(KA_TICKETS, sm_count());
+  pl.slice_bytes = align_up((size_t)pl.G * 2 * KP_ROWS * (dw + 2) * sizeof(float), 256);
   return pl;
 }
 
-template <typename XT, int DW, int NG>
+template <typename XT, int DW>
 static int launch_prompt_inst(const PromptPlan& pl, const CUtensorMap& qmap, const AttendParams& p, cudaStream_t s) {
-  auto kern = kv_prompt_kernel<XT, DW, NG>;
+  auto kern = kv_prompt_kernel<XT, DW>;
   struct AttrTag {};
   const int arc = once_per_device<AttrTag>([&]() {
     cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     cudaGetLastError();
-    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem(DW, NG));
+    return (int)cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem(DW));
   });
   if (arc != 0) return fail(JGQ_ERR_CUDA, "kv_attend: cannot raise the dynamic shared memory limit");
-  kern<<<(unsigned)pl.G, kp_threads(NG), kp_smem(DW, NG), s>>>(qmap, p);
+  kern<<<(unsigned)pl.G, KP_THREADS, kp_smem(DW), s>>>(qmap, p);
   return check_launch("kv_prompt");
 }
 
 template <typename XT>
 static int launch_prompt(const PromptPlan& pl, const CUtensorMap& qmap, const AttendParams& p, int dw, cudaStream_t s) {
-  if (dw == 64) return pl.groups == 2 ? launch_prompt_inst<XT, 64, 2>(pl, qmap, p, s) : launch_prompt_inst<XT, 64, 1>(pl, qmap, p, s);
-  return pl.groups == 2 ? launch_prompt_inst<XT, 128, 2>(pl, qmap, p, s) : launch_prompt_inst<XT, 128, 1>(pl, qmap, p, s);
+  return dw == 64 ? launch_prompt_inst<XT, 64>(pl, qmap, p, s) : launch_prompt_inst<XT, 128>(pl, qmap, p, s);
 }
 
 int launch_kv_prompt(const PromptPlan& pl, AttendParams& p, int dw, int q_dtype, cudaStream_t s) {
