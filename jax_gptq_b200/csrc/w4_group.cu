@@ -427,7 +427,11 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   JGQ_REQUIRE(aligned(ws, 256), JGQ_ERR_ALIGN, "w4_group_matmul: workspace must be 256-byte aligned");
   cudaStream_t s = (cudaStream_t)stream;
   const bool dense = aligned(packed, 16) && aligned(x, 16);
-  if (!transpose_b && M <= kGroupDecodeRows && dense && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) && aligned(scale, 16) && aligned(zero, 16)) {
+  const PairPlan pp = dense ? group_pairs(M, N, K, x_dtype, transpose_b, group_size) : PairPlan{};
+  // 17 to 32 rows of 16 bits on large weights: on pairs that share the tiles (bf16, groups of 128, 17 and 32 rows: 4096 x 4096 20.7
+  // and 20.8 us for 21.7 and 26.2; 8192 x 2048 22 for 23 and 28; 11008 x 4096 36.5 for 38 and 43; but 4096 x 2048 17.6 for 14.8 and 18.6)
+  const bool paired = pp.use && M > 16 && K * N >= 1 << 24 && pp.splits > 1;
+  if (!transpose_b && M <= kGroupDecodeRows && dense && !paired && aligned(out, x_dtype == JGQ_F32 ? 16 : 8) && aligned(scale, 16) && aligned(zero, 16)) {
     const int64_t step = x_dtype == JGQ_F32 ? std::min(M, kGroupPassRows) : M;
     const GemvPlan whole = plan_w4_gemv(step, N, K, x_dtype, group_size, (int)zb);
     if (whole.use) {
@@ -442,8 +446,7 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
       return rc;
     }
   }
-  const PairPlan pp = group_pairs(M, N, K, x_dtype, transpose_b, group_size);
-  if (pp.use && dense) {
+  if (pp.use) {
     rc = fits(pp.ws_bytes);
     return rc ? rc : launch_w4_pair(pp, x, x_dtype, packed, zero, scale, zs_dtype, out, M, N, K, transpose_b, group_size, ws, s);
   }

@@ -72,7 +72,7 @@ def test_product_and_gradient(G, M, K, N, group, x):
 
 @pytest.mark.parametrize('M,K,N,group', [(33, 5002, 272, 96), (40, 11008, 256, 32), (64, 2998, 1008, 64), (96, 1030, 4096, 128), (130, 4096, 4112, 128),
                                          (257, 3000, 528, 32), (300, 2050, 2064, 160), (512, 8200, 256, 8224), (700, 1536, 1536, 64),
-                                         (1000, 8200, 4112, 128), (1024, 4110, 8208, 32), (1001, 4104, 11008, 96), (390, 11008, 2064, 64)])
+                                         (1000, 8200, 4112, 128), (1024, 4110, 8208, 32), (1001, 4104, 11008, 96), (390, 11008, 2064, 64), (17, 4096, 4112, 64), (32, 11008, 2064, 32)])
 @pytest.mark.parametrize('x', ['f16', 'bf16'])
 def test_tiles_shared_along_the_contraction(G, M, K, N, group, x):
     """Few tiles and a long contraction in either direction: odd numbers of stages per slice, groups that straddle the slices,
