@@ -156,18 +156,23 @@ class KVCache:
         self.v_scale = torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=d)
 
     def _rows(self, t, name, heads):
-        """(tensor with a contiguous last axis, dtype code) of (tokens, heads, head_dim) rows."""
+        """(tensor with a contiguous last axis, its shape, its strides) of (tokens, heads, head_dim) rows."""
         if type(t) is not torch.Tensor or t.get_device() != self.device.index:
             t = _cuda(t, name, self.device)
         if t.dtype not in _DT:
             raise TypeError(f'{name} must be float32, float16 or bfloat16, not {t.dtype}')
-        if t.dim() != 3 or (heads is not None and t.size(1) != heads) or t.size(2) != self.head_dim:
-            raise ValueError(f'{name} must have shape (tokens, {"heads" if heads is None else heads}, {self.head_dim}), not {tuple(t.shape)}')
+        shape = t.shape
+        if len(shape) != 3 or (heads is not None and shape[1] != heads) or shape[2] != self.head_dim:
+            raise ValueError(f'{name} must have shape (tokens, {"heads" if heads is None else heads}, {self.head_dim}), not {tuple(shape)}')
         if t.requires_grad:
             if torch.is_grad_enabled():
                 raise ValueError(f'{name} requires a gradient; the cache has none (detach it)')
             t = t.detach()
-        return t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
+        strides = t.stride()
+        if strides[2] != 1 and shape[2] != 1:
+            t = t.contiguous()
+            strides = t.stride()
+        return t, shape, strides
 
     def write(self, k, v, slots):
         """Quantizes row t of `k` and `v` (tokens, kv_heads, head_dim) into token slot `slots[t]` (int64; page * page_size +
@@ -177,12 +182,14 @@ class KVCache:
         them (runs of one page that lie apart in one call spoil each other's codes; two calls do not).  Where a
         page's first token is written its scale is set anew; later tokens that need more make it grow by a power of two,
         and the codes that are there are rounded to it.  NaN is stored as 0, infinities as the largest code."""
-        k, v = self._rows(k, 'k', self.kv_heads), self._rows(v, 'v', self.kv_heads)
-        if k.shape != v.shape or k.dtype != v.dtype:
-            raise ValueError(f'k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ')
-        slots = _vector(slots, 'slots', torch.int64, k.shape[0], self.device)
-        _launch(self.device.index, lib.jgq_kv_write, k.data_ptr(), v.data_ptr(), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                slots.data_ptr(), k.shape[0], self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+        k, shape, ks = self._rows(k, 'k', self.kv_heads)
+        v, v_shape, vs = self._rows(v, 'v', self.kv_heads)
+        if shape != v_shape or k.dtype != v.dtype:
+            raise ValueError(f'k {tuple(shape)} {k.dtype} and v {tuple(v_shape)} {v.dtype} differ')
+        tokens = shape[0]
+        slots = _vector(slots, 'slots', torch.int64, tokens, self.device)
+        _launch(self.device.index, lib.jgq_kv_write, k.data_ptr(), v.data_ptr(), _DT[k.dtype], ks[0], ks[1], vs[0], vs[1],
+                slots.data_ptr(), tokens, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                 self.num_pages, self.page_size, self.kv_heads, self.head_dim)
 
     def read(self, pages, dtype=torch.float32):
@@ -193,7 +200,7 @@ class KVCache:
         pages = _vector(pages, 'pages', torch.int64, None, self.device)
         shape = (pages.shape[0], self.kv_heads, self.page_size, self.head_dim)
         k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         _launch(self.device.index, lib.jgq_kv_read, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                 self.num_pages, self.page_size, self.kv_heads, self.head_dim, pages.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), _DT[dtype])
         return k, v
@@ -208,51 +215,53 @@ class KVCache:
         only steers the choice of kernel.  Rows that see nothing are zero.  Rows behind the last request are zero in a
         new result and left as they were in `out`.  A page number outside the cache makes its rows NaN.  `scale` defaults to
         head_dim ** -0.5.  With `return_lse` also the logarithm of the sum of exponentials, fp32 (tokens, heads)."""
-        q = self._rows(q, 'q', None)
-        d = self.device
+        q, shape, strides = self._rows(q, 'q', None)
+        d, tokens, heads = self.device, shape[0], shape[1]
         if block_table.dim() != 2 or block_table.dtype != torch.int32:
             raise ValueError('block_table must be a 2-D int32 tensor')
         table = block_table if type(block_table) is torch.Tensor and block_table.get_device() == d.index else _cuda(block_table, 'block_table', d)
-        if table.stride(1) != 1 and table.shape[1] > 1:
+        n, width = table.shape
+        pitch = table.stride()
+        if pitch[1] != 1 and width > 1:
             table = table.contiguous()
-        n, heads = table.size(0), q.size(1)
+            pitch = table.stride()
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f'{heads} query heads are no multiple of {self.kv_heads} kv heads')
         lengths = _vector(lengths, 'lengths', torch.int32, n, d)
         if cu_seqlens is None:
-            if q.size(0) != n:
-                raise ValueError(f'{q.shape[0]} rows of q for {n} requests without cu_seqlens')
+            if tokens != n:
+                raise ValueError(f'{tokens} rows of q for {n} requests without cu_seqlens')
             most = 1
         else:
             cu_seqlens = _vector(cu_seqlens, 'cu_seqlens', torch.int32, n + 1, d)
-            most = max(1, q.shape[0] if max_new is None else int(max_new))
+            most = max(1, tokens if max_new is None else int(max_new))
         fresh = out is None
         if fresh:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         else:
             _cuda(out, 'out', d)
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
                 raise ValueError(f'out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}')
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=d) if return_lse else None
-        if _current_device() == d.index:
-            self._attend(q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh)
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=d) if return_lse else None
+        index, code = d.index, _DT[q.dtype]
+        args = (q.data_ptr(), code, strides[0], strides[1], out.data_ptr(), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                self.v_scale.data_ptr(), self.num_pages, self.page_size, table.data_ptr(), pitch[0], width, lengths.data_ptr(), _ptr(cu_seqlens),
+                tokens, n, most, heads, self.kv_heads, self.head_dim, float(self.head_dim ** -0.5 if scale is None else scale),
+                _lib.KV_ZERO_REST if fresh else 0)
+        if _current_device() == index:
+            self._attend(args, heads, most, code, index)
         else:
-            with torch.cuda.device(d):
-                self._attend(q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh)
+            with torch.cuda.device(index):
+                self._attend(args, heads, most, code, index)
         return (out, lse) if return_lse else out
 
-    def _attend(self, q, table, lengths, cu_seqlens, n, heads, most, scale, out, lse, fresh):
-        code, index = _DT[q.dtype], self.device.index
+    def _attend(self, args, heads, most, code, index):
         need = self._ws_bytes.get((heads, most, code))
         if need is None:
             if len(self._ws_bytes) >= 1024:
                 self._ws_bytes.clear()
             need = self._ws_bytes[heads, most, code] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, code)
         stream = _raw_stream(index)
-        rc = lib.jgq_kv_attend(q.data_ptr(), code, q.stride(0), q.stride(1), out.data_ptr(), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(),
-                               self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.num_pages, self.page_size, table.data_ptr(),
-                               table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(cu_seqlens), q.shape[0], n, most,
-                               heads, self.kv_heads, self.head_dim, float(self.head_dim ** -0.5 if scale is None else scale),
-                               _lib.KV_ZERO_REST if fresh else 0, _scratch(need, 'kv', index, stream), need, stream)
+        rc = lib.jgq_kv_attend(*args, _scratch(need, 'kv', index, stream), need, stream)
         if rc:
             check(rc)
