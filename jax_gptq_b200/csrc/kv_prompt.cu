@@ -295,7 +295,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
         }
       }
     } else if (warp >= W_EXPAND) {
-      // ===================== codes into operands: one or two warps each for keys and values =====================
+      // ===================== codes into operands: four warps for the keys', two for the values' =====================
       const int part = warp >= W_EXPAND + EWK, share = part ? warp - W_EXPAND - EWK : warp - W_EXPAND;
       uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
       // lane's 16-byte piece i = lane + 32 j: row and chunk of the operand; the row's low bits, which swizzle, follow j's parity at most
