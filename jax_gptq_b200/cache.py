@@ -213,7 +213,8 @@ class KVCache:
         of them; with it (int32, requests + 1) rows cu_seqlens[r] .. cu_seqlens[r + 1] - 1 are the last ones, and each sees the
         tokens up to its own.  `max_new` is the largest number of rows of a request that is expected (default: all of q); it
         only steers the choice of kernel.  Rows that see nothing are zero.  Rows behind the last request are zero in a
-        new result and left as they were in `out`.  A page number outside the cache makes its rows NaN.  `scale` defaults to
+        new result and left as they were in `out`.  A page number outside the cache makes its rows NaN (scales
+        that are not finite spoil the rows that see their page, and no others).  `scale` defaults to
         head_dim ** -0.5.  With `return_lse` also the logarithm of the sum of exponentials, fp32 (tokens, heads)."""
         q, shape, strides = self._rows(q, 'q', None)
         d, tokens, heads = self.device, shape[0], shape[1]

@@ -601,7 +601,8 @@ extern "C" int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride,
               (long long)q_heads, (long long)kv_heads);
   JGQ_REQUIRE(tokens >= 0 && requests >= 0 && pages > 0 && table_width >= 0 && max_new >= 1, JGQ_ERR_ARG, "kv_attend: bad sizes");
   JGQ_REQUIRE(cu_seqlens || tokens == requests, JGQ_ERR_ARG, "kv_attend: %lld tokens for %lld requests without cu_seqlens", (long long)tokens, (long long)requests);
-  JGQ_REQUIRE(tokens <= (1 << 24) && requests <= (1 << 20) && q_heads <= 4096 && pages <= 2147483647LL && table_width * page_size <= 2147483647LL - 64,
+  JGQ_REQUIRE(tokens <= (1 << 24) && requests <= (1 << 20) && q_heads <= 4096 && tokens * (q_heads / kv_heads) <= 2147483647LL - 1024 &&
+                  pages <= 2147483647LL && table_width * page_size <= 2147483647LL - 64,
               JGQ_ERR_LIMIT, "kv_attend: shape too large");
   if (tokens == 0) return JGQ_OK;
   JGQ_REQUIRE(q && out && k && v && k_scale && v_scale && lengths && (block_table || table_width == 0), JGQ_ERR_ARG, "kv_attend: null pointer");

@@ -59,6 +59,7 @@ def test_cache_entry_points_refuse(jlib):  # noqa: F811
     assert attend(n=64) == -3 and attend(ws=None) == -3
     assert attend(ws=128) == -2 and attend(q=257) == -2
     assert attend(width=1 << 26, page=256) == -5
+    assert attend(tokens=1 << 22, cu=256, hq=1024, hkv=1) == -5            # rows per kv head are counted in 32 bits
 
     def write(k=256, dt=F16, slots=256, tokens=4, pages=8, page=64, H=2, D=64, codes=256):
         return lib.jgq_kv_write(k, 256, dt, H * D, D, H * D, D, slots, tokens, codes, 256, 256, 256, pages, page, H, D, None)
