@@ -248,3 +248,24 @@ def test_a_workspace_of_the_stated_size_is_enough(G, x, new, Hq, H, D):
     assert rc == 0, lib.jgq_last_error()
     assert torch.equal(out, cache.attend(q, table, n, cu_seqlens=cu, max_new=new))
     assert bool((ws[need:] == 171).all()) and not bool(ws[:16384].any())
+
+
+@pytest.mark.parametrize('new', [1, 90])
+def test_requests_that_share_pages_and_calls_on_two_streams(G, new):
+    """A prefix that two requests have in common lies in the same pages; calls on two streams at once do not meet."""
+    lengths = [640, 700, 64 * 9]
+    cache, table, gen = filled(G, lengths, 2, 64, 64, 12)
+    table[1, :8] = table[0, :8]
+    table[2, :9] = table[0, 3]                                            # one page nine times
+    q = torch.randn((3 * new, 8, 64), generator=gen, device='cuda').half()
+    out = check(cache, table, q, lengths, [new] * 3)
+    cu, n = i32([0, new, 2 * new, 3 * new]), i32(lengths)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(cache.attend(q, table, n, cu_seqlens=cu, max_new=new))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) for part in got for o in part)
