@@ -623,7 +623,6 @@ extern "C" int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride,
   p.group = (int)(q_heads / kv_heads); p.D = (int)head_dim; p.P = page_size; p.pages = (int)pages;
   p.vec_q = aligned(q, 16) && q_token_stride * xb % 16 == 0 && q_head_stride * xb % 16 == 0;
   p.vec_o = head_dim % 4 == 0 && aligned(out, 4 * xb);
-  p.vec_o8 = head_dim % 8 == 0 && aligned(out, 16);
   p.zero_rest = (flags & JGQ_KV_ZERO_REST) != 0;
   p.G = pl.prompt.use ? pl.prompt.G : pl.G;
   p.scale = scale * 1.4426950408889634f;

@@ -17,7 +17,7 @@ struct AttendParams {
   int32_t* tickets; float* slices;
   int T, B, W, Hq, Hkv, group, D, P, pages;
   int q_map;                   // prompts: rows of q come by TMA
-  int vec_q, vec_o, vec_o8;    // 16-byte loads of q, stores of four and of eight channels are legal
+  int vec_q, vec_o;            // 16-byte loads of q, stores of four channels are legal
   int zero_rest;               // rows behind the last sequence are zeroed
   int G;                       // CTAs
   float scale;                 // of the scores, times log2(e)
