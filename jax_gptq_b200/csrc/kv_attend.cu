@@ -33,6 +33,10 @@
 // items (its first and its last), so two slices per CTA are all the scratch there is.
 // Where the rows of a sequence make several row tiles, the earlier ones see fewer tokens: tile counts are a linear function
 // rounded down, whose sums have a closed form (floor_sum).
+//
+// Measured (replayed): 64 sequences up to 32768 tokens, 64 / 8 heads of 128, bf16, one token each (833 MB of codes): 148 us, 5.6 TB/s, 0.86 of
+// the measured copy; 700 tokens of one sequence, 12 heads of 64, fp32: 12.5 us, of which the launch and the cut are 3, one tile's chain and
+// the join the rest.  Up to 16 rows of 16 bits the warps share tiles (the same bytes for every row), above each has rows of its own.
 #include "kv_attend.cuh"
 #include "trace.cuh"
 #include <algorithm>
