@@ -80,7 +80,7 @@ __device__ __forceinline__ float row_element(const Row16<XT>& r, int i) {      /
 // The codes of four elements, in excess 128, as a word: rne(x / s) with the quotient rounded to fp32.  x times a reciprocal
 // 2^-21 too small and one as much too large, each rounded to a whole number by adding 1.5 * 2^23 (one fused operation, the sum's
 // low byte is the number): where both give the same, the quotient and its rounding to fp32, which lie between, do too.
-// Otherwise, and where elements are not finite or the reciprocal is not normal (lo = NaN), the elements are divided.
+// Otherwise, and where elements are not finite or the reciprocal is not normal (`divide`), the elements are divided.
 static __device__ __noinline__ uint32_t encode4_divided(float x0, float x1, float x2, float x3, float s) {
   const float x[4] = {x0, x1, x2, x3};
   uint32_t r = 0;
@@ -95,18 +95,19 @@ static __device__ __noinline__ uint32_t encode4_divided(float x0, float x1, floa
 static __device__ __noinline__ void store_bytes(uint8_t* dst, uint32_t c, int a, int b) {
   for (int i = a; i < b; ++i) dst[i] = (uint8_t)(c >> (8 * i));
 }
-struct Reciprocal { float s, lo, hi; };
+struct Reciprocal { float s, lo, hi; uint32_t divide; };
 __device__ __forceinline__ Reciprocal reciprocal(float s, bool finite) {
   Reciprocal r;
   r.s = s > 0.f ? s : 1.f;
   const float inv = __fdiv_rn(1.f, r.s);
   const bool ok = finite && r.s >= 1.1754943508222875e-38f && inv >= 1.1754943508222875e-38f;
-  r.lo = ok ? inv * 0.99999952316284180f : __int_as_float(0x7fc00000);
+  r.lo = inv * 0.99999952316284180f;
   r.hi = inv * 1.0000004768371582f;
+  r.divide = ok ? 0u : 1u;                               // two NaN of such elements would pass for a quotient
   return r;
 }
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4], const Reciprocal& q) {
-  uint32_t b[4], differ = 0;
+  uint32_t b[4], differ = q.divide;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     b[i] = __float_as_uint(fmaf(x[i], q.lo, 12582912.f));
