@@ -12,7 +12,9 @@
  *     it, never synchronises and never allocates.  The device that owns the stream
  *     must be the current device of the calling thread; calls may come from several
  *     host threads (one per device).  Scratch memory is supplied by the caller
- *     (`ws`, `ws_bytes`; size from the matching *_workspace_bytes);
+ *     (`ws`, `ws_bytes`; size from the matching *_workspace_bytes).  A call may be
+ *     several launches that meet in it: threads that share a stream and a workspace
+ *     hold a lock of their own around each call;
  *   - return value 0 = enqueued, negative = host-side validation error, nothing
  *     was launched; jgq_last_error() returns the thread-local message;
  *   - device-side conditions (non-positive pivot / NaN in the Cholesky) are

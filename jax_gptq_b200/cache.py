@@ -10,7 +10,8 @@ of a serving loop, for every layer between two `quantized_matmul`s:
 
 Everything is enqueued on the current stream, nothing synchronises, and the arguments stay on the device, so a step can be
 captured into a CUDA graph (its outputs and workspaces then belong to the graph).  All tensors are CUDA tensors of one
-device; the call makes that device current for its launches.
+device; the call makes that device current for its launches.  Calls may come from several host threads: those on one stream run one
+after the other.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _DT, _dev, _ptr, _scratch
+from .gptq import _DT, _dev, _ptr, _scratch, _stream_lock
 
 PAGE_SIZES = (64, 128, 256)
 
@@ -60,11 +61,13 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 
 def _launch(index, call, *args):
     """`call` with the current stream of device `index`, on which it runs, behind its arguments."""
-    if _current_device() == index:
-        rc = call(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = call(*args, _raw_stream(index))
+    stream = _raw_stream(index)
+    with _stream_lock(index, stream):
+        if _current_device() == index:
+            rc = call(*args, stream)
+        else:
+            with torch.cuda.device(index):
+                rc = call(*args, stream)
     if rc:
         check(rc)
 
@@ -263,6 +266,7 @@ class KVCache:
                 self._ws_bytes.clear()
             need = self._ws_bytes[heads, most, code] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, code)
         stream = _raw_stream(index)
-        rc = lib.jgq_kv_attend(*args, _scratch(need, 'kv', index, stream), need, stream)
+        with _stream_lock(index, stream):
+            rc = lib.jgq_kv_attend(*args, _scratch(need, 'kv', index, stream), need, stream)
         if rc:
             check(rc)

@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _check_groups, _DT
+from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _stream_lock, _check_groups, _DT
 
 _functorch_active = torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._get_tracing_state
@@ -71,10 +71,12 @@ def _launch(x, w, zero, scale, transpose_b):
     out = x.new_empty((M, out_n))
     dev = _current_device()
     need = _workspace_bytes(dev, M, Nw, Kw, transpose_b)
-    ws = _workspace(need, zeroed=True, tag='w4').data_ptr() if need else 0
-    flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
-    rc = lib.jgq_w4_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(),
-                           _ZS[zero.dtype], out.data_ptr(), M, Nw, Kw, flags, ws, need, _raw_stream(dev))
+    stream = _raw_stream(dev)
+    with _stream_lock(dev, stream):
+        ws = _workspace(need, zeroed=True, tag='w4').data_ptr() if need else 0
+        flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
+        rc = lib.jgq_w4_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(),
+                               _ZS[zero.dtype], out.data_ptr(), M, Nw, Kw, flags, ws, need, stream)
     if rc:
         check(rc)
     return out if len(shape) == 2 else out.reshape(shape[:-1] + (out_n,))
@@ -85,9 +87,10 @@ def _enqueue_groups(x, w, zero, scale, out, M, N, K, group_size, transpose_b, de
     if need is None:
         need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
     stream = _raw_stream(dev)
-    flags = _lib.W4_TRANSPOSE_B if transpose_b else _lib.W4_WEIGHTS_SETTLED if _settled_groups(w, zero, scale) else 0
-    rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
-                                 out.data_ptr(), M, N, K, group_size, flags, _scratch(need, 'w4g', dev, stream), need, stream)
+    with _stream_lock(dev, stream):
+        flags = _lib.W4_TRANSPOSE_B if transpose_b else _lib.W4_WEIGHTS_SETTLED if _settled_groups(w, zero, scale) else 0
+        rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
+                                     out.data_ptr(), M, N, K, group_size, flags, _scratch(need, 'w4g', dev, stream), need, stream)
     if rc:
         check(rc)
 
@@ -179,7 +182,8 @@ def _group_matmul(x, w, zero, scale, group_size, transpose_b):
 
 def quantized_matmul(x, quantized_matrix, transpose_b=False):
     """x @ dequant(quantized_matrix) (or its transpose); result in x's dtype.  A matrix with a ``group_size`` has a scale and
-    a zero point per group of rows and channel, one without per channel."""
+    a zero point per group of rows and channel, one without per channel.  Calls may come from several host threads, also on
+    one stream."""
     if type(x) is torch.Tensor and x.is_cuda and x.dtype in _DT:
         as_np, xd = False, x
     else:
