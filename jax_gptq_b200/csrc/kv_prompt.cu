@@ -305,13 +305,16 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
       const uint32_t row_step = part ? 8 * 128 : (32 / KP) * 128, odd = !part && KP == 8 ? 64u : 0u;
       const uint32_t c0 = ((2 * (col & 3)) ^ (row0 & 7)) << 4, c1 = c0 ^ 16;
       constexpr int STEPS = UNIT / 16 / 32;            // of the operand's warps together
-      float vs_next = 1.f;
+      const float* scales = part ? p.v_scale : p.k_scale;
+      float scale_next = 1.f;
       int page_1 = 0;
-      if (part && nt > 0) { bool bad; vs_next = p.v_scale[block_of(page_of(0), bad)]; page_1 = page_of(1); }
+      bool bad;
+      if (nt > 0) { scale_next = scales[block_of(page_of(0), bad)]; page_1 = page_of(1); }
       for (int k = 0; k < nt && ok; ++k) {
         const uint32_t c = done + k, u = 2 * c + part, slot = u % KP_RAW, buf = c % NG;
-        const float vs = vs_next;                      // one tile ahead
-        if (part) { bool bad; vs_next = p.v_scale[block_of(page_1, bad)]; page_1 = page_of(k + 2); }
+        const float scale = scale_next;                // one tile ahead
+        scale_next = scales[block_of(page_1, bad)];
+        page_1 = page_of(k + 2);
         ok = __all_sync(0xffffffffu, mbar_wait_suspended(&raw_full[slot], (u / KP_RAW) & 1, abort_flag));
         if (ok && c >= NG) ok = __all_sync(0xffffffffu, mbar_wait_suspended(&empty[buf], (c / NG + 1) & 1, abort_flag));
         if (!ok) break;
@@ -336,13 +339,13 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
         constexpr std::integral_constant<int, EWK> of_k{};
         constexpr std::integral_constant<int, EWV> of_v{};
         auto key = [](uint32_t w, uint32_t sel) { return BF ? code_pair_bf16(w, sel) : code_pair_f16(w, sel); };
-        if (!part) {                                   // keys: of q's type, signed as the scale of the scores is
-          if (p.scale < 0.f) expand(of_k, [=](uint32_t w, uint32_t sel) { return key(w, sel) ^ 0x80008000u; });
-          else               expand(of_k, key);
-        } else if (vs > 0.f) {
+        if (!part) {                                   // keys: of q's type, signed as the product of their scale and the scores' is
+          if ((p.scale < 0.f) != (scale < 0.f)) expand(of_k, [=](uint32_t w, uint32_t sel) { return key(w, sel) ^ 0x80008000u; });
+          else                                  expand(of_k, key);
+        } else if (scale > 0.f) {
           expand(of_v, [](uint32_t w, uint32_t sel) { return code_pair_f16(w, sel); });
         } else {                                       // values of a zero scale are zero, of a negative one negative
-          const uint32_t keep = vs == 0.f ? 0u : 0xffffffffu, flip = vs < 0.f ? 0x80008000u : 0u;
+          const uint32_t keep = scale == 0.f ? 0u : 0xffffffffu, flip = scale < 0.f ? 0x80008000u : 0u;
           expand(of_v, [=](uint32_t w, uint32_t sel) { return (code_pair_f16(w, sel) & keep) ^ flip; });
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -360,7 +363,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
       bool bad;
       int64_t block = nt > 0 ? block_of(page_of(0), bad) : 0;
       int page_1 = page_of(1);
-      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : attend_key_scale(p.k_scale[block])) : 0.f, vs = nt > 0 ? fabsf(p.v_scale[block]) : 0.f, lv = log2f(vs);
+      float ks = nt > 0 ? (bad ? __int_as_float(0x7fc00000) : attend_key_scale(fabsf(p.k_scale[block]))) : 0.f, vs = nt > 0 ? fabsf(p.v_scale[block]) : 0.f, lv = log2f(vs);
       for (int k = 0; k < nt; ++k) {
         const uint32_t c = done + k, b = c & 1;
         const int tile = pc.t_first + k;
@@ -377,7 +380,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
         }
         const bool masked = partial || (tile + 1) * KV_TILE > least;
         const int seen = limit - tile * KV_TILE;       // columns of the tile that this row sees
-        const float f = q_factor * ks;                 // not negative
+        const float f = q_factor * ks;                 // not negative: the signs are the codes'
         uint32_t ph[32];
         float sum, back;
         // p' = 2^(score + lv - ref) = 2^(score - m - back); a second time where a row needs a new reference (one copy of the code)
@@ -454,7 +457,7 @@ kv_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const AttendParams p)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * grp + b]);
-        ks = bad ? __int_as_float(0x7fc00000) : attend_key_scale(ks_next);
+        ks = bad ? __int_as_float(0x7fc00000) : attend_key_scale(fabsf(ks_next));
         vs = fabsf(vs_next);
         lv = log2f(vs);
       }

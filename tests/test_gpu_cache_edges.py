@@ -1,11 +1,13 @@
-"""Calls at the edges of what the paged cache allows: rows that are not finite inside longer runs, scales below the normal range."""
+"""Calls at the edges of what the paged cache allows: rows that are not finite inside longer runs, scales below the normal range
+and below zero."""
 import importlib
 
 import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_cache import DT, codes_of, write_reference
+from tests.test_gpu_cache import DT, codes_of, filled, i32, write_reference
+from tests.test_gpu_prompt_attention import reference
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +63,26 @@ def test_runs_whose_scale_has_no_reciprocal(G, x, heads, dim, top):
         t[5:14] = 0
         t[:, :, 16:32] = 0
     check_write(G, k.to(DT[x]), v.to(DT[x]), slots, 2, 64)
+
+
+@pytest.mark.parametrize('x', ['f16', 'bf16', 'f32'])
+@pytest.mark.parametrize('new', [1, 20, 100, 300])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('scale', [None, -0.2])
+def test_negative_scales_of_keys(G, x, new, D, scale):
+    """A page with a negative scale is one with a positive scale and negated codes, whatever the scores' range in its tiles is."""
+    lengths = [700, 400]
+    cache, table, gen = filled(G, lengths, 2, D, 64, D + new)
+    cache.k.clamp_(min=1)                                                 # every code has a negative
+    cache.k_scale[::2] *= 4                                               # scores some 50 powers of two apart
+    same = G.KVCache(cache.num_pages, 2, D, 64)
+    for name in ('k', 'v', 'k_scale', 'v_scale'):
+        getattr(same, name).copy_(getattr(cache, name))
+    cache.k_scale[::3] *= -1
+    same.k[::3] = (256 - same.k[::3].int()).to(torch.uint8)
+    q = (2 * torch.randn((2 * new, 4, D), generator=gen, device='cuda')).to(DT[x])
+    out, lse = cache.attend(q, table, i32(lengths), i32([0, new, 2 * new]), new, scale=scale, return_lse=True)
+    want, wl, tol, tl = reference(same, table, q, lengths, [new, new], D ** -0.5 if scale is None else scale)
+    off = (out.double() - want).abs()
+    assert bool((off <= tol).all()), f'{float((off / tol).max())} of the tolerance'
+    assert bool(((lse.double() - wl).abs() <= tl).all())
