@@ -15,6 +15,7 @@ after the other.
 """
 from __future__ import annotations
 
+import math
 from collections import namedtuple
 
 import torch
@@ -218,7 +219,8 @@ class KVCache:
         only steers the choice of kernel.  Rows that see nothing are zero.  Rows behind the last request are zero in a
         new result and left as they were in `out`.  A page number outside the cache makes its rows NaN (scales
         that are not finite spoil the rows that see their page, and no others).  `scale` defaults to
-        head_dim ** -0.5.  With `return_lse` also the logarithm of the sum of exponentials, fp32 (tokens, heads)."""
+        head_dim ** -0.5.  With `return_lse` also the logarithm of the sum of exponentials, fp32 (tokens, heads), -inf in rows that
+        see nothing and in those behind the last request."""
         q, shape, strides = self._rows(q, 'q', None)
         d, tokens, heads = self.device, shape[0], shape[1]
         if block_table.dim() != 2 or block_table.dtype != torch.int32:
@@ -246,7 +248,9 @@ class KVCache:
             _cuda(out, 'out', d)
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
                 raise ValueError(f'out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}')
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=d) if return_lse else None
+        lse = None
+        if return_lse:                   # new in either case: KV_ZERO_REST, which sets the rows behind the last request, goes with a new result
+            lse = torch.empty(shape[:2], dtype=torch.float32, device=d) if fresh else torch.full(shape[:2], -math.inf, dtype=torch.float32, device=d)
         index, code = d.index, _DT[q.dtype]
         args = (q.data_ptr(), code, strides[0], strides[1], out.data_ptr(), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
                 self.v_scale.data_ptr(), self.num_pages, self.page_size, table.data_ptr(), pitch[0], width, lengths.data_ptr(), _ptr(cu_seqlens),

@@ -86,3 +86,17 @@ def test_negative_scales_of_keys(G, x, new, D, scale):
     off = (out.double() - want).abs()
     assert bool((off <= tol).all()), f'{float((off / tol).max())} of the tolerance'
     assert bool(((lse.double() - wl).abs() <= tl).all())
+
+
+@pytest.mark.parametrize('new', [3, 90])
+def test_lse_behind_the_last_request_beside_a_given_result(G, new):
+    lengths = [200, 100]
+    cache, table, gen = filled(G, lengths, 2, 64, 64, 3)
+    q = torch.randn((2 * new + 40, 4, 64), generator=gen, device='cuda').half()
+    cu = i32([0, new, 2 * new])
+    _, want = cache.attend(q, table, i32(lengths), cu, new, return_lse=True)
+    out = torch.full_like(q, 7.0)
+    used = torch.full(want.shape, 3.0, device='cuda')                  # what the allocator hands out next
+    del used
+    _, lse = cache.attend(q, table, i32(lengths), cu, new, out=out, return_lse=True)
+    assert torch.equal(lse, want) and bool((lse[2 * new:] == -float('inf')).all()) and bool((out[2 * new:] == 7).all())
