@@ -609,7 +609,7 @@ extern "C" int jgq_kv_attend(const void* q, int q_dtype, int64_t q_token_stride,
                   pages <= 2147483647LL && table_width * page_size <= 2147483647LL - 64,
               JGQ_ERR_LIMIT, "kv_attend: shape too large");
   if (tokens == 0) return JGQ_OK;
-  JGQ_REQUIRE(q && out && k && v && k_scale && v_scale && lengths && (block_table || table_width == 0), JGQ_ERR_ARG, "kv_attend: null pointer");
+  JGQ_REQUIRE(q && out && k && v && k_scale && v_scale && (requests == 0 || (lengths && (block_table || table_width == 0))), JGQ_ERR_ARG, "kv_attend: null pointer");
   const size_t xb = dtype_size(q_dtype);
   JGQ_REQUIRE(aligned(q, xb) && aligned(out, xb) && aligned(k, 16) && aligned(v, 16), JGQ_ERR_ALIGN, "kv_attend: misaligned pointer");
   const size_t need = jgq_kv_attend_workspace_bytes(q_heads, kv_heads, head_dim, max_new, q_dtype);

@@ -100,3 +100,15 @@ def test_lse_behind_the_last_request_beside_a_given_result(G, new):
     del used
     _, lse = cache.attend(q, table, i32(lengths), cu, new, out=out, return_lse=True)
     assert torch.equal(lse, want) and bool((lse[2 * new:] == -float('inf')).all()) and bool((out[2 * new:] == 7).all())
+
+
+@pytest.mark.parametrize('new', [1, 90])
+def test_rows_of_no_request(G, new):
+    """A step without requests: all rows lie behind the last one."""
+    cache, _, gen = filled(G, [10], 2, 64, 64, 3)
+    q = torch.randn((5, 4, 64), generator=gen, device='cuda').half()
+    none, table = i32([]), torch.zeros((0, 4), dtype=torch.int32, device='cuda')
+    got, lse = cache.attend(q, table, none, i32([0]), new, return_lse=True)
+    assert bool((got == 0).all()) and bool((lse == -float('inf')).all())
+    out = torch.full_like(q, 7.0)
+    assert bool((cache.attend(q, table, none, i32([0]), new, out=out) == 7).all())
