@@ -240,8 +240,8 @@ int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed,
  *     (natural logarithm of the sum of exponentials) may be null.  Sequence r has lengths[r] tokens (at most
  *     table_width * page_size are looked at) in the pages block_table[r][...]; its rows are cu_seqlens[r] .. cu_seqlens[r + 1] - 1, or
  *     row r where cu_seqlens is null; row i of n sees the first lengths[r] - n + i + 1 tokens, and is zero where that is none.
- *     max_new is the expected largest n (a larger one is computed all the same).  Rows behind cu_seqlens[requests] are left as
- *     they were, in out and lse, or become zero (lse: -infinity) with JGQ_KV_ZERO_REST.  A page number outside [0, pages) makes its rows NaN;
+ *     max_new is the expected largest n (a larger one is computed all the same).  Rows behind cu_seqlens[requests] and in front
+ *     of cu_seqlens[0] are left as they were, in out and lse, or become zero (lse: -infinity) with JGQ_KV_ZERO_REST.  A page number outside [0, pages) makes its rows NaN;
  *     scales that are not finite make the rows that see their page something that is not.
  *     The first 16384 bytes of the workspace must be zero before its first use (the kernels leave them zero).
  * jgq_kv_reserve: pages of finished requests (finished[r] != 0; may be null) back to the stack free_pages[0 .. free_count), pages

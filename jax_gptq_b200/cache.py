@@ -216,11 +216,11 @@ class KVCache:
         Request r has `lengths[r]` tokens, in the pages `block_table[r]`.  Without `cu_seqlens` row r of q is the last
         of them; with it (int32, requests + 1) rows cu_seqlens[r] .. cu_seqlens[r + 1] - 1 are the last ones, and each sees the
         tokens up to its own.  `max_new` is the largest number of rows of a request that is expected (default: all of q); it
-        only steers the choice of kernel.  Rows that see nothing are zero.  Rows behind the last request are zero in a
-        new result and left as they were in `out`.  A page number outside the cache makes its rows NaN (scales
+        only steers the choice of kernel.  Rows that see nothing are zero.  Rows of no request (behind the
+        last one, or in front of cu_seqlens[0]) are zero in a new result and left as they were in `out`.  A page number outside the cache makes its rows NaN (scales
         that are not finite spoil the rows that see their page, and no others).  `scale` defaults to
         head_dim ** -0.5.  With `return_lse` also the logarithm of the sum of exponentials, fp32 (tokens, heads), -inf in rows that
-        see nothing and in those behind the last request."""
+        see nothing and in those of no request."""
         q, shape, strides = self._rows(q, 'q', None)
         d, tokens, heads = self.device, shape[0], shape[1]
         if block_table.dim() != 2 or block_table.dtype != torch.int32:
@@ -249,7 +249,7 @@ class KVCache:
             if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
                 raise ValueError(f'out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}')
         lse = None
-        if return_lse:                   # new in either case: KV_ZERO_REST, which sets the rows behind the last request, goes with a new result
+        if return_lse:                   # new in either case: KV_ZERO_REST, which sets the rows of no request, goes with a new result
             lse = torch.empty(shape[:2], dtype=torch.float32, device=d) if fresh else torch.full(shape[:2], -math.inf, dtype=torch.float32, device=d)
         index, code = d.index, _DT[q.dtype]
         args = (q.data_ptr(), code, strides[0], strides[1], out.data_ptr(), _ptr(lse), self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),

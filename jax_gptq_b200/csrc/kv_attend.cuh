@@ -18,7 +18,7 @@ struct AttendParams {
   int T, B, W, Hq, Hkv, group, D, P, pages;
   int q_map;                   // prompts: rows of q come by TMA
   int vec_q, vec_o;            // 16-byte loads of q, stores of four channels are legal
-  int zero_rest;               // rows behind the last sequence are zeroed
+  int zero_rest;               // rows of no sequence are zeroed
   int G;                       // CTAs
   float scale;                 // of the scores, times log2(e)
 };
@@ -236,15 +236,19 @@ struct AttendCursor {
   }
 };
 
-// rows of q behind the last sequence become zero
+// rows of q behind the last sequence, and in front of the first, become zero
 template <typename XT, int THREADS>
 __device__ __forceinline__ void attend_zero_rest(const AttendParams& p) {
   if (!p.zero_rest || !p.cu) return;
-  const int64_t first = max(0, min(p.cu[p.B], p.T)), count = (p.T - first) * p.Hq * p.D, at = blockIdx.x * (int64_t)THREADS + threadIdx.x;
-  XT* o = reinterpret_cast<XT*>(p.out) + first * p.Hq * p.D;
-  for (int64_t i = at; i < count; i += (int64_t)gridDim.x * THREADS) o[i] = from_f32<XT>(0.f);
-  if (p.lse)
-    for (int64_t i = first * p.Hq + at; i < (int64_t)p.T * p.Hq; i += (int64_t)gridDim.x * THREADS) p.lse[i] = -INFINITY;
+  const int64_t front = max(0, min(p.cu[0], p.T)), behind = max(0, min(p.cu[p.B], p.T)), at = blockIdx.x * (int64_t)THREADS + threadIdx.x;
+  auto clear = [&](int64_t first, int64_t rows) {
+    XT* o = reinterpret_cast<XT*>(p.out) + first * p.Hq * p.D;
+    for (int64_t i = at; i < rows * p.Hq * p.D; i += (int64_t)gridDim.x * THREADS) o[i] = from_f32<XT>(0.f);
+    if (p.lse)
+      for (int64_t i = at; i < rows * p.Hq; i += (int64_t)gridDim.x * THREADS) p.lse[first * p.Hq + i] = -INFINITY;
+  };
+  if (front > 0) clear(0, min(front, behind));
+  clear(behind, p.T - behind);
 }
 
 // where row `col` of an item goes: the row of (token, head)

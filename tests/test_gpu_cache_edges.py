@@ -112,3 +112,20 @@ def test_rows_of_no_request(G, new):
     assert bool((got == 0).all()) and bool((lse == -float('inf')).all())
     out = torch.full_like(q, 7.0)
     assert bool((cache.attend(q, table, none, i32([0]), new, out=out) == 7).all())
+
+
+@pytest.mark.parametrize('x', ['f16', 'f32'])
+@pytest.mark.parametrize('new', [3, 90])
+def test_rows_in_front_of_the_first_request(G, new, x):
+    lengths = [200, 100]
+    cache, table, gen = filled(G, lengths, 2, 64, 64, 3)
+    q = torch.randn((2 * new + 7, 4, 64), generator=gen, device='cuda').to(DT[x])
+    want, wl = cache.attend(q[5:], table, i32(lengths), i32([0, new, 2 * new]), new, return_lse=True)
+    used = torch.full_like(q, 3.0)                                        # what the allocator hands out next
+    del used
+    got, lse = cache.attend(q, table, i32(lengths), i32([5, new + 5, 2 * new + 5]), new, return_lse=True)
+    assert torch.equal(got[5:], want) and torch.equal(lse[5:], wl)
+    assert bool((got[:5] == 0).all()) and bool((lse[:5] == -float('inf')).all())
+    out = torch.full_like(q, 7.0)
+    cache.attend(q, table, i32(lengths), i32([5, new + 5, 2 * new + 5]), new, out=out)
+    assert torch.equal(out[5:-2], want[:-2]) and bool((out[:5] == 7).all()) and bool((out[-2:] == 7).all())
