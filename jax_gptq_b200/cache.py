@@ -19,6 +19,7 @@ import math
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
@@ -172,6 +173,8 @@ class KVCache:
             if torch.is_grad_enabled():
                 raise ValueError(f'{name} requires a gradient; the cache has none (detach it)')
             t = t.detach()
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name} has a tangent; the cache has none (detach it)')
         strides = t.stride()
         if strides[2] != 1 and shape[2] != 1:
             t = t.contiguous()

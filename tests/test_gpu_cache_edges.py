@@ -5,6 +5,7 @@ import importlib
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from tests.test_gpu_cache import DT, codes_of, filled, i32, write_reference
 from tests.test_gpu_prompt_attention import reference
@@ -129,3 +130,17 @@ def test_rows_in_front_of_the_first_request(G, new, x):
     out = torch.full_like(q, 7.0)
     cache.attend(q, table, i32(lengths), i32([5, new + 5, 2 * new + 5]), new, out=out)
     assert torch.equal(out[5:-2], want[:-2]) and bool((out[:5] == 7).all()) and bool((out[-2:] == 7).all())
+
+
+def test_forward_mode_tangents_are_refused(G):
+    cache, table, gen = filled(G, [10], 2, 64, 64, 3)
+    q = torch.randn((1, 4, 64), generator=gen, device='cuda')
+    kv, slots = torch.randn((1, 2, 64), generator=gen, device='cuda'), torch.tensor([3], device='cuda')
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(q, torch.ones_like(q))
+        with pytest.raises(ValueError, match='tangent'):
+            cache.attend(dual, table, i32([10]))
+        with pytest.raises(ValueError, match='tangent'):
+            cache.write(kv, fwAD.make_dual(kv, torch.ones_like(kv)), slots)
+        cache.attend(q, table, i32([10]))                                 # nothing depends on these
+        cache.write(kv, kv, slots)

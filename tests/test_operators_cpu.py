@@ -125,3 +125,24 @@ def test_grouped_workspaces(jlib):  # noqa: F811
                         call = lambda ws, n: lib.jgq_w4_group_matmul(256, xd, 256, 256, 256, jlib.F32, 256, M, N, K, g, flags, ws, n, None)
                         assert call(256, 16383) == -3 and call(None, need) == -3
                         assert call(8, need) == -2
+
+
+def test_rows_with_a_tangent_are_refused(jlib):  # noqa: F811
+    """Keys, values and queries of the cache have no derivative; a forward-mode one would be lost."""
+    import types
+
+    import torch
+    import torch.autograd.forward_ad as fwAD
+    from jax_gptq_b200.cache import KVCache
+    cache = KVCache.__new__(KVCache)
+    cache.device, cache.head_dim = types.SimpleNamespace(index=-1), 8    # -1: what CPU tensors answer
+    t = torch.zeros((3, 2, 8))
+    assert cache._rows(t, 'q', None)[1] == (3, 2, 8)
+    with fwAD.dual_level():
+        assert cache._rows(t, 'q', 2)[0] is t
+        with pytest.raises(ValueError, match='tangent'):
+            cache._rows(fwAD.make_dual(t, torch.ones_like(t)), 'q', None)
+        with torch.no_grad(), pytest.raises(ValueError, match='tangent'):
+            cache._rows(fwAD.make_dual(t, torch.ones_like(t)).transpose(0, 1), 'q', None)
+    with pytest.raises(ValueError, match='gradient'):
+        cache._rows(t.clone().requires_grad_(), 'q', None)
