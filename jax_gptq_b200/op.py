@@ -175,6 +175,8 @@ def _group_matmul(x, w, zero, scale, group_size, transpose_b):
         _check_groups(2, 0, 2 * rows, channels, group_size, scale, zero)
     if not (x.get_device() == w.get_device() == zero.get_device() == scale.get_device()):
         raise ValueError(f'x is on {x.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
+    if (zero.requires_grad or scale.requires_grad) and torch.is_grad_enabled():
+        raise ValueError('scales and zero points of groups have no gradient: only x has one (detach them)')
     if _needs_function(x, zero, scale):
         return _GroupMatmul.apply(x, w, zero, scale, group_size, transpose_b)
     return _launch_groups(x, w, zero, scale, group_size, transpose_b)
@@ -182,8 +184,9 @@ def _group_matmul(x, w, zero, scale, group_size, transpose_b):
 
 def quantized_matmul(x, quantized_matrix, transpose_b=False):
     """x @ dequant(quantized_matrix) (or its transpose); result in x's dtype.  A matrix with a ``group_size`` has a scale and
-    a zero point per group of rows and channel, one without per channel.  Calls may come from several host threads, also on
-    one stream."""
+    a zero point per group of rows and channel, one without per channel.  Only x has a gradient: scales and zero points of groups
+    that require one are refused, those per channel count as constants (op.py:71-81).  Calls may come from several host
+    threads, also on one stream."""
     if type(x) is torch.Tensor and x.is_cuda and x.dtype in _DT:
         as_np, xd = False, x
     else:

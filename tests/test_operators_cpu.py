@@ -146,3 +146,15 @@ def test_rows_with_a_tangent_are_refused(jlib):  # noqa: F811
             cache._rows(fwAD.make_dual(t, torch.ones_like(t)).transpose(0, 1), 'q', None)
     with pytest.raises(ValueError, match='gradient'):
         cache._rows(t.clone().requires_grad_(), 'q', None)
+
+
+def test_trainable_scales_of_groups_are_refused(jlib):  # noqa: F811
+    import torch
+    from jax_gptq_b200.op import _group_matmul
+    w, x = torch.zeros((32, 16), dtype=torch.uint8), torch.zeros((3, 64))
+    for trained in range(2):
+        parts = [torch.zeros((2, 16)), torch.ones((2, 16))]
+        parts[trained].requires_grad_()
+        for flip in (False, True):
+            with pytest.raises(ValueError, match='no gradient'):
+                _group_matmul(x[:, :16] if flip else x, w, *parts, 32, flip)
