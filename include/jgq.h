@@ -248,7 +248,7 @@ int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* packed,
  *     for lengths[r] + added[r] tokens of every request from it into block_table, held[r] (pages of a request) with them;
  *     then slots and positions of the added tokens (-1 and 0 behind the last one, up to max_tokens), cu_seqlens (requests + 1) and
  *     lengths_out = lengths + added.  All or nothing: otherwise a bit is or-ed into *status, no page is taken, every slot
- *     is -1, cu_seqlens is zero and lengths_out = lengths.  Any page_size >= 1.
+ *     is -1, cu_seqlens is zero and lengths_out = lengths; pages of finished requests are back on the stack all the same.  Any page_size >= 1.
  * jgq_capture_id: 0 if the stream is not being captured, else a number of the capture (host; launches nothing). */
 enum { JGQ_KV_ZERO_REST = 1 };
 enum { JGQ_KV_NO_PAGES = 1, JGQ_KV_ROW_FULL = 2, JGQ_KV_TOO_MANY_TOKENS = 4, JGQ_KV_BAD_LENGTH = 8, JGQ_KV_BAD_TABLE = 16 };

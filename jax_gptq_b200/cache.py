@@ -105,7 +105,8 @@ class PageTable:
         that takes the place.  Pages that a request already holds are kept, also when its length is set back.
         `max_tokens` bounds the sum of `added` and is the length of the slot map.  All or nothing: a step that does not fit
         (too few pages or columns, too many tokens, a negative length) takes no page, its slots are all -1, cu_seqlens
-        is zero, the lengths stay, and `status` says why."""
+        is zero, the lengths stay, and `status` says why.  What finished requests held goes back to the stack all the
+        same, before the step is weighed: the call may be made again, with the same `finished` or without."""
         d, n = self.device, self.requests
         lengths, added = _vector(lengths, 'lengths', torch.int32, n, d), _vector(added, 'added', torch.int32, n, d)
         if finished is not None:

@@ -6,7 +6,8 @@
 //   every request gets the pages it lacks for lengths[r] + added[r] tokens, requests in order, popped from the stack;
 //   slots / positions of the added tokens, cu_seqlens over the requests, lengths behind the step.
 // All or nothing: if a request's tokens do not fit its row of the table, the stack has too few pages, more tokens are added than
-// the slot map holds or a length is negative, no page is taken, every slot is -1, cu_seqlens is zero, lengths stay.
+// the slot map holds or a length is negative, no page is taken, every slot is -1, cu_seqlens is zero, lengths stay.  The first of these
+// three is done by then: it does not depend on the rest, and doing it again does nothing.
 //
 // Latency-bound: one CTA of 1024 threads scans the requests (1024 at a time) twice, once for the totals; pages and, up to
 // KT_SMALL of them, slots are handed out by all threads, each finding its request by bisection in the scanned sums.  Larger

@@ -144,3 +144,23 @@ def test_forward_mode_tangents_are_refused(G):
             cache.write(kv, fwAD.make_dual(kv, torch.ones_like(kv)), slots)
         cache.attend(q, table, i32([10]))                                 # nothing depends on these
         cache.write(kv, kv, slots)
+
+
+def test_a_refused_step_has_taken_back_what_finished_requests_held(G):
+    """Nothing is handed out, but the pages of those who left are free; the same call again, then one that fits."""
+    table = G.PageTable(3, 4, 6, 64)
+    table.reserve(i32([0, 0, 0]), i32([100, 60, 128]), 300)
+    held = table.block_table.tolist()
+    gone = torch.tensor([False, True, True], device='cuda')
+    for _ in range(2):
+        got = table.reserve(i32([100, 0, 0]), i32([1, 256, 256]), 600, finished=gone)         # eight pages of four
+        assert got.slots.tolist() == [-1] * 600 and got.cu_seqlens.tolist() == [0] * 4 and got.lengths.tolist() == [100, 0, 0]
+        assert table.held.tolist() == [2, 0, 0] and int(table.free_count) == 4
+        assert table.block_table.tolist() == [held[0], [-1] * 4, [-1] * 4]
+        with pytest.raises(RuntimeError, match='too few free pages'):
+            table.check()
+    got = table.reserve(i32([100, 0, 0]), i32([1, 64, 65]), 130)
+    table.check()
+    assert table.held.tolist() == [2, 1, 2] and got.lengths.tolist() == [101, 64, 65]
+    pages = [p for row in table.block_table.tolist() for p in row if p >= 0]
+    assert sorted(pages + table.free[:int(table.free_count)].tolist()) == list(range(6))
