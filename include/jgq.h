@@ -215,7 +215,8 @@ int jgq_w4_matmul_noalloc(const void* x, int x_dtype, const uint8_t* packed,
  *     w[k, n] = scale[k / group_size, n] * (code[k, n] - zero[k / group_size, n])
  * jgq_group_params: jgq_col_params of every group.  jgq_gptq_quantize_groups: jgq_gptq_quantize with those params; a block
  * of the loop must lie in one group (group_size % block_size == 0).  jgq_w4_group_matmul: jgq_w4_matmul with them; the
- * first 16384 bytes of its workspace must be zero before its first use (the kernels leave them zero). */
+ * first 16384 bytes of its workspace must be zero before its first use (the kernels leave them zero).  Where N % 4 != 0 or packed is
+ * not 4-byte aligned it reads whole aligned words, up to 3 bytes in front of and behind `packed` with them (and ignores those). */
 int jgq_group_params(const float* W, int64_t K, int64_t N, int group_size, int maxq, float* scale, float* zero, void* stream);
 int jgq_gptq_quantize_groups(float* W, const float* L, const float* scale, const float* zero,
                              int64_t K, int64_t N, int group_size, int block_size, int maxq,

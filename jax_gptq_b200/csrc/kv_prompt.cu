@@ -16,8 +16,10 @@
 // The sum of exponentials has a reference of its own, the running maximum of the scores (kept within 2^12): it takes p' before the
 // rounding, 64 of them at a time, times 2^(reference - log2(v_scale) - maximum) (two units of 2^-23 off at most, as 2^x is).
 //
-// Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit, which bounds
-// the softmax warps: 1600 clocks of a tile's 2650 go by between the first score and the last p' of 256 rows).
+// Per tile and 128 rows: 512 tensor clocks (DW = 128), 8192 exponentials (512 clocks of the special function unit); a tile of 256 rows takes
+// 2650 clocks.  No unit is full (a capture shows the special function unit 26 % busy, the tensor pipe 24 %, issue 43 %): the softmax
+// warps' chain bounds it, 1600 clocks between the first score and the last p', in which a thread loads 32 scores, waits for them and
+// computes, twice.
 // Measured: four chunks of 512 rows, 32 heads of 128, up to 4096 tokens (f16): 95 us, 36 GFLOP; 2048 rows, 16384 tokens, 32 / 8 heads
 // (bf16): 640 us, 0.8 PFLOP/s.  Copies of the softmax loop cost more than a second pass over a tile: with three of them 109 and 684 us.
 //

@@ -16,9 +16,10 @@
 // A CTA looks through `chunk` rows for the runs that begin there; which rows follow on their predecessors is found once, as a
 // mask, for the chunk and what its last run may reach.  Runs of one row (a decode step) go to a warp each, without a barrier.
 //
-// Measured (f16, 32 heads of 128, 6 x 2000 rows into pages of 128): write 105 us (295 MB, 2.8 TB/s), read 64 (4.6 TB/s).  The write issues 20
-// instructions per element: bound by the conversions' ALU work and instruction fetch.  256 single rows of 8 heads, bf16, and their pages
-// read back: 30 us (49 with IEEE divisions and a CTA per row).
+// Measured (f16, 32 heads of 128, 6 x 2000 rows into pages of 128): write 107 us (295 MB, 2.7 TB/s), read 64 to 76 (4.6 to 4.0 TB/s).  A CTA
+// loads, takes the maximum and encodes one run after the other, with nothing of the next one under way: a capture of the write shows the wait for
+// loads as the first stall, issue 64 %, ALU 54 % (20 instructions per element), and 18 % of the cycles idle at the end.  256 single rows of 8
+// heads, bf16: write 9.4 us (1.6 MB: launch and one chain of load, maximum, codes), read of their pages 21; both 30 (49 with IEEE divisions and a CTA per row).
 #include "kv_cache.cuh"
 #include <algorithm>
 #include <cstring>

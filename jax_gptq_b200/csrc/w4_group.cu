@@ -20,8 +20,11 @@
 // the result's own rounding); fp32 activations as three (all 24 bits).
 // A long contraction with few tiles is split; the CTA that draws a tile's last ticket adds the slices in order.
 //
+// What is rounded is relative to scale |code - 8|: a weight of zero (code and zero point both 0, say) may bring 2^-14 of scale |x| (fp32:
+// 2^-21) instead of nothing in the transposed product, whose planes hold x scale while the zero point's sum does not.
+//
 // Bound by the legacy tensor path and what feeds it (three planes of fp32 activations): 1024 x 4096 x 4096 fp32 502 us, 205
-// TFLOP/s executed; transposed 554.  Small ones by latency: 137 x 272 x 909 fp32 13.5 us, transposed 14.8.
+// TFLOP/s executed; transposed 553.  Small ones by latency: 137 x 272 x 909 fp32 13.5 us, transposed 14.8.
 #include "w4_common.cuh"
 #include "w4_plans.cuh"
 #include <algorithm>
@@ -45,7 +48,7 @@ struct GroupParams {
   int32_t* tickets;            // one per tile of a split contraction, zero between launches
   int64_t M, N, K;
   int64_t rows, depth;         // weight rows of the product (N or K) and its contraction length (K or N)
-  int group, groups;
+  int group;
   int chunks_per_split, splits;
   int vec_w;                   // 4-byte loads of codes are legal
   int vec_x;                   // 16-byte loads of activations are legal
@@ -125,7 +128,7 @@ w4_group_kernel(const GroupParams p) {
         const uint8_t* src = p.packed + br * p.N + n;
         if (p.vec_w) {
           w = *reinterpret_cast<const uint32_t*>(src);       // N % 4 == 0: the word is inside the row
-        } else {                                             // out of the one or two aligned words that hold its bytes
+        } else {                                             // out of the one or two aligned words that hold its bytes, others' bytes masked
           const uintptr_t at = reinterpret_cast<uintptr_t>(src);
           const uint32_t shift = 8 * (uint32_t)(at & 3), left = (uint32_t)min((int64_t)4, p.N - n);
           const uint32_t* lo = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
@@ -458,7 +461,7 @@ extern "C" int jgq_w4_group_matmul(const void* x, int x_dtype, const uint8_t* pa
   p.x = x; p.packed = packed; p.zero = zero; p.scale = scale; p.out = out;
   p.M = M; p.N = N; p.K = K;
   p.rows = transpose_b ? K : N; p.depth = transpose_b ? N : K;
-  p.group = group_size; p.groups = (int)cdiv(K, group_size);
+  p.group = group_size;
   p.chunks_per_split = pl.chunks_per_split; p.splits = pl.splits;
   p.vec_w = N % 4 == 0 && aligned(packed, 4);
   p.vec_x = p.depth * xb % 16 == 0 && aligned(x, 16);
