@@ -23,7 +23,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _DT, _dev, _ptr, _scratch, _stream_lock
+from .gptq import _DT, _dev, _ptr, _scratch, _stream_locks
 
 PAGE_SIZES = (64, 128, 256)
 
@@ -64,7 +64,7 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 def _launch(index, call, *args):
     """`call` with the current stream of device `index`, on which it runs, behind its arguments."""
     stream = _raw_stream(index)
-    with _stream_lock(index, stream):
+    with _stream_locks[index, stream]:
         if _current_device() == index:
             rc = call(*args, stream)
         else:
@@ -274,7 +274,7 @@ class KVCache:
                 self._ws_bytes.clear()
             need = self._ws_bytes[heads, most, code] = lib.jgq_kv_attend_workspace_bytes(heads, self.kv_heads, self.head_dim, most, code)
         stream = _raw_stream(index)
-        with _stream_lock(index, stream):
+        with _stream_locks[index, stream]:
             rc = lib.jgq_kv_attend(*args, _scratch(need, 'kv', index, stream), need, stream)
         if rc:
             check(rc)

@@ -81,25 +81,23 @@ def _workspace(nbytes, zeroed=False, tag='ws'):
     return buf
 
 
-_stream_locks = {}
-
-
-def _stream_lock(dev, stream):
-    """Held from the lookup of a (device, stream) workspace until the call that uses it has enqueued its launches.  Another host
+class _StreamLocks(dict):
+    """[device, stream]: held from the lookup of their workspace until the call that uses it has enqueued its launches.  Another host
     thread on the same stream can then neither have the buffer replaced, and freed, in between (a later launch may reuse its memory:
     it runs behind these), nor put launches of its own between those of one call."""
-    key = (dev, stream)
-    lock = _stream_locks.get(key)
-    return _stream_locks.setdefault(key, threading.RLock()) if lock is None else lock
+
+    def __missing__(self, key):
+        return self.setdefault(key, threading.RLock())
 
 
+_stream_locks = _StreamLocks()
 _scratch_ws, _capture_ws = {}, {}
 _capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _scratch(nbytes, tag, dev, stream):
     """Address of a zeroed workspace of the current device `dev` and its current stream for kernels that leave their tickets
-    zero, good while the caller holds `_stream_lock`.  While the stream is being captured the buffer belongs to that capture
+    zero, good while the caller holds `_stream_locks[dev, stream]`.  While the stream is being captured the buffer belongs to that capture
     (allocated and cleared inside it, once), so that no two graphs, and no graph and an eager call, ever share one."""
     key = (dev, stream, tag)
     if not _capturing():

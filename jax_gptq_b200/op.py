@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _stream_lock, _check_groups, _DT
+from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _stream_locks, _check_groups, _DT
 
 _functorch_active = torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._get_tracing_state
@@ -72,7 +72,7 @@ def _launch(x, w, zero, scale, transpose_b):
     dev = _current_device()
     need = _workspace_bytes(dev, M, Nw, Kw, transpose_b)
     stream = _raw_stream(dev)
-    with _stream_lock(dev, stream):
+    with _stream_locks[dev, stream]:
         ws = _workspace(need, zeroed=True, tag='w4').data_ptr() if need else 0
         flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
         rc = lib.jgq_w4_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(),
@@ -87,7 +87,7 @@ def _enqueue_groups(x, w, zero, scale, out, M, N, K, group_size, transpose_b, de
     if need is None:
         need = _workspace_bytes(dev, M, N, K, transpose_b, group_size)
     stream = _raw_stream(dev)
-    with _stream_lock(dev, stream):
+    with _stream_locks[dev, stream]:
         flags = _lib.W4_TRANSPOSE_B if transpose_b else _lib.W4_WEIGHTS_SETTLED if _settled_groups(w, zero, scale) else 0
         rc = lib.jgq_w4_group_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(), _ZS[zero.dtype],
                                      out.data_ptr(), M, N, K, group_size, flags, _scratch(need, 'w4g', dev, stream), need, stream)
@@ -175,9 +175,9 @@ def _group_matmul(x, w, zero, scale, group_size, transpose_b):
         _check_groups(2, 0, 2 * rows, channels, group_size, scale, zero)
     if not (x.get_device() == w.get_device() == zero.get_device() == scale.get_device()):
         raise ValueError(f'x is on {x.device}, the matrix on {w.device}, {zero.device}, {scale.device}')
-    if (zero.requires_grad or scale.requires_grad) and torch.is_grad_enabled():
-        raise ValueError('scales and zero points of groups have no gradient: only x has one (detach them)')
     if _needs_function(x, zero, scale):
+        if (zero.requires_grad or scale.requires_grad) and torch.is_grad_enabled():
+            raise ValueError('scales and zero points of groups have no gradient: only x has one (detach them)')
         return _GroupMatmul.apply(x, w, zero, scale, group_size, transpose_b)
     return _launch_groups(x, w, zero, scale, group_size, transpose_b)
 
