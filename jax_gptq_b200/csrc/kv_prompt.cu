@@ -21,7 +21,7 @@
 // warps' chain bounds it, 1600 clocks between the first score and the last p', in which a thread loads 32 scores, waits for them and
 // computes, twice.
 // Measured: four chunks of 512 rows, 32 heads of 128, up to 4096 tokens (f16): 95 us, 36 GFLOP; 2048 rows, 16384 tokens, 32 / 8 heads
-// (bf16): 640 us, 0.8 PFLOP/s.  Copies of the softmax loop cost more than a second pass over a tile: with three of them 109 and 684 us.
+// (bf16): 645 us, 0.8 PFLOP/s.  Copies of the softmax loop cost more than a second pass over a tile: with three of them 109 and 684 us.
 //
 // Roles: warps 0 .. 7 softmax, then one warp for copies (q; a ring of four units of raw codes), one that issues the MMAs,
 // four (with one 118 us instead of 101) that turn the keys' codes into an operand, two for the values' (128-byte

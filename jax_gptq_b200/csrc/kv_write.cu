@@ -16,7 +16,7 @@
 // A CTA looks through `chunk` rows for the runs that begin there; which rows follow on their predecessors is found once, as a
 // mask, for the chunk and what its last run may reach.  Runs of one row (a decode step) go to a warp each, without a barrier.
 //
-// Measured (f16, 32 heads of 128, 6 x 2000 rows into pages of 128): write 107 us (295 MB, 2.7 TB/s), read 64 to 76 (4.6 to 4.0 TB/s).  A CTA
+// Measured (f16, 32 heads of 128, 6 x 2000 rows into pages of 128): write 107 us (295 MB, 2.7 TB/s), read 76 (302 MB, 4.0 TB/s; 56 behind the write).  A CTA
 // loads, takes the maximum and encodes one run after the other, with nothing of the next one under way: a capture of the write shows the wait for
 // loads as the first stall, issue 64 %, ALU 54 % (20 instructions per element), and 18 % of the cycles idle at the end.  256 single rows of 8
 // heads, bf16: write 9.4 us (1.6 MB: launch and one chain of load, maximum, codes), read of their pages 21; both 30 (49 with IEEE divisions and a CTA per row).
