@@ -68,15 +68,14 @@ def _ptr(t):
 _ws_cache = {}
 
 
-def _workspace(nbytes, zeroed=False, tag='ws'):
-    """Per (device, stream) scratch buffer, grown on demand.  `zeroed` buffers are
-    created with zeros and handed only to kernels that restore the zeros."""
+def _workspace(nbytes, tag='ws'):
+    """Per (device, stream) scratch buffer, grown on demand."""
     dev = torch.cuda.current_device()
     key = (dev, torch._C._cuda_getCurrentRawStream(dev), tag)
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         size = max(int(nbytes), 1 << 20)
-        buf = (torch.zeros if zeroed else torch.empty)(size, dtype=torch.uint8, device=_dev())
+        buf = torch.empty(size, dtype=torch.uint8, device=_dev())
         _ws_cache[key] = buf
     return buf
 
@@ -91,25 +90,28 @@ class _StreamLocks(dict):
 
 
 _stream_locks = _StreamLocks()
+_TICKETS = 16384         # bytes at the front of a workspace that the kernels want zero, and leave so
 _scratch_ws, _capture_ws = {}, {}
 _capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _scratch(nbytes, tag, dev, stream):
-    """Address of a zeroed workspace of the current device `dev` and its current stream for kernels that leave their tickets
-    zero, good while the caller holds `_stream_locks[dev, stream]`.  While the stream is being captured the buffer belongs to that capture
-    (allocated and cleared inside it, once), so that no two graphs, and no graph and an eager call, ever share one."""
+    """Address of a workspace of the current device `dev` and its current stream, with zero tickets, for kernels that leave them
+    zero; good while the caller holds `_stream_locks[dev, stream]`.  While the stream is being captured the buffer belongs to that capture
+    (allocated inside it, its tickets cleared there once), so that no two graphs, and no graph and an eager call, ever share one."""
     key = (dev, stream, tag)
     if not _capturing():
         have = _scratch_ws.get(key)
         if have is None or have[0] < nbytes:
-            buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=torch.device('cuda', dev))
+            buf = torch.empty(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=torch.device('cuda', dev))
+            buf[:_TICKETS].zero_()
             have = _scratch_ws[key] = (buf.numel(), buf.data_ptr(), buf)
         return have[1]
     capture = lib.jgq_capture_id(stream)
     owner, buf = _capture_ws.get(key, (0, None))
     if owner != capture or buf.numel() < nbytes:
-        buf = torch.zeros(int(nbytes), dtype=torch.uint8, device=torch.device('cuda', dev))
+        buf = torch.empty(int(nbytes), dtype=torch.uint8, device=torch.device('cuda', dev))
+        buf[:_TICKETS].zero_()
         _capture_ws[key] = (capture, buf)
     return buf.data_ptr()
 

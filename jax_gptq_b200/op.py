@@ -14,7 +14,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
-from .gptq import _to_dev, _out, _is_np, _workspace, _scratch, _stream_locks, _check_groups, _DT
+from .gptq import _to_dev, _out, _is_np, _scratch, _stream_locks, _check_groups, _DT
 
 _functorch_active = torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._get_tracing_state
@@ -73,7 +73,7 @@ def _launch(x, w, zero, scale, transpose_b):
     need = _workspace_bytes(dev, M, Nw, Kw, transpose_b)
     stream = _raw_stream(dev)
     with _stream_locks[dev, stream]:
-        ws = _workspace(need, zeroed=True, tag='w4').data_ptr() if need else 0
+        ws = _scratch(need, 'w4', dev, stream) if need else 0
         flags = (_lib.W4_TRANSPOSE_B if transpose_b else 0) | (_lib.W4_WEIGHTS_SETTLED if _settled(w) else 0)
         rc = lib.jgq_w4_matmul(x.data_ptr(), _DT[x.dtype], w.data_ptr(), zero.data_ptr(), scale.data_ptr(),
                                _ZS[zero.dtype], out.data_ptr(), M, Nw, Kw, flags, ws, need, stream)
